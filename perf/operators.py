@@ -227,19 +227,13 @@ def _frequencies(case):
 def prepare(case, seed):
     g, dt = _gen(seed), DTYPES[case["dtype"]]
     s = {"case": case}
-    if own:
-        s["nxg"] = _nxg()
     if case["op"] == "rope":
         lens = _lengths(case)
         T, H, D = sum(lens), case["heads"], case["dim"]
         # fused: the heads to turn are the first of a projection's rows, as many again (the values) behind
         s["x"] = _randn(g, dt, T, H + (H + 1) // 2, D)[:, :H] if case["fused"] else _randn(g, dt, T, H, D)
         s["cu"] = torch.from_numpy(_offsets(lens)).cuda()
-        if own:
-            f, s["mscale"] = s["nxg"].rope_frequencies(case["rot"], case["base"], case["scaling"], case["factor"],
-                                                       case["train_len"])
-        else:
-            f, s["mscale"] = _frequencies(case)
+        f, s["mscale"] = _frequencies(case)
         s["freq"] = torch.from_numpy(f).cuda()
         s["lens"] = lens
         return s
@@ -271,6 +265,7 @@ def prepare(case, seed):
         s["dout"] = (0.1 * torch.randn(T, H, D, device="cuda", generator=g)).to(dt)
     s["cu_q"], s["cu_k"] = (torch.from_numpy(_offsets(n)).cuda() for n in (lens, keys))
     s["lens"], s["keys"] = lens, keys
+    s["groups"] = _groups(case)                     # of use to the plain form
     return s
 
 
@@ -279,7 +274,7 @@ def prepare(case, seed):
 def run(s):
     case = s["case"]
     if own:
-        nxg = s["nxg"]
+        nxg = _nxg()
         if case["op"] == "rope":
             return nxg.rope_rows(s["x"], s["freq"], s["cu"], layout=case["layout"], mscale=s["mscale"],
                                  inverse=case["inverse"])
@@ -352,8 +347,33 @@ def _span(case, n, m, r, rows):
     return lo, max(lo, hi)
 
 
+def _groups(case):
+    """The documents in groups of like lengths, padded to one batch each: the rows of q and k of
+    [document][position], row 0 behind a document's end, and the lengths."""
+    lens, keys = np.array(_lengths(case)), np.array(_lengths(case, "keys"))
+    t0, k0 = _offsets(lens)[:-1], _offsets(keys)[:-1]
+    left, out = sorted(range(len(lens)), key=lambda d: (-keys[d], -lens[d])), []
+    while left:
+        n, m = lens[left].max(), keys[left[0]]
+        most = max(1, CHUNK // (case["heads"] * max(1, n * m)))
+        # all at once where they are few, else those of at least two thirds of the longest
+        near = left if len(left) <= most else [d for d in left if 3 * keys[d] >= 2 * m][:most]
+        left = [d for d in left if d not in near]
+        n, m = lens[near].max(), keys[near].max()
+        i, j = np.arange(n)[None, :], np.arange(m)[None, :]
+        nd, md = lens[near][:, None], keys[near][:, None]
+        pad = lambda start, at, size: torch.from_numpy(np.where(at < size, start[near][:, None] + at, 0)).cuda()  # noqa: E731
+        # where each row of the documents is in the padded batch, one after another
+        flat = lambda at, size: torch.from_numpy(np.flatnonzero(at < size)).cuda()  # noqa: E731
+        dst = lambda start, at, size: torch.from_numpy((start[near][:, None] + at)[at < size]).cuda()  # noqa: E731
+        out.append({"n": int(n), "m": int(m), "q": pad(t0, i, nd), "k": pad(k0, j, md),
+                    "q_flat": flat(i, nd), "q_row": dst(t0, i, nd), "k_flat": flat(j, md), "k_row": dst(k0, j, md),
+                    "nd": torch.from_numpy(nd).cuda(), "md": torch.from_numpy(md).cuda(), "alike": bool((nd == n).all() and (md == m).all())})
+    return out
+
+
 def _plain_attention(s, train):
-    """Per document, all heads at a time, in pieces of the queries."""
+    """Groups of documents as padded batches, all heads at a time, in pieces of the queries."""
     case, q, k, v = s["case"], s["q"], s["k"], s["v"]
     H, G, D, R = case["heads"], case["kv_heads"], case["dim"], case["heads"] // case["kv_heads"]
     scale, left, right = case["dim"] ** -0.5, case["left"], case["right"]
@@ -361,56 +381,62 @@ def _plain_attention(s, train):
     if train:
         dq = torch.empty(q.shape, dtype=q.dtype, device="cuda")
         dk, dv = (torch.empty(t.shape, dtype=t.dtype, device="cuda") for t in (k, v))
-    t0 = k0 = 0
-    for n, m in zip(s["lens"], s["keys"]):
-        kh = k[k0:k0 + m].float().transpose(0, 1)                                    # G, m, D
-        vh = v[k0:k0 + m].float().transpose(0, 1).contiguous()
-        kt, kh = kh.transpose(1, 2).contiguous(), kh.contiguous()
+    for g in s["groups"]:
+        B, n, m = g["nd"].shape[0], g["n"], g["m"]
+        if m == 0:                                   # documents without keys
+            out[g["q_row"]] = 0
+            if train:
+                dq[g["q_row"]] = 0
+            continue
+        heads = lambda t, rows: t[rows].float().transpose(1, 2).reshape(-1, rows.shape[1], D)       # noqa: E731
+        kh, vh = heads(k, g["k"]), heads(v, g["k"])                                                  # B * G, m, D
+        kt = kh.transpose(1, 2).contiguous()
+        gq, y = (torch.empty(B, n, H, D, device="cuda") for _ in range(2))
         if train:
             vt = vh.transpose(1, 2).contiguous()
             gk, gv = torch.zeros_like(kh), torch.zeros_like(vh)
-        # with a window a piece sees few keys beside its own: pieces of its size
-        step = max(1, CHUNK // (H * max(1, m)))
-        if left >= 0:
+        step = max(1, CHUNK // (B * H * m))
+        if left >= 0 and g["alike"]:                 # a piece sees few keys beside its own: pieces of that size
             step = min(step, max(256, left + max(right, 0)))
         for r in range(0, n, step):
             rows = min(step, n - r)
-            lo, hi = _span(case, n, m, r, rows)
-            part = slice(t0 + r, t0 + r + rows)
-            # G, R * rows, D: a KV head's queries one after another
-            qh = q[part].float().view(rows, G, R, D).permute(1, 2, 0, 3).reshape(G, R * rows, D)
+            lo, hi = _span(case, n, m, r, rows) if g["alike"] else (0, m)
+            if lo >= hi:
+                lo, hi = 0, m
+            # B * G, R * rows, D: a KV head's queries one after another
+            split = lambda t: t[g["q"][:, r:r + rows]].float().view(B, rows, G, R, D).permute(0, 2, 3, 1, 4).reshape(B * G, R * rows, D)  # noqa: E731
+            join = lambda t: t.view(B, G, R, rows, D).permute(0, 3, 1, 2, 4).reshape(B, rows, H, D)   # noqa: E731
+            qh = split(q)
             sc = torch.bmm(qh, kt[:, :, lo:hi].contiguous()).mul_(scale)
-            if left >= 0 or right >= 0:
-                i = torch.arange(r, r + rows, device="cuda")[:, None] + (m - n)
-                j = torch.arange(lo, hi, device="cuda")[None, :]
-                hide = torch.zeros(rows, hi - lo, dtype=torch.bool, device="cuda")
+            if left >= 0 or right >= 0 or not g["alike"]:
+                j = torch.arange(lo, hi, device="cuda")[None, None, :]
+                at = torch.arange(r, r + rows, device="cuda")[None, :, None] + (g["md"] - g["nd"])[:, :, None]
+                hide = j >= g["md"][:, :, None]
                 if left >= 0:
-                    hide |= j < i - left
+                    hide = hide | (j < at - left)
                 if right >= 0:
-                    hide |= j > i + right
-                sc.view(G, R, rows, hi - lo).masked_fill_(hide, -math.inf)
-            if hi > lo:
-                top = sc.amax(2, keepdim=True)
-                p = sc.sub_(torch.where(top == -math.inf, torch.zeros_like(top), top)).exp_()
-                total = p.sum(2, keepdim=True)
-                p.div_(torch.where(total == 0, torch.ones_like(total), total))
-            else:
-                p = sc
-            y = torch.bmm(p, vh[:, lo:hi].contiguous())
-            out[part] = y.view(G, R, rows, D).permute(2, 0, 1, 3).reshape(rows, H, D).to(q.dtype)
+                    hide = hide | (j > at + right)
+                sc.view(B, G * R, rows, hi - lo).masked_fill_(hide.expand(B, rows, hi - lo)[:, None], -math.inf)
+            top = sc.amax(2, keepdim=True)
+            p = sc.sub_(torch.where(top == -math.inf, torch.zeros_like(top), top)).exp_()
+            total = p.sum(2, keepdim=True)
+            p.div_(torch.where(total == 0, torch.ones_like(total), total))
+            y[:, r:r + rows] = join(torch.bmm(p, vh[:, lo:hi].contiguous()))
             if not train:
                 continue
-            do = s["dout"][part].float().view(rows, G, R, D).permute(1, 2, 0, 3).reshape(G, R * rows, D)
+            do = split(s["dout"])
+            if not g["alike"]:                       # rows behind a document's end
+                do.view(B, G * R, rows, D).mul_((torch.arange(r, r + rows, device="cuda") < g["nd"]).view(B, 1, rows, 1))
             gv[:, lo:hi] += torch.bmm(p.transpose(1, 2).contiguous(), do)
             dp = torch.bmm(do, vt[:, :, lo:hi].contiguous())
             ds = dp.sub_((dp * p).sum(2, keepdim=True)).mul_(p).mul_(scale)
-            gq = torch.bmm(ds, kh[:, lo:hi].contiguous())
-            dq[part] = gq.view(G, R, rows, D).permute(2, 0, 1, 3).reshape(rows, H, D).to(q.dtype)
+            gq[:, r:r + rows] = join(torch.bmm(ds, kh[:, lo:hi].contiguous()))
             gk[:, lo:hi] += torch.bmm(ds.transpose(1, 2).contiguous(), qh)
+        out[g["q_row"]] = y.view(B * n, H, D)[g["q_flat"]].to(q.dtype)
         if train:
-            dk[k0:k0 + m] = gk.transpose(0, 1).to(k.dtype)
-            dv[k0:k0 + m] = gv.transpose(0, 1).to(v.dtype)
-        t0, k0 = t0 + n, k0 + m
+            dq[g["q_row"]] = gq.view(B * n, H, D)[g["q_flat"]].to(q.dtype)
+            rows = lambda t: t.view(B, G, m, D).transpose(1, 2).reshape(B * m, G, D)[g["k_flat"]]      # noqa: E731
+            dk[g["k_row"]], dv[g["k_row"]] = rows(gk).to(k.dtype), rows(gv).to(v.dtype)
     return (out, dq, dk, dv) if train else out
 
 
