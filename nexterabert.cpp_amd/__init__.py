@@ -10,6 +10,9 @@ stream as the HIP stream:
   linear_i8(weight, qact, residual)         op_linear_i8           src/nexterabert.cpp:969-1007
   Builder.linear(name, x, residual)         builder::linear        src/nexterabert.cpp:1121-1143
 
+and, with no counterpart in the reference, floating-point row operators with their gradients (rows.py,
+include/nxg_rows.h): rope_rows, layer_norm_rows, attention_rows.
+
 Errors follow the reference: bad input raises ValueError (rc 1), allocation
 MemoryError (rc 2), device failures RuntimeError (rc 3). There is no CPU
 fallback: without the built library or a gfx950 GPU every device call raises.
@@ -124,6 +127,16 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
         "nxg_linear_i8_relu2_q8_rows": ([P, P, P, i32, i32, P, P, P], i32),
         "nxg_linear_f32_relu2_q8_rows": ([P, P, i32, i32, P, P, P, P, P], i32),
         "nxg_linear_f32_relu2_q8": ([P, P, P, i32, i32, P, P, P, P, P], i32),
+        # include/nxg_rows.h
+        "nxg_rope_frequencies": ([i32, ctypes.c_double, i32, ctypes.c_double, i32, P, P], i32),
+        "nxg_rope_rows": ([i32, P, i32, i32, i32, P, i32, i32, ctypes.c_float, i32, P, P, i32, P, P], i32),
+        "nxg_layer_norm_rows": ([i32, P, i64, P, P, i32, ctypes.c_float, i32, i32, P, i64, P, P, P], i32),
+        "nxg_layer_norm_rows_workspace_bytes": ([i32, i32], i64),
+        "nxg_layer_norm_rows_backward": ([i32, P, i64, P, i64, P, P, P, i32, i32, i32, P, i64, P, P, P, i64, P], i32),
+        "nxg_attention_rows_workspace_bytes": ([P], i64),
+        "nxg_attention_rows": ([P, P, P, P, P, P, P, i64, P], i32),
+        "nxg_attention_rows_backward_workspace_bytes": ([P], i64),
+        "nxg_attention_rows_backward": ([P, P, P, P, P, P, P, P, P, P, P, i64, P], i32),
         "nxg_gemm_kernel_name": ([i32, i32, i32, i32, i32], ctypes.c_char_p),
         # include/nxg_gguf.h
         "nxg_gguf_open": ([ctypes.c_char_p, ctypes.POINTER(P)], i32),
@@ -1262,3 +1275,7 @@ class Builder:
     def reset(self) -> None:
         """Drops the quantized copies (the reference rebuilds its graph per forward)."""
         self.qcache.clear()
+
+
+from .rows import (attention_rows, attention_rows_backward, attention_rows_backward_workspace_bytes,  # noqa: E402
+                   layer_norm_rows, layer_norm_rows_backward, layer_norm_rows_workspace_bytes, rope_frequencies, rope_rows)

@@ -84,18 +84,25 @@ def build(verbose: bool = False) -> Path:
     rocm = Path(_hipcc()).resolve().parent.parent
     _run(["g++", *common, "-D__HIP_PLATFORM_AMD__", f"-I{rocm / 'include'}", "-c", CSRC / "nxg_encoder.cpp",
           "-o", OBJ / "nxg_encoder.o"], verbose)
-    cmd = [str(c) for c in (_hipcc(), *hip_only, *common, "-Rpass-analysis=kernel-resource-usage",
-                            "-c", CSRC / "nxg_linear.hip", "-o", OBJ / "nxg_linear.o")]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    r = subprocess.run(cmd, stderr=subprocess.PIPE, text=True)
-    if r.returncode != 0:
-        sys.stderr.write(r.stderr)
-        raise subprocess.CalledProcessError(r.returncode, cmd)
-    (OBJ / "kernel_resources.txt").write_text(_check_resources(r.stderr) + "\n")
+    # the row operators owe no order of roundings to the reference: products and sums contract to fma there
+    rows_common = ["-ffp-contract=fast" if c == "-ffp-contract=off" else c for c in common] + ["-Wno-inline-asm"]
+    cmds = [[str(c) for c in (_hipcc(), *hip_only, *flags, "-Rpass-analysis=kernel-resource-usage",
+                              "-c", CSRC / f"{src}.hip", "-o", OBJ / f"{src}.o")]
+            for src, flags in (("nxg_linear", common), ("nxg_rows", rows_common), ("nxg_attn_rows", rows_common))]
+    runs = []
+    for cmd in cmds:
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        runs.append(subprocess.Popen(cmd, stderr=subprocess.PIPE, text=True))
+    errs = [r.communicate()[1] for r in runs]
+    for cmd, r, err in zip(cmds, runs, errs):
+        if r.returncode != 0:
+            sys.stderr.write(err)
+            raise subprocess.CalledProcessError(r.returncode, cmd)
+    (OBJ / "kernel_resources.txt").write_text("\n".join(map(_check_resources, errs)) + "\n")
     tmp = LIB.with_suffix(".so.tmp")
     _run([_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-pthread",
-          OBJ / "nxg_linear.o", OBJ / "nxg_host.o", OBJ / "nxg_gguf.o", OBJ / "nxg_encoder.o", "-o", tmp], verbose)
+          OBJ / "nxg_linear.o", OBJ / "nxg_rows.o", OBJ / "nxg_attn_rows.o", OBJ / "nxg_host.o", OBJ / "nxg_gguf.o", OBJ / "nxg_encoder.o", "-o", tmp], verbose)
     os.replace(tmp, LIB)
     tmp = API_LIB.with_suffix(".so.tmp")
     _run(["g++", "-O2", "-fPIC", "-std=c++17", "-Wall", "-fvisibility=hidden", "-DNEXTERA_SHARED", "-DNEXTERA_BUILD",

@@ -1,0 +1,1043 @@
+// nxg_attn_rows.hip -- gfx950 attention over packed 16-bit rows, forward and backward, and its C ABI
+// (include/nxg_rows.h).
+//
+// One KV head's queries are taken as "pairs" (token, query head of the group), pair p = token * R + r
+// with R = n_head / n_kv_head, so that the R heads that share K and V share their tiles too. Every
+// product is an MFMA 32x32x16 with the wave's own 32 rows as the columns of the result:
+//
+//   forward, dQ   S^T = K Q^T     a lane holds 16 keys' scores of one pair (its column)
+//   dK, dV        S   = Q K^T     a lane holds 16 pairs' scores of one key
+//
+// A lane's registers of such a result are, without a move between lanes, the operand of the product
+// that follows (P V, dS K, P^T dO, dS^T Q): 32x32x16 wants 8 values of the contracted index per lane, and
+// the order of that index is free as long as the other operand has the same. That other operand is
+// the tile in LDS read in columns, which ds_read_b64_tr_b16 does 4 rows at a time.
+//
+// Softmax statistics, products and sums are fp32. P and dS are rounded to the inputs' type for the second
+// products (at most half a step of a value in 0..1, its sign alternating over the keys; the sum stays
+// fp32); fp16, whose range they would leave, carries them scaled by powers of two.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+
+#include "nxg_rows.h"
+#include "nxg_internal.h"
+
+namespace {
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
+
+// fp16 alone: P is carried as 2^15 P in the backward pass (P <= 1, fp16 ends at 65504), so that weights
+// down to 2^-29 keep all their bits
+constexpr int P_SHIFT = 15;
+constexpr int N_MAX = 256;     // workgroups of the delta kernel, and row maxima they leave for fp16
+
+template <class E> struct type_of;
+template <> struct type_of<__bf16> {
+    typedef v8b v8;
+    static constexpr bool HALF = false;
+    static __device__ __forceinline__ v16f mfma(v8 a, v8 b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct type_of<_Float16> {
+    typedef v8h v8;
+    static constexpr bool HALF = true;
+    static __device__ __forceinline__ v16f mfma(v8 a, v8 b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+struct rows {
+    char * data;
+    int64_t ts, hs;            // strides in bytes
+};
+
+struct attn_p {
+    rows q, k, v, out, dout, dq, dk, dv;
+    float * lse;               // [T_q][H]
+    float * delta;             // [T_q][H]
+    float * maxima;            // [N_MAX][2]: largest |dout row|^2 and |v row|^2 (fp16)
+    float * part;              // partial sums of the split forward pass
+    const int32_t * cu_q, * cu_k;
+    int32_t n_seqs, T_q, T_k, H, G, R, D, left, right, n_slots, n_split;
+    float scale;
+};
+
+// ---------------------------------------------------------------------------
+// small pieces
+// ---------------------------------------------------------------------------
+
+__device__ __align__(16) const uint32_t zeros16[4] = {};
+
+// 16 bytes per lane from global memory straight into LDS (lane l to lds + 16 l). From inline asm, so
+// that the compiler does not wait for every prefetch before an LDS read; wait_all() and a barrier do.
+__device__ __forceinline__ void dma16(const void * g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(g), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_addr(const void * p) { return (uint32_t) (uintptr_t) (lds_void *) p; }
+
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// max over the two halves of the wave
+__device__ __forceinline__ float half_max(float x) {
+    const v2u r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const v2u r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Row offsets as the caller gave them, kept inside the arrays whatever they hold.
+__device__ __forceinline__ int offset(const int32_t * cu, int d, int T) { return min(max(cu[d], 0), T); }
+
+// The document of a tile slot. Document d owns the slots from floor(cu[d] * mul / tile) + d, which are at
+// least as many as its ceil(len * mul / tile) tiles, so the slots need no pass over the lengths: T * mul /
+// tile + n_seqs of them in all. 64 documents are tried at a time.
+__device__ __forceinline__ int64_t slot_of(const int32_t * cu, int d, int T, int mul, int tile) {
+    return (int64_t) offset(cu, d, T) * mul / tile + d;
+}
+__device__ __forceinline__ int find_doc(const int32_t * cu, int n_seqs, int T, int mul, int tile, int slot) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = n_seqs;               // the document is in lo .. lo + n - 1
+    while (n > 1) {
+        const int step = (n + 63) >> 6;
+        const int d = lo + lane * step;
+        const bool at = lane * step < n && slot_of(cu, d, T, mul, tile) <= slot;
+        const int last = max(__popcll(__ballot(at)) - 1, 0);
+        n = min(step, n - last * step);
+        lo += last * step;
+    }
+    return uni(lo);
+}
+
+struct doc {
+    int q0, n, k0, m;          // first query row, queries, first key row, keys
+};
+__device__ __forceinline__ doc doc_of(const attn_p & p, int d) {
+    doc r;
+    r.q0 = uni(offset(p.cu_q, d, p.T_q));
+    r.n = uni(max(offset(p.cu_q, d + 1, p.T_q) - r.q0, 0));
+    r.k0 = uni(offset(p.cu_k, d, p.T_k));
+    r.m = uni(max(offset(p.cu_k, d + 1, p.T_k) - r.k0, 0));
+    return r;
+}
+// The keys lo .. hi - 1 of query token t.
+__device__ __forceinline__ int key_lo(const attn_p & p, const doc & c, int t) {
+    return p.left < 0 ? 0 : min(max(t + c.m - c.n - p.left, 0), c.m);
+}
+__device__ __forceinline__ int key_hi(const attn_p & p, const doc & c, int t) {
+    return p.right < 0 ? c.m : min(max(t + c.m - c.n + p.right + 1, 0), c.m);
+}
+// The query tokens lo .. hi - 1 that see key j.
+__device__ __forceinline__ int tok_lo(const attn_p & p, const doc & c, int j) {
+    return p.right < 0 ? 0 : min(max(j - (c.m - c.n) - p.right, 0), c.n);
+}
+__device__ __forceinline__ int tok_hi(const attn_p & p, const doc & c, int j) {
+    return p.left < 0 ? c.n : min(max(j - (c.m - c.n) + p.left + 1, 0), c.n);
+}
+
+// ---------------------------------------------------------------------------
+// tiles in LDS
+// ---------------------------------------------------------------------------
+//
+// A tile is rows of SP = 64 or 128 values (the head's D, zeros behind it). The 16-byte chunk c of row r is
+// at chunk c ^ swz(r) of the row: 8 neighbouring rows of one chunk fill all banks (reads of rows: 32 rows
+// of one chunk per half wave), and so do 4 neighbouring rows of a pair of chunks (reads of columns).
+
+__device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+
+template <int DT> constexpr int SP = DT <= 2 ? 64 : 128;
+
+// Loads NR rows by the NT threads of a workgroup (NT = 256) or a wave (64): row r from src(r), a pointer to
+// its D values or null for zeros.
+template <int DT, int NR, int NT, class Src>
+__device__ __forceinline__ void load_rows(uint32_t lds, int D, Src src) {
+    constexpr int CH = SP<DT> / 8;
+    const int t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
+    const uint32_t wave0 = NT == 64 ? 0 : uni(threadIdx.x >> 6) * 1024;
+#pragma unroll
+    for (int it = 0; it < NR * CH / NT; ++it) {
+        const int r = (it * NT + t) / CH, c = (t % CH) ^ swz(r);
+        const char * s = src(r);
+        dma16(s && c * 8 < D ? s + c * 16 : (const char *) zeros16, lds + wave0 + it * NT * 16);
+    }
+}
+
+// Operand of 32 rows: lane l's row l % 32, values 16 s + 8 (l / 32) + 0..7.
+template <class E, int DT>
+__device__ __forceinline__ typename type_of<E>::v8 row_operand(const E * tile, int r0, int s) {
+    const int lane = threadIdx.x & 63, r = lane & 31;
+    const int c = (2 * s + (lane >> 5)) ^ swz(r);
+    return *reinterpret_cast<const typename type_of<E>::v8 *>(tile + (r0 + r) * SP<DT> + c * 8);
+}
+
+// Operand of 32 columns d0 .. d0 + 31 (lane l's column d0 + l % 32), rows r0 + 4 (l / 32) + {0..3, 8..11}: the
+// rows of registers 0..7 of a 32x32 result (r0 a multiple of 16).
+template <class E, int DT>
+__device__ __forceinline__ typename type_of<E>::v8 col_operand(const E * tile, int r0, int d0) {
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    typedef __attribute__((address_space(3))) v4s lds_v4s;
+    v4s x[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int r = r0 + 8 * k + 4 * (g >> 1) + (i >> 2);
+        const int c = (d0 / 8 + 2 * (g & 1) + ((i & 3) >> 1)) ^ swz(r);
+        x[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_v4s *) (lds_void *) (tile + r * SP<DT> + c * 8 + (i & 1) * 4));
+    }
+    typename type_of<E>::v8 out;
+    __builtin_memcpy(&out, x, 16);
+    return out;
+}
+
+// Register i of lane l of a 32x32 result is row 8 (i / 4) + 4 (l / 32) + i % 4 of column l % 32.
+__device__ __forceinline__ constexpr int reg_row(int i) { return 8 * (i / 4) + i % 4; }
+
+// Registers 8 a .. 8 a + 7 as the operand of the next product.
+template <class E>
+__device__ __forceinline__ typename type_of<E>::v8 pack(const v16f & x, int a) {
+    typename type_of<E>::v8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = (E) x[8 * a + j];
+    return o;
+}
+
+// The wave's own 32 rows of D values as an operand in registers, from src (this lane's row).
+template <class E, int DT>
+__device__ __forceinline__ void load_operand(typename type_of<E>::v8 (&x)[2 * DT], const char * src, int D) {
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int s = 0; s < 2 * DT; ++s) {
+        v4i z = {0, 0, 0, 0};
+        if (16 * s + 8 * h < D) z = *reinterpret_cast<const v4i *>(src + (16 * s + 8 * h) * 2);
+        __builtin_memcpy(&x[s], &z, 16);
+    }
+}
+
+// The wave's 32 columns of DT 32x32 results as rows of D values in memory, scaled by f: through a tile
+// of 32 rows of LDS, so that a row is written in 16-byte pieces one after another. dst(c): column c's row, or null.
+template <class E, int DT, class Dst>
+__device__ __forceinline__ void store_columns(E * tile, const v16f (&acc)[DT], float f, int D, Dst dst) {
+    typedef E v4e __attribute__((ext_vector_type(4)));
+    constexpr int CH = SP<DT> / 8;
+    const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v4e e;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = (E) (acc[d][4 * k + i] * f);
+            const int c = (4 * d + k) ^ swz(col);
+            *reinterpret_cast<v4e *>(tile + col * SP<DT> + c * 8 + 4 * h) = e;
+        }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int it = 0; it < 32 * CH / 64; ++it) {
+        const int r = (it * 64 + lane) / CH, c = lane % CH;
+        char * o = dst(r);
+        const v4i x = *reinterpret_cast<const v4i *>(tile + r * SP<DT> + (c ^ swz(r)) * 8);
+        if (o && c * 8 < D) *reinterpret_cast<v4i *>(o + c * 16) = x;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+
+// Running softmax of the wave's 32 pairs: m the reference of the exponentials (the largest score so far, or
+// up to 8 powers of two below it), l the half wave's share of the sum, o = sum p v.
+template <int DT>
+struct fwd_state {
+    float m, l;
+    v16f o[DT];
+};
+
+// 32 NK keys of a tile. lo, hi: the lane's pair sees keys lo .. hi - 1 of the tile (MASK only).
+template <class E, int DT, int NK, bool MASK>
+__device__ __forceinline__ void fwd_tile(fwd_state<DT> & st, const typename type_of<E>::v8 (&q)[2 * DT], const E * kt,
+                                         const E * vt, float c, int lo, int hi) {
+    typedef type_of<E> TY;
+    const int h = (threadIdx.x & 63) >> 5;
+    v16f s[NK];
+#pragma unroll
+    for (int a = 0; a < NK; ++a) {
+        s[a] = v16f{};
+#pragma unroll
+        for (int d = 0; d < 2 * DT; ++d) s[a] = TY::mfma(row_operand<E, DT>(kt, 32 * a, d), q[d], s[a]);
+    }
+    if (MASK) {
+        const int l0 = lo - 4 * h;
+        const unsigned n = hi > lo ? hi - lo : 0;
+#pragma unroll
+        for (int a = 0; a < NK; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if ((unsigned) (32 * a + reg_row(i) - l0) >= n) s[a][i] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int a = 0; a < NK; ++a)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[a][i]);
+    mx = half_max(mx);
+    // a new reference only where it would be passed by more than 2^8: P stays below 256, far from the
+    // end of either type, and most tiles leave o alone
+    const bool up = (mx - st.m) * c > 8.0f || (st.m == -INFINITY && mx > -INFINITY);
+    if (__any(up)) {
+        const float m1 = up ? mx : st.m;
+        const float f = up ? __builtin_amdgcn_exp2f((st.m - m1) * c) : 1.0f;
+        st.m = m1;
+        st.l *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st.o[d][i] *= f;
+    }
+    const float mc = st.m == -INFINITY ? 0.0f : st.m * c;
+#pragma unroll
+    for (int a = 0; a < NK; ++a) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[a][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a][i], c, -mc));
+            st.l += s[a][i];
+        }
+    }
+#pragma unroll
+    for (int a = 0; a < 2 * NK; ++a) {
+        const typename TY::v8 pa = pack<E>(s[a / 2], a % 2);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) st.o[d] = TY::mfma(col_operand<E, DT>(vt, 16 * a, 32 * d), pa, st.o[d]);
+    }
+}
+
+// A workgroup: 128 pairs of one document and KV head, a wave each 32 of them; 64 keys at a time.
+template <class E, int DT>
+__global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
+    constexpr int BM = 128, BN = 64, TILE = BN * SP<DT>;
+    __shared__ __align__(1024) E sk[2][TILE], sv[2][TILE];
+    const int g = blockIdx.x % p.G, slot = p.n_slots - 1 - blockIdx.x / p.G;
+    const int d = find_doc(p.cu_q, p.n_seqs, p.T_q, p.R, BM, slot);
+    const doc c = doc_of(p, d);
+    const int64_t p0l = (slot - slot_of(p.cu_q, d, p.T_q, p.R, BM)) * BM;
+    const int np = c.n * p.R;
+    if (p0l < 0 || p0l >= np) return;
+    const int p0 = uni((int) p0l);
+
+    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    const int pw = p0 + 32 * wave;
+    const bool active = pw < np;
+    const int pc = min(pw + (lane & 31), np - 1), tok = pc / p.R, head = g * p.R + pc % p.R;
+    typename type_of<E>::v8 q[2 * DT];
+    load_operand<E, DT>(q, p.q.data + (c.q0 + tok) * p.q.ts + head * p.q.hs, p.D);
+
+    const int lo = key_lo(p, c, tok), hi = key_hi(p, c, tok);
+    // keys of the workgroup, and of the wave: some pair's, and every pair's
+    const int t_end = (min(p0 + BM, np) - 1) / p.R;
+    const int j_lo = key_lo(p, c, p0 / p.R) / BN, j_hi = (key_hi(p, c, t_end) + BN - 1) / BN;
+    const int ta = uni(min(pw, np - 1) / p.R), tb = uni(min(pw + 31, np - 1) / p.R);
+    const int some_lo = key_lo(p, c, ta), some_hi = key_hi(p, c, tb), all_lo = key_lo(p, c, tb), all_hi = key_hi(p, c, ta);
+
+    const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
+    const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
+    auto load = [&](int j, int buf) {
+        const int j0 = j * BN, left = c.m - j0;
+        load_rows<DT, BN, 256>(lds_addr(sk[buf]), p.D, [&](int r) { return r < left ? kb + (int64_t) (j0 + r) * p.k.ts : nullptr; });
+        load_rows<DT, BN, 256>(lds_addr(sv[buf]), p.D, [&](int r) { return r < left ? vb + (int64_t) (j0 + r) * p.v.ts : nullptr; });
+    };
+
+    fwd_state<DT> st;
+    st.m = -INFINITY;
+    st.l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DT; ++k) st.o[k] = v16f{};
+    const float cs = p.scale * LOG2E;
+    if (j_lo < j_hi) load(j_lo, 0);
+    for (int j = j_lo; j < j_hi; ++j) {
+        const int buf = (j - j_lo) & 1, j0 = j * BN;
+        wait_all();
+        barrier();
+        if (j + 1 < j_hi) load(j + 1, buf ^ 1);
+        if (!active || j0 >= some_hi || j0 + BN <= some_lo) continue;
+        if (j0 >= all_lo && j0 + BN <= all_hi) fwd_tile<E, DT, 2, false>(st, q, sk[buf], sv[buf], cs, 0, 0);
+        else fwd_tile<E, DT, 2, true>(st, q, sk[buf], sv[buf], cs, lo - j0, hi - j0);
+    }
+    barrier();
+    if (!active) return;
+    const float l = half_sum(st.l);
+    if (h == 0 && pw + lane < np) {
+        p.lse[(int64_t) (c.q0 + tok) * p.H + head] = st.m == -INFINITY ? -INFINITY : st.m * p.scale + LN2 * __builtin_amdgcn_logf(l);
+    }
+    E * tile = (wave < 2 ? sk[0] : sv[0]) + (wave & 1) * 32 * SP<DT>;
+    store_columns<E, DT>(tile, st.o, l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l), p.D, [&](int r) -> char * {
+        const int pr = pw + r;
+        if (pr >= np) return nullptr;
+        return p.out.data + (int64_t) (c.q0 + pr / p.R) * p.out.ts + (g * p.R + pr % p.R) * p.out.hs;
+    });
+}
+
+// Few pairs: a workgroup takes 32 of them, its four waves every fourth 32 keys of the split's share, each through
+// LDS of its own; the waves' sums are joined in LDS. With n_split > 1 the shares of a document's keys go to
+// different workgroups, which leave sums (o, m, l) that attn_rows_join_kernel joins.
+template <class E, int DT>
+__global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
+    constexpr int BM = 32, BN = 32, TILE = BN * SP<DT>;
+    __shared__ __align__(1024) E lds[4][2][2][TILE];       // wave, buffer, K or V
+    __shared__ float sm[4][32], sl[4][32];
+    const int g = blockIdx.x % p.G, rest = blockIdx.x / p.G, split = rest % p.n_split, slot = rest / p.n_split;
+    const int d = find_doc(p.cu_q, p.n_seqs, p.T_q, p.R, BM, slot);
+    const doc c = doc_of(p, d);
+    const int64_t p0l = (slot - slot_of(p.cu_q, d, p.T_q, p.R, BM)) * BM;
+    const int np = c.n * p.R;
+    if (p0l < 0 || p0l >= np) return;
+    const int p0 = uni((int) p0l);
+
+    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int pc = min(p0 + (lane & 31), np - 1), tok = pc / p.R, head = g * p.R + pc % p.R;
+    typename type_of<E>::v8 q[2 * DT];
+    load_operand<E, DT>(q, p.q.data + (c.q0 + tok) * p.q.ts + head * p.q.hs, p.D);
+    const int lo = key_lo(p, c, tok), hi = key_hi(p, c, tok);
+    const int ta = uni(p0 / p.R), tb = uni(min(p0 + 31, np - 1) / p.R);
+    const int all_lo = key_lo(p, c, tb), all_hi = key_hi(p, c, ta);
+    const int t_lo = key_lo(p, c, ta) / BN, t_hi = (key_hi(p, c, tb) + BN - 1) / BN;
+    // the split's share of the tiles t_lo .. t_hi - 1
+    const int share = (max(t_hi - t_lo, 0) + p.n_split - 1) / p.n_split;
+    const int j_lo = t_lo + split * share, j_hi = min(j_lo + share, t_hi);
+
+    const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
+    const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
+    auto load = [&](int j, int buf) {
+        const int j0 = j * BN, left = c.m - j0;
+        load_rows<DT, BN, 64>(lds_addr(lds[wave][buf][0]), p.D, [&](int r) { return r < left ? kb + (int64_t) (j0 + r) * p.k.ts : nullptr; });
+        load_rows<DT, BN, 64>(lds_addr(lds[wave][buf][1]), p.D, [&](int r) { return r < left ? vb + (int64_t) (j0 + r) * p.v.ts : nullptr; });
+    };
+    fwd_state<DT> st;
+    st.m = -INFINITY;
+    st.l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DT; ++k) st.o[k] = v16f{};
+    const float cs = p.scale * LOG2E;
+    int buf = 0;
+    if (j_lo + wave < j_hi) load(j_lo + wave, 0);
+    for (int j = j_lo + wave; j < j_hi; j += 4, buf ^= 1) {
+        wait_all();
+        if (j + 4 < j_hi) load(j + 4, buf ^ 1);
+        const int j0 = j * BN;
+        if (j0 >= all_lo && j0 + BN <= all_hi) fwd_tile<E, DT, 1, false>(st, q, lds[wave][buf][0], lds[wave][buf][1], cs, 0, 0);
+        else fwd_tile<E, DT, 1, true>(st, q, lds[wave][buf][0], lds[wave][buf][1], cs, lo - j0, hi - j0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next load writes it
+    }
+    // join the waves: each leaves its sums in its own LDS, [column][d] as fp32 (32 SP values, as 4 tiles hold)
+    const float l = half_sum(st.l);
+    if (lane < 32) {
+        sm[wave][lane] = st.m;
+        sl[wave][lane] = l;
+    }
+    float * so = reinterpret_cast<float *>(&lds[wave][0][0][0]);
+#pragma unroll
+    for (int k = 0; k < DT; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const v4f x = {st.o[k][4 * i], st.o[k][4 * i + 1], st.o[k][4 * i + 2], st.o[k][4 * i + 3]};
+            *reinterpret_cast<v4f *>(so + (lane & 31) * SP<DT> + 32 * k + 8 * i + 4 * (lane >> 5)) = x;
+        }
+    barrier();
+    constexpr int CH = SP<DT> / 8;
+    constexpr int WAVE_F = 2 * 2 * TILE / 2;                // floats of a wave's LDS
+    const float * all = reinterpret_cast<const float *>(&lds[0][0][0][0]);
+    for (int idx = threadIdx.x; idx < 32 * CH; idx += 256) {
+        const int r = idx / CH, cc = idx % CH, pr = p0 + r;
+        if (pr >= np || cc * 8 >= p.D) continue;
+        float m = -INFINITY, lt = 0.0f, x[8] = {};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) m = fmaxf(m, sm[w][r]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = sm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((sm[w][r] - m) * cs);
+            lt += f * sl[w][r];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] += sm[w][r] == -INFINITY ? 0.0f : f * all[w * WAVE_F + r * SP<DT> + cc * 8 + i];
+        }
+        const int64_t row = (int64_t) (c.q0 + pr / p.R) * p.H + g * p.R + pr % p.R;
+        if (p.n_split > 1) {
+            float * o = p.part + ((int64_t) split * p.T_q * p.H + row) * (p.D + 8);
+            *reinterpret_cast<v4f *>(o + 8 + cc * 8) = v4f{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<v4f *>(o + 8 + cc * 8 + 4) = v4f{x[4], x[5], x[6], x[7]};
+            if (cc == 0) {
+                o[0] = m;
+                o[1] = lt;
+            }
+            continue;
+        }
+        const float f = lt > 0.0f ? 1.0f / lt : (lt == 0.0f ? 0.0f : lt);
+        typename type_of<E>::v8 e;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = (E) (x[i] * f);
+        *reinterpret_cast<typename type_of<E>::v8 *>(p.out.data + (int64_t) (c.q0 + pr / p.R) * p.out.ts +
+                                                     (g * p.R + pr % p.R) * p.out.hs + cc * 16) = e;
+        if (cc == 0) p.lse[row] = m == -INFINITY ? -INFINITY : m * p.scale + LN2 * __builtin_amdgcn_logf(lt);
+    }
+}
+
+// The splits' sums of a (token, head) row joined: 16 lanes a row, 8 values each.
+template <class E>
+__global__ __launch_bounds__(256) void attn_rows_join_kernel(attn_p p) {
+    const int64_t row = (int64_t) blockIdx.x * 16 + threadIdx.x / 16, n_rows = (int64_t) p.T_q * p.H;
+    const int cc = threadIdx.x % 16;
+    if (row >= n_rows || cc * 8 >= p.D) return;
+    const int tok = (int) (row / p.H), head = (int) (row % p.H);
+    // rows of no document have no sums
+    const int end = offset(p.cu_q, p.n_seqs, p.T_q);
+    if (tok >= end || tok < offset(p.cu_q, 0, p.T_q)) return;
+    const float cs = p.scale * LOG2E;
+    float m = -INFINITY, l = 0.0f, x[8] = {};
+    for (int s = 0; s < p.n_split; ++s) m = fmaxf(m, p.part[(s * n_rows + row) * (p.D + 8)]);
+    for (int s = 0; s < p.n_split; ++s) {
+        const float * o = p.part + (s * n_rows + row) * (p.D + 8);
+        if (o[0] == -INFINITY && o[1] == 0.0f) continue;
+        const float f = __builtin_amdgcn_exp2f((o[0] - m) * cs);
+        l += f * o[1];
+        const v4f a = *reinterpret_cast<const v4f *>(o + 8 + cc * 8), b = *reinterpret_cast<const v4f *>(o + 12 + cc * 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] += f * a[i];
+            x[4 + i] += f * b[i];
+        }
+    }
+    const float f = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    typename type_of<E>::v8 e;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = (E) (x[i] * f);
+    *reinterpret_cast<typename type_of<E>::v8 *>(p.out.data + (int64_t) tok * p.out.ts + head * p.out.hs + cc * 16) = e;
+    if (cc == 0) p.lse[row] = m == -INFINITY ? -INFINITY : m * p.scale + LN2 * __builtin_amdgcn_logf(l);
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+
+// delta = sum(dout out) of each (token, head) row; for fp16 the largest squared norms of dout's and v's
+// rows, from which the gradients' kernels take the power of two that dS is carried with. 16 lanes a row.
+template <class E>
+__global__ __launch_bounds__(256) void attn_rows_delta_kernel(attn_p p) {
+    typedef typename type_of<E>::v8 v8;
+    const int cc = threadIdx.x % 16, sub = threadIdx.x / 16;
+    float top_o = 0.0f, top_v = 0.0f;
+    auto sum16 = [](float x) {
+#pragma unroll
+        for (int k = 8; k; k >>= 1) x += __shfl_xor(x, k, 16);
+        return x;
+    };
+    const int64_t n_rows = (int64_t) p.T_q * p.H;
+    for (int64_t row = (int64_t) blockIdx.x * 16 + sub; row < n_rows; row += (int64_t) gridDim.x * 16) {
+        const int64_t tok = row / p.H, head = row % p.H;
+        float s = 0.0f, n2 = 0.0f;
+        if (cc * 8 < p.D) {
+            const v8 a = *reinterpret_cast<const v8 *>(p.dout.data + tok * p.dout.ts + head * p.dout.hs + cc * 16);
+            const v8 b = *reinterpret_cast<const v8 *>(p.out.data + tok * p.out.ts + head * p.out.hs + cc * 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s += (float) a[i] * (float) b[i];
+                n2 += (float) a[i] * (float) a[i];
+            }
+        }
+        s = sum16(s);
+        if (cc == 0) p.delta[row] = s;
+        if (type_of<E>::HALF) top_o = fmaxf(top_o, sum16(n2));
+    }
+    if (!type_of<E>::HALF) return;
+    const int64_t n_v = (int64_t) p.T_k * p.G;
+    for (int64_t row = (int64_t) blockIdx.x * 16 + sub; row < n_v; row += (int64_t) gridDim.x * 16) {
+        float n2 = 0.0f;
+        if (cc * 8 < p.D) {
+            const v8 a = *reinterpret_cast<const v8 *>(p.v.data + row / p.G * p.v.ts + row % p.G * p.v.hs + cc * 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) n2 += (float) a[i] * (float) a[i];
+        }
+        top_v = fmaxf(top_v, sum16(n2));
+    }
+    __shared__ float so[16], sv[16];
+    if (cc == 0) {
+        so[sub] = top_o;
+        sv[sub] = top_v;
+    }
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        float a = so[threadIdx.x], b = sv[threadIdx.x];
+#pragma unroll
+        for (int k = 8; k; k >>= 1) {
+            a = fmaxf(a, __shfl_xor(a, k, 16));
+            b = fmaxf(b, __shfl_xor(b, k, 16));
+        }
+        if (threadIdx.x == 0) {
+            p.maxima[2 * blockIdx.x] = a;
+            p.maxima[2 * blockIdx.x + 1] = b;
+        }
+    }
+}
+
+// fp16: the power of two that dS is carried with, 2^k with |dS| 2^k <= 2^15: |dP - delta| is at most twice the
+// product of the largest norms of dout's and v's rows, and P is at most 1. 1 where the norms are no help.
+template <class E>
+__device__ __forceinline__ float ds_factor(const attn_p & p) {
+    if constexpr (!type_of<E>::HALF) return 1.0f;
+    const int lane = threadIdx.x & 63;
+    float a = 0.0f, b = 0.0f;
+    for (int i = lane; i < N_MAX; i += 64) {
+        a = fmaxf(a, p.maxima[2 * i]);
+        b = fmaxf(b, p.maxima[2 * i + 1]);
+    }
+#pragma unroll
+    for (int k = 32; k; k >>= 1) {
+        a = fmaxf(a, __shfl_xor(a, k));
+        b = fmaxf(b, __shfl_xor(b, k));
+    }
+    const float bound = 2.0f * sqrtf(a) * sqrtf(b);
+    if (!(bound > 0.0f) || !(bound < INFINITY)) return 1.0f;
+    int e;
+    (void) frexpf(bound, &e);                        // bound < 2^e
+    return ldexpf(1.0f, min(max(15 - e, -30), 60));
+}
+
+// dQ: the forward pass's tiling. dQ^T = scale K^T dS^T.
+template <class E, int DT, bool MASK>
+__device__ __forceinline__ void dq_tile(v16f (&dq)[DT], const typename type_of<E>::v8 (&q)[2 * DT],
+                                        const typename type_of<E>::v8 (&go)[2 * DT], const E * kt, const E * vt, float c,
+                                        float lse2, float sigma, float delta_s, int lo, int hi) {
+    typedef type_of<E> TY;
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+        v16f s = {}, dp = {};
+#pragma unroll
+        for (int d = 0; d < 2 * DT; ++d) s = TY::mfma(row_operand<E, DT>(kt, 32 * a, d), q[d], s);
+#pragma unroll
+        for (int d = 0; d < 2 * DT; ++d) dp = TY::mfma(row_operand<E, DT>(vt, 32 * a, d), go[d], dp);
+        const int l0 = lo - 4 * h;
+        const unsigned n = hi > lo ? hi - lo : 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2));
+            s[i] = pr * __builtin_fmaf(dp[i], sigma, -delta_s);
+            if (MASK && (unsigned) (32 * a + reg_row(i) - l0) >= n) s[i] = 0.0f;
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const typename TY::v8 ds = pack<E>(s, b);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dq[d] = TY::mfma(col_operand<E, DT>(kt, 32 * a + 16 * b, 32 * d), ds, dq[d]);
+        }
+    }
+}
+
+template <class E, int DT>
+__global__ __launch_bounds__(256, DT <= 3 ? 2 : 1) void attn_rows_dq_kernel(attn_p p) {
+    constexpr int BM = 128, BN = 64, TILE = BN * SP<DT>;
+    __shared__ __align__(1024) E sk[2][TILE], sv[2][TILE];
+    const int g = blockIdx.x % p.G, slot = p.n_slots - 1 - blockIdx.x / p.G;
+    const int d = find_doc(p.cu_q, p.n_seqs, p.T_q, p.R, BM, slot);
+    const doc c = doc_of(p, d);
+    const int64_t p0l = (slot - slot_of(p.cu_q, d, p.T_q, p.R, BM)) * BM;
+    const int np = c.n * p.R;
+    if (p0l < 0 || p0l >= np) return;
+    const int p0 = uni((int) p0l);
+
+    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int pw = p0 + 32 * wave;
+    const bool active = pw < np;
+    const int pc = min(pw + (lane & 31), np - 1), tok = pc / p.R, head = g * p.R + pc % p.R;
+    typename type_of<E>::v8 q[2 * DT], go[2 * DT];
+    load_operand<E, DT>(q, p.q.data + (c.q0 + tok) * p.q.ts + head * p.q.hs, p.D);
+    load_operand<E, DT>(go, p.dout.data + (c.q0 + tok) * p.dout.ts + head * p.dout.hs, p.D);
+    const int64_t row = (int64_t) (c.q0 + tok) * p.H + head;
+    const float factor = ds_factor<E>(p), sigma = type_of<E>::HALF ? factor : 1.0f;
+    const float lse = p.lse[row], delta_s = p.delta[row] * sigma;
+    const float lse2 = lse * LOG2E;
+
+    const int lo = key_lo(p, c, tok), hi = key_hi(p, c, tok);
+    const int t_end = (min(p0 + BM, np) - 1) / p.R;
+    const int j_lo = key_lo(p, c, p0 / p.R) / BN, j_hi = (key_hi(p, c, t_end) + BN - 1) / BN;
+    const int ta = uni(min(pw, np - 1) / p.R), tb = uni(min(pw + 31, np - 1) / p.R);
+    const int some_lo = key_lo(p, c, ta), some_hi = key_hi(p, c, tb), all_lo = key_lo(p, c, tb), all_hi = key_hi(p, c, ta);
+
+    const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
+    const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
+    auto load = [&](int j, int buf) {
+        const int j0 = j * BN, left = c.m - j0;
+        load_rows<DT, BN, 256>(lds_addr(sk[buf]), p.D, [&](int r) { return r < left ? kb + (int64_t) (j0 + r) * p.k.ts : nullptr; });
+        load_rows<DT, BN, 256>(lds_addr(sv[buf]), p.D, [&](int r) { return r < left ? vb + (int64_t) (j0 + r) * p.v.ts : nullptr; });
+    };
+    v16f dq[DT];
+#pragma unroll
+    for (int k = 0; k < DT; ++k) dq[k] = v16f{};
+    const float cs = p.scale * LOG2E;
+    if (j_lo < j_hi) load(j_lo, 0);
+    for (int j = j_lo; j < j_hi; ++j) {
+        const int buf = (j - j_lo) & 1, j0 = j * BN;
+        wait_all();
+        barrier();
+        if (j + 1 < j_hi) load(j + 1, buf ^ 1);
+        if (!active || j0 >= some_hi || j0 + BN <= some_lo) continue;
+        if (j0 >= all_lo && j0 + BN <= all_hi) dq_tile<E, DT, false>(dq, q, go, sk[buf], sv[buf], cs, lse2, sigma, delta_s, 0, 0);
+        else dq_tile<E, DT, true>(dq, q, go, sk[buf], sv[buf], cs, lse2, sigma, delta_s, lo - j0, hi - j0);
+    }
+    barrier();
+    if (!active) return;
+    E * tile = (wave < 2 ? sk[0] : sv[0]) + (wave & 1) * 32 * SP<DT>;
+    store_columns<E, DT>(tile, dq, p.scale / factor, p.D, [&](int r) -> char * {
+        const int pr = pw + r;
+        if (pr >= np) return nullptr;
+        return p.dq.data + (int64_t) (c.q0 + pr / p.R) * p.dq.ts + (g * p.R + pr % p.R) * p.dq.hs;
+    });
+}
+
+// dK, dV: a wave has 32 keys, the workgroup goes over the pairs that see its 128, 64 at a time.
+template <class E, int DT, bool MASK>
+__device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const typename type_of<E>::v8 (&k)[2 * DT],
+                                         const typename type_of<E>::v8 (&v)[2 * DT], const E * qt, const E * ot,
+                                         const float * lse2, const float * delta_s, float c, float sigma, int lo, int hi) {
+    typedef type_of<E> TY;
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+        v16f s = {}, dp = {};
+#pragma unroll
+        for (int d = 0; d < 2 * DT; ++d) s = TY::mfma(row_operand<E, DT>(qt, 32 * a, d), k[d], s);
+#pragma unroll
+        for (int d = 0; d < 2 * DT; ++d) dp = TY::mfma(row_operand<E, DT>(ot, 32 * a, d), v[d], dp);
+        const int l0 = lo - 4 * h;
+        const unsigned n = hi > lo ? hi - lo : 0;
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+            const v4f ls = *reinterpret_cast<const v4f *>(lse2 + 32 * a + 8 * i4 + 4 * h);
+            const v4f de = *reinterpret_cast<const v4f *>(delta_s + 32 * a + 8 * i4 + 4 * h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = 4 * i4 + j;
+                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[j]));
+                dp[i] = s[i] * __builtin_fmaf(dp[i], sigma, -de[j]);
+                if (MASK && (unsigned) (32 * a + reg_row(i) - l0) >= n) s[i] = dp[i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const typename TY::v8 pp = pack<E>(s, b), ds = pack<E>(dp, b);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                dv[d] = TY::mfma(col_operand<E, DT>(ot, 32 * a + 16 * b, 32 * d), pp, dv[d]);
+                dk[d] = TY::mfma(col_operand<E, DT>(qt, 32 * a + 16 * b, 32 * d), ds, dk[d]);
+            }
+        }
+    }
+}
+
+template <class E, int DT>
+__global__ __launch_bounds__(256, DT <= 2 ? 2 : 1) void attn_rows_dkv_kernel(attn_p p) {
+    constexpr int BK = 128, BQ = 64, TILE = BQ * SP<DT>;
+    __shared__ __align__(1024) E sq[2][TILE], so[2][TILE];
+    __shared__ __align__(16) float s_lse[2][BQ], s_delta[2][BQ];
+    const int g = blockIdx.x % p.G, slot = blockIdx.x / p.G;
+    const int d = find_doc(p.cu_k, p.n_seqs, p.T_k, 1, BK, slot);
+    const doc c = doc_of(p, d);
+    const int64_t kl = (slot - slot_of(p.cu_k, d, p.T_k, 1, BK)) * BK;
+    if (kl < 0 || kl >= c.m) return;
+    const int kb0 = uni((int) kl), np = c.n * p.R;
+
+    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int kw = kb0 + 32 * wave;
+    const bool active = kw < c.m;
+    const int key = min(kw + (lane & 31), c.m - 1);
+    typename type_of<E>::v8 k[2 * DT], v[2 * DT];
+    load_operand<E, DT>(k, p.k.data + (int64_t) (c.k0 + key) * p.k.ts + g * p.k.hs, p.D);
+    load_operand<E, DT>(v, p.v.data + (int64_t) (c.k0 + key) * p.v.ts + g * p.v.hs, p.D);
+    const float factor = ds_factor<E>(p);
+    // P is carried as 2^15 P, so dS's factor has it already
+    const float sigma = type_of<E>::HALF ? ldexpf(factor, -P_SHIFT) : 1.0f;
+
+    const int lo = tok_lo(p, c, key) * p.R, hi = tok_hi(p, c, key) * p.R;
+    const int k_end = min(kb0 + BK, c.m) - 1;
+    const int j_lo = tok_lo(p, c, kb0) * p.R / BQ, j_hi = (tok_hi(p, c, k_end) * p.R + BQ - 1) / BQ;
+    const int ka = uni(min(kw, c.m - 1)), ke = uni(min(kw + 31, c.m - 1));
+    const int some_lo = tok_lo(p, c, ka) * p.R, some_hi = tok_hi(p, c, ke) * p.R;
+    const int all_lo = tok_lo(p, c, ke) * p.R, all_hi = tok_hi(p, c, ka) * p.R;
+
+    float row_value = 0.0f;      // threads 0..63: a pair's lse, 64..127: its delta, of the tile being loaded
+    auto load = [&](int j, int buf) {
+        const int j0 = j * BQ;
+        auto at = [&](const rows & x, int r) -> const char * {
+            const int pr = j0 + r;
+            return pr < np ? x.data + (int64_t) (c.q0 + pr / p.R) * x.ts + (g * p.R + pr % p.R) * x.hs : nullptr;
+        };
+        load_rows<DT, BQ, 256>(lds_addr(sq[buf]), p.D, [&](int r) { return at(p.q, r); });
+        load_rows<DT, BQ, 256>(lds_addr(so[buf]), p.D, [&](int r) { return at(p.dout, r); });
+        if (threadIdx.x < 2 * BQ) {
+            const int pr = j0 + (threadIdx.x & (BQ - 1));
+            const bool ok = pr < np, is_lse = threadIdx.x < BQ;
+            const int64_t row = (int64_t) (c.q0 + min(pr, np - 1) / p.R) * p.H + g * p.R + min(pr, np - 1) % p.R;
+            const float x = (is_lse ? p.lse : p.delta)[row];
+            // pairs behind the document: P = 2^-inf = 0
+            row_value = is_lse ? (ok ? x * LOG2E - (type_of<E>::HALF ? P_SHIFT : 0) : INFINITY) : (ok ? x * sigma : 0.0f);
+        }
+    };
+    auto put = [&](int buf) {
+        if (threadIdx.x < BQ) s_lse[buf][threadIdx.x] = row_value;
+        else if (threadIdx.x < 2 * BQ) s_delta[buf][threadIdx.x - BQ] = row_value;
+    };
+    v16f dk[DT], dv[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) dk[i] = dv[i] = v16f{};
+    const float cs = p.scale * LOG2E;
+    if (j_lo < j_hi) {
+        load(j_lo, 0);
+        put(0);
+    }
+    for (int j = j_lo; j < j_hi; ++j) {
+        const int buf = (j - j_lo) & 1, j0 = j * BQ;
+        wait_all();
+        barrier();
+        if (j + 1 < j_hi) load(j + 1, buf ^ 1);
+        if (active && j0 < some_hi && j0 + BQ > some_lo) {
+            if (j0 >= all_lo && j0 + BQ <= all_hi)
+                dkv_tile<E, DT, false>(dk, dv, k, v, sq[buf], so[buf], s_lse[buf], s_delta[buf], cs, sigma, 0, 0);
+            else dkv_tile<E, DT, true>(dk, dv, k, v, sq[buf], so[buf], s_lse[buf], s_delta[buf], cs, sigma, lo - j0, hi - j0);
+        }
+        if (j + 1 < j_hi) put(buf ^ 1);
+    }
+    barrier();
+    if (!active) return;
+    E * tile = (wave < 2 ? sq[0] : so[0]) + (wave & 1) * 32 * SP<DT>;
+    auto dst = [&](const rows & x) {
+        return [&, x](int r) -> char * { return kw + r < c.m ? x.data + (int64_t) (c.k0 + kw + r) * x.ts + g * x.hs : nullptr; };
+    };
+    store_columns<E, DT>(tile, dv, type_of<E>::HALF ? 1.0f / (1 << P_SHIFT) : 1.0f, p.D, dst(p.dv));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    store_columns<E, DT>(tile, dk, p.scale / factor, p.D, dst(p.dk));
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+int64_t slots(int64_t T, int64_t mul, int64_t tile, int64_t n_seqs) { return T * mul / tile + n_seqs; }
+
+constexpr int64_t MAX_T = 1 << 30;
+
+int32_t check_params(const char * what, const nxg_attention_rows_params * a, attn_p & p) {
+    if (!a) return nxg_fail(NXG_EINVAL, "%s: null parameters", what);
+    if (a->type != NXG_TYPE_F16 && a->type != NXG_TYPE_BF16) {
+        return nxg_fail(NXG_EINVAL, "%s: type %d (rows must be F16 or BF16)", what, a->type);
+    }
+    if (a->head_dim < 8 || a->head_dim > 128 || a->head_dim % 8) {
+        return nxg_fail(NXG_EINVAL, "%s: head_dim=%d (a multiple of 8 up to 128)", what, a->head_dim);
+    }
+    if (a->n_head < 1 || a->n_kv_head < 1 || a->n_head % a->n_kv_head) {
+        return nxg_fail(NXG_EINVAL, "%s: n_head=%d n_kv_head=%d", what, a->n_head, a->n_kv_head);
+    }
+    if (a->T_q < 0 || a->T_k < 0 || a->n_seqs < 0 || a->T_q > MAX_T || a->T_k > MAX_T) {
+        return nxg_fail(NXG_EINVAL, "%s: T_q=%d T_k=%d n_seqs=%d", what, a->T_q, a->T_k, a->n_seqs);
+    }
+    if (a->left < -1 || a->right < -1) return nxg_fail(NXG_EINVAL, "%s: left=%d right=%d (-1: no limit)", what, a->left, a->right);
+    if (!(a->scale > 0.0f) || !(a->scale < INFINITY)) return nxg_fail(NXG_EINVAL, "%s: scale must be positive and finite", what);
+    p = attn_p{};
+    p.H = a->n_head;
+    p.G = a->n_kv_head;
+    p.R = p.H / p.G;
+    p.D = a->head_dim;
+    p.T_q = a->T_q;
+    p.T_k = a->T_k;
+    p.n_seqs = a->n_seqs;
+    p.left = std::min(a->left, (int32_t) MAX_T - 1);
+    p.right = std::min(a->right, (int32_t) MAX_T - 1);
+    p.scale = a->scale;
+    p.cu_q = a->cu_q;
+    p.cu_k = a->cu_k;
+    if ((int64_t) p.T_q * p.R > INT32_MAX - 256 ||
+        (slots(p.T_q, p.R, 32, p.n_seqs)) * p.G > INT32_MAX / 64 || slots(p.T_k, 1, 128, p.n_seqs) * p.G > INT32_MAX) {
+        return nxg_fail(NXG_EINVAL, "%s: T_q=%d T_k=%d of %d heads is too large", what, p.T_q, p.T_k, p.H);
+    }
+    p.n_split = 1;
+    return NXG_OK;
+}
+
+int32_t check_rows(const char * what, const char * name, const nxg_rows * x, int64_t T, int n_head, int D, bool written, rows & r) {
+    if (T == 0) return NXG_OK;
+    if (!x || !x->data) return nxg_fail(NXG_EINVAL, "%s: %s is null", what, name);
+    if ((uintptr_t) x->data & 15) return nxg_fail(NXG_EINVAL, "%s: %s must be 16-byte aligned", what, name);
+    r.data = (char *) x->data;
+    r.ts = T == 1 ? 0 : x->token_stride;
+    r.hs = n_head == 1 ? 0 : x->head_stride;
+    const int64_t most = INT64_MAX / 16;
+    if (r.ts < 0 || r.hs < 0 || r.ts % 8 || r.hs % 8 || r.ts > most / T || r.hs > most / n_head) {
+        return nxg_fail(NXG_EINVAL, "%s: %s has strides %lld, %lld (multiples of 8)", what, name, (long long) r.ts, (long long) r.hs);
+    }
+    if (written) {           // no two rows of an output overlap
+        const int64_t in_n = r.hs <= r.ts || T == 1 ? n_head : T, in_s = r.hs <= r.ts || T == 1 ? r.hs : r.ts;
+        const int64_t out_n = in_s == r.hs ? T : n_head, out_s = in_s == r.hs ? r.ts : r.hs;
+        if ((in_n > 1 && in_s < D) || (out_n > 1 && out_s < (in_n - 1) * in_s + D)) {
+            return nxg_fail(NXG_EINVAL, "%s: rows of %s overlap (strides %lld, %lld)", what, name, (long long) r.ts, (long long) r.hs);
+        }
+    }
+    r.ts *= 2;
+    r.hs *= 2;
+    return NXG_OK;
+}
+
+#define NXG_TRY(call) do { const int32_t rc_ = (call); if (rc_) return rc_; } while (0)
+
+// Launches one of a kernel's instances by type and head size.
+#define NXG_BY_TYPE(type, D, LAUNCH)                                               \
+    do {                                                                           \
+        if ((type) == NXG_TYPE_BF16) { typedef __bf16 E; NXG_BY_DIM(D, LAUNCH); }  \
+        else { typedef _Float16 E; NXG_BY_DIM(D, LAUNCH); }                        \
+    } while (0)
+#define NXG_BY_DIM(D, LAUNCH)                                                      \
+    do {                                                                           \
+        if ((D) <= 32) { constexpr int DT = 1; LAUNCH; }                           \
+        else if ((D) <= 64) { constexpr int DT = 2; LAUNCH; }                      \
+        else if ((D) <= 96) { constexpr int DT = 3; LAUNCH; }                      \
+        else { constexpr int DT = 4; LAUNCH; }                                     \
+    } while (0)
+
+// The few-pairs kernel where tiles of 128 pairs would leave most CUs idle, its keys split until there are
+// two workgroups a CU, 256 keys of the average document at least to each.
+struct fwd_plan {
+    bool few;
+    int n_split;
+};
+fwd_plan plan_forward(const attn_p & p) {
+    const int64_t cus = nxg_device_cus();
+    fwd_plan f{false, 1};
+    if (slots(p.T_q, p.R, 128, p.n_seqs) * p.G >= cus) {
+        // documents of few pairs each: tiles of 128 would be nearly empty
+        if ((int64_t) p.T_q * p.R > 32LL * p.n_seqs) return f;
+    }
+    f.few = true;
+    const int64_t wgs = slots(p.T_q, p.R, 32, p.n_seqs) * p.G;
+    const int64_t keys = p.T_k / std::max(1, p.n_seqs);
+    f.n_split = (int) std::max<int64_t>(1, std::min({2 * cus / wgs, keys / 256, (int64_t) 64}));
+    return f;
+}
+
+} // namespace
+
+extern "C" {
+
+int64_t nxg_attention_rows_workspace_bytes(const nxg_attention_rows_params * a) {
+    attn_p p;
+    const int32_t rc = check_params("attention_rows_workspace_bytes", a, p);
+    if (rc) return -rc;
+    if (p.T_q == 0 || p.n_seqs == 0) return 0;
+    const fwd_plan f = plan_forward(p);
+    return f.n_split > 1 ? (int64_t) f.n_split * p.T_q * p.H * (p.D + 8) * 4 : 0;
+}
+
+int32_t nxg_attention_rows(const nxg_attention_rows_params * a, const nxg_rows * q, const nxg_rows * k, const nxg_rows * v,
+                           const nxg_rows * out, float * lse, void * workspace, int64_t workspace_bytes, void * stream) {
+    const char * what = "attention_rows";
+    attn_p p;
+    NXG_TRY(check_params(what, a, p));
+    NXG_TRY(check_rows(what, "q", q, p.T_q, p.H, p.D, false, p.q));
+    NXG_TRY(check_rows(what, "k", k, p.T_k, p.G, p.D, false, p.k));
+    NXG_TRY(check_rows(what, "v", v, p.T_k, p.G, p.D, false, p.v));
+    NXG_TRY(check_rows(what, "out", out, p.T_q, p.H, p.D, true, p.out));
+    if (workspace_bytes < 0 || (workspace_bytes > 0 && !workspace) || ((uintptr_t) workspace & 15)) {
+        return nxg_fail(NXG_EINVAL, "%s: workspace must be 16-byte aligned memory of workspace_bytes", what);
+    }
+    if (p.T_q == 0 || p.n_seqs == 0) return NXG_OK;
+    if (!p.cu_q || !p.cu_k || !lse) return nxg_fail(NXG_EINVAL, "%s: cu_q, cu_k or lse is null", what);
+    NXG_TRY(nxg_check_device());
+    p.lse = lse;
+    fwd_plan f = plan_forward(p);
+    if (f.n_split > 1) f.n_split = (int) std::min<int64_t>(f.n_split, workspace_bytes / ((int64_t) p.T_q * p.H * (p.D + 8) * 4));
+    f.n_split = std::max(1, f.n_split);
+    p.n_split = f.n_split;
+    p.part = (float *) workspace;
+    hipStream_t s = (hipStream_t) stream;
+    p.n_slots = (int32_t) slots(p.T_q, p.R, f.few ? 32 : 128, p.n_seqs);
+    const unsigned grid = (unsigned) ((int64_t) p.n_slots * p.G * p.n_split);
+    if (f.few) {
+        NXG_BY_TYPE(a->type, p.D, (attn_rows_few_kernel<E, DT><<<grid, 256, 0, s>>>(p)));
+        NXG_TRY(nxg_launch_check(what));
+        if (p.n_split == 1) return NXG_OK;
+        const unsigned rows_grid = (unsigned) (((int64_t) p.T_q * p.H + 15) / 16);
+        if (a->type == NXG_TYPE_BF16) attn_rows_join_kernel<__bf16><<<rows_grid, 256, 0, s>>>(p);
+        else attn_rows_join_kernel<_Float16><<<rows_grid, 256, 0, s>>>(p);
+        return nxg_launch_check(what);
+    }
+    NXG_BY_TYPE(a->type, p.D, (attn_rows_fwd_kernel<E, DT><<<grid, 256, 0, s>>>(p)));
+    return nxg_launch_check(what);
+}
+
+int64_t nxg_attention_rows_backward_workspace_bytes(const nxg_attention_rows_params * a) {
+    attn_p p;
+    const int32_t rc = check_params("attention_rows_backward_workspace_bytes", a, p);
+    if (rc) return -rc;
+    return 8 * N_MAX + 4 * (int64_t) p.T_q * p.H;
+}
+
+int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const nxg_rows * dout, const nxg_rows * q,
+                                    const nxg_rows * k, const nxg_rows * v, const nxg_rows * out, const float * lse,
+                                    const nxg_rows * dq, const nxg_rows * dk, const nxg_rows * dv, void * workspace,
+                                    int64_t workspace_bytes, void * stream) {
+    const char * what = "attention_rows_backward";
+    attn_p p;
+    NXG_TRY(check_params(what, a, p));
+    NXG_TRY(check_rows(what, "dout", dout, p.T_q, p.H, p.D, false, p.dout));
+    NXG_TRY(check_rows(what, "q", q, p.T_q, p.H, p.D, false, p.q));
+    NXG_TRY(check_rows(what, "k", k, p.T_k, p.G, p.D, false, p.k));
+    NXG_TRY(check_rows(what, "v", v, p.T_k, p.G, p.D, false, p.v));
+    NXG_TRY(check_rows(what, "out", out, p.T_q, p.H, p.D, false, p.out));
+    NXG_TRY(check_rows(what, "dq", dq, p.T_q, p.H, p.D, true, p.dq));
+    NXG_TRY(check_rows(what, "dk", dk, p.T_k, p.G, p.D, true, p.dk));
+    NXG_TRY(check_rows(what, "dv", dv, p.T_k, p.G, p.D, true, p.dv));
+    if (p.n_seqs == 0 || (p.T_q == 0 && p.T_k == 0)) return NXG_OK;
+    if (!p.cu_q || !p.cu_k || (p.T_q > 0 && !lse)) return nxg_fail(NXG_EINVAL, "%s: cu_q, cu_k or lse is null", what);
+    if (!workspace || ((uintptr_t) workspace & 15) || workspace_bytes < 8 * N_MAX + 4 * (int64_t) p.T_q * p.H) {
+        return nxg_fail(NXG_EINVAL, "%s: workspace must be 16-byte aligned memory of %lld bytes", what,
+                        (long long) (8 * N_MAX + 4 * (int64_t) p.T_q * p.H));
+    }
+    NXG_TRY(nxg_check_device());
+    p.lse = (float *) lse;
+    p.maxima = (float *) workspace;
+    p.delta = p.maxima + 2 * N_MAX;
+    hipStream_t s = (hipStream_t) stream;
+    if (p.T_q > 0) {
+        if (a->type == NXG_TYPE_BF16) {
+            const int64_t n = ((int64_t) p.T_q * p.H + 15) / 16;
+            attn_rows_delta_kernel<__bf16><<<(unsigned) std::min<int64_t>(n, 8 * N_MAX), 256, 0, s>>>(p);
+        } else {
+            attn_rows_delta_kernel<_Float16><<<N_MAX, 256, 0, s>>>(p);
+        }
+        NXG_TRY(nxg_launch_check(what));
+        p.n_slots = (int32_t) slots(p.T_q, p.R, 128, p.n_seqs);
+        NXG_BY_TYPE(a->type, p.D, (attn_rows_dq_kernel<E, DT><<<(unsigned) (p.n_slots * p.G), 256, 0, s>>>(p)));
+        NXG_TRY(nxg_launch_check(what));
+    }
+    if (p.T_k > 0) {
+        p.n_slots = (int32_t) slots(p.T_k, 1, 128, p.n_seqs);
+        NXG_BY_TYPE(a->type, p.D, (attn_rows_dkv_kernel<E, DT><<<(unsigned) (p.n_slots * p.G), 256, 0, s>>>(p)));
+        NXG_TRY(nxg_launch_check(what));
+    }
+    return NXG_OK;
+}
+
+} // extern "C"

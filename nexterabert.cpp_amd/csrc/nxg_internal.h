@@ -13,4 +13,16 @@ void nxg_tile_rows(const int8_t * rows, int n_rows, int n_in, int KS, int8_t * t
 // Records the message returned by nxg_last_error() on this thread.
 void nxg_set_error(const char * msg);
 
+// Records a formatted message and returns `code`.
+int nxg_fail(int code, const char * fmt, ...) __attribute__((format(printf, 2, 3)));
+
+// NXG_OK if the current device is a gfx950 GPU.
+int nxg_check_device(void);
+
+// Compute units of the device that nxg_check_device last saw on this thread (256 before its first call).
+int nxg_device_cus(void);
+
+// NXG_OK, or NXG_EDEVICE with the error of the launch just made.
+int nxg_launch_check(const char * what);
+
 #endif

@@ -3883,6 +3883,20 @@ bool qact_dims_of(int T, int n_in, qact_dims & d) {
 
 } // namespace
 
+int nxg_fail(int code, const char * fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    nxg_set_error(buf);
+    return code;
+}
+
+int nxg_check_device(void) { return check_device(); }
+int nxg_device_cus(void) { return device_cus(); }
+int nxg_launch_check(const char * what) { return launch_check(what); }
+
 struct nxg_weight {
     int32_t n_in = 0, n_out = 0, n_blk = 0, KS = 0, NP = 0;
     int8_t * w = nullptr;    // NP x KS*64 bytes in fragment tiles
