@@ -76,6 +76,7 @@ struct attn_p {
     const int32_t * cu_q, * cu_k;
     int32_t n_seqs, T_q, T_k, H, G, R, D, left, right, n_slots, n_split;
     float scale;
+    bool near_k, near_q;       // a tile's rows are within 32-bit offsets of its first (of q and dout: and lie alike in every tile)
 };
 
 // ---------------------------------------------------------------------------
@@ -89,11 +90,19 @@ __device__ __align__(16) const uint32_t zeros16[4] = {};
 __device__ __forceinline__ void dma16(const void * g, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(g), "s"(lds) : "memory", "m0");
 }
+// The same from a scalar base: lane l copies the 16 bytes at base + off_l.
+__device__ __forceinline__ void dma16s(const char * base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
 __device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_addr(const void * p) { return (uint32_t) (uintptr_t) (lds_void *) p; }
 
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ const char * uni(const char * p) {
+    const uint64_t v = (uint64_t) (uintptr_t) p;
+    return (const char *) (uintptr_t) (((uint64_t) (uint32_t) uni((int) (v >> 32)) << 32) | (uint32_t) uni((int) (uint32_t) v));
+}
 
 // max over the two halves of the wave
 __device__ __forceinline__ float half_max(float x) {
@@ -166,19 +175,61 @@ __device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 
 
 template <int DT> constexpr int SP = DT <= 2 ? 64 : 128;
 
-// Loads NR rows by the NT threads of a workgroup (NT = 256) or a wave (64): row r from src(r), a pointer to
-// its D values or null for zeros.
-template <int DT, int NR, int NT, class Src>
-__device__ __forceinline__ void load_rows(uint32_t lds, int D, Src src) {
-    constexpr int CH = SP<DT> / 8;
-    const int t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
-    const uint32_t wave0 = NT == 64 ? 0 : uni(threadIdx.x >> 6) * 1024;
-#pragma unroll
-    for (int it = 0; it < NR * CH / NT; ++it) {
-        const int r = (it * NT + t) / CH, c = (t % CH) ^ swz(r);
-        const char * s = src(r);
-        dma16(s && c * 8 < D ? s + c * 16 : (const char *) zeros16, lds + wave0 + it * NT * 16);
+// Copies NR rows by the NT threads of a workgroup (NT = 256) or a wave (64) into a tile. A thread's places
+// within a tile are computed once; a tile is a new scalar base. Chunks behind D are never written: clear()
+// before.
+template <int DT, int NR, int NT>
+struct tile_loader {
+    static constexpr int CH = SP<DT> / 8, N = NR * CH / NT, STEP = NT / CH;
+    uint32_t off[N];
+    int r0, c0, D;
+
+    static __device__ __forceinline__ int thread() { return NT == 64 ? threadIdx.x & 63 : threadIdx.x; }
+    static __device__ __forceinline__ uint32_t wave_at() { return NT == 64 ? 0 : uni((int) (threadIdx.x >> 6)) * 1024; }
+    // The chunk of the thread's k'th row: the same for all where 8 divides STEP, else (4) every other row's
+    // neighbour, as swz() of a row 4 further says.
+    __device__ __forceinline__ int chunk(int k) const {
+        static_assert(STEP % 4 == 0 && 4 * STEP >= 16, "swz of the rows of a thread");
+        return STEP % 8 == 0 ? c0 : c0 ^ (k & 1);
     }
+
+    // at(r): the byte of row r from a tile's base
+    template <class At>
+    __device__ __forceinline__ tile_loader(int D_, At at) : D(D_) {
+        const int t = thread();
+        r0 = t / CH;
+        c0 = (t % CH) ^ swz(r0);
+#pragma unroll
+        for (int k = 0; k < N; ++k) off[k] = (uint32_t) at(r0 + k * STEP) + chunk(k) * 16;
+    }
+    // every row from base + at(r)
+    __device__ __forceinline__ void load(const char * base, uint32_t lds) const {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (chunk(k) * 8 < D) dma16s(base, off[k], lds + wave_at() + k * NT * 16);
+    }
+    // row r from src(r), zeros where that is null
+    template <class Src>
+    __device__ __forceinline__ void load_each(uint32_t lds, Src src) const {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const char * s = src(r0 + k * STEP);
+            if (chunk(k) * 8 < D) dma16(s ? s + chunk(k) * 16 : (const char *) zeros16, lds + wave_at() + k * NT * 16);
+        }
+    }
+};
+
+// The tile of keys j0 .. of a document's m, rows ts bytes apart from `first`.
+template <class L>
+__device__ __forceinline__ void load_keys(const L & l, uint32_t lds, const char * first, int64_t ts, int j0, int m, bool near) {
+    constexpr int NR = L::N * L::STEP;
+    if (near && j0 + NR <= m) l.load(uni(first + j0 * ts), lds);
+    else l.load_each(lds, [&](int r) { return j0 + r < m ? first + (j0 + r) * ts : nullptr; });
+}
+
+// Zeros the chunks behind D of n tiles' memory (all of it), before the first load.
+__device__ __forceinline__ void clear(void * lds, int bytes, int thread, int threads) {
+    for (int i = thread * 16; i < bytes; i += threads * 16) *reinterpret_cast<v4i *>((char *) lds + i) = v4i{0, 0, 0, 0};
 }
 
 // Operand of 32 rows: lane l's row l % 32, values 16 s + 8 (l / 32) + 0..7.
@@ -224,11 +275,18 @@ __device__ __forceinline__ typename type_of<E>::v8 pack(const v16f & x, int a) {
 template <class E, int DT>
 __device__ __forceinline__ void load_operand(typename type_of<E>::v8 (&x)[2 * DT], const char * src, int D) {
     const int h = (threadIdx.x & 63) >> 5;
+    v4i z[2 * DT];
 #pragma unroll
     for (int s = 0; s < 2 * DT; ++s) {
-        v4i z = {0, 0, 0, 0};
-        if (16 * s + 8 * h < D) z = *reinterpret_cast<const v4i *>(src + (16 * s + 8 * h) * 2);
-        __builtin_memcpy(&x[s], &z, 16);
+        z[s] = v4i{0, 0, 0, 0};
+        if (16 * s + 8 * h < D) z[s] = *reinterpret_cast<const v4i *>(src + (16 * s + 8 * h) * 2);
+    }
+    // arrived here, not at their first use: that is in a loop, where the compiler would wait for the tiles
+    // under way as well
+#pragma unroll
+    for (int s = 0; s < 2 * DT; ++s) {
+        asm volatile("" : "+v"(z[s]));
+        __builtin_memcpy(&x[s], &z[s], 16);
     }
 }
 
@@ -264,18 +322,28 @@ __device__ __forceinline__ void store_columns(E * tile, const v16f (&acc)[DT], f
 // forward
 // ---------------------------------------------------------------------------
 
-// Running softmax of the wave's 32 pairs: m the reference of the exponentials (the largest score so far, or
-// up to 8 powers of two below it), l the half wave's share of the sum, o = sum p v.
+// Running softmax of the wave's 32 pairs. mc: the exponentials' reference in powers of two, the largest score
+// so far or up to 2^8 below it, so that most tiles leave the sums alone (P stays below 256, far from the
+// end of either type); top: the score past which it moves (-inf before the first); l: the half wave's
+// share of sum p; o = sum p v.
 template <int DT>
 struct fwd_state {
-    float m, l;
+    float top, mc, l;
     v16f o[DT];
+
+    __device__ __forceinline__ void init() {
+        top = -INFINITY;
+        mc = l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < DT; ++k) o[k] = v16f{};
+    }
 };
 
-// 32 NK keys of a tile. lo, hi: the lane's pair sees keys lo .. hi - 1 of the tile (MASK only).
-template <class E, int DT, int NK, bool MASK>
+// 32 NK keys of a tile. lo, hi: the lane's pair sees keys lo .. hi - 1 of the tile (with `mask` alone: a
+// tile that every pair sees has no masks).
+template <class E, int DT, int NK>
 __device__ __forceinline__ void fwd_tile(fwd_state<DT> & st, const typename type_of<E>::v8 (&q)[2 * DT], const E * kt,
-                                         const E * vt, float c, int lo, int hi) {
+                                         const E * vt, float c, bool mask, int lo, int hi) {
     typedef type_of<E> TY;
     const int h = (threadIdx.x & 63) >> 5;
     v16f s[NK];
@@ -285,7 +353,7 @@ __device__ __forceinline__ void fwd_tile(fwd_state<DT> & st, const typename type
 #pragma unroll
         for (int d = 0; d < 2 * DT; ++d) s[a] = TY::mfma(row_operand<E, DT>(kt, 32 * a, d), q[d], s[a]);
     }
-    if (MASK) {
+    if (mask) {
         const int l0 = lo - 4 * h;
         const unsigned n = hi > lo ? hi - lo : 0;
 #pragma unroll
@@ -300,28 +368,25 @@ __device__ __forceinline__ void fwd_tile(fwd_state<DT> & st, const typename type
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[a][i]);
     mx = half_max(mx);
-    // a new reference only where it would be passed by more than 2^8: P stays below 256, far from the
-    // end of either type, and most tiles leave o alone
-    const bool up = (mx - st.m) * c > 8.0f || (st.m == -INFINITY && mx > -INFINITY);
-    if (__any(up)) {
-        const float m1 = up ? mx : st.m;
-        const float f = up ? __builtin_amdgcn_exp2f((st.m - m1) * c) : 1.0f;
-        st.m = m1;
-        st.l *= f;
+    if (__any(mx > st.top)) {
+        if (mx > st.top) {
+            const float mc = mx * c, f = fminf(__builtin_amdgcn_exp2f(st.mc - mc), 1.0f);   // 1: nothing summed yet
+            st.mc = mc;
+            st.top = mx + 8.0f / c;
+            st.l *= f;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+            for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) st.o[d][i] *= f;
-    }
-    const float mc = st.m == -INFINITY ? 0.0f : st.m * c;
-#pragma unroll
-    for (int a = 0; a < NK; ++a) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[a][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a][i], c, -mc));
-            st.l += s[a][i];
+                for (int i = 0; i < 16; ++i) st.o[d][i] *= f;
         }
     }
+#pragma unroll
+    for (int a = 0; a < NK; ++a)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[a][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a][i], c, -st.mc));
+            st.l += s[a][i];
+        }
 #pragma unroll
     for (int a = 0; a < 2 * NK; ++a) {
         const typename TY::v8 pa = pack<E>(s[a / 2], a % 2);
@@ -359,17 +424,19 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
 
     const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
     const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
+    const tile_loader<DT, BN, 256> lk(p.D, [&](int r) { return r * p.k.ts; }), lv(p.D, [&](int r) { return r * p.v.ts; });
     auto load = [&](int j, int buf) {
-        const int j0 = j * BN, left = c.m - j0;
-        load_rows<DT, BN, 256>(lds_addr(sk[buf]), p.D, [&](int r) { return r < left ? kb + (int64_t) (j0 + r) * p.k.ts : nullptr; });
-        load_rows<DT, BN, 256>(lds_addr(sv[buf]), p.D, [&](int r) { return r < left ? vb + (int64_t) (j0 + r) * p.v.ts : nullptr; });
+        load_keys(lk, lds_addr(sk[buf]), kb, p.k.ts, j * BN, c.m, p.near_k);
+        load_keys(lv, lds_addr(sv[buf]), vb, p.v.ts, j * BN, c.m, p.near_k);
     };
+    if (p.D != 32 * DT) {
+        clear(sk, sizeof(sk), threadIdx.x, 256);
+        clear(sv, sizeof(sv), threadIdx.x, 256);
+        barrier();
+    }
 
     fwd_state<DT> st;
-    st.m = -INFINITY;
-    st.l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < DT; ++k) st.o[k] = v16f{};
+    st.init();
     const float cs = p.scale * LOG2E;
     if (j_lo < j_hi) load(j_lo, 0);
     for (int j = j_lo; j < j_hi; ++j) {
@@ -378,14 +445,13 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
         barrier();
         if (j + 1 < j_hi) load(j + 1, buf ^ 1);
         if (!active || j0 >= some_hi || j0 + BN <= some_lo) continue;
-        if (j0 >= all_lo && j0 + BN <= all_hi) fwd_tile<E, DT, 2, false>(st, q, sk[buf], sv[buf], cs, 0, 0);
-        else fwd_tile<E, DT, 2, true>(st, q, sk[buf], sv[buf], cs, lo - j0, hi - j0);
+        fwd_tile<E, DT, 2>(st, q, sk[buf], sv[buf], cs, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
     }
     barrier();
     if (!active) return;
     const float l = half_sum(st.l);
     if (h == 0 && pw + lane < np) {
-        p.lse[(int64_t) (c.q0 + tok) * p.H + head] = st.m == -INFINITY ? -INFINITY : st.m * p.scale + LN2 * __builtin_amdgcn_logf(l);
+        p.lse[(int64_t) (c.q0 + tok) * p.H + head] = LN2 * (st.mc + __builtin_amdgcn_logf(l));
     }
     E * tile = (wave < 2 ? sk[0] : sv[0]) + (wave & 1) * 32 * SP<DT>;
     store_columns<E, DT>(tile, st.o, l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l), p.D, [&](int r) -> char * {
@@ -425,16 +491,17 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
 
     const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
     const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
+    const tile_loader<DT, BN, 64> lk(p.D, [&](int r) { return r * p.k.ts; }), lv(p.D, [&](int r) { return r * p.v.ts; });
     auto load = [&](int j, int buf) {
-        const int j0 = j * BN, left = c.m - j0;
-        load_rows<DT, BN, 64>(lds_addr(lds[wave][buf][0]), p.D, [&](int r) { return r < left ? kb + (int64_t) (j0 + r) * p.k.ts : nullptr; });
-        load_rows<DT, BN, 64>(lds_addr(lds[wave][buf][1]), p.D, [&](int r) { return r < left ? vb + (int64_t) (j0 + r) * p.v.ts : nullptr; });
+        load_keys(lk, lds_addr(lds[wave][buf][0]), kb, p.k.ts, j * BN, c.m, p.near_k);
+        load_keys(lv, lds_addr(lds[wave][buf][1]), vb, p.v.ts, j * BN, c.m, p.near_k);
     };
+    if (p.D != 32 * DT) {
+        clear(lds[wave], sizeof(lds[wave]), lane, 64);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
     fwd_state<DT> st;
-    st.m = -INFINITY;
-    st.l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < DT; ++k) st.o[k] = v16f{};
+    st.init();
     const float cs = p.scale * LOG2E;
     int buf = 0;
     if (j_lo + wave < j_hi) load(j_lo + wave, 0);
@@ -442,14 +509,13 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
         wait_all();
         if (j + 4 < j_hi) load(j + 4, buf ^ 1);
         const int j0 = j * BN;
-        if (j0 >= all_lo && j0 + BN <= all_hi) fwd_tile<E, DT, 1, false>(st, q, lds[wave][buf][0], lds[wave][buf][1], cs, 0, 0);
-        else fwd_tile<E, DT, 1, true>(st, q, lds[wave][buf][0], lds[wave][buf][1], cs, lo - j0, hi - j0);
+        fwd_tile<E, DT, 1>(st, q, lds[wave][buf][0], lds[wave][buf][1], cs, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next load writes it
     }
     // join the waves: each leaves its sums in its own LDS, [column][d] as fp32 (32 SP values, as 4 tiles hold)
     const float l = half_sum(st.l);
     if (lane < 32) {
-        sm[wave][lane] = st.m;
+        sm[wave][lane] = st.top == -INFINITY ? -INFINITY : st.mc;
         sl[wave][lane] = l;
     }
     float * so = reinterpret_cast<float *>(&lds[wave][0][0][0]);
@@ -472,7 +538,7 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
         for (int w = 0; w < 4; ++w) m = fmaxf(m, sm[w][r]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = sm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((sm[w][r] - m) * cs);
+            const float f = sm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][r] - m);
             lt += f * sl[w][r];
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] += sm[w][r] == -INFINITY ? 0.0f : f * all[w * WAVE_F + r * SP<DT> + cc * 8 + i];
@@ -494,7 +560,7 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
         for (int i = 0; i < 8; ++i) e[i] = (E) (x[i] * f);
         *reinterpret_cast<typename type_of<E>::v8 *>(p.out.data + (int64_t) (c.q0 + pr / p.R) * p.out.ts +
                                                      (g * p.R + pr % p.R) * p.out.hs + cc * 16) = e;
-        if (cc == 0) p.lse[row] = m == -INFINITY ? -INFINITY : m * p.scale + LN2 * __builtin_amdgcn_logf(lt);
+        if (cc == 0) p.lse[row] = m == -INFINITY && lt == 0.0f ? -INFINITY : LN2 * (m + __builtin_amdgcn_logf(lt));
     }
 }
 
@@ -508,13 +574,12 @@ __global__ __launch_bounds__(256) void attn_rows_join_kernel(attn_p p) {
     // rows of no document have no sums
     const int end = offset(p.cu_q, p.n_seqs, p.T_q);
     if (tok >= end || tok < offset(p.cu_q, 0, p.T_q)) return;
-    const float cs = p.scale * LOG2E;
     float m = -INFINITY, l = 0.0f, x[8] = {};
     for (int s = 0; s < p.n_split; ++s) m = fmaxf(m, p.part[(s * n_rows + row) * (p.D + 8)]);
     for (int s = 0; s < p.n_split; ++s) {
         const float * o = p.part + (s * n_rows + row) * (p.D + 8);
         if (o[0] == -INFINITY && o[1] == 0.0f) continue;
-        const float f = __builtin_amdgcn_exp2f((o[0] - m) * cs);
+        const float f = __builtin_amdgcn_exp2f(o[0] - m);
         l += f * o[1];
         const v4f a = *reinterpret_cast<const v4f *>(o + 8 + cc * 8), b = *reinterpret_cast<const v4f *>(o + 12 + cc * 8);
 #pragma unroll
@@ -528,7 +593,7 @@ __global__ __launch_bounds__(256) void attn_rows_join_kernel(attn_p p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) e[i] = (E) (x[i] * f);
     *reinterpret_cast<typename type_of<E>::v8 *>(p.out.data + (int64_t) tok * p.out.ts + head * p.out.hs + cc * 16) = e;
-    if (cc == 0) p.lse[row] = m == -INFINITY ? -INFINITY : m * p.scale + LN2 * __builtin_amdgcn_logf(l);
+    if (cc == 0) p.lse[row] = m == -INFINITY && l == 0.0f ? -INFINITY : LN2 * (m + __builtin_amdgcn_logf(l));
 }
 
 // ---------------------------------------------------------------------------
@@ -619,10 +684,10 @@ __device__ __forceinline__ float ds_factor(const attn_p & p) {
 }
 
 // dQ: the forward pass's tiling. dQ^T = scale K^T dS^T.
-template <class E, int DT, bool MASK>
+template <class E, int DT>
 __device__ __forceinline__ void dq_tile(v16f (&dq)[DT], const typename type_of<E>::v8 (&q)[2 * DT],
                                         const typename type_of<E>::v8 (&go)[2 * DT], const E * kt, const E * vt, float c,
-                                        float lse2, float sigma, float delta_s, int lo, int hi) {
+                                        float lse2, float sigma, float delta_s, bool mask, int lo, int hi) {
     typedef type_of<E> TY;
     const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
@@ -632,13 +697,17 @@ __device__ __forceinline__ void dq_tile(v16f (&dq)[DT], const typename type_of<E
         for (int d = 0; d < 2 * DT; ++d) s = TY::mfma(row_operand<E, DT>(kt, 32 * a, d), q[d], s);
 #pragma unroll
         for (int d = 0; d < 2 * DT; ++d) dp = TY::mfma(row_operand<E, DT>(vt, 32 * a, d), go[d], dp);
-        const int l0 = lo - 4 * h;
-        const unsigned n = hi > lo ? hi - lo : 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2));
             s[i] = pr * __builtin_fmaf(dp[i], sigma, -delta_s);
-            if (MASK && (unsigned) (32 * a + reg_row(i) - l0) >= n) s[i] = 0.0f;
+        }
+        if (mask) {
+            const int l0 = lo - 4 * h;
+            const unsigned n = hi > lo ? hi - lo : 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if ((unsigned) (32 * a + reg_row(i) - l0) >= n) s[i] = 0.0f;
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -650,7 +719,7 @@ __device__ __forceinline__ void dq_tile(v16f (&dq)[DT], const typename type_of<E
 }
 
 template <class E, int DT>
-__global__ __launch_bounds__(256, DT <= 3 ? 2 : 1) void attn_rows_dq_kernel(attn_p p) {
+__global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
     constexpr int BM = 128, BN = 64, TILE = BN * SP<DT>;
     __shared__ __align__(1024) E sk[2][TILE], sv[2][TILE];
     const int g = blockIdx.x % p.G, slot = p.n_slots - 1 - blockIdx.x / p.G;
@@ -681,11 +750,16 @@ __global__ __launch_bounds__(256, DT <= 3 ? 2 : 1) void attn_rows_dq_kernel(attn
 
     const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
     const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
+    const tile_loader<DT, BN, 256> lk(p.D, [&](int r) { return r * p.k.ts; }), lv(p.D, [&](int r) { return r * p.v.ts; });
     auto load = [&](int j, int buf) {
-        const int j0 = j * BN, left = c.m - j0;
-        load_rows<DT, BN, 256>(lds_addr(sk[buf]), p.D, [&](int r) { return r < left ? kb + (int64_t) (j0 + r) * p.k.ts : nullptr; });
-        load_rows<DT, BN, 256>(lds_addr(sv[buf]), p.D, [&](int r) { return r < left ? vb + (int64_t) (j0 + r) * p.v.ts : nullptr; });
+        load_keys(lk, lds_addr(sk[buf]), kb, p.k.ts, j * BN, c.m, p.near_k);
+        load_keys(lv, lds_addr(sv[buf]), vb, p.v.ts, j * BN, c.m, p.near_k);
     };
+    if (p.D != 32 * DT) {
+        clear(sk, sizeof(sk), threadIdx.x, 256);
+        clear(sv, sizeof(sv), threadIdx.x, 256);
+        barrier();
+    }
     v16f dq[DT];
 #pragma unroll
     for (int k = 0; k < DT; ++k) dq[k] = v16f{};
@@ -697,8 +771,7 @@ __global__ __launch_bounds__(256, DT <= 3 ? 2 : 1) void attn_rows_dq_kernel(attn
         barrier();
         if (j + 1 < j_hi) load(j + 1, buf ^ 1);
         if (!active || j0 >= some_hi || j0 + BN <= some_lo) continue;
-        if (j0 >= all_lo && j0 + BN <= all_hi) dq_tile<E, DT, false>(dq, q, go, sk[buf], sv[buf], cs, lse2, sigma, delta_s, 0, 0);
-        else dq_tile<E, DT, true>(dq, q, go, sk[buf], sv[buf], cs, lse2, sigma, delta_s, lo - j0, hi - j0);
+        dq_tile<E, DT>(dq, q, go, sk[buf], sv[buf], cs, lse2, sigma, delta_s, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
     }
     barrier();
     if (!active) return;
@@ -711,10 +784,10 @@ __global__ __launch_bounds__(256, DT <= 3 ? 2 : 1) void attn_rows_dq_kernel(attn
 }
 
 // dK, dV: a wave has 32 keys, the workgroup goes over the pairs that see its 128, 64 at a time.
-template <class E, int DT, bool MASK>
+template <class E, int DT>
 __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const typename type_of<E>::v8 (&k)[2 * DT],
                                          const typename type_of<E>::v8 (&v)[2 * DT], const E * qt, const E * ot,
-                                         const float * lse2, const float * delta_s, float c, float sigma, int lo, int hi) {
+                                         const float * lse2, const float * delta_s, float c, float sigma, bool mask, int lo, int hi) {
     typedef type_of<E> TY;
     const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
@@ -724,8 +797,6 @@ __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const t
         for (int d = 0; d < 2 * DT; ++d) s = TY::mfma(row_operand<E, DT>(qt, 32 * a, d), k[d], s);
 #pragma unroll
         for (int d = 0; d < 2 * DT; ++d) dp = TY::mfma(row_operand<E, DT>(ot, 32 * a, d), v[d], dp);
-        const int l0 = lo - 4 * h;
-        const unsigned n = hi > lo ? hi - lo : 0;
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) {
             const v4f ls = *reinterpret_cast<const v4f *>(lse2 + 32 * a + 8 * i4 + 4 * h);
@@ -735,8 +806,14 @@ __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const t
                 const int i = 4 * i4 + j;
                 s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[j]));
                 dp[i] = s[i] * __builtin_fmaf(dp[i], sigma, -de[j]);
-                if (MASK && (unsigned) (32 * a + reg_row(i) - l0) >= n) s[i] = dp[i] = 0.0f;
             }
+        }
+        if (mask) {
+            const int l0 = lo - 4 * h;
+            const unsigned n = hi > lo ? hi - lo : 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if ((unsigned) (32 * a + reg_row(i) - l0) >= n) s[i] = dp[i] = 0.0f;
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -780,15 +857,27 @@ __global__ __launch_bounds__(256, DT <= 2 ? 2 : 1) void attn_rows_dkv_kernel(att
     const int some_lo = tok_lo(p, c, ka) * p.R, some_hi = tok_hi(p, c, ke) * p.R;
     const int all_lo = tok_lo(p, c, ke) * p.R, all_hi = tok_hi(p, c, ka) * p.R;
 
+    const tile_loader<DT, BQ, 256> lq(p.D, [&](int r) { return r / p.R * p.q.ts + r % p.R * p.q.hs; });
+    const tile_loader<DT, BQ, 256> l_out(p.D, [&](int r) { return r / p.R * p.dout.ts + r % p.R * p.dout.hs; });
+    if (p.D != 32 * DT) {
+        clear(sq, sizeof(sq), threadIdx.x, 256);
+        clear(so, sizeof(so), threadIdx.x, 256);
+        barrier();
+    }
     float row_value = 0.0f;      // threads 0..63: a pair's lse, 64..127: its delta, of the tile being loaded
     auto load = [&](int j, int buf) {
         const int j0 = j * BQ;
-        auto at = [&](const rows & x, int r) -> const char * {
-            const int pr = j0 + r;
-            return pr < np ? x.data + (int64_t) (c.q0 + pr / p.R) * x.ts + (g * p.R + pr % p.R) * x.hs : nullptr;
-        };
-        load_rows<DT, BQ, 256>(lds_addr(sq[buf]), p.D, [&](int r) { return at(p.q, r); });
-        load_rows<DT, BQ, 256>(lds_addr(so[buf]), p.D, [&](int r) { return at(p.dout, r); });
+        if (p.near_q && j0 + BQ <= np) {
+            lq.load(uni(p.q.data + (int64_t) (c.q0 + j0 / p.R) * p.q.ts + g * p.R * p.q.hs), lds_addr(sq[buf]));
+            l_out.load(uni(p.dout.data + (int64_t) (c.q0 + j0 / p.R) * p.dout.ts + g * p.R * p.dout.hs), lds_addr(so[buf]));
+        } else {
+            auto at = [&](const rows & x, int r) -> const char * {
+                const int pr = j0 + r;
+                return pr < np ? x.data + (int64_t) (c.q0 + pr / p.R) * x.ts + (g * p.R + pr % p.R) * x.hs : nullptr;
+            };
+            lq.load_each(lds_addr(sq[buf]), [&](int r) { return at(p.q, r); });
+            l_out.load_each(lds_addr(so[buf]), [&](int r) { return at(p.dout, r); });
+        }
         if (threadIdx.x < 2 * BQ) {
             const int pr = j0 + (threadIdx.x & (BQ - 1));
             const bool ok = pr < np, is_lse = threadIdx.x < BQ;
@@ -816,9 +905,7 @@ __global__ __launch_bounds__(256, DT <= 2 ? 2 : 1) void attn_rows_dkv_kernel(att
         barrier();
         if (j + 1 < j_hi) load(j + 1, buf ^ 1);
         if (active && j0 < some_hi && j0 + BQ > some_lo) {
-            if (j0 >= all_lo && j0 + BQ <= all_hi)
-                dkv_tile<E, DT, false>(dk, dv, k, v, sq[buf], so[buf], s_lse[buf], s_delta[buf], cs, sigma, 0, 0);
-            else dkv_tile<E, DT, true>(dk, dv, k, v, sq[buf], so[buf], s_lse[buf], s_delta[buf], cs, sigma, lo - j0, hi - j0);
+            dkv_tile<E, DT>(dk, dv, k, v, sq[buf], so[buf], s_lse[buf], s_delta[buf], cs, sigma, j0 < all_lo || j0 + BQ > all_hi, lo - j0, hi - j0);
         }
         if (j + 1 < j_hi) put(buf ^ 1);
     }
@@ -876,6 +963,13 @@ int32_t check_params(const char * what, const nxg_attention_rows_params * a, att
     }
     p.n_split = 1;
     return NXG_OK;
+}
+
+// Whether 64 rows' offsets from the first fit 32 bits: keys one after another, and pairs, whose places
+// repeat from tile to tile where R divides 64.
+bool near_rows(const rows & x) { return x.ts <= (INT32_MAX - 4096) / 64; }
+bool near_pairs(const rows & x, int R) {
+    return 64 % R == 0 && x.ts <= (INT32_MAX - 4096) / 128 && x.hs <= (INT32_MAX - 4096) / 2 / R;
 }
 
 int32_t check_rows(const char * what, const char * name, const nxg_rows * x, int64_t T, int n_head, int D, bool written, rows & r) {
@@ -966,6 +1060,7 @@ int32_t nxg_attention_rows(const nxg_attention_rows_params * a, const nxg_rows *
     if (!p.cu_q || !p.cu_k || !lse) return nxg_fail(NXG_EINVAL, "%s: cu_q, cu_k or lse is null", what);
     NXG_TRY(nxg_check_device());
     p.lse = lse;
+    p.near_k = near_rows(p.k) && near_rows(p.v);
     fwd_plan f = plan_forward(p);
     if (f.n_split > 1) f.n_split = (int) std::min<int64_t>(f.n_split, workspace_bytes / ((int64_t) p.T_q * p.H * (p.D + 8) * 4));
     f.n_split = std::max(1, f.n_split);
@@ -1017,6 +1112,8 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
     }
     NXG_TRY(nxg_check_device());
     p.lse = (float *) lse;
+    p.near_k = near_rows(p.k) && near_rows(p.v);
+    p.near_q = near_pairs(p.q, p.R) && near_pairs(p.dout, p.R);
     p.maxima = (float *) workspace;
     p.delta = p.maxima + 2 * N_MAX;
     hipStream_t s = (hipStream_t) stream;
