@@ -70,7 +70,7 @@ struct rows {
 struct attn_p {
     rows q, k, v, out, dout, dq, dk, dv;
     float * lse;               // [T_q][H]
-    float * delta;             // [T_q][H]
+    float * lse2, * ndelta;    // for the backward pass, a KV head's pairs one after another ([G][T_q R]): log2 of the sums, -delta
     float * maxima;            // [N_MAX][2]: largest |dout row|^2 and |v row|^2 (fp16)
     float * part;              // partial sums of the split forward pass
     const int32_t * cu_q, * cu_k;
@@ -93,6 +93,10 @@ __device__ __forceinline__ void dma16(const void * g, uint32_t lds) {
 // The same from a scalar base: lane l copies the 16 bytes at base + off_l.
 __device__ __forceinline__ void dma16s(const char * base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+// 4 bytes per lane (lane l to lds + 4 l).
+__device__ __forceinline__ void dma4(const void * g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(g), "s"(lds) : "memory", "m0");
 }
 __device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -175,46 +179,51 @@ __device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 
 
 template <int DT> constexpr int SP = DT <= 2 ? 64 : 128;
 
-// Copies NR rows by the NT threads of a workgroup (NT = 256) or a wave (64) into a tile. A thread's places
-// within a tile are computed once; a tile is a new scalar base. Chunks behind D are never written: clear()
-// before.
+// Copies NR rows by the NT threads of a workgroup (NT = 256) or a wave (64) into a tile. A thread's place
+// within a tile is computed once; a tile is a new scalar base, and so is each of a thread's rows (STEP
+// rows further). Chunks behind D are never written: clear() before.
 template <int DT, int NR, int NT>
 struct tile_loader {
     static constexpr int CH = SP<DT> / 8, N = NR * CH / NT, STEP = NT / CH;
-    uint32_t off[N];
     int r0, c0, D;
+    uint32_t off;              // of row r0 from the tile's base
+    int64_t step;              // of STEP rows
 
     static __device__ __forceinline__ int thread() { return NT == 64 ? threadIdx.x & 63 : threadIdx.x; }
     static __device__ __forceinline__ uint32_t wave_at() { return NT == 64 ? 0 : uni((int) (threadIdx.x >> 6)) * 1024; }
     // The chunk of the thread's k'th row: the same for all where 8 divides STEP, else (4) every other row's
     // neighbour, as swz() of a row 4 further says.
     __device__ __forceinline__ int chunk(int k) const {
-        static_assert(STEP % 4 == 0 && 4 * STEP >= 16, "swz of the rows of a thread");
+        static_assert(STEP % 4 == 0, "swz of the rows of a thread");
         return STEP % 8 == 0 ? c0 : c0 ^ (k & 1);
     }
 
-    // at(r): the byte of row r from a tile's base
-    template <class At>
-    __device__ __forceinline__ tile_loader(int D_, At at) : D(D_) {
+    __device__ __forceinline__ tile_loader(int D_) : D(D_) {
         const int t = thread();
         r0 = t / CH;
         c0 = (t % CH) ^ swz(r0);
-#pragma unroll
-        for (int k = 0; k < N; ++k) off[k] = (uint32_t) at(r0 + k * STEP) + chunk(k) * 16;
     }
-    // every row from base + at(r)
+    // Rows ts bytes apart; or pairs, R to a token (R divides STEP), heads hs bytes apart.
+    __device__ __forceinline__ void rows_at(int64_t ts) {
+        off = (uint32_t) (r0 * ts);
+        step = STEP * ts;
+    }
+    __device__ __forceinline__ void pairs_at(int R, int64_t ts, int64_t hs) {
+        off = (uint32_t) (r0 / R * ts + r0 % R * hs);
+        step = STEP / R * ts;
+    }
     __device__ __forceinline__ void load(const char * base, uint32_t lds) const {
 #pragma unroll
         for (int k = 0; k < N; ++k)
-            if (chunk(k) * 8 < D) dma16s(base, off[k], lds + wave_at() + k * NT * 16);
+            if (chunk(k) * 8 < D) dma16s(base + k * step, off + chunk(k) * 16, lds + wave_at() + k * NT * 16);
     }
     // row r from src(r), zeros where that is null
     template <class Src>
     __device__ __forceinline__ void load_each(uint32_t lds, Src src) const {
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < N; ++k) {
             const char * s = src(r0 + k * STEP);
-            if (chunk(k) * 8 < D) dma16(s ? s + chunk(k) * 16 : (const char *) zeros16, lds + wave_at() + k * NT * 16);
+            if (chunk(k) * 8 < D) dma16(s ? s + chunk(k) * 16 : (const char *) zeros16, uni((int) (lds + wave_at() + k * NT * 16)));
         }
     }
 };
@@ -232,28 +241,40 @@ __device__ __forceinline__ void clear(void * lds, int bytes, int thread, int thr
     for (int i = thread * 16; i < bytes; i += threads * 16) *reinterpret_cast<v4i *>((char *) lds + i) = v4i{0, 0, 0, 0};
 }
 
-// Operand of 32 rows: lane l's row l % 32, values 16 s + 8 (l / 32) + 0..7.
-template <class E, int DT>
-__device__ __forceinline__ typename type_of<E>::v8 row_operand(const E * tile, int r0, int s) {
-    const int lane = threadIdx.x & 63, r = lane & 31;
-    const int c = (2 * s + (lane >> 5)) ^ swz(r);
-    return *reinterpret_cast<const typename type_of<E>::v8 *>(tile + (r0 + r) * SP<DT> + c * 8);
+// A lane's places in a tile, as byte offsets whose chunk is varied by an exclusive or.
+struct lane_at {
+    uint32_t row, col;
+};
+template <int DT>
+__device__ __forceinline__ lane_at lane_places() {
+    const int lane = threadIdx.x & 63, r = lane & 31, i = lane & 15, g = lane >> 4;
+    const int cr = 4 * (g >> 1) + (i >> 2);
+    lane_at o;
+    o.row = r * SP<DT> * 2 + (((lane >> 5) ^ swz(r)) << 4);
+    o.col = cr * SP<DT> * 2 + (((2 * (g & 1) + ((i & 3) >> 1)) ^ swz(cr)) << 4) + (i & 1) * 8;
+    return o;
 }
 
-// Operand of 32 columns d0 .. d0 + 31 (lane l's column d0 + l % 32), rows r0 + 4 (l / 32) + {0..3, 8..11}: the
-// rows of registers 0..7 of a 32x32 result (r0 a multiple of 16).
+// Operand of 32 rows from r0: lane l's row r0 + l % 32, values 16 s + 8 (l / 32) + 0..7. `at`: the tile's LDS
+// address + lane_at.row.
 template <class E, int DT>
-__device__ __forceinline__ typename type_of<E>::v8 col_operand(const E * tile, int r0, int d0) {
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+__device__ __forceinline__ typename type_of<E>::v8 row_operand(uint32_t at, int r0, int s) {
+    typedef __attribute__((address_space(3))) v4i lds_v4i;
+    const v4i x = *(lds_v4i *) (uintptr_t) ((at ^ (s << 5)) + r0 * SP<DT> * 2);
+    typename type_of<E>::v8 out;
+    __builtin_memcpy(&out, &x, 16);
+    return out;
+}
+
+// Operand of the 32 columns from 32 d, rows r0 + 4 (l / 32) + {0..3, 8..11}: the rows of registers 0..7 of a
+// 32x32 result (r0 a multiple of 16). `at`: the tile's LDS address + lane_at.col.
+template <class E, int DT>
+__device__ __forceinline__ typename type_of<E>::v8 col_operand(uint32_t at, int r0, int d) {
     typedef __attribute__((address_space(3))) v4s lds_v4s;
     v4s x[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int r = r0 + 8 * k + 4 * (g >> 1) + (i >> 2);
-        const int c = (d0 / 8 + 2 * (g & 1) + ((i & 3) >> 1)) ^ swz(r);
-        x[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_v4s *) (lds_void *) (tile + r * SP<DT> + c * 8 + (i & 1) * 4));
-    }
+    for (int k = 0; k < 2; ++k)
+        x[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *) (uintptr_t) ((at ^ (d << 6)) + (r0 + 8 * k) * SP<DT> * 2));
     typename type_of<E>::v8 out;
     __builtin_memcpy(&out, x, 16);
     return out;
@@ -342,8 +363,8 @@ struct fwd_state {
 // 32 NK keys of a tile. lo, hi: the lane's pair sees keys lo .. hi - 1 of the tile (with `mask` alone: a
 // tile that every pair sees has no masks).
 template <class E, int DT, int NK>
-__device__ __forceinline__ void fwd_tile(fwd_state<DT> & st, const typename type_of<E>::v8 (&q)[2 * DT], const E * kt,
-                                         const E * vt, float c, bool mask, int lo, int hi) {
+__device__ __forceinline__ void fwd_tile(fwd_state<DT> & st, const typename type_of<E>::v8 (&q)[2 * DT], lane_at at, uint32_t kt,
+                                         uint32_t vt, float c, bool mask, int lo, int hi) {
     typedef type_of<E> TY;
     const int h = (threadIdx.x & 63) >> 5;
     v16f s[NK];
@@ -351,7 +372,7 @@ __device__ __forceinline__ void fwd_tile(fwd_state<DT> & st, const typename type
     for (int a = 0; a < NK; ++a) {
         s[a] = v16f{};
 #pragma unroll
-        for (int d = 0; d < 2 * DT; ++d) s[a] = TY::mfma(row_operand<E, DT>(kt, 32 * a, d), q[d], s[a]);
+        for (int d = 0; d < 2 * DT; ++d) s[a] = TY::mfma(row_operand<E, DT>(kt + at.row, 32 * a, d), q[d], s[a]);
     }
     if (mask) {
         const int l0 = lo - 4 * h;
@@ -391,7 +412,7 @@ __device__ __forceinline__ void fwd_tile(fwd_state<DT> & st, const typename type
     for (int a = 0; a < 2 * NK; ++a) {
         const typename TY::v8 pa = pack<E>(s[a / 2], a % 2);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) st.o[d] = TY::mfma(col_operand<E, DT>(vt, 16 * a, 32 * d), pa, st.o[d]);
+        for (int d = 0; d < DT; ++d) st.o[d] = TY::mfma(col_operand<E, DT>(vt + at.col, 16 * a, d), pa, st.o[d]);
     }
 }
 
@@ -424,7 +445,9 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
 
     const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
     const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
-    const tile_loader<DT, BN, 256> lk(p.D, [&](int r) { return r * p.k.ts; }), lv(p.D, [&](int r) { return r * p.v.ts; });
+    tile_loader<DT, BN, 256> lk(p.D), lv(p.D);
+    lk.rows_at(p.k.ts);
+    lv.rows_at(p.v.ts);
     auto load = [&](int j, int buf) {
         load_keys(lk, lds_addr(sk[buf]), kb, p.k.ts, j * BN, c.m, p.near_k);
         load_keys(lv, lds_addr(sv[buf]), vb, p.v.ts, j * BN, c.m, p.near_k);
@@ -438,6 +461,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     fwd_state<DT> st;
     st.init();
     const float cs = p.scale * LOG2E;
+    const lane_at at = lane_places<DT>();
     if (j_lo < j_hi) load(j_lo, 0);
     for (int j = j_lo; j < j_hi; ++j) {
         const int buf = (j - j_lo) & 1, j0 = j * BN;
@@ -445,7 +469,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
         barrier();
         if (j + 1 < j_hi) load(j + 1, buf ^ 1);
         if (!active || j0 >= some_hi || j0 + BN <= some_lo) continue;
-        fwd_tile<E, DT, 2>(st, q, sk[buf], sv[buf], cs, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
+        fwd_tile<E, DT, 2>(st, q, at, lds_addr(sk[buf]), lds_addr(sv[buf]), cs, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
     }
     barrier();
     if (!active) return;
@@ -491,7 +515,9 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
 
     const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
     const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
-    const tile_loader<DT, BN, 64> lk(p.D, [&](int r) { return r * p.k.ts; }), lv(p.D, [&](int r) { return r * p.v.ts; });
+    tile_loader<DT, BN, 64> lk(p.D), lv(p.D);
+    lk.rows_at(p.k.ts);
+    lv.rows_at(p.v.ts);
     auto load = [&](int j, int buf) {
         load_keys(lk, lds_addr(lds[wave][buf][0]), kb, p.k.ts, j * BN, c.m, p.near_k);
         load_keys(lv, lds_addr(lds[wave][buf][1]), vb, p.v.ts, j * BN, c.m, p.near_k);
@@ -503,13 +529,14 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
     fwd_state<DT> st;
     st.init();
     const float cs = p.scale * LOG2E;
+    const lane_at at = lane_places<DT>();
     int buf = 0;
     if (j_lo + wave < j_hi) load(j_lo + wave, 0);
     for (int j = j_lo + wave; j < j_hi; j += 4, buf ^= 1) {
         wait_all();
         if (j + 4 < j_hi) load(j + 4, buf ^ 1);
         const int j0 = j * BN;
-        fwd_tile<E, DT, 1>(st, q, lds[wave][buf][0], lds[wave][buf][1], cs, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
+        fwd_tile<E, DT, 1>(st, q, at, lds_addr(lds[wave][buf][0]), lds_addr(lds[wave][buf][1]), cs, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next load writes it
     }
     // join the waves: each leaves its sums in its own LDS, [column][d] as fp32 (32 SP values, as 4 tiles hold)
@@ -600,7 +627,7 @@ __global__ __launch_bounds__(256) void attn_rows_join_kernel(attn_p p) {
 // backward
 // ---------------------------------------------------------------------------
 
-// delta = sum(dout out) of each (token, head) row; for fp16 the largest squared norms of dout's and v's
+// -delta = -sum(dout out) and log2 of the sums of each (token, head) row; for fp16 the largest squared norms of dout's and v's
 // rows, from which the gradients' kernels take the power of two that dS is carried with. 16 lanes a row.
 template <class E>
 __global__ __launch_bounds__(256) void attn_rows_delta_kernel(attn_p p) {
@@ -614,7 +641,8 @@ __global__ __launch_bounds__(256) void attn_rows_delta_kernel(attn_p p) {
     };
     const int64_t n_rows = (int64_t) p.T_q * p.H;
     for (int64_t row = (int64_t) blockIdx.x * 16 + sub; row < n_rows; row += (int64_t) gridDim.x * 16) {
-        const int64_t tok = row / p.H, head = row % p.H;
+        // in the order of lse2 and ndelta: a KV head's pairs one after another
+        const int64_t pr = row % ((int64_t) p.T_q * p.R), tok = pr / p.R, head = row / ((int64_t) p.T_q * p.R) * p.R + pr % p.R;
         float s = 0.0f, n2 = 0.0f;
         if (cc * 8 < p.D) {
             const v8 a = *reinterpret_cast<const v8 *>(p.dout.data + tok * p.dout.ts + head * p.dout.hs + cc * 16);
@@ -626,7 +654,10 @@ __global__ __launch_bounds__(256) void attn_rows_delta_kernel(attn_p p) {
             }
         }
         s = sum16(s);
-        if (cc == 0) p.delta[row] = s;
+        if (cc == 0) {
+            p.lse2[row] = p.lse[tok * p.H + head] * LOG2E - (type_of<E>::HALF ? P_SHIFT : 0);
+            p.ndelta[row] = -s;
+        }
         if (type_of<E>::HALF) top_o = fmaxf(top_o, sum16(n2));
     }
     if (!type_of<E>::HALF) return;
@@ -660,8 +691,9 @@ __global__ __launch_bounds__(256) void attn_rows_delta_kernel(attn_p p) {
     }
 }
 
-// fp16: the power of two that dS is carried with, 2^k with |dS| 2^k <= 2^15: |dP - delta| is at most twice the
-// product of the largest norms of dout's and v's rows, and P is at most 1. 1 where the norms are no help.
+// fp16: the factor from (2^15 P) (dP - delta) to dS as it is carried, 2^k dS with |dS| 2^k <= 2^15: |dP - delta| is at
+// most twice the product of the largest norms of dout's and v's rows, and P is at most 1. k = 0 where the
+// norms are no help.
 template <class E>
 __device__ __forceinline__ float ds_factor(const attn_p & p) {
     if constexpr (!type_of<E>::HALF) return 1.0f;
@@ -677,30 +709,31 @@ __device__ __forceinline__ float ds_factor(const attn_p & p) {
         b = fmaxf(b, __shfl_xor(b, k));
     }
     const float bound = 2.0f * sqrtf(a) * sqrtf(b);
-    if (!(bound > 0.0f) || !(bound < INFINITY)) return 1.0f;
+    if (!(bound > 0.0f) || !(bound < INFINITY)) return ldexpf(1.0f, -P_SHIFT);
     int e;
     (void) frexpf(bound, &e);                        // bound < 2^e
-    return ldexpf(1.0f, min(max(15 - e, -30), 60));
+    return ldexpf(1.0f, min(max(15 - e, -30), 60) - P_SHIFT);
 }
 
 // dQ: the forward pass's tiling. dQ^T = scale K^T dS^T.
 template <class E, int DT>
 __device__ __forceinline__ void dq_tile(v16f (&dq)[DT], const typename type_of<E>::v8 (&q)[2 * DT],
-                                        const typename type_of<E>::v8 (&go)[2 * DT], const E * kt, const E * vt, float c,
-                                        float lse2, float sigma, float delta_s, bool mask, int lo, int hi) {
+                                        const typename type_of<E>::v8 (&go)[2 * DT], lane_at at, uint32_t kt, uint32_t vt, float c,
+                                        float lse2, float ndelta, float factor, bool mask, int lo, int hi) {
     typedef type_of<E> TY;
     const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
         v16f s = {}, dp = {};
 #pragma unroll
-        for (int d = 0; d < 2 * DT; ++d) s = TY::mfma(row_operand<E, DT>(kt, 32 * a, d), q[d], s);
+        for (int d = 0; d < 2 * DT; ++d) s = TY::mfma(row_operand<E, DT>(kt + at.row, 32 * a, d), q[d], s);
 #pragma unroll
-        for (int d = 0; d < 2 * DT; ++d) dp = TY::mfma(row_operand<E, DT>(vt, 32 * a, d), go[d], dp);
+        for (int d = 0; d < 2 * DT; ++d) dp = TY::mfma(row_operand<E, DT>(vt + at.row, 32 * a, d), go[d], dp);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2));
-            s[i] = pr * __builtin_fmaf(dp[i], sigma, -delta_s);
+            s[i] = pr * (dp[i] + ndelta);
+            if (TY::HALF) s[i] *= factor;
         }
         if (mask) {
             const int l0 = lo - 4 * h;
@@ -713,7 +746,7 @@ __device__ __forceinline__ void dq_tile(v16f (&dq)[DT], const typename type_of<E
         for (int b = 0; b < 2; ++b) {
             const typename TY::v8 ds = pack<E>(s, b);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) dq[d] = TY::mfma(col_operand<E, DT>(kt, 32 * a + 16 * b, 32 * d), ds, dq[d]);
+            for (int d = 0; d < DT; ++d) dq[d] = TY::mfma(col_operand<E, DT>(kt + at.col, 32 * a + 16 * b, d), ds, dq[d]);
         }
     }
 }
@@ -737,10 +770,10 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
     typename type_of<E>::v8 q[2 * DT], go[2 * DT];
     load_operand<E, DT>(q, p.q.data + (c.q0 + tok) * p.q.ts + head * p.q.hs, p.D);
     load_operand<E, DT>(go, p.dout.data + (c.q0 + tok) * p.dout.ts + head * p.dout.hs, p.D);
-    const int64_t row = (int64_t) (c.q0 + tok) * p.H + head;
-    const float factor = ds_factor<E>(p), sigma = type_of<E>::HALF ? factor : 1.0f;
-    const float lse = p.lse[row], delta_s = p.delta[row] * sigma;
-    const float lse2 = lse * LOG2E;
+    const int64_t row = ((int64_t) g * p.T_q + c.q0) * p.R + pc;
+    const float factor = ds_factor<E>(p), ds_scale = type_of<E>::HALF ? ldexpf(factor, P_SHIFT) : 1.0f;
+    float lse2 = p.lse2[row], ndelta = p.ndelta[row];
+    asm volatile("" : "+v"(lse2), "+v"(ndelta));
 
     const int lo = key_lo(p, c, tok), hi = key_hi(p, c, tok);
     const int t_end = (min(p0 + BM, np) - 1) / p.R;
@@ -750,7 +783,9 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
 
     const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
     const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
-    const tile_loader<DT, BN, 256> lk(p.D, [&](int r) { return r * p.k.ts; }), lv(p.D, [&](int r) { return r * p.v.ts; });
+    tile_loader<DT, BN, 256> lk(p.D), lv(p.D);
+    lk.rows_at(p.k.ts);
+    lv.rows_at(p.v.ts);
     auto load = [&](int j, int buf) {
         load_keys(lk, lds_addr(sk[buf]), kb, p.k.ts, j * BN, c.m, p.near_k);
         load_keys(lv, lds_addr(sv[buf]), vb, p.v.ts, j * BN, c.m, p.near_k);
@@ -764,6 +799,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
 #pragma unroll
     for (int k = 0; k < DT; ++k) dq[k] = v16f{};
     const float cs = p.scale * LOG2E;
+    const lane_at at = lane_places<DT>();
     if (j_lo < j_hi) load(j_lo, 0);
     for (int j = j_lo; j < j_hi; ++j) {
         const int buf = (j - j_lo) & 1, j0 = j * BN;
@@ -771,64 +807,84 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
         barrier();
         if (j + 1 < j_hi) load(j + 1, buf ^ 1);
         if (!active || j0 >= some_hi || j0 + BN <= some_lo) continue;
-        dq_tile<E, DT>(dq, q, go, sk[buf], sv[buf], cs, lse2, sigma, delta_s, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
+        dq_tile<E, DT>(dq, q, go, at, lds_addr(sk[buf]), lds_addr(sv[buf]), cs, lse2, ndelta, factor, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
     }
     barrier();
     if (!active) return;
     E * tile = (wave < 2 ? sk[0] : sv[0]) + (wave & 1) * 32 * SP<DT>;
-    store_columns<E, DT>(tile, dq, p.scale / factor, p.D, [&](int r) -> char * {
+    store_columns<E, DT>(tile, dq, p.scale / ds_scale, p.D, [&](int r) -> char * {
         const int pr = pw + r;
         if (pr >= np) return nullptr;
         return p.dq.data + (int64_t) (c.q0 + pr / p.R) * p.dq.ts + (g * p.R + pr % p.R) * p.dq.hs;
     });
 }
 
-// dK, dV: a wave has 32 keys, the workgroup goes over the pairs that see its 128, 64 at a time.
+// Ends a phase of N products of one LDS read each, with two reads ahead of the products: more would not
+// fit the registers.
+template <int N>
+__device__ __forceinline__ void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+    for (int i = 0; i < N - 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// dK, dV: a wave has 32 keys, the workgroup goes over the pairs that see its 128, 64 at a time, a wave 32 at a
+// time: qt, ot their rows of q and dout, lse2, ndelta their sums, pairs lo .. hi - 1 of them seen by the key.
 template <class E, int DT>
 __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const typename type_of<E>::v8 (&k)[2 * DT],
-                                         const typename type_of<E>::v8 (&v)[2 * DT], const E * qt, const E * ot,
-                                         const float * lse2, const float * delta_s, float c, float sigma, bool mask, int lo, int hi) {
+                                         const typename type_of<E>::v8 (&v)[2 * DT], lane_at at, uint32_t qt, uint32_t ot,
+                                         const float * lse2, const float * ndelta, float c, float factor, bool mask, int lo, int hi) {
     typedef type_of<E> TY;
     const int h = (threadIdx.x & 63) >> 5;
+    v16f s = {}, dp;
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-        v16f s = {}, dp = {};
+    for (int d = 0; d < 2 * DT; ++d) s = TY::mfma(row_operand<E, DT>(qt + at.row, 0, d), k[d], s);
+    if (DT >= 3) reads_ahead<2 * DT>();
 #pragma unroll
-        for (int d = 0; d < 2 * DT; ++d) s = TY::mfma(row_operand<E, DT>(qt, 32 * a, d), k[d], s);
+    for (int i4 = 0; i4 < 4; ++i4) {              // dP - delta: the sums start there
+        const v4f de = *reinterpret_cast<const v4f *>(ndelta + 8 * i4 + 4 * h);
 #pragma unroll
-        for (int d = 0; d < 2 * DT; ++d) dp = TY::mfma(row_operand<E, DT>(ot, 32 * a, d), v[d], dp);
+        for (int j = 0; j < 4; ++j) dp[4 * i4 + j] = de[j];
+    }
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-            const v4f ls = *reinterpret_cast<const v4f *>(lse2 + 32 * a + 8 * i4 + 4 * h);
-            const v4f de = *reinterpret_cast<const v4f *>(delta_s + 32 * a + 8 * i4 + 4 * h);
+    for (int d = 0; d < 2 * DT; ++d) dp = TY::mfma(row_operand<E, DT>(ot + at.row, 0, d), v[d], dp);
+    if (DT >= 3) reads_ahead<2 * DT>();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = 4 * i4 + j;
-                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[j]));
-                dp[i] = s[i] * __builtin_fmaf(dp[i], sigma, -de[j]);
-            }
+    for (int i4 = 0; i4 < 4; ++i4) {
+        const v4f ls = *reinterpret_cast<const v4f *>(lse2 + 8 * i4 + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = 4 * i4 + j;
+            s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[j]));
+            dp[i] *= s[i];
+            if (TY::HALF) dp[i] *= factor;
         }
-        if (mask) {
-            const int l0 = lo - 4 * h;
-            const unsigned n = hi > lo ? hi - lo : 0;
+    }
+    if (mask) {
+        const int l0 = lo - 4 * h;
+        const unsigned n = hi > lo ? hi - lo : 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if ((unsigned) (32 * a + reg_row(i) - l0) >= n) s[i] = dp[i] = 0.0f;
-        }
+        for (int i = 0; i < 16; ++i)
+            if ((unsigned) (reg_row(i) - l0) >= n) s[i] = dp[i] = 0.0f;
+    }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const typename TY::v8 pp = pack<E>(s, b), ds = pack<E>(dp, b);
+    for (int b = 0; b < 2; ++b) {
+        const typename TY::v8 pp = pack<E>(s, b), ds = pack<E>(dp, b);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                dv[d] = TY::mfma(col_operand<E, DT>(ot, 32 * a + 16 * b, 32 * d), pp, dv[d]);
-                dk[d] = TY::mfma(col_operand<E, DT>(qt, 32 * a + 16 * b, 32 * d), ds, dk[d]);
-            }
+        for (int d = 0; d < DT; ++d) {
+            dv[d] = TY::mfma(col_operand<E, DT>(ot + at.col, 16 * b, d), pp, dv[d]);
+            dk[d] = TY::mfma(col_operand<E, DT>(qt + at.col, 16 * b, d), ds, dk[d]);
         }
     }
 }
 
 template <class E, int DT>
-__global__ __launch_bounds__(256, DT <= 2 ? 2 : 1) void attn_rows_dkv_kernel(attn_p p) {
+__global__ __launch_bounds__(256, 2) void attn_rows_dkv_kernel(attn_p p) {
     constexpr int BK = 128, BQ = 64, TILE = BQ * SP<DT>;
     __shared__ __align__(1024) E sq[2][TILE], so[2][TILE];
     __shared__ __align__(16) float s_lse[2][BQ], s_delta[2][BQ];
@@ -846,9 +902,7 @@ __global__ __launch_bounds__(256, DT <= 2 ? 2 : 1) void attn_rows_dkv_kernel(att
     typename type_of<E>::v8 k[2 * DT], v[2 * DT];
     load_operand<E, DT>(k, p.k.data + (int64_t) (c.k0 + key) * p.k.ts + g * p.k.hs, p.D);
     load_operand<E, DT>(v, p.v.data + (int64_t) (c.k0 + key) * p.v.ts + g * p.v.hs, p.D);
-    const float factor = ds_factor<E>(p);
-    // P is carried as 2^15 P, so dS's factor has it already
-    const float sigma = type_of<E>::HALF ? ldexpf(factor, -P_SHIFT) : 1.0f;
+    const float factor = ds_factor<E>(p), ds_scale = type_of<E>::HALF ? ldexpf(factor, P_SHIFT) : 1.0f;
 
     const int lo = tok_lo(p, c, key) * p.R, hi = tok_hi(p, c, key) * p.R;
     const int k_end = min(kb0 + BK, c.m) - 1;
@@ -857,14 +911,14 @@ __global__ __launch_bounds__(256, DT <= 2 ? 2 : 1) void attn_rows_dkv_kernel(att
     const int some_lo = tok_lo(p, c, ka) * p.R, some_hi = tok_hi(p, c, ke) * p.R;
     const int all_lo = tok_lo(p, c, ke) * p.R, all_hi = tok_hi(p, c, ka) * p.R;
 
-    const tile_loader<DT, BQ, 256> lq(p.D, [&](int r) { return r / p.R * p.q.ts + r % p.R * p.q.hs; });
-    const tile_loader<DT, BQ, 256> l_out(p.D, [&](int r) { return r / p.R * p.dout.ts + r % p.R * p.dout.hs; });
+    tile_loader<DT, BQ, 256> lq(p.D), l_out(p.D);
+    lq.pairs_at(p.R, p.q.ts, p.q.hs);
+    l_out.pairs_at(p.R, p.dout.ts, p.dout.hs);
     if (p.D != 32 * DT) {
         clear(sq, sizeof(sq), threadIdx.x, 256);
         clear(so, sizeof(so), threadIdx.x, 256);
         barrier();
     }
-    float row_value = 0.0f;      // threads 0..63: a pair's lse, 64..127: its delta, of the tile being loaded
     auto load = [&](int j, int buf) {
         const int j0 = j * BQ;
         if (p.near_q && j0 + BQ <= np) {
@@ -878,36 +932,28 @@ __global__ __launch_bounds__(256, DT <= 2 ? 2 : 1) void attn_rows_dkv_kernel(att
             lq.load_each(lds_addr(sq[buf]), [&](int r) { return at(p.q, r); });
             l_out.load_each(lds_addr(so[buf]), [&](int r) { return at(p.dout, r); });
         }
-        if (threadIdx.x < 2 * BQ) {
-            const int pr = j0 + (threadIdx.x & (BQ - 1));
-            const bool ok = pr < np, is_lse = threadIdx.x < BQ;
-            const int64_t row = (int64_t) (c.q0 + min(pr, np - 1) / p.R) * p.H + g * p.R + min(pr, np - 1) % p.R;
-            const float x = (is_lse ? p.lse : p.delta)[row];
-            // pairs behind the document: P = 2^-inf = 0
-            row_value = is_lse ? (ok ? x * LOG2E - (type_of<E>::HALF ? P_SHIFT : 0) : INFINITY) : (ok ? x * sigma : 0.0f);
-        }
-    };
-    auto put = [&](int buf) {
-        if (threadIdx.x < BQ) s_lse[buf][threadIdx.x] = row_value;
-        else if (threadIdx.x < 2 * BQ) s_delta[buf][threadIdx.x - BQ] = row_value;
+        // the pairs' sums: waves 0 and 1, a value a lane (behind the document: whatever is there, masked)
+        if (wave < 2) dma4((wave ? p.ndelta : p.lse2) + ((int64_t) g * p.T_q + c.q0) * p.R + j0 + lane, lds_addr(wave ? s_delta[buf] : s_lse[buf]));
     };
     v16f dk[DT], dv[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) dk[i] = dv[i] = v16f{};
     const float cs = p.scale * LOG2E;
-    if (j_lo < j_hi) {
-        load(j_lo, 0);
-        put(0);
-    }
+    const lane_at at = lane_places<DT>();
+    if (j_lo < j_hi) load(j_lo, 0);
     for (int j = j_lo; j < j_hi; ++j) {
         const int buf = (j - j_lo) & 1, j0 = j * BQ;
         wait_all();
         barrier();
         if (j + 1 < j_hi) load(j + 1, buf ^ 1);
         if (active && j0 < some_hi && j0 + BQ > some_lo) {
-            dkv_tile<E, DT>(dk, dv, k, v, sq[buf], so[buf], s_lse[buf], s_delta[buf], cs, sigma, j0 < all_lo || j0 + BQ > all_hi, lo - j0, hi - j0);
+            const bool mask = j0 < all_lo || j0 + BQ > all_hi;
+#pragma unroll 1
+            for (int a = 0; a < BQ; a += 32) {
+                dkv_tile<E, DT>(dk, dv, k, v, at, lds_addr(sq[buf]) + a * SP<DT> * 2, lds_addr(so[buf]) + a * SP<DT> * 2, s_lse[buf] + a,
+                                s_delta[buf] + a, cs, factor, mask, lo - j0 - a, hi - j0 - a);
+            }
         }
-        if (j + 1 < j_hi) put(buf ^ 1);
     }
     barrier();
     if (!active) return;
@@ -917,7 +963,7 @@ __global__ __launch_bounds__(256, DT <= 2 ? 2 : 1) void attn_rows_dkv_kernel(att
     };
     store_columns<E, DT>(tile, dv, type_of<E>::HALF ? 1.0f / (1 << P_SHIFT) : 1.0f, p.D, dst(p.dv));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    store_columns<E, DT>(tile, dk, p.scale / factor, p.D, dst(p.dk));
+    store_columns<E, DT>(tile, dk, p.scale / ds_scale, p.D, dst(p.dk));
 }
 
 // ---------------------------------------------------------------------------
@@ -966,10 +1012,10 @@ int32_t check_params(const char * what, const nxg_attention_rows_params * a, att
 }
 
 // Whether 64 rows' offsets from the first fit 32 bits: keys one after another, and pairs, whose places
-// repeat from tile to tile where R divides 64.
+// repeat from tile to tile where R divides the rows of a thread's step (16).
 bool near_rows(const rows & x) { return x.ts <= (INT32_MAX - 4096) / 64; }
 bool near_pairs(const rows & x, int R) {
-    return 64 % R == 0 && x.ts <= (INT32_MAX - 4096) / 128 && x.hs <= (INT32_MAX - 4096) / 2 / R;
+    return 16 % R == 0 && x.ts <= (INT32_MAX - 4096) / 128 && x.hs <= (INT32_MAX - 4096) / 2 / R;
 }
 
 int32_t check_rows(const char * what, const char * name, const nxg_rows * x, int64_t T, int n_head, int D, bool written, rows & r) {
@@ -996,6 +1042,10 @@ int32_t check_rows(const char * what, const char * name, const nxg_rows * x, int
 }
 
 #define NXG_TRY(call) do { const int32_t rc_ = (call); if (rc_) return rc_; } while (0)
+
+// Values of a row array of the backward pass: one a (token, head), and a tile's reach behind the last.
+int64_t row_values(const attn_p & p) { return (int64_t) p.T_q * p.H + 64; }
+int64_t backward_bytes(const attn_p & p) { return (2 * N_MAX + 2 * row_values(p)) * 4; }
 
 // Launches one of a kernel's instances by type and head size.
 #define NXG_BY_TYPE(type, D, LAUNCH)                                               \
@@ -1086,7 +1136,7 @@ int64_t nxg_attention_rows_backward_workspace_bytes(const nxg_attention_rows_par
     attn_p p;
     const int32_t rc = check_params("attention_rows_backward_workspace_bytes", a, p);
     if (rc) return -rc;
-    return 8 * N_MAX + 4 * (int64_t) p.T_q * p.H;
+    return backward_bytes(p);
 }
 
 int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const nxg_rows * dout, const nxg_rows * q,
@@ -1106,16 +1156,17 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
     NXG_TRY(check_rows(what, "dv", dv, p.T_k, p.G, p.D, true, p.dv));
     if (p.n_seqs == 0 || (p.T_q == 0 && p.T_k == 0)) return NXG_OK;
     if (!p.cu_q || !p.cu_k || (p.T_q > 0 && !lse)) return nxg_fail(NXG_EINVAL, "%s: cu_q, cu_k or lse is null", what);
-    if (!workspace || ((uintptr_t) workspace & 15) || workspace_bytes < 8 * N_MAX + 4 * (int64_t) p.T_q * p.H) {
+    if (!workspace || ((uintptr_t) workspace & 15) || workspace_bytes < backward_bytes(p)) {
         return nxg_fail(NXG_EINVAL, "%s: workspace must be 16-byte aligned memory of %lld bytes", what,
-                        (long long) (8 * N_MAX + 4 * (int64_t) p.T_q * p.H));
+                        (long long) backward_bytes(p));
     }
     NXG_TRY(nxg_check_device());
     p.lse = (float *) lse;
     p.near_k = near_rows(p.k) && near_rows(p.v);
     p.near_q = near_pairs(p.q, p.R) && near_pairs(p.dout, p.R);
     p.maxima = (float *) workspace;
-    p.delta = p.maxima + 2 * N_MAX;
+    p.lse2 = p.maxima + 2 * N_MAX;
+    p.ndelta = p.lse2 + row_values(p);
     hipStream_t s = (hipStream_t) stream;
     if (p.T_q > 0) {
         if (a->type == NXG_TYPE_BF16) {
