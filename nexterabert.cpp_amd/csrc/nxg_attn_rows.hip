@@ -172,12 +172,16 @@ __device__ __forceinline__ int tok_hi(const attn_p & p, const doc & c, int j) {
 // ---------------------------------------------------------------------------
 //
 // A tile is rows of SP = 64 or 128 values (the head's D, zeros behind it). The 16-byte chunk c of row r is
-// at chunk c ^ swz(r) of the row: 8 neighbouring rows of one chunk fill all banks (reads of rows: 32 rows
-// of one chunk per half wave), and so do 4 neighbouring rows of a pair of chunks (reads of columns).
-
-__device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+// at chunk c ^ swz(r) of the row, so that a cycle of LDS (64 banks of 4 bytes) is filled both by 16 rows'
+// same chunk (reads of rows, 16 lanes a cycle) and by 4 rows' 4 neighbouring chunks (reads of columns, 32 lanes
+// a cycle). swz(a ^ b) = swz(a) ^ swz(b).
 
 template <int DT> constexpr int SP = DT <= 2 ? 64 : 128;
+
+template <int DT>
+__device__ __forceinline__ constexpr int swz(int r) {
+    return SP<DT> == 64 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3) : (r & 3) << 2 | ((r >> 2) & 3);
+}
 
 // Copies NR rows by the NT threads of a workgroup (NT = 256) or a wave (64) into a tile. A thread's place
 // within a tile is computed once; a tile is a new scalar base, and so is each of a thread's rows (STEP
@@ -187,21 +191,17 @@ struct tile_loader {
     static constexpr int CH = SP<DT> / 8, N = NR * CH / NT, STEP = NT / CH;
     int r0, c0, D;
     uint32_t off;              // of row r0 from the tile's base
+    uint32_t wave_at;          // the wave's first row in the tile
     int64_t step;              // of STEP rows
 
-    static __device__ __forceinline__ int thread() { return NT == 64 ? threadIdx.x & 63 : threadIdx.x; }
-    static __device__ __forceinline__ uint32_t wave_at() { return NT == 64 ? 0 : uni((int) (threadIdx.x >> 6)) * 1024; }
-    // The chunk of the thread's k'th row: the same for all where 8 divides STEP, else (4) every other row's
-    // neighbour, as swz() of a row 4 further says.
-    __device__ __forceinline__ int chunk(int k) const {
-        static_assert(STEP % 4 == 0, "swz of the rows of a thread");
-        return STEP % 8 == 0 ? c0 : c0 ^ (k & 1);
-    }
+    // The chunk of the thread's k'th row, r0 + k STEP = r0 ^ k STEP.
+    __device__ __forceinline__ int chunk(int k) const { return c0 ^ swz<DT>(k * STEP); }
 
     __device__ __forceinline__ tile_loader(int D_) : D(D_) {
-        const int t = thread();
+        const int t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
+        wave_at = NT == 64 ? 0 : uni((int) (threadIdx.x >> 6)) * 1024;
         r0 = t / CH;
-        c0 = (t % CH) ^ swz(r0);
+        c0 = (t % CH) ^ swz<DT>(r0);
     }
     // Rows ts bytes apart; or pairs, R to a token (R divides STEP), heads hs bytes apart.
     __device__ __forceinline__ void rows_at(int64_t ts) {
@@ -215,7 +215,7 @@ struct tile_loader {
     __device__ __forceinline__ void load(const char * base, uint32_t lds) const {
 #pragma unroll
         for (int k = 0; k < N; ++k)
-            if (chunk(k) * 8 < D) dma16s(base + k * step, off + chunk(k) * 16, lds + wave_at() + k * NT * 16);
+            if (chunk(k) * 8 < D) dma16s(base + k * step, off + chunk(k) * 16, lds + wave_at + k * NT * 16);
     }
     // row r from src(r), zeros where that is null
     template <class Src>
@@ -223,18 +223,40 @@ struct tile_loader {
 #pragma unroll 1
         for (int k = 0; k < N; ++k) {
             const char * s = src(r0 + k * STEP);
-            if (chunk(k) * 8 < D) dma16(s ? s + chunk(k) * 16 : (const char *) zeros16, uni((int) (lds + wave_at() + k * NT * 16)));
+            if (chunk(k) * 8 < D) dma16(s ? s + chunk(k) * 16 : (const char *) zeros16, uni((int) (lds + wave_at + k * NT * 16)));
         }
     }
 };
 
-// The tile of keys j0 .. of a document's m, rows ts bytes apart from `first`.
-template <class L>
-__device__ __forceinline__ void load_keys(const L & l, uint32_t lds, const char * first, int64_t ts, int j0, int m, bool near) {
-    constexpr int NR = L::N * L::STEP;
-    if (near && j0 + NR <= m) l.load(uni(first + j0 * ts), lds);
-    else l.load_each(lds, [&](int r) { return j0 + r < m ? first + (j0 + r) * ts : nullptr; });
-}
+// The tiles of a document's m keys one after another, K and V: the next one starts at key j0.
+template <int DT, int NR, int NT>
+struct key_stream {
+    tile_loader<DT, NR, NT> lk, lv;
+    const char * k, * v;       // of the next tile's first rows
+    int j0, m, step;           // keys from one tile to the next
+    int64_t kts, vts;
+    bool near;
+
+    __device__ __forceinline__ key_stream(const attn_p & p, const doc & c, int g, int first, int step_)
+        : lk(p.D), lv(p.D), j0(first), m(c.m), step(step_), kts(p.k.ts), vts(p.v.ts), near(p.near_k) {
+        lk.rows_at(kts);
+        lv.rows_at(vts);
+        k = uni(p.k.data + (c.k0 + (int64_t) first) * kts + g * p.k.hs);
+        v = uni(p.v.data + (c.k0 + (int64_t) first) * vts + g * p.v.hs);
+    }
+    __device__ __forceinline__ void next(uint32_t lds_k, uint32_t lds_v) {
+        if (near && j0 + NR <= m) {
+            lk.load(k, lds_k);
+            lv.load(v, lds_v);
+        } else {
+            lk.load_each(lds_k, [&](int r) { return j0 + r < m ? k + r * kts : nullptr; });
+            lv.load_each(lds_v, [&](int r) { return j0 + r < m ? v + r * vts : nullptr; });
+        }
+        j0 += step;
+        k += step * kts;
+        v += step * vts;
+    }
+};
 
 // Zeros the chunks behind D of n tiles' memory (all of it), before the first load.
 __device__ __forceinline__ void clear(void * lds, int bytes, int thread, int threads) {
@@ -250,8 +272,8 @@ __device__ __forceinline__ lane_at lane_places() {
     const int lane = threadIdx.x & 63, r = lane & 31, i = lane & 15, g = lane >> 4;
     const int cr = 4 * (g >> 1) + (i >> 2);
     lane_at o;
-    o.row = r * SP<DT> * 2 + (((lane >> 5) ^ swz(r)) << 4);
-    o.col = cr * SP<DT> * 2 + (((2 * (g & 1) + ((i & 3) >> 1)) ^ swz(cr)) << 4) + (i & 1) * 8;
+    o.row = r * SP<DT> * 2 + (((lane >> 5) ^ swz<DT>(r)) << 4);
+    o.col = cr * SP<DT> * 2 + (((2 * (g & 1) + ((i & 3) >> 1)) ^ swz<DT>(cr)) << 4) + (i & 1) * 8;
     return o;
 }
 
@@ -274,7 +296,7 @@ __device__ __forceinline__ typename type_of<E>::v8 col_operand(uint32_t at, int 
     v4s x[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
-        x[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *) (uintptr_t) ((at ^ (d << 6)) + (r0 + 8 * k) * SP<DT> * 2));
+        x[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *) (uintptr_t) ((at ^ (d << 6 | swz<DT>(8 * k) << 4)) + (r0 + 8 * k) * SP<DT> * 2));
     typename type_of<E>::v8 out;
     __builtin_memcpy(&out, x, 16);
     return out;
@@ -325,7 +347,7 @@ __device__ __forceinline__ void store_columns(E * tile, const v16f (&acc)[DT], f
             v4e e;
 #pragma unroll
             for (int i = 0; i < 4; ++i) e[i] = (E) (acc[d][4 * k + i] * f);
-            const int c = (4 * d + k) ^ swz(col);
+            const int c = (4 * d + k) ^ swz<DT>(col);
             *reinterpret_cast<v4e *>(tile + col * SP<DT> + c * 8 + 4 * h) = e;
         }
     }
@@ -334,7 +356,7 @@ __device__ __forceinline__ void store_columns(E * tile, const v16f (&acc)[DT], f
     for (int it = 0; it < 32 * CH / 64; ++it) {
         const int r = (it * 64 + lane) / CH, c = lane % CH;
         char * o = dst(r);
-        const v4i x = *reinterpret_cast<const v4i *>(tile + r * SP<DT> + (c ^ swz(r)) * 8);
+        const v4i x = *reinterpret_cast<const v4i *>(tile + r * SP<DT> + (c ^ swz<DT>(r)) * 8);
         if (o && c * 8 < D) *reinterpret_cast<v4i *>(o + c * 16) = x;
     }
 }
@@ -343,22 +365,25 @@ __device__ __forceinline__ void store_columns(E * tile, const v16f (&acc)[DT], f
 // forward
 // ---------------------------------------------------------------------------
 
-// Running softmax of the wave's 32 pairs. mc: the exponentials' reference in powers of two, the largest score
-// so far or up to 2^8 below it, so that most tiles leave the sums alone (P stays below 256, far from the
-// end of either type); top: the score past which it moves (-inf before the first); l: the half wave's
-// share of sum p; o = sum p v.
+// Running softmax of the wave's 32 pairs. mc: the exponentials' reference in powers of two (-inf before the
+// first key); l: the half wave's share of sum p; o = sum p v.
 template <int DT>
 struct fwd_state {
-    float top, mc, l;
+    float mc, l;
     v16f o[DT];
 
-    __device__ __forceinline__ void init() {
-        top = -INFINITY;
-        mc = l = 0.0f;
+    // some: the lane's pair sees a key at all
+    __device__ __forceinline__ void init(bool some) {
+        mc = some ? -INFINITY : 0.0f;
+        l = 0.0f;
 #pragma unroll
         for (int k = 0; k < DT; ++k) o[k] = v16f{};
     }
 };
+
+// A tile's scores that may raise the reference: their sum with the old one past 2^14 (so P stays in either
+// type's range). The largest score is looked for in those tiles alone, the first and a few more.
+constexpr float RAISE = 16384.0f;
 
 // 32 NK keys of a tile. lo, hi: the lane's pair sees keys lo .. hi - 1 of the tile (with `mask` alone: a
 // tile that every pair sees has no masks).
@@ -366,48 +391,63 @@ template <class E, int DT, int NK>
 __device__ __forceinline__ void fwd_tile(fwd_state<DT> & st, const typename type_of<E>::v8 (&q)[2 * DT], lane_at at, uint32_t kt,
                                          uint32_t vt, float c, bool mask, int lo, int hi) {
     typedef type_of<E> TY;
-    const int h = (threadIdx.x & 63) >> 5;
     v16f s[NK];
+    auto scores = [&] {
+        // within the loop below, whose second turn is rare: nothing of it is to be computed before
+        uint32_t k_at = kt + at.row;
+        int l0 = lo - 4 * ((int) (threadIdx.x & 63) >> 5);
+        asm volatile("" : "+v"(k_at), "+v"(l0));
 #pragma unroll
-    for (int a = 0; a < NK; ++a) {
-        s[a] = v16f{};
+        for (int a = 0; a < NK; ++a) {
+            s[a] = v16f{};
 #pragma unroll
-        for (int d = 0; d < 2 * DT; ++d) s[a] = TY::mfma(row_operand<E, DT>(kt + at.row, 32 * a, d), q[d], s[a]);
-    }
-    if (mask) {
-        const int l0 = lo - 4 * h;
-        const unsigned n = hi > lo ? hi - lo : 0;
+            for (int d = 0; d < 2 * DT; ++d) s[a] = TY::mfma(row_operand<E, DT>(k_at, 32 * a, d), q[d], s[a]);
+        }
+        if (mask) {
+            const unsigned n = hi > lo ? hi - lo : 0;
+#pragma unroll
+            for (int a = 0; a < NK; ++a)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if ((unsigned) (32 * a + reg_row(i) - l0) >= n) s[a][i] = -INFINITY;
+        }
+    };
+    auto weights = [&](float mc) {
+        float t[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int a = 0; a < NK; ++a)
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if ((unsigned) (32 * a + reg_row(i) - l0) >= n) s[a][i] = -INFINITY;
+            for (int i = 0; i < 16; ++i) {
+                s[a][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a][i], c, -mc));
+                t[i & 1] += s[a][i];
+            }
+        return t[0] + t[1];
+    };
+    // a new reference: the largest score so far
+    auto raise = [&] {
+        float mx = s[0][0];
+#pragma unroll
+        for (int a = 0; a < NK; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[a][i]);
+        const float mc = fmaxf(st.mc, half_max(mx) * c);
+        const float f = st.mc == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.mc - mc);
+        st.mc = mc;
+        st.l *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st.o[d][i] *= f;
+    };
+    float t;
+    for (bool up = __any(st.mc == -INFINITY);;) {
+        scores();
+        if (up) raise();
+        t = weights(st.mc == -INFINITY ? 0.0f : st.mc);
+        if (up || !__any(!(t <= RAISE))) break;
+        up = true;
     }
-    float mx = s[0][0];
-#pragma unroll
-    for (int a = 0; a < NK; ++a)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[a][i]);
-    mx = half_max(mx);
-    if (__any(mx > st.top)) {
-        if (mx > st.top) {
-            const float mc = mx * c, f = fminf(__builtin_amdgcn_exp2f(st.mc - mc), 1.0f);   // 1: nothing summed yet
-            st.mc = mc;
-            st.top = mx + 8.0f / c;
-            st.l *= f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) st.o[d][i] *= f;
-        }
-    }
-#pragma unroll
-    for (int a = 0; a < NK; ++a)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[a][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a][i], c, -st.mc));
-            st.l += s[a][i];
-        }
+    st.l += t;
 #pragma unroll
     for (int a = 0; a < 2 * NK; ++a) {
         const typename TY::v8 pa = pack<E>(s[a / 2], a % 2);
@@ -443,15 +483,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     const int ta = uni(min(pw, np - 1) / p.R), tb = uni(min(pw + 31, np - 1) / p.R);
     const int some_lo = key_lo(p, c, ta), some_hi = key_hi(p, c, tb), all_lo = key_lo(p, c, tb), all_hi = key_hi(p, c, ta);
 
-    const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
-    const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
-    tile_loader<DT, BN, 256> lk(p.D), lv(p.D);
-    lk.rows_at(p.k.ts);
-    lv.rows_at(p.v.ts);
-    auto load = [&](int j, int buf) {
-        load_keys(lk, lds_addr(sk[buf]), kb, p.k.ts, j * BN, c.m, p.near_k);
-        load_keys(lv, lds_addr(sv[buf]), vb, p.v.ts, j * BN, c.m, p.near_k);
-    };
+    key_stream<DT, BN, 256> keys(p, c, g, j_lo * BN, BN);
     if (p.D != 32 * DT) {
         clear(sk, sizeof(sk), threadIdx.x, 256);
         clear(sv, sizeof(sv), threadIdx.x, 256);
@@ -459,15 +491,15 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     }
 
     fwd_state<DT> st;
-    st.init();
+    st.init(lo < hi);
     const float cs = p.scale * LOG2E;
     const lane_at at = lane_places<DT>();
-    if (j_lo < j_hi) load(j_lo, 0);
+    if (j_lo < j_hi) keys.next(lds_addr(sk[0]), lds_addr(sv[0]));
     for (int j = j_lo; j < j_hi; ++j) {
         const int buf = (j - j_lo) & 1, j0 = j * BN;
         wait_all();
         barrier();
-        if (j + 1 < j_hi) load(j + 1, buf ^ 1);
+        if (j + 1 < j_hi) keys.next(lds_addr(sk[buf ^ 1]), lds_addr(sv[buf ^ 1]));
         if (!active || j0 >= some_hi || j0 + BN <= some_lo) continue;
         fwd_tile<E, DT, 2>(st, q, at, lds_addr(sk[buf]), lds_addr(sv[buf]), cs, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
     }
@@ -513,28 +545,20 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
     const int share = (max(t_hi - t_lo, 0) + p.n_split - 1) / p.n_split;
     const int j_lo = t_lo + split * share, j_hi = min(j_lo + share, t_hi);
 
-    const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
-    const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
-    tile_loader<DT, BN, 64> lk(p.D), lv(p.D);
-    lk.rows_at(p.k.ts);
-    lv.rows_at(p.v.ts);
-    auto load = [&](int j, int buf) {
-        load_keys(lk, lds_addr(lds[wave][buf][0]), kb, p.k.ts, j * BN, c.m, p.near_k);
-        load_keys(lv, lds_addr(lds[wave][buf][1]), vb, p.v.ts, j * BN, c.m, p.near_k);
-    };
+    key_stream<DT, BN, 64> keys(p, c, g, (j_lo + wave) * BN, 4 * BN);
     if (p.D != 32 * DT) {
         clear(lds[wave], sizeof(lds[wave]), lane, 64);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     fwd_state<DT> st;
-    st.init();
+    st.init(lo < hi);
     const float cs = p.scale * LOG2E;
     const lane_at at = lane_places<DT>();
     int buf = 0;
-    if (j_lo + wave < j_hi) load(j_lo + wave, 0);
+    if (j_lo + wave < j_hi) keys.next(lds_addr(lds[wave][0][0]), lds_addr(lds[wave][0][1]));
     for (int j = j_lo + wave; j < j_hi; j += 4, buf ^= 1) {
         wait_all();
-        if (j + 4 < j_hi) load(j + 4, buf ^ 1);
+        if (j + 4 < j_hi) keys.next(lds_addr(lds[wave][buf ^ 1][0]), lds_addr(lds[wave][buf ^ 1][1]));
         const int j0 = j * BN;
         fwd_tile<E, DT, 1>(st, q, at, lds_addr(lds[wave][buf][0]), lds_addr(lds[wave][buf][1]), cs, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next load writes it
@@ -542,7 +566,7 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
     // join the waves: each leaves its sums in its own LDS, [column][d] as fp32 (32 SP values, as 4 tiles hold)
     const float l = half_sum(st.l);
     if (lane < 32) {
-        sm[wave][lane] = st.top == -INFINITY ? -INFINITY : st.mc;
+        sm[wave][lane] = l == 0.0f ? -INFINITY : st.mc;
         sl[wave][lane] = l;
     }
     float * so = reinterpret_cast<float *>(&lds[wave][0][0][0]);
@@ -781,15 +805,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
     const int ta = uni(min(pw, np - 1) / p.R), tb = uni(min(pw + 31, np - 1) / p.R);
     const int some_lo = key_lo(p, c, ta), some_hi = key_hi(p, c, tb), all_lo = key_lo(p, c, tb), all_hi = key_hi(p, c, ta);
 
-    const char * kb = p.k.data + (int64_t) c.k0 * p.k.ts + g * p.k.hs;
-    const char * vb = p.v.data + (int64_t) c.k0 * p.v.ts + g * p.v.hs;
-    tile_loader<DT, BN, 256> lk(p.D), lv(p.D);
-    lk.rows_at(p.k.ts);
-    lv.rows_at(p.v.ts);
-    auto load = [&](int j, int buf) {
-        load_keys(lk, lds_addr(sk[buf]), kb, p.k.ts, j * BN, c.m, p.near_k);
-        load_keys(lv, lds_addr(sv[buf]), vb, p.v.ts, j * BN, c.m, p.near_k);
-    };
+    key_stream<DT, BN, 256> keys(p, c, g, j_lo * BN, BN);
     if (p.D != 32 * DT) {
         clear(sk, sizeof(sk), threadIdx.x, 256);
         clear(sv, sizeof(sv), threadIdx.x, 256);
@@ -800,12 +816,12 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
     for (int k = 0; k < DT; ++k) dq[k] = v16f{};
     const float cs = p.scale * LOG2E;
     const lane_at at = lane_places<DT>();
-    if (j_lo < j_hi) load(j_lo, 0);
+    if (j_lo < j_hi) keys.next(lds_addr(sk[0]), lds_addr(sv[0]));
     for (int j = j_lo; j < j_hi; ++j) {
         const int buf = (j - j_lo) & 1, j0 = j * BN;
         wait_all();
         barrier();
-        if (j + 1 < j_hi) load(j + 1, buf ^ 1);
+        if (j + 1 < j_hi) keys.next(lds_addr(sk[buf ^ 1]), lds_addr(sv[buf ^ 1]));
         if (!active || j0 >= some_hi || j0 + BN <= some_lo) continue;
         dq_tile<E, DT>(dq, q, go, at, lds_addr(sk[buf]), lds_addr(sv[buf]), cs, lse2, ndelta, factor, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
     }
