@@ -94,9 +94,9 @@ __device__ __forceinline__ void dma16(const void * g, uint32_t lds) {
 __device__ __forceinline__ void dma16s(const char * base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
-// 4 bytes per lane (lane l to lds + 4 l).
-__device__ __forceinline__ void dma4(const void * g, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(g), "s"(lds) : "memory", "m0");
+// 4 bytes per lane (lane l's at base + off_l to lds + 4 l).
+__device__ __forceinline__ void dma4s(const void * base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
 __device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -189,72 +189,82 @@ __device__ __forceinline__ constexpr int swz(int r) {
 template <int DT, int NR, int NT>
 struct tile_loader {
     static constexpr int CH = SP<DT> / 8, N = NR * CH / NT, STEP = NT / CH;
-    int r0, c0, D;
-    uint32_t off;              // of row r0 from the tile's base
+    int D;
+    uint32_t off;              // of the thread's first row r0 from the tile's base
     uint32_t wave_at;          // the wave's first row in the tile
     int64_t step;              // of STEP rows
 
+    static __device__ __forceinline__ int row_of(int t) { return (NT == 64 ? t & 63 : t) / CH; }
     // The chunk of the thread's k'th row, r0 + k STEP = r0 ^ k STEP.
-    __device__ __forceinline__ int chunk(int k) const { return c0 ^ swz<DT>(k * STEP); }
+    static __device__ __forceinline__ int chunk_of(int t, int k) { return (t % CH) ^ swz<DT>(row_of(t)) ^ swz<DT>(k * STEP); }
 
-    __device__ __forceinline__ tile_loader(int D_) : D(D_) {
-        const int t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
-        wave_at = NT == 64 ? 0 : uni((int) (threadIdx.x >> 6)) * 1024;
-        r0 = t / CH;
-        c0 = (t % CH) ^ swz<DT>(r0);
-    }
+    __device__ __forceinline__ tile_loader(int D_) : D(D_), wave_at(NT == 64 ? 0 : uni((int) (threadIdx.x >> 6)) * 1024) {}
     // Rows ts bytes apart; or pairs, R to a token (R divides STEP), heads hs bytes apart.
     __device__ __forceinline__ void rows_at(int64_t ts) {
-        off = (uint32_t) (r0 * ts);
+        off = (uint32_t) (row_of(threadIdx.x) * ts);
         step = STEP * ts;
     }
     __device__ __forceinline__ void pairs_at(int R, int64_t ts, int64_t hs) {
+        const int r0 = row_of(threadIdx.x);
         off = (uint32_t) (r0 / R * ts + r0 % R * hs);
         step = STEP / R * ts;
     }
     __device__ __forceinline__ void load(const char * base, uint32_t lds) const {
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (chunk(k) * 8 < D) dma16s(base + k * step, off + chunk(k) * 16, lds + wave_at + k * NT * 16);
+        for (int k = 0; k < N; ++k) {
+            const int c = chunk_of(threadIdx.x, k);
+            if (c * 8 < D) dma16s(base + k * step, off + c * 16, lds + wave_at + k * NT * 16);
+        }
     }
     // row r from src(r), zeros where that is null
     template <class Src>
     __device__ __forceinline__ void load_each(uint32_t lds, Src src) const {
+        int t = threadIdx.x;
+        asm volatile("" : "+v"(t));        // few tiles come here: nothing of it is kept in registers
 #pragma unroll 1
         for (int k = 0; k < N; ++k) {
-            const char * s = src(r0 + k * STEP);
-            if (chunk(k) * 8 < D) dma16(s ? s + chunk(k) * 16 : (const char *) zeros16, uni((int) (lds + wave_at + k * NT * 16)));
+            const char * s = src(row_of(t) + k * STEP);
+            const int c = chunk_of(t, k);
+            if (c * 8 < D) dma16(s ? s + c * 16 : (const char *) zeros16, uni((int) (lds + wave_at + k * NT * 16)));
         }
     }
 };
 
-// The tiles of a document's m keys one after another, K and V: the next one starts at key j0.
+// The tiles of a document's m keys one after another, K and V each by itself; K's start k_ahead keys further.
 template <int DT, int NR, int NT>
 struct key_stream {
     tile_loader<DT, NR, NT> lk, lv;
     const char * k, * v;       // of the next tile's first rows
-    int j0, m, step;           // keys from one tile to the next
+    int jk, jv, m, step;       // their keys; keys from one tile to the next
     int64_t kts, vts;
     bool near;
 
-    __device__ __forceinline__ key_stream(const attn_p & p, const doc & c, int g, int first, int step_)
-        : lk(p.D), lv(p.D), j0(first), m(c.m), step(step_), kts(p.k.ts), vts(p.v.ts), near(p.near_k) {
+    __device__ __forceinline__ key_stream(const attn_p & p, const doc & c, int g, int first, int step_, int k_ahead = 0)
+        : lk(p.D), lv(p.D), jk(first + k_ahead), jv(first), m(c.m), step(step_), kts(p.k.ts), vts(p.v.ts), near(p.near_k) {
         lk.rows_at(kts);
         lv.rows_at(vts);
-        k = uni(p.k.data + (c.k0 + (int64_t) first) * kts + g * p.k.hs);
-        v = uni(p.v.data + (c.k0 + (int64_t) first) * vts + g * p.v.hs);
+        k = uni(p.k.data + (c.k0 + (int64_t) jk) * kts + g * p.k.hs);
+        v = uni(p.v.data + (c.k0 + (int64_t) jv) * vts + g * p.v.hs);
+    }
+    __device__ __forceinline__ void next_k(uint32_t lds) {
+        if (near && jk + NR <= m) lk.load(k, lds);
+        else lk.load_each(lds, [&](int r) { return jk + r < m ? k + r * kts : nullptr; });
+        jk += step;
+        k += step * kts;
+    }
+    // the tile before the first, as far as it is within the document (with k_ahead)
+    __device__ __forceinline__ void first_k(uint32_t lds) {
+        lk.load_each(lds, [&](int r) { return (unsigned) (jk - step + r) < (unsigned) m ? k + (r - step) * kts : nullptr; });
+    }
+    __device__ __forceinline__ void next_v(uint32_t lds) {
+        if (near && jv + NR <= m) lv.load(v, lds);
+        else lv.load_each(lds, [&](int r) { return jv + r < m ? v + r * vts : nullptr; });
+        jv += step;
+        v += step * vts;
     }
     __device__ __forceinline__ void next(uint32_t lds_k, uint32_t lds_v) {
-        if (near && j0 + NR <= m) {
-            lk.load(k, lds_k);
-            lv.load(v, lds_v);
-        } else {
-            lk.load_each(lds_k, [&](int r) { return j0 + r < m ? k + r * kts : nullptr; });
-            lv.load_each(lds_v, [&](int r) { return j0 + r < m ? v + r * vts : nullptr; });
-        }
-        j0 += step;
-        k += step * kts;
-        v += step * vts;
+        next_k(lds_k);
+        next_v(lds_v);
     }
 };
 
@@ -381,55 +391,47 @@ struct fwd_state {
     }
 };
 
-// A tile's scores that may raise the reference: their sum with the old one past 2^14 (so P stays in either
-// type's range). The largest score is looked for in those tiles alone, the first and a few more.
+// A sum of weights past which the reference is raised: P stays in either type's range, and the largest score is
+// looked for in few tiles, the first and some after it.
 constexpr float RAISE = 16384.0f;
 
-// 32 NK keys of a tile. lo, hi: the lane's pair sees keys lo .. hi - 1 of the tile (with `mask` alone: a
-// tile that every pair sees has no masks).
-template <class E, int DT, int NK>
-__device__ __forceinline__ void fwd_tile(fwd_state<DT> & st, const typename type_of<E>::v8 (&q)[2 * DT], lane_at at, uint32_t kt,
-                                         uint32_t vt, float c, bool mask, int lo, int hi) {
-    typedef type_of<E> TY;
-    v16f s[NK];
-    auto scores = [&] {
-        // within the loop below, whose second turn is rare: nothing of it is to be computed before
-        uint32_t k_at = kt + at.row;
-        int l0 = lo - 4 * ((int) (threadIdx.x & 63) >> 5);
-        asm volatile("" : "+v"(k_at), "+v"(l0));
+// Scores of the wave's pairs with the 32 keys from row r0 of the tile.
+template <class E, int DT>
+__device__ __forceinline__ v16f fwd_scores(const typename type_of<E>::v8 (&q)[2 * DT], uint32_t kt, int r0) {
+    v16f s = {};
 #pragma unroll
-        for (int a = 0; a < NK; ++a) {
-            s[a] = v16f{};
+    for (int d = 0; d < 2 * DT; ++d) s = type_of<E>::mfma(row_operand<E, DT>(kt, r0, d), q[d], s);
+    return s;
+}
+
+// Scores outside the lane's keys lo .. hi - 1 of the 32: -inf.
+__device__ __forceinline__ void fwd_mask(v16f & s, int lo, int hi) {
+    const int l0 = lo - 4 * ((int) (threadIdx.x & 63) >> 5);
+    const unsigned n = hi > lo ? hi - lo : 0;
 #pragma unroll
-            for (int d = 0; d < 2 * DT; ++d) s[a] = TY::mfma(row_operand<E, DT>(k_at, 32 * a, d), q[d], s[a]);
-        }
-        if (mask) {
-            const unsigned n = hi > lo ? hi - lo : 0;
+    for (int i = 0; i < 16; ++i)
+        if ((unsigned) (reg_row(i) - l0) >= n) s[i] = -INFINITY;
+}
+
+__device__ __forceinline__ float fwd_exp(v16f & w, const v16f & s, float c, float mc) {
+    float t[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int a = 0; a < NK; ++a)
+    for (int i = 0; i < 16; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -mc));
+        t[i & 1] += w[i];
+    }
+    return t[0] + t[1];
+}
+
+// The weights of 32 keys from their scores, with a new reference where the old one is passed: the largest
+// score so far.
+template <int DT>
+__device__ __forceinline__ void fwd_weights(v16f & w, const v16f & s, fwd_state<DT> & st, float c) {
+    float t = fwd_exp(w, s, c, st.mc);
+    if (__any(!(t <= RAISE))) {
+        float mx = s[0];
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if ((unsigned) (32 * a + reg_row(i) - l0) >= n) s[a][i] = -INFINITY;
-        }
-    };
-    auto weights = [&](float mc) {
-        float t[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int a = 0; a < NK; ++a)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[a][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a][i], c, -mc));
-                t[i & 1] += s[a][i];
-            }
-        return t[0] + t[1];
-    };
-    // a new reference: the largest score so far
-    auto raise = [&] {
-        float mx = s[0][0];
-#pragma unroll
-        for (int a = 0; a < NK; ++a)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[a][i]);
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
         const float mc = fmaxf(st.mc, half_max(mx) * c);
         const float f = st.mc == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.mc - mc);
         st.mc = mc;
@@ -438,25 +440,26 @@ __device__ __forceinline__ void fwd_tile(fwd_state<DT> & st, const typename type
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) st.o[d][i] *= f;
-    };
-    float t;
-    for (bool up = __any(st.mc == -INFINITY);;) {
-        scores();
-        if (up) raise();
-        t = weights(st.mc == -INFINITY ? 0.0f : st.mc);
-        if (up || !__any(!(t <= RAISE))) break;
-        up = true;
+        t = fwd_exp(w, s, c, mc == -INFINITY ? 0.0f : mc);
     }
     st.l += t;
+}
+
+// o += V^T P^T for the 32 keys from row r0 of the tile.
+template <class E, int DT>
+__device__ __forceinline__ void fwd_values(fwd_state<DT> & st, const v16f & w, uint32_t vt, int r0) {
 #pragma unroll
-    for (int a = 0; a < 2 * NK; ++a) {
-        const typename TY::v8 pa = pack<E>(s[a / 2], a % 2);
+    for (int a = 0; a < 2; ++a) {
+        const typename type_of<E>::v8 pa = pack<E>(w, a);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) st.o[d] = TY::mfma(col_operand<E, DT>(vt + at.col, 16 * a, d), pa, st.o[d]);
+        for (int d = 0; d < DT; ++d) st.o[d] = type_of<E>::mfma(col_operand<E, DT>(vt, r0 + 16 * a, d), pa, st.o[d]);
     }
 }
 
-// A workgroup: 128 pairs of one document and KV head, a wave each 32 of them; 64 keys at a time.
+// A workgroup: 128 pairs of one document and KV head, a wave each 32 of them; 64 keys at a time. The scores of
+// the next 32 keys are computed beside the exponentials of these, which take about as long as both products:
+// K's tiles start 32 keys behind V's. Every wave takes every tile of the workgroup (the windows of its 128 pairs
+// differ by few keys), so that the loop has no branches between the products.
 template <class E, int DT>
 __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     constexpr int BM = 128, BN = 64, TILE = BN * SP<DT>;
@@ -469,7 +472,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     if (p0l < 0 || p0l >= np) return;
     const int p0 = uni((int) p0l);
 
-    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int pw = p0 + 32 * wave;
     const bool active = pw < np;
     const int pc = min(pw + (lane & 31), np - 1), tok = pc / p.R, head = g * p.R + pc % p.R;
@@ -481,9 +484,9 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     const int t_end = (min(p0 + BM, np) - 1) / p.R;
     const int j_lo = key_lo(p, c, p0 / p.R) / BN, j_hi = (key_hi(p, c, t_end) + BN - 1) / BN;
     const int ta = uni(min(pw, np - 1) / p.R), tb = uni(min(pw + 31, np - 1) / p.R);
-    const int some_lo = key_lo(p, c, ta), some_hi = key_hi(p, c, tb), all_lo = key_lo(p, c, tb), all_hi = key_hi(p, c, ta);
+    const int all_lo = key_lo(p, c, tb), all_hi = key_hi(p, c, ta);
 
-    key_stream<DT, BN, 256> keys(p, c, g, j_lo * BN, BN);
+    key_stream<DT, BN, 256> keys(p, c, g, j_lo * BN, BN, 32);
     if (p.D != 32 * DT) {
         clear(sk, sizeof(sk), threadIdx.x, 256);
         clear(sv, sizeof(sv), threadIdx.x, 256);
@@ -494,20 +497,40 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     st.init(lo < hi);
     const float cs = p.scale * LOG2E;
     const lane_at at = lane_places<DT>();
-    if (j_lo < j_hi) keys.next(lds_addr(sk[0]), lds_addr(sv[0]));
-    for (int j = j_lo; j < j_hi; ++j) {
-        const int buf = (j - j_lo) & 1, j0 = j * BN;
+    v16f s0, s1, w;
+    if (j_lo < j_hi) {
+        keys.first_k(lds_addr(sk[1]));
+        keys.next_k(lds_addr(sk[0]));
+        keys.next_v(lds_addr(sv[0]));
         wait_all();
         barrier();
-        if (j + 1 < j_hi) keys.next(lds_addr(sk[buf ^ 1]), lds_addr(sv[buf ^ 1]));
-        if (!active || j0 >= some_hi || j0 + BN <= some_lo) continue;
-        fwd_tile<E, DT, 2>(st, q, at, lds_addr(sk[buf]), lds_addr(sv[buf]), cs, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
+        s0 = fwd_scores<E, DT>(q, lds_addr(sk[1]) + at.row, 32);
+    }
+    for (int j = j_lo; j < j_hi; ++j) {
+        const int buf = (j - j_lo) & 1, j0 = j * BN;
+        const uint32_t kt = lds_addr(sk[buf]) + at.row, vt = lds_addr(sv[buf]) + at.col;
+        const bool mask = j0 < all_lo || j0 + BN > all_hi;
+        wait_all();
+        barrier();
+        if (j + 1 < j_hi) {
+            keys.next_k(lds_addr(sk[buf ^ 1]));
+            keys.next_v(lds_addr(sv[buf ^ 1]));
+        }
+        if (mask) fwd_mask(s0, lo - j0, hi - j0);
+        s1 = fwd_scores<E, DT>(q, kt, 0);
+        fwd_weights<DT>(w, s0, st, cs);
+        fwd_values<E, DT>(st, w, vt, 0);
+        if (mask) fwd_mask(s1, lo - j0 - 32, hi - j0 - 32);
+        s0 = fwd_scores<E, DT>(q, kt, 32);             // of the next tile's first keys
+        fwd_weights<DT>(w, s1, st, cs);
+        fwd_values<E, DT>(st, w, vt, 32);
     }
     barrier();
     if (!active) return;
     const float l = half_sum(st.l);
-    if (h == 0 && pw + lane < np) {
-        p.lse[(int64_t) (c.q0 + tok) * p.H + head] = LN2 * (st.mc + __builtin_amdgcn_logf(l));
+    if (lane < 32 && pw + lane < np) {
+        const int pr = pw + lane;
+        p.lse[(int64_t) (c.q0 + pr / p.R) * p.H + g * p.R + pr % p.R] = LN2 * (st.mc + __builtin_amdgcn_logf(l));
     }
     E * tile = (wave < 2 ? sk[0] : sv[0]) + (wave & 1) * 32 * SP<DT>;
     store_columns<E, DT>(tile, st.o, l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l), p.D, [&](int r) -> char * {
@@ -560,7 +583,10 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
         wait_all();
         if (j + 4 < j_hi) keys.next(lds_addr(lds[wave][buf ^ 1][0]), lds_addr(lds[wave][buf ^ 1][1]));
         const int j0 = j * BN;
-        fwd_tile<E, DT, 1>(st, q, at, lds_addr(lds[wave][buf][0]), lds_addr(lds[wave][buf][1]), cs, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
+v16f s = fwd_scores<E, DT>(q, lds_addr(lds[wave][buf][0]) + at.row, 0), w;
+        if (j0 < all_lo || j0 + BN > all_hi) fwd_mask(s, lo - j0, hi - j0);
+        fwd_weights<DT>(w, s, st, cs);
+        fwd_values<E, DT>(st, w, lds_addr(lds[wave][buf][1]) + at.col, 0);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next load writes it
     }
     // join the waves: each leaves its sums in its own LDS, [column][d] as fp32 (32 SP values, as 4 tiles hold)
@@ -920,7 +946,6 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dkv_kernel(attn_p p) {
     load_operand<E, DT>(v, p.v.data + (int64_t) (c.k0 + key) * p.v.ts + g * p.v.hs, p.D);
     const float factor = ds_factor<E>(p), ds_scale = type_of<E>::HALF ? ldexpf(factor, P_SHIFT) : 1.0f;
 
-    const int lo = tok_lo(p, c, key) * p.R, hi = tok_hi(p, c, key) * p.R;
     const int k_end = min(kb0 + BK, c.m) - 1;
     const int j_lo = tok_lo(p, c, kb0) * p.R / BQ, j_hi = (tok_hi(p, c, k_end) * p.R + BQ - 1) / BQ;
     const int ka = uni(min(kw, c.m - 1)), ke = uni(min(kw + 31, c.m - 1));
@@ -949,7 +974,12 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dkv_kernel(attn_p p) {
             l_out.load_each(lds_addr(so[buf]), [&](int r) { return at(p.dout, r); });
         }
         // the pairs' sums: waves 0 and 1, a value a lane (behind the document: whatever is there, masked)
-        if (wave < 2) dma4((wave ? p.ndelta : p.lse2) + ((int64_t) g * p.T_q + c.q0) * p.R + j0 + lane, lds_addr(wave ? s_delta[buf] : s_lse[buf]));
+        if (wave < 2) {
+            int t = threadIdx.x;
+            asm volatile("" : "+v"(t));
+            const float * from = (wave ? p.ndelta : p.lse2) + ((int64_t) g * p.T_q + c.q0) * p.R + j0;
+            dma4s(uni((const char *) from), (t & 63) * 4, lds_addr(wave ? s_delta[buf] : s_lse[buf]));
+        }
     };
     v16f dk[DT], dv[DT];
 #pragma unroll
@@ -964,10 +994,18 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dkv_kernel(attn_p p) {
         if (j + 1 < j_hi) load(j + 1, buf ^ 1);
         if (active && j0 < some_hi && j0 + BQ > some_lo) {
             const bool mask = j0 < all_lo || j0 + BQ > all_hi;
+            int lo = 0, hi = 0;
+            if (mask) {                // few tiles: the lane's bounds are not kept in registers
+                int t = threadIdx.x;
+                asm volatile("" : "+v"(t));
+                const int j = min(kw + (t & 31), c.m - 1);
+                lo = tok_lo(p, c, j) * p.R - j0;
+                hi = tok_hi(p, c, j) * p.R - j0;
+            }
 #pragma unroll 1
             for (int a = 0; a < BQ; a += 32) {
                 dkv_tile<E, DT>(dk, dv, k, v, at, lds_addr(sq[buf]) + a * SP<DT> * 2, lds_addr(so[buf]) + a * SP<DT> * 2, s_lse[buf] + a,
-                                s_delta[buf] + a, cs, factor, mask, lo - j0 - a, hi - j0 - a);
+                                s_delta[buf] + a, cs, factor, mask, lo - a, hi - a);
             }
         }
     }
