@@ -349,7 +349,9 @@ template <class E, int DT, class Dst>
 __device__ __forceinline__ void store_columns(E * tile, const v16f (&acc)[DT], float f, int D, Dst dst) {
     typedef E v4e __attribute__((ext_vector_type(4)));
     constexpr int CH = SP<DT> / 8;
-    const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));            // nothing of this is kept in registers over the loop before
+    const int col = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
 #pragma unroll
@@ -680,7 +682,7 @@ __global__ __launch_bounds__(256) void attn_rows_join_kernel(attn_p p) {
 // -delta = -sum(dout out) and log2 of the sums of each (token, head) row; for fp16 the largest squared norms of dout's and v's
 // rows, from which the gradients' kernels take the power of two that dS is carried with. 16 lanes a row.
 template <class E>
-__global__ __launch_bounds__(256) void attn_rows_delta_kernel(attn_p p) {
+__global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
     typedef typename type_of<E>::v8 v8;
     const int cc = threadIdx.x % 16, sub = threadIdx.x / 16;
     float top_o = 0.0f, top_v = 0.0f;
@@ -689,50 +691,68 @@ __global__ __launch_bounds__(256) void attn_rows_delta_kernel(attn_p p) {
         for (int k = 8; k; k >>= 1) x += __shfl_xor(x, k, 16);
         return x;
     };
-    const int64_t n_rows = (int64_t) p.T_q * p.H;
-    for (int64_t row = (int64_t) blockIdx.x * 16 + sub; row < n_rows; row += (int64_t) gridDim.x * 16) {
-        // in the order of lse2 and ndelta: a KV head's pairs one after another
-        const int64_t pr = row % ((int64_t) p.T_q * p.R), tok = pr / p.R, head = row / ((int64_t) p.T_q * p.R) * p.R + pr % p.R;
-        float s = 0.0f, n2 = 0.0f;
-        if (cc * 8 < p.D) {
-            const v8 a = *reinterpret_cast<const v8 *>(p.dout.data + tok * p.dout.ts + head * p.dout.hs + cc * 16);
-            const v8 b = *reinterpret_cast<const v8 *>(p.out.data + tok * p.out.ts + head * p.out.hs + cc * 16);
+    // in the order of lse2 and ndelta, a KV head's pairs one after another; two rows at a time under way
+    const int n_pairs = p.T_q * p.R, all = p.G * ((n_pairs + 127) / 128);
+    for (int w = blockIdx.x; w < all; w += gridDim.x) {
+        const int g = w % p.G, p0 = w / p.G * 128 + sub;
+        v8 a[2], b[2];
+        int64_t at[2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                s += (float) a[i] * (float) b[i];
-                n2 += (float) a[i] * (float) a[i];
+        for (int k = 0; k < 2; ++k) {
+            const int pr = p0 + 64 * k;
+            at[k] = -1;
+            if (pr >= n_pairs) continue;
+            const int64_t tok = pr / p.R, head = g * p.R + pr % p.R;
+            at[k] = tok * p.H + head;
+            if (cc * 8 < p.D) {
+                a[k] = *reinterpret_cast<const v8 *>(p.dout.data + tok * p.dout.ts + head * p.dout.hs + cc * 16);
+                b[k] = *reinterpret_cast<const v8 *>(p.out.data + tok * p.out.ts + head * p.out.hs + cc * 16);
             }
         }
-        s = sum16(s);
-        if (cc == 0) {
-            p.lse2[row] = p.lse[tok * p.H + head] * LOG2E - (type_of<E>::HALF ? P_SHIFT : 0);
-            p.ndelta[row] = -s;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (at[k] < 0) continue;          // the 16 lanes of a row alike
+            float s = 0.0f, n2 = 0.0f;
+            if (cc * 8 < p.D) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    s += (float) a[k][i] * (float) b[k][i];
+                    n2 += (float) a[k][i] * (float) a[k][i];
+                }
+            }
+            s = sum16(s);
+            if (cc == 0) {
+                const int64_t row = (int64_t) g * n_pairs + p0 + 64 * k;
+                p.lse2[row] = p.lse[at[k]] * LOG2E - (type_of<E>::HALF ? P_SHIFT : 0);
+                p.ndelta[row] = -s;
+            }
+            if (type_of<E>::HALF) top_o = fmaxf(top_o, sum16(n2));
         }
-        if (type_of<E>::HALF) top_o = fmaxf(top_o, sum16(n2));
     }
     if (!type_of<E>::HALF) return;
-    const int64_t n_v = (int64_t) p.T_k * p.G;
-    for (int64_t row = (int64_t) blockIdx.x * 16 + sub; row < n_v; row += (int64_t) gridDim.x * 16) {
+    const int n_v = p.T_k * p.G;
+    for (int64_t row = (int64_t) blockIdx.x * 64 + sub; row < n_v; row += (int64_t) gridDim.x * 64) {
         float n2 = 0.0f;
         if (cc * 8 < p.D) {
-            const v8 a = *reinterpret_cast<const v8 *>(p.v.data + row / p.G * p.v.ts + row % p.G * p.v.hs + cc * 16);
+            const int tok = (int) row / p.G, g = (int) row % p.G;
+            const v8 a = *reinterpret_cast<const v8 *>(p.v.data + tok * p.v.ts + g * p.v.hs + cc * 16);
 #pragma unroll
             for (int i = 0; i < 8; ++i) n2 += (float) a[i] * (float) a[i];
         }
         top_v = fmaxf(top_v, sum16(n2));
     }
-    __shared__ float so[16], sv[16];
+    __shared__ float so[64], sv[64];
     if (cc == 0) {
         so[sub] = top_o;
         sv[sub] = top_v;
     }
     __syncthreads();
-    if (threadIdx.x < 16) {
+    if (threadIdx.x < 64) {
         float a = so[threadIdx.x], b = sv[threadIdx.x];
 #pragma unroll
-        for (int k = 8; k; k >>= 1) {
-            a = fmaxf(a, __shfl_xor(a, k, 16));
-            b = fmaxf(b, __shfl_xor(b, k, 16));
+        for (int k = 32; k; k >>= 1) {
+            a = fmaxf(a, __shfl_xor(a, k));
+            b = fmaxf(b, __shfl_xor(b, k));
         }
         if (threadIdx.x == 0) {
             p.maxima[2 * blockIdx.x] = a;
@@ -925,11 +945,15 @@ __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const t
     }
 }
 
-template <class E, int DT>
-__global__ __launch_bounds__(256, 2) void attn_rows_dkv_kernel(attn_p p) {
-    constexpr int BK = 128, BQ = 64, TILE = BQ * SP<DT>;
+// A workgroup: 128 keys, 4 waves of 32; QG groups of waves with the same keys take every QG'th 32 pairs and
+// add their sums at the end. One group, several workgroups a CU: a workgroup's start and end hide behind the
+// others. QG groups, one workgroup a CU: for launches that fit the CUs at once, where it would be a CU's longest
+// workgroup, alone at the end with a quarter of the waves, that takes the time.
+template <class E, int DT, int QG>
+__global__ __launch_bounds__(256 * QG, 2) void attn_rows_dkv_kernel(attn_p p) {
+    constexpr int BK = 128, SUB = QG == 1 ? 2 : 1, BQ = 32 * QG * SUB, TILE = BQ * SP<DT>;
     __shared__ __align__(1024) E sq[2][TILE], so[2][TILE];
-    __shared__ __align__(16) float s_lse[2][BQ], s_delta[2][BQ];
+    __shared__ __align__(16) float s_lse[2][128], s_delta[2][128];       // BQ of them used
     const int g = blockIdx.x % p.G, slot = blockIdx.x / p.G;
     const int d = find_doc(p.cu_k, p.n_seqs, p.T_k, 1, BK, slot);
     const doc c = doc_of(p, d);
@@ -937,7 +961,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dkv_kernel(attn_p p) {
     if (kl < 0 || kl >= c.m) return;
     const int kb0 = uni((int) kl), np = c.n * p.R;
 
-    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wave = uni(threadIdx.x >> 6) % 4, group = uni(threadIdx.x >> 8), lane = threadIdx.x & 63;
     const int kw = kb0 + 32 * wave;
     const bool active = kw < c.m;
     const int key = min(kw + (lane & 31), c.m - 1);
@@ -952,12 +976,12 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dkv_kernel(attn_p p) {
     const int some_lo = tok_lo(p, c, ka) * p.R, some_hi = tok_hi(p, c, ke) * p.R;
     const int all_lo = tok_lo(p, c, ke) * p.R, all_hi = tok_hi(p, c, ka) * p.R;
 
-    tile_loader<DT, BQ, 256> lq(p.D), l_out(p.D);
+    tile_loader<DT, BQ, 256 * QG> lq(p.D), l_out(p.D);
     lq.pairs_at(p.R, p.q.ts, p.q.hs);
     l_out.pairs_at(p.R, p.dout.ts, p.dout.hs);
     if (p.D != 32 * DT) {
-        clear(sq, sizeof(sq), threadIdx.x, 256);
-        clear(so, sizeof(so), threadIdx.x, 256);
+        clear(sq, sizeof(sq), threadIdx.x, 256 * QG);
+        clear(so, sizeof(so), threadIdx.x, 256 * QG);
         barrier();
     }
     auto load = [&](int j, int buf) {
@@ -973,12 +997,12 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dkv_kernel(attn_p p) {
             lq.load_each(lds_addr(sq[buf]), [&](int r) { return at(p.q, r); });
             l_out.load_each(lds_addr(so[buf]), [&](int r) { return at(p.dout, r); });
         }
-        // the pairs' sums: waves 0 and 1, a value a lane (behind the document: whatever is there, masked)
-        if (wave < 2) {
+        // the pairs' sums, 64 a wave (behind the document: whatever is there, masked)
+        if (group == 0 && wave < 2 * ((BQ + 63) / 64)) {
             int t = threadIdx.x;
             asm volatile("" : "+v"(t));
-            const float * from = (wave ? p.ndelta : p.lse2) + ((int64_t) g * p.T_q + c.q0) * p.R + j0;
-            dma4s(uni((const char *) from), (t & 63) * 4, lds_addr(wave ? s_delta[buf] : s_lse[buf]));
+            const float * from = (wave & 1 ? p.ndelta : p.lse2) + ((int64_t) g * p.T_q + c.q0) * p.R + j0 + (wave >> 1) * 64;
+            dma4s(uni((const char *) from), (t & 63) * 4, lds_addr((wave & 1 ? s_delta[buf] : s_lse[buf]) + (wave >> 1) * 64));
         }
     };
     v16f dk[DT], dv[DT];
@@ -1003,13 +1027,48 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dkv_kernel(attn_p p) {
                 hi = tok_hi(p, c, j) * p.R - j0;
             }
 #pragma unroll 1
-            for (int a = 0; a < BQ; a += 32) {
+            for (int a = 32 * SUB * group; a < 32 * SUB * (group + 1); a += 32) {
                 dkv_tile<E, DT>(dk, dv, k, v, at, lds_addr(sq[buf]) + a * SP<DT> * 2, lds_addr(so[buf]) + a * SP<DT> * 2, s_lse[buf] + a,
                                 s_delta[buf] + a, cs, factor, mask, lo - a, hi - a);
             }
         }
     }
     barrier();
+    if constexpr (QG > 1) {
+        // the groups' sums one after another into the first's, through LDS
+        int t = threadIdx.x;
+        asm volatile("" : "+v"(t));            // not kept in a register over the loop
+        float * sums = reinterpret_cast<float *>(wave < 2 ? sq : so) + (wave & 1) * DT * 16 * 64 + (t & 63) * 4;
+        static_assert(2 * DT * 16 * 64 * 4 <= (int) sizeof(sq), "two waves' sums in half of the tiles");
+        auto join = [&](v16f (&x)[DT]) {
+#pragma unroll
+            for (int q = 1; q < QG; ++q) {
+                if (group == q) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *reinterpret_cast<v4f *>(sums + (4 * d + i) * 256) = v4f{x[d][4 * i], x[d][4 * i + 1], x[d][4 * i + 2], x[d][4 * i + 3]};
+                }
+                barrier();
+                if (group == 0) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const v4f y = *reinterpret_cast<const v4f *>(sums + (4 * d + i) * 256);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) x[d][4 * i + k] += y[k];
+                            if (i & 1) __builtin_amdgcn_sched_barrier(0);      // not all reads at once: registers
+                        }
+                }
+                barrier();
+            }
+        };
+        join(dv);
+        join(dk);
+        if (group) return;
+    }
     if (!active) return;
     E * tile = (wave < 2 ? sq[0] : so[0]) + (wave & 1) * 32 * SP<DT>;
     auto dst = [&](const rows & x) {
@@ -1057,7 +1116,7 @@ int32_t check_params(const char * what, const nxg_attention_rows_params * a, att
     p.scale = a->scale;
     p.cu_q = a->cu_q;
     p.cu_k = a->cu_k;
-    if ((int64_t) p.T_q * p.R > INT32_MAX - 256 ||
+    if ((int64_t) p.T_q * p.H > INT32_MAX - 256 || (int64_t) p.T_k * p.G > INT32_MAX ||
         (slots(p.T_q, p.R, 32, p.n_seqs)) * p.G > INT32_MAX / 64 || slots(p.T_k, 1, 128, p.n_seqs) * p.G > INT32_MAX) {
         return nxg_fail(NXG_EINVAL, "%s: T_q=%d T_k=%d of %d heads is too large", what, p.T_q, p.T_k, p.H);
     }
@@ -1098,21 +1157,24 @@ int32_t check_rows(const char * what, const char * name, const nxg_rows * x, int
 #define NXG_TRY(call) do { const int32_t rc_ = (call); if (rc_) return rc_; } while (0)
 
 // Values of a row array of the backward pass: one a (token, head), and a tile's reach behind the last.
-int64_t row_values(const attn_p & p) { return (int64_t) p.T_q * p.H + 64; }
+int64_t row_values(const attn_p & p) { return (int64_t) p.T_q * p.H + 128; }
 int64_t backward_bytes(const attn_p & p) { return (2 * N_MAX + 2 * row_values(p)) * 4; }
 
+// dK, dV: launches of at most this many workgroups a CU take several groups of waves for one.
+constexpr unsigned DKV_GROUPS = 3;
+
 // Launches one of a kernel's instances by type and head size.
-#define NXG_BY_TYPE(type, D, LAUNCH)                                               \
+#define NXG_BY_TYPE(type, D, ...)                                                  \
     do {                                                                           \
-        if ((type) == NXG_TYPE_BF16) { typedef __bf16 E; NXG_BY_DIM(D, LAUNCH); }  \
-        else { typedef _Float16 E; NXG_BY_DIM(D, LAUNCH); }                        \
+        if ((type) == NXG_TYPE_BF16) { typedef __bf16 E; NXG_BY_DIM(D, __VA_ARGS__); }  \
+        else { typedef _Float16 E; NXG_BY_DIM(D, __VA_ARGS__); }                   \
     } while (0)
-#define NXG_BY_DIM(D, LAUNCH)                                                      \
+#define NXG_BY_DIM(D, ...)                                                         \
     do {                                                                           \
-        if ((D) <= 32) { constexpr int DT = 1; LAUNCH; }                           \
-        else if ((D) <= 64) { constexpr int DT = 2; LAUNCH; }                      \
-        else if ((D) <= 96) { constexpr int DT = 3; LAUNCH; }                      \
-        else { constexpr int DT = 4; LAUNCH; }                                     \
+        if ((D) <= 32) { constexpr int DT = 1; __VA_ARGS__; }                           \
+        else if ((D) <= 64) { constexpr int DT = 2; __VA_ARGS__; }                      \
+        else if ((D) <= 96) { constexpr int DT = 3; __VA_ARGS__; }                      \
+        else { constexpr int DT = 4; __VA_ARGS__; }                                     \
     } while (0)
 
 // The few-pairs kernel where tiles of 128 pairs would leave most CUs idle, its keys split until there are
@@ -1224,10 +1286,10 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
     hipStream_t s = (hipStream_t) stream;
     if (p.T_q > 0) {
         if (a->type == NXG_TYPE_BF16) {
-            const int64_t n = ((int64_t) p.T_q * p.H + 15) / 16;
-            attn_rows_delta_kernel<__bf16><<<(unsigned) std::min<int64_t>(n, 8 * N_MAX), 256, 0, s>>>(p);
+            const int64_t n = ((int64_t) p.T_q * p.R + 127) / 128 * p.G;
+            attn_rows_delta_kernel<__bf16><<<(unsigned) std::min<int64_t>(n, 4 * N_MAX), 1024, 0, s>>>(p);
         } else {
-            attn_rows_delta_kernel<_Float16><<<N_MAX, 256, 0, s>>>(p);
+            attn_rows_delta_kernel<_Float16><<<N_MAX, 1024, 0, s>>>(p);
         }
         NXG_TRY(nxg_launch_check(what));
         p.n_slots = (int32_t) slots(p.T_q, p.R, 128, p.n_seqs);
@@ -1236,7 +1298,13 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
     }
     if (p.T_k > 0) {
         p.n_slots = (int32_t) slots(p.T_k, 1, 128, p.n_seqs);
-        NXG_BY_TYPE(a->type, p.D, (attn_rows_dkv_kernel<E, DT><<<(unsigned) (p.n_slots * p.G), 256, 0, s>>>(p)));
+        const unsigned grid = (unsigned) (p.n_slots * p.G);
+        const bool groups = grid <= DKV_GROUPS * (unsigned) nxg_device_cus();
+        NXG_BY_TYPE(a->type, p.D, {
+            constexpr int QG = DT <= 2 ? 3 : 2;
+            if (groups) attn_rows_dkv_kernel<E, DT, QG><<<grid, 256 * QG, 0, s>>>(p);
+            else attn_rows_dkv_kernel<E, DT, 1><<<grid, 256, 0, s>>>(p);
+        });
         NXG_TRY(nxg_launch_check(what));
     }
     return NXG_OK;
