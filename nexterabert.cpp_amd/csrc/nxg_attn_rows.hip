@@ -74,7 +74,7 @@ struct attn_p {
     float * maxima;            // [N_MAX][2]: largest |dout row|^2 and |v row|^2 (fp16)
     float * part;              // partial sums of the split forward pass
     const int32_t * cu_q, * cu_k;
-    int32_t n_seqs, T_q, T_k, H, G, R, D, left, right, n_slots, n_split;
+    int32_t n_seqs, T_q, T_k, H, G, R, D, left, right, n_slots, n_split, order;
     float scale;
     bool near_k, near_q;       // a tile's rows are within 32-bit offsets of its first (of q and dout: and lie alike in every tile)
 };
@@ -152,6 +152,108 @@ __device__ __forceinline__ doc doc_of(const attn_p & p, int d) {
     r.m = uni(max(offset(p.cu_k, d + 1, p.T_k) - r.k0, 0));
     return r;
 }
+
+// Sum of the lanes up to this one.
+__device__ __forceinline__ int scan64(int x) {
+#define NXG_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false)
+    NXG_STEP(0x111, 0xf);      // row_shr 1, 2, 4, 8
+    NXG_STEP(0x112, 0xf);
+    NXG_STEP(0x114, 0xf);
+    NXG_STEP(0x118, 0xf);
+    NXG_STEP(0x142, 0xa);      // row_bcast 15, 31
+    NXG_STEP(0x143, 0xc);
+#undef NXG_STEP
+    return x;
+}
+
+// What a workgroup does: a tile (BM query-head pairs, or keys) of a document.
+struct job {
+    doc c;
+    int tile;                  // -1: nothing
+};
+
+// The order of a launch's workgroups, so that the last to start are short ones.
+enum { BY_ROWS, BY_LENGTH, BY_LEVEL };
+
+// The slot's job. A document has ceil(len mul / size) tiles, by its queries or its keys (by_keys). BY_ROWS: slots as
+// find_doc() gives them. For up to 64 documents, a lane each: BY_LENGTH takes the longest documents first
+// (full windows: a tile's work is its document's length), BY_LEVEL the tiles with the most work of all documents
+// first (windows open on one side: a tile's work is its number, from the end where from_end).
+__device__ __forceinline__ job find_job(const attn_p & p, bool by_keys, int mul, int size, int slot, int order, bool from_end) {
+    job r;
+    r.tile = -1;
+    const int32_t * cu = by_keys ? p.cu_k : p.cu_q;
+    const int T = by_keys ? p.T_k : p.T_q;
+    if (order == BY_ROWS || p.n_seqs > 64) {
+        const int d = find_doc(cu, p.n_seqs, T, mul, size, slot);
+        r.c = doc_of(p, d);
+        const int64_t at = slot - slot_of(cu, d, T, mul, size);
+        const int64_t len = (int64_t) (by_keys ? r.c.m : r.c.n) * mul;
+        if (at >= 0 && at * size < len) r.tile = uni((int) (from_end ? (len + size - 1) / size - 1 - at : at));
+        return r;
+    }
+    const int lane = threadIdx.x & 63, d = min(lane, p.n_seqs - 1);
+    const int q0 = offset(p.cu_q, d, p.T_q), n = max(offset(p.cu_q, d + 1, p.T_q) - q0, 0);
+    const int k0 = offset(p.cu_k, d, p.T_k), m = max(offset(p.cu_k, d + 1, p.T_k) - k0, 0);
+    const int count = lane < p.n_seqs ? (int) (((int64_t) (by_keys ? m : n) * mul + size - 1) / size) : 0;
+    int rank = 0;              // documents of more tiles, or as many and before this one
+    for (int j = 0; j < p.n_seqs; ++j) {
+        const int cj = __builtin_amdgcn_readlane(count, j);
+        rank += cj > count || (cj == count && j < lane);
+    }
+    if (lane >= p.n_seqs) rank = lane;
+    const int c = __builtin_amdgcn_ds_permute(rank << 2, count);       // lane r: the r'th most
+    const int upto = scan64(c);
+    int doc_rank, tile;
+    if (order == BY_LENGTH) {
+        const uint64_t here = __ballot(slot < upto);
+        if (!here) return r;
+        doc_rank = __builtin_ctzll(here);
+        tile = slot - (__builtin_amdgcn_readlane(upto, doc_rank) - __builtin_amdgcn_readlane(c, doc_rank));
+    } else {
+        // tiles of the first r + 1 documents above the next one's count
+        const int next = lane < 63 ? __shfl_down(c, 1) : 0;
+        const int above = upto - (lane + 1) * next;
+        const uint64_t here = __ballot(slot < above);
+        if (!here) return r;
+        const int last = __builtin_ctzll(here);
+        const int k = slot - (last ? __builtin_amdgcn_readlane(above, last - 1) : 0);
+        tile = __builtin_amdgcn_readlane(c, last) - 1 - k / (last + 1);
+        doc_rank = k % (last + 1);
+    }
+    const int at = __builtin_ctzll(__ballot(rank == doc_rank));
+    if (from_end && order == BY_LEVEL) tile = __builtin_amdgcn_readlane(count, at) - 1 - tile;
+    r.c.q0 = __builtin_amdgcn_readlane(q0, at);
+    r.c.n = __builtin_amdgcn_readlane(n, at);
+    r.c.k0 = __builtin_amdgcn_readlane(k0, at);
+    r.c.m = __builtin_amdgcn_readlane(m, at);
+    r.tile = uni(tile);
+    return r;
+}
+
+// The same for a whole workgroup: found by its first wave, through LDS (with a barrier).
+__device__ __forceinline__ job workgroup_job(const attn_p & p, bool by_keys, int mul, int size, int slot, bool from_end, int * lds) {
+    if (p.order == BY_ROWS) return find_job(p, by_keys, mul, size, slot, BY_ROWS, from_end);
+    if (uni(threadIdx.x >> 6) == 0) {
+        const job f = find_job(p, by_keys, mul, size, slot, p.order, from_end);
+        if (threadIdx.x == 0) {
+            lds[0] = f.c.q0;
+            lds[1] = f.c.n;
+            lds[2] = f.c.k0;
+            lds[3] = f.c.m;
+            lds[4] = f.tile;
+        }
+    }
+    barrier();
+    job r;
+    r.c.q0 = uni(lds[0]);
+    r.c.n = uni(lds[1]);
+    r.c.k0 = uni(lds[2]);
+    r.c.m = uni(lds[3]);
+    r.tile = uni(lds[4]);
+    return r;
+}
+
 // The keys lo .. hi - 1 of query token t.
 __device__ __forceinline__ int key_lo(const attn_p & p, const doc & c, int t) {
     return p.left < 0 ? 0 : min(max(t + c.m - c.n - p.left, 0), c.m);
@@ -315,6 +417,22 @@ __device__ __forceinline__ typename type_of<E>::v8 col_operand(uint32_t at, int 
 // Register i of lane l of a 32x32 result is row 8 (i / 4) + 4 (l / 32) + i % 4 of column l % 32.
 __device__ __forceinline__ constexpr int reg_row(int i) { return 8 * (i / 4) + i % 4; }
 
+// Sets the registers whose row is not in the lane's lo .. hi - 1 to x; sides: 1 if a row may be below lo, 2 if one may be
+// past hi (of the wave's 32 columns; at no side most tiles).
+__device__ __forceinline__ void mask_rows(v16f & s, int sides, int lo, int hi, float x) {
+    const int h4 = 4 * ((int) (threadIdx.x & 63) >> 5);
+    if (sides & 1) {
+        const int l = lo - h4;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = reg_row(i) < l ? x : s[i];
+    }
+    if (sides & 2) {
+        const int l = hi - h4;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = reg_row(i) >= l ? x : s[i];
+    }
+}
+
 // Registers 8 a .. 8 a + 7 as the operand of the next product.
 template <class E>
 __device__ __forceinline__ typename type_of<E>::v8 pack(const v16f & x, int a) {
@@ -406,21 +524,12 @@ __device__ __forceinline__ v16f fwd_scores(const typename type_of<E>::v8 (&q)[2 
     return s;
 }
 
-// Scores outside the lane's keys lo .. hi - 1 of the 32: -inf.
-__device__ __forceinline__ void fwd_mask(v16f & s, int lo, int hi) {
-    const int l0 = lo - 4 * ((int) (threadIdx.x & 63) >> 5);
-    const unsigned n = hi > lo ? hi - lo : 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if ((unsigned) (reg_row(i) - l0) >= n) s[i] = -INFINITY;
-}
-
 __device__ __forceinline__ float fwd_exp(v16f & w, const v16f & s, float c, float mc) {
-    float t[2] = {0.0f, 0.0f};
+    float t[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -mc));
-        t[i & 1] += w[i];
+        t[i & 1] = i < 2 ? w[i] : t[i & 1] + w[i];
     }
     return t[0] + t[1];
 }
@@ -466,13 +575,12 @@ template <class E, int DT>
 __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     constexpr int BM = 128, BN = 64, TILE = BN * SP<DT>;
     __shared__ __align__(1024) E sk[2][TILE], sv[2][TILE];
-    const int g = blockIdx.x % p.G, slot = p.n_slots - 1 - blockIdx.x / p.G;
-    const int d = find_doc(p.cu_q, p.n_seqs, p.T_q, p.R, BM, slot);
-    const doc c = doc_of(p, d);
-    const int64_t p0l = (slot - slot_of(p.cu_q, d, p.T_q, p.R, BM)) * BM;
-    const int np = c.n * p.R;
-    if (p0l < 0 || p0l >= np) return;
-    const int p0 = uni((int) p0l);
+    __shared__ int s_job[8];
+    const int g = blockIdx.x % p.G;
+    const job todo = workgroup_job(p, false, p.R, BM, blockIdx.x / p.G, p.right >= 0 ? p.order == BY_ROWS : p.left >= 0 && p.order != BY_ROWS, s_job);
+    if (todo.tile < 0) return;
+    const doc c = todo.c;
+    const int np = c.n * p.R, p0 = todo.tile * BM;
 
     const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int pw = p0 + 32 * wave;
@@ -511,18 +619,18 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     for (int j = j_lo; j < j_hi; ++j) {
         const int buf = (j - j_lo) & 1, j0 = j * BN;
         const uint32_t kt = lds_addr(sk[buf]) + at.row, vt = lds_addr(sv[buf]) + at.col;
-        const bool mask = j0 < all_lo || j0 + BN > all_hi;
+        const int sides = (j0 < all_lo ? 1 : 0) | (j0 + BN > all_hi ? 2 : 0);
         wait_all();
         barrier();
         if (j + 1 < j_hi) {
             keys.next_k(lds_addr(sk[buf ^ 1]));
             keys.next_v(lds_addr(sv[buf ^ 1]));
         }
-        if (mask) fwd_mask(s0, lo - j0, hi - j0);
+        if (sides) mask_rows(s0, sides, lo - j0, hi - j0, -INFINITY);
         s1 = fwd_scores<E, DT>(q, kt, 0);
         fwd_weights<DT>(w, s0, st, cs);
         fwd_values<E, DT>(st, w, vt, 0);
-        if (mask) fwd_mask(s1, lo - j0 - 32, hi - j0 - 32);
+        if (sides) mask_rows(s1, sides, lo - j0 - 32, hi - j0 - 32, -INFINITY);
         s0 = fwd_scores<E, DT>(q, kt, 32);             // of the next tile's first keys
         fwd_weights<DT>(w, s1, st, cs);
         fwd_values<E, DT>(st, w, vt, 32);
@@ -551,12 +659,10 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
     __shared__ __align__(1024) E lds[4][2][2][TILE];       // wave, buffer, K or V
     __shared__ float sm[4][32], sl[4][32];
     const int g = blockIdx.x % p.G, rest = blockIdx.x / p.G, split = rest % p.n_split, slot = rest / p.n_split;
-    const int d = find_doc(p.cu_q, p.n_seqs, p.T_q, p.R, BM, slot);
-    const doc c = doc_of(p, d);
-    const int64_t p0l = (slot - slot_of(p.cu_q, d, p.T_q, p.R, BM)) * BM;
-    const int np = c.n * p.R;
-    if (p0l < 0 || p0l >= np) return;
-    const int p0 = uni((int) p0l);
+    const job todo = find_job(p, false, p.R, BM, slot, BY_ROWS, false);
+    if (todo.tile < 0) return;
+    const doc c = todo.c;
+    const int np = c.n * p.R, p0 = todo.tile * BM;
 
     const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int pc = min(p0 + (lane & 31), np - 1), tok = pc / p.R, head = g * p.R + pc % p.R;
@@ -586,7 +692,8 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
         if (j + 4 < j_hi) keys.next(lds_addr(lds[wave][buf ^ 1][0]), lds_addr(lds[wave][buf ^ 1][1]));
         const int j0 = j * BN;
 v16f s = fwd_scores<E, DT>(q, lds_addr(lds[wave][buf][0]) + at.row, 0), w;
-        if (j0 < all_lo || j0 + BN > all_hi) fwd_mask(s, lo - j0, hi - j0);
+        const int sides = (j0 < all_lo ? 1 : 0) | (j0 + BN > all_hi ? 2 : 0);
+        if (sides) mask_rows(s, sides, lo - j0, hi - j0, -INFINITY);
         fwd_weights<DT>(w, s, st, cs);
         fwd_values<E, DT>(st, w, lds_addr(lds[wave][buf][1]) + at.col, 0);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next load writes it
@@ -680,26 +787,28 @@ __global__ __launch_bounds__(256) void attn_rows_join_kernel(attn_p p) {
 // ---------------------------------------------------------------------------
 
 // -delta = -sum(dout out) and log2 of the sums of each (token, head) row; for fp16 the largest squared norms of dout's and v's
-// rows, from which the gradients' kernels take the power of two that dS is carried with. 16 lanes a row.
-template <class E>
+// rows, from which the gradients' kernels take the power of two that dS is carried with. L lanes a row (8 for heads of
+// up to 64).
+template <class E, int L>
 __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
     typedef typename type_of<E>::v8 v8;
-    const int cc = threadIdx.x % 16, sub = threadIdx.x / 16;
+    constexpr int ROWS = 1024 / L;
+    const int cc = threadIdx.x % L, sub = threadIdx.x / L;
     float top_o = 0.0f, top_v = 0.0f;
-    auto sum16 = [](float x) {
+    auto sum = [](float x) {
 #pragma unroll
-        for (int k = 8; k; k >>= 1) x += __shfl_xor(x, k, 16);
+        for (int k = L / 2; k; k >>= 1) x += __shfl_xor(x, k, L);
         return x;
     };
     // in the order of lse2 and ndelta, a KV head's pairs one after another; two rows at a time under way
-    const int n_pairs = p.T_q * p.R, all = p.G * ((n_pairs + 127) / 128);
+    const int n_pairs = p.T_q * p.R, all = p.G * ((n_pairs + 2 * ROWS - 1) / (2 * ROWS));
     for (int w = blockIdx.x; w < all; w += gridDim.x) {
-        const int g = w % p.G, p0 = w / p.G * 128 + sub;
+        const int g = w % p.G, p0 = w / p.G * (2 * ROWS) + sub;
         v8 a[2], b[2];
         int64_t at[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const int pr = p0 + 64 * k;
+            const int pr = p0 + ROWS * k;
             at[k] = -1;
             if (pr >= n_pairs) continue;
             const int64_t tok = pr / p.R, head = g * p.R + pr % p.R;
@@ -711,7 +820,7 @@ __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            if (at[k] < 0) continue;          // the 16 lanes of a row alike
+            if (at[k] < 0) continue;          // a row's lanes alike
             float s = 0.0f, n2 = 0.0f;
             if (cc * 8 < p.D) {
 #pragma unroll
@@ -720,18 +829,18 @@ __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
                     n2 += (float) a[k][i] * (float) a[k][i];
                 }
             }
-            s = sum16(s);
+            s = sum(s);
             if (cc == 0) {
-                const int64_t row = (int64_t) g * n_pairs + p0 + 64 * k;
+                const int64_t row = (int64_t) g * n_pairs + p0 + ROWS * k;
                 p.lse2[row] = p.lse[at[k]] * LOG2E - (type_of<E>::HALF ? P_SHIFT : 0);
                 p.ndelta[row] = -s;
             }
-            if (type_of<E>::HALF) top_o = fmaxf(top_o, sum16(n2));
+            if (type_of<E>::HALF) top_o = fmaxf(top_o, sum(n2));
         }
     }
     if (!type_of<E>::HALF) return;
     const int n_v = p.T_k * p.G;
-    for (int64_t row = (int64_t) blockIdx.x * 64 + sub; row < n_v; row += (int64_t) gridDim.x * 64) {
+    for (int64_t row = (int64_t) blockIdx.x * ROWS + sub; row < n_v; row += (int64_t) gridDim.x * ROWS) {
         float n2 = 0.0f;
         if (cc * 8 < p.D) {
             const int tok = (int) row / p.G, g = (int) row % p.G;
@@ -739,9 +848,9 @@ __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) n2 += (float) a[i] * (float) a[i];
         }
-        top_v = fmaxf(top_v, sum16(n2));
+        top_v = fmaxf(top_v, sum(n2));
     }
-    __shared__ float so[64], sv[64];
+    __shared__ float so[ROWS], sv[ROWS];
     if (cc == 0) {
         so[sub] = top_o;
         sv[sub] = top_v;
@@ -749,6 +858,10 @@ __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
     __syncthreads();
     if (threadIdx.x < 64) {
         float a = so[threadIdx.x], b = sv[threadIdx.x];
+        if (ROWS > 64) {
+            a = fmaxf(a, so[threadIdx.x + ROWS - 64]);
+            b = fmaxf(b, sv[threadIdx.x + ROWS - 64]);
+        }
 #pragma unroll
         for (int k = 32; k; k >>= 1) {
             a = fmaxf(a, __shfl_xor(a, k));
@@ -789,9 +902,8 @@ __device__ __forceinline__ float ds_factor(const attn_p & p) {
 template <class E, int DT>
 __device__ __forceinline__ void dq_tile(v16f (&dq)[DT], const typename type_of<E>::v8 (&q)[2 * DT],
                                         const typename type_of<E>::v8 (&go)[2 * DT], lane_at at, uint32_t kt, uint32_t vt, float c,
-                                        float lse2, float ndelta, float factor, bool mask, int lo, int hi) {
+                                        float lse2, float ndelta, float factor, int sides, int lo, int hi) {
     typedef type_of<E> TY;
-    const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
         v16f s = {}, dp = {};
@@ -805,13 +917,7 @@ __device__ __forceinline__ void dq_tile(v16f (&dq)[DT], const typename type_of<E
             s[i] = pr * (dp[i] + ndelta);
             if (TY::HALF) s[i] *= factor;
         }
-        if (mask) {
-            const int l0 = lo - 4 * h;
-            const unsigned n = hi > lo ? hi - lo : 0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if ((unsigned) (32 * a + reg_row(i) - l0) >= n) s[i] = 0.0f;
-        }
+        if (sides) mask_rows(s, sides, lo - 32 * a, hi - 32 * a, 0.0f);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const typename TY::v8 ds = pack<E>(s, b);
@@ -825,13 +931,12 @@ template <class E, int DT>
 __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
     constexpr int BM = 128, BN = 64, TILE = BN * SP<DT>;
     __shared__ __align__(1024) E sk[2][TILE], sv[2][TILE];
-    const int g = blockIdx.x % p.G, slot = p.n_slots - 1 - blockIdx.x / p.G;
-    const int d = find_doc(p.cu_q, p.n_seqs, p.T_q, p.R, BM, slot);
-    const doc c = doc_of(p, d);
-    const int64_t p0l = (slot - slot_of(p.cu_q, d, p.T_q, p.R, BM)) * BM;
-    const int np = c.n * p.R;
-    if (p0l < 0 || p0l >= np) return;
-    const int p0 = uni((int) p0l);
+    __shared__ int s_job[8];
+    const int g = blockIdx.x % p.G;
+    const job todo = workgroup_job(p, false, p.R, BM, blockIdx.x / p.G, p.right >= 0 ? p.order == BY_ROWS : p.left >= 0 && p.order != BY_ROWS, s_job);
+    if (todo.tile < 0) return;
+    const doc c = todo.c;
+    const int np = c.n * p.R, p0 = todo.tile * BM;
 
     const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int pw = p0 + 32 * wave;
@@ -869,7 +974,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
         barrier();
         if (j + 1 < j_hi) keys.next(lds_addr(sk[buf ^ 1]), lds_addr(sv[buf ^ 1]));
         if (!active || j0 >= some_hi || j0 + BN <= some_lo) continue;
-        dq_tile<E, DT>(dq, q, go, at, lds_addr(sk[buf]), lds_addr(sv[buf]), cs, lse2, ndelta, factor, j0 < all_lo || j0 + BN > all_hi, lo - j0, hi - j0);
+        dq_tile<E, DT>(dq, q, go, at, lds_addr(sk[buf]), lds_addr(sv[buf]), cs, lse2, ndelta, factor, (j0 < all_lo ? 1 : 0) | (j0 + BN > all_hi ? 2 : 0), lo - j0, hi - j0);
     }
     barrier();
     if (!active) return;
@@ -896,20 +1001,21 @@ __device__ __forceinline__ void reads_ahead() {
 }
 
 // dK, dV: a wave has 32 keys, the workgroup goes over the pairs that see its 128, 64 at a time, a wave 32 at a
-// time: qt, ot their rows of q and dout, lse2, ndelta their sums, pairs lo .. hi - 1 of them seen by the key.
+// time: qt, ot their rows of q and dout, lse2, ndelta (LDS addresses as well) their sums, pairs lo .. hi - 1 of them seen by the key.
 template <class E, int DT>
 __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const typename type_of<E>::v8 (&k)[2 * DT],
                                          const typename type_of<E>::v8 (&v)[2 * DT], lane_at at, uint32_t qt, uint32_t ot,
-                                         const float * lse2, const float * ndelta, float c, float factor, bool mask, int lo, int hi) {
+                                         uint32_t lse2, uint32_t ndelta, float c, float factor, int sides, int lo, int hi) {
     typedef type_of<E> TY;
-    const int h = (threadIdx.x & 63) >> 5;
+    typedef __attribute__((address_space(3))) v4f lds_v4f;
+    const uint32_t h16 = (threadIdx.x & 32) >> 1;      // 4 values for the second half wave
     v16f s = {}, dp;
 #pragma unroll
     for (int d = 0; d < 2 * DT; ++d) s = TY::mfma(row_operand<E, DT>(qt + at.row, 0, d), k[d], s);
     if (DT >= 3) reads_ahead<2 * DT>();
 #pragma unroll
     for (int i4 = 0; i4 < 4; ++i4) {              // dP - delta: the sums start there
-        const v4f de = *reinterpret_cast<const v4f *>(ndelta + 8 * i4 + 4 * h);
+        const v4f de = *(lds_v4f *) (uintptr_t) (ndelta + h16 + 32 * i4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) dp[4 * i4 + j] = de[j];
     }
@@ -918,7 +1024,7 @@ __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const t
     if (DT >= 3) reads_ahead<2 * DT>();
 #pragma unroll
     for (int i4 = 0; i4 < 4; ++i4) {
-        const v4f ls = *reinterpret_cast<const v4f *>(lse2 + 8 * i4 + 4 * h);
+        const v4f ls = *(lds_v4f *) (uintptr_t) (lse2 + h16 + 32 * i4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int i = 4 * i4 + j;
@@ -927,12 +1033,9 @@ __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const t
             if (TY::HALF) dp[i] *= factor;
         }
     }
-    if (mask) {
-        const int l0 = lo - 4 * h;
-        const unsigned n = hi > lo ? hi - lo : 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if ((unsigned) (reg_row(i) - l0) >= n) s[i] = dp[i] = 0.0f;
+    if (sides) {
+        mask_rows(s, sides, lo, hi, 0.0f);
+        mask_rows(dp, sides, lo, hi, 0.0f);
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -954,12 +1057,12 @@ __global__ __launch_bounds__(256 * QG, 2) void attn_rows_dkv_kernel(attn_p p) {
     constexpr int BK = 128, SUB = QG == 1 ? 2 : 1, BQ = 32 * QG * SUB, TILE = BQ * SP<DT>;
     __shared__ __align__(1024) E sq[2][TILE], so[2][TILE];
     __shared__ __align__(16) float s_lse[2][128], s_delta[2][128];       // BQ of them used
-    const int g = blockIdx.x % p.G, slot = blockIdx.x / p.G;
-    const int d = find_doc(p.cu_k, p.n_seqs, p.T_k, 1, BK, slot);
-    const doc c = doc_of(p, d);
-    const int64_t kl = (slot - slot_of(p.cu_k, d, p.T_k, 1, BK)) * BK;
-    if (kl < 0 || kl >= c.m) return;
-    const int kb0 = uni((int) kl), np = c.n * p.R;
+    __shared__ int s_job[8];
+    const int g = blockIdx.x % p.G;
+    const job todo = workgroup_job(p, true, 1, BK, blockIdx.x / p.G, p.right >= 0 && p.order != BY_ROWS, s_job);
+    if (todo.tile < 0) return;
+    const doc c = todo.c;
+    const int np = c.n * p.R, kb0 = todo.tile * BK;
 
     const int wave = uni(threadIdx.x >> 6) % 4, group = uni(threadIdx.x >> 8), lane = threadIdx.x & 63;
     const int kw = kb0 + 32 * wave;
@@ -1017,9 +1120,9 @@ __global__ __launch_bounds__(256 * QG, 2) void attn_rows_dkv_kernel(attn_p p) {
         barrier();
         if (j + 1 < j_hi) load(j + 1, buf ^ 1);
         if (active && j0 < some_hi && j0 + BQ > some_lo) {
-            const bool mask = j0 < all_lo || j0 + BQ > all_hi;
+            const int sides = (j0 < all_lo ? 1 : 0) | (j0 + BQ > all_hi ? 2 : 0);
             int lo = 0, hi = 0;
-            if (mask) {                // few tiles: the lane's bounds are not kept in registers
+            if (sides) {               // few tiles: the lane's bounds are not kept in registers
                 int t = threadIdx.x;
                 asm volatile("" : "+v"(t));
                 const int j = min(kw + (t & 31), c.m - 1);
@@ -1028,8 +1131,8 @@ __global__ __launch_bounds__(256 * QG, 2) void attn_rows_dkv_kernel(attn_p p) {
             }
 #pragma unroll 1
             for (int a = 32 * SUB * group; a < 32 * SUB * (group + 1); a += 32) {
-                dkv_tile<E, DT>(dk, dv, k, v, at, lds_addr(sq[buf]) + a * SP<DT> * 2, lds_addr(so[buf]) + a * SP<DT> * 2, s_lse[buf] + a,
-                                s_delta[buf] + a, cs, factor, mask, lo - a, hi - a);
+                dkv_tile<E, DT>(dk, dv, k, v, at, lds_addr(sq[buf]) + a * SP<DT> * 2, lds_addr(so[buf]) + a * SP<DT> * 2, lds_addr(s_lse[buf]) + 4 * a,
+                                lds_addr(s_delta[buf]) + 4 * a, cs, factor, sides, lo - a, hi - a);
             }
         }
     }
@@ -1160,9 +1263,6 @@ int32_t check_rows(const char * what, const char * name, const nxg_rows * x, int
 int64_t row_values(const attn_p & p) { return (int64_t) p.T_q * p.H + 128; }
 int64_t backward_bytes(const attn_p & p) { return (2 * N_MAX + 2 * row_values(p)) * 4; }
 
-// dK, dV: launches of at most this many workgroups a CU take several groups of waves for one.
-constexpr unsigned DKV_GROUPS = 3;
-
 // Launches one of a kernel's instances by type and head size.
 #define NXG_BY_TYPE(type, D, ...)                                                  \
     do {                                                                           \
@@ -1176,6 +1276,13 @@ constexpr unsigned DKV_GROUPS = 3;
         else if ((D) <= 96) { constexpr int DT = 3; __VA_ARGS__; }                      \
         else { constexpr int DT = 4; __VA_ARGS__; }                                     \
     } while (0)
+
+// Documents in the order of their rows where the workgroups fit the CUs at once, where there is one
+// document or more than a wave has lanes, or where every tile's work is alike.
+int work_order(const attn_p & p, int64_t workgroups) {
+    if (p.n_seqs < 2 || p.n_seqs > 64 || workgroups <= 2 * nxg_device_cus() || (p.left >= 0 && p.right >= 0)) return BY_ROWS;
+    return p.left < 0 && p.right < 0 ? BY_LENGTH : BY_LEVEL;
+}
 
 // The few-pairs kernel where tiles of 128 pairs would leave most CUs idle, its keys split until there are
 // two workgroups a CU, 256 keys of the average document at least to each.
@@ -1244,6 +1351,7 @@ int32_t nxg_attention_rows(const nxg_attention_rows_params * a, const nxg_rows *
         else attn_rows_join_kernel<_Float16><<<rows_grid, 256, 0, s>>>(p);
         return nxg_launch_check(what);
     }
+    p.order = work_order(p, grid);
     NXG_BY_TYPE(a->type, p.D, (attn_rows_fwd_kernel<E, DT><<<grid, 256, 0, s>>>(p)));
     return nxg_launch_check(what);
 }
@@ -1285,21 +1393,29 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
     p.ndelta = p.lse2 + row_values(p);
     hipStream_t s = (hipStream_t) stream;
     if (p.T_q > 0) {
+        const int L = p.D <= 64 ? 8 : 16;
+        const int64_t n = ((int64_t) p.T_q * p.R + 2048 / L - 1) / (2048 / L) * p.G;
         if (a->type == NXG_TYPE_BF16) {
-            const int64_t n = ((int64_t) p.T_q * p.R + 127) / 128 * p.G;
-            attn_rows_delta_kernel<__bf16><<<(unsigned) std::min<int64_t>(n, 4 * N_MAX), 1024, 0, s>>>(p);
+            const unsigned grid = (unsigned) std::min<int64_t>(n, 4 * N_MAX);
+            if (L == 8) attn_rows_delta_kernel<__bf16, 8><<<grid, 1024, 0, s>>>(p);
+            else attn_rows_delta_kernel<__bf16, 16><<<grid, 1024, 0, s>>>(p);
         } else {
-            attn_rows_delta_kernel<_Float16><<<N_MAX, 1024, 0, s>>>(p);
+            if (L == 8) attn_rows_delta_kernel<_Float16, 8><<<N_MAX, 1024, 0, s>>>(p);
+            else attn_rows_delta_kernel<_Float16, 16><<<N_MAX, 1024, 0, s>>>(p);
         }
         NXG_TRY(nxg_launch_check(what));
         p.n_slots = (int32_t) slots(p.T_q, p.R, 128, p.n_seqs);
+        p.order = work_order(p, (int64_t) p.n_slots * p.G);
         NXG_BY_TYPE(a->type, p.D, (attn_rows_dq_kernel<E, DT><<<(unsigned) (p.n_slots * p.G), 256, 0, s>>>(p)));
         NXG_TRY(nxg_launch_check(what));
     }
     if (p.T_k > 0) {
         p.n_slots = (int32_t) slots(p.T_k, 1, 128, p.n_seqs);
         const unsigned grid = (unsigned) (p.n_slots * p.G);
-        const bool groups = grid <= DKV_GROUPS * (unsigned) nxg_device_cus();
+        p.order = work_order(p, grid);
+        // documents' ends differ in work where one side of the window is open and the other not
+        const bool uneven = (p.left < 0) != (p.right < 0);
+        const bool groups = grid <= (uneven ? 3u : 1u) * (unsigned) nxg_device_cus();
         NXG_BY_TYPE(a->type, p.D, {
             constexpr int QG = DT <= 2 ? 3 : 2;
             if (groups) attn_rows_dkv_kernel<E, DT, QG><<<grid, 256 * QG, 0, s>>>(p);
