@@ -492,6 +492,88 @@ __device__ __forceinline__ void store_columns(E * tile, const v16f (&acc)[DT], f
 }
 
 // ---------------------------------------------------------------------------
+// sums taken again
+// ---------------------------------------------------------------------------
+//
+// A product over a tile takes in every row of it, those that a pair does not see with weight 0. If such a row
+// holds an infinity or a NaN, 0 times it is NaN. So a result that is not finite, where rows that some
+// pair of the wave does not see hold such values, is taken again from the definition, over the seen rows alone.
+// That costs nothing until it happens.
+
+// Bit c: column c of the wave's sums (both half waves) is not finite.
+template <int DT>
+__device__ __forceinline__ uint32_t bad_columns(const v16f (&x)[DT]) {
+    float z = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z = __builtin_fmaf(x[d][i], 0.0f, z);
+    const uint64_t b = __ballot(z != 0.0f || z != z);
+    return (uint32_t) b | (uint32_t) (b >> 32);
+}
+
+// Does any of the rows a .. b - 1 hold a value that is not finite? row(i): its D values.
+template <class E, class Row>
+__device__ __forceinline__ bool holds_bad(int a, int b, int D, Row row) {
+    const int lane = threadIdx.x & 63, chunks = D / 8;
+    bool bad = false;
+    for (int i = lane; i < (b - a) * chunks; i += 64) {
+        const typename type_of<E>::v8 x = *reinterpret_cast<const typename type_of<E>::v8 *>(row(a + i / chunks) + i % chunks * 16);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) bad |= !(fabsf((float) x[k]) < INFINITY);
+    }
+    return __any(bad);
+}
+
+template <class E>
+__device__ __forceinline__ float dot(const char * a, const char * b, int D) {
+    float s = 0.0f;
+    for (int d = 0; d < D; d += 8) {
+        const typename type_of<E>::v8 x = *reinterpret_cast<const typename type_of<E>::v8 *>(a + 2 * d);
+        const typename type_of<E>::v8 y = *reinterpret_cast<const typename type_of<E>::v8 *>(b + 2 * d);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s = __builtin_fmaf((float) x[k], (float) y[k], s);
+    }
+    return s;
+}
+
+// The wave's sum over j in a .. b - 1 of weight(j) times row(j): lane l has values l and 64 + l. lds: 64 floats.
+template <class E, class Weight, class Row>
+__device__ __forceinline__ void add_rows(float (&x)[2], int a, int b, int D, float * lds, Weight weight, Row row) {
+    const int lane = threadIdx.x & 63;
+    for (int j = a; j < b; j += 64) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        lds[lane] = j + lane < b ? weight(j + lane) : 0.0f;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int k = 0; k < min(64, b - j); ++k) {
+            const E * r = reinterpret_cast<const E *>(row(j + k));
+            const float w = lds[k];
+            if (lane < D) x[0] += w * (float) r[lane];
+            if (64 + lane < D) x[1] += w * (float) r[64 + lane];
+        }
+    }
+}
+
+template <class E>
+__device__ __forceinline__ void store_row(char * to, const float (&x)[2], float f, int D) {
+    const int lane = threadIdx.x & 63;
+    E * o = reinterpret_cast<E *>(to);
+    if (lane < D) o[lane] = (E) (x[0] * f);
+    if (64 + lane < D) o[64 + lane] = (E) (x[1] * f);
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int k = 32; k; k >>= 1) x = fmaxf(x, __shfl_xor(x, k));
+    return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int k = 32; k; k >>= 1) x += __shfl_xor(x, k);
+    return x;
+}
+
+// ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
 
@@ -565,6 +647,32 @@ __device__ __forceinline__ void fwd_values(fwd_state<DT> & st, const v16f & w, u
 #pragma unroll
         for (int d = 0; d < DT; ++d) st.o[d] = type_of<E>::mfma(col_operand<E, DT>(vt, r0 + 16 * a, d), pa, st.o[d]);
     }
+}
+
+// One pair's sums again, over its keys among the tiles first, first + step, ... below end of `size` keys: mc, l (its
+// whole sum) and o as in fwd_state, lane l with o's values l and 64 + l.
+template <class E>
+__device__ __forceinline__ void fwd_again(const attn_p & p, const doc & c, int g, int pair, int first, int step, int end, int size,
+                                          float * lds, float & mc, float & l, float (&o)[2]) {
+    const int tok = pair / p.R, head = g * p.R + pair % p.R, lane = threadIdx.x & 63;
+    const int lo = key_lo(p, c, tok), hi = key_hi(p, c, tok);
+    const char * q = p.q.data + (c.q0 + tok) * p.q.ts + head * p.q.hs;
+    const char * k = p.k.data + c.k0 * p.k.ts + g * p.k.hs, * v = p.v.data + c.k0 * p.v.ts + g * p.v.hs;
+    const float cs = p.scale * LOG2E;
+    float mx = -INFINITY, t = 0.0f;
+    for (int j = first; j < end; j += step)
+        for (int i = max(j * size, lo) + lane; i < min((j + 1) * size, hi); i += 64) mx = fmaxf(mx, dot<E>(q, k + i * p.k.ts, p.D));
+    mx = wave_max(mx) * cs;
+    mc = mx == -INFINITY ? 0.0f : mx;
+    o[0] = o[1] = 0.0f;
+    for (int j = first; j < end; j += step) {
+        add_rows<E>(o, max(j * size, lo), min((j + 1) * size, hi), p.D, lds, [&](int i) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(dot<E>(q, k + i * p.k.ts, p.D), cs, -mc));
+            t += w;
+            return w;
+        }, [&](int i) { return v + i * p.v.ts; });
+    }
+    l = wave_sum(t);
 }
 
 // A workgroup: 128 pairs of one document and KV head, a wave each 32 of them; 64 keys at a time. The scores of
@@ -643,11 +751,23 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
         p.lse[(int64_t) (c.q0 + pr / p.R) * p.H + g * p.R + pr % p.R] = LN2 * (st.mc + __builtin_amdgcn_logf(l));
     }
     E * tile = (wave < 2 ? sk[0] : sv[0]) + (wave & 1) * 32 * SP<DT>;
+    uint32_t bad = bad_columns<DT>(st.o);
     store_columns<E, DT>(tile, st.o, l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l), p.D, [&](int r) -> char * {
         const int pr = pw + r;
         if (pr >= np) return nullptr;
         return p.out.data + (int64_t) (c.q0 + pr / p.R) * p.out.ts + (g * p.R + pr % p.R) * p.out.hs;
     });
+    if (!bad) return;
+    auto v_row = [&](int j) { return p.v.data + (int64_t) (c.k0 + j) * p.v.ts + g * p.v.hs; };
+    if (!holds_bad<E>(j_lo * BN, min(all_lo, c.m), p.D, v_row) && !holds_bad<E>(max(all_hi, 0), min(j_hi * BN, c.m), p.D, v_row)) return;
+    for (; bad; bad &= bad - 1) {
+        const int pair = pw + __builtin_ctz(bad);
+        if (pair >= np) break;
+        float mc, l, o[2];
+        fwd_again<E>(p, c, g, pair, j_lo, 1, j_hi, BN, reinterpret_cast<float *>(tile), mc, l, o);
+        store_row<E>(p.out.data + (int64_t) (c.q0 + pair / p.R) * p.out.ts + (g * p.R + pair % p.R) * p.out.hs, o,
+                     l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l), p.D);
+    }
 }
 
 // Few pairs: a workgroup takes 32 of them, its four waves every fourth 32 keys of the split's share, each through
@@ -657,7 +777,7 @@ template <class E, int DT>
 __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
     constexpr int BM = 32, BN = 32, TILE = BN * SP<DT>;
     __shared__ __align__(1024) E lds[4][2][2][TILE];       // wave, buffer, K or V
-    __shared__ float sm[4][32], sl[4][32];
+    __shared__ float sm[4][32], sl[4][32], s_weights[4][64];
     const int g = blockIdx.x % p.G, rest = blockIdx.x / p.G, split = rest % p.n_split, slot = rest / p.n_split;
     const job todo = find_job(p, false, p.R, BM, slot, BY_ROWS, false);
     if (todo.tile < 0) return;
@@ -712,6 +832,23 @@ v16f s = fwd_scores<E, DT>(q, lds_addr(lds[wave][buf][0]) + at.row, 0), w;
             const v4f x = {st.o[k][4 * i], st.o[k][4 * i + 1], st.o[k][4 * i + 2], st.o[k][4 * i + 3]};
             *reinterpret_cast<v4f *>(so + (lane & 31) * SP<DT> + 32 * k + 8 * i + 4 * (lane >> 5)) = x;
         }
+    if (uint32_t bad = bad_columns<DT>(st.o)) {
+        auto v_row = [&](int j) { return p.v.data + (int64_t) (c.k0 + j) * p.v.ts + g * p.v.hs; };
+        if (holds_bad<E>(t_lo * BN, min(all_lo, c.m), p.D, v_row) || holds_bad<E>(max(all_hi, 0), min(t_hi * BN, c.m), p.D, v_row)) {
+            for (; bad; bad &= bad - 1) {
+                const int col = __builtin_ctz(bad);
+                if (p0 + col >= np) break;
+                float mc, l, o[2];
+                fwd_again<E>(p, c, g, p0 + col, j_lo + wave, 4, j_hi, BN, s_weights[wave], mc, l, o);
+                if (lane == 0) {
+                    sm[wave][col] = l == 0.0f ? -INFINITY : mc;
+                    sl[wave][col] = l;
+                }
+                so[col * SP<DT> + lane] = o[0];
+                if (SP<DT> > 64) so[col * SP<DT> + 64 + lane] = o[1];
+            }
+        }
+    }
     barrier();
     constexpr int CH = SP<DT> / 8;
     constexpr int WAVE_F = 2 * 2 * TILE / 2;                // floats of a wave's LDS
@@ -800,6 +937,9 @@ __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
         for (int k = L / 2; k; k >>= 1) x += __shfl_xor(x, k, L);
         return x;
     };
+    // the largest norms: of documents' rows alone
+    const int q_lo = offset(p.cu_q, 0, p.T_q), q_hi = offset(p.cu_q, p.n_seqs, p.T_q);
+    const int k_lo = offset(p.cu_k, 0, p.T_k), k_hi = offset(p.cu_k, p.n_seqs, p.T_k);
     // in the order of lse2 and ndelta, a KV head's pairs one after another; two rows at a time under way
     const int n_pairs = p.T_q * p.R, all = p.G * ((n_pairs + 2 * ROWS - 1) / (2 * ROWS));
     for (int w = blockIdx.x; w < all; w += gridDim.x) {
@@ -835,12 +975,16 @@ __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
                 p.lse2[row] = p.lse[at[k]] * LOG2E - (type_of<E>::HALF ? P_SHIFT : 0);
                 p.ndelta[row] = -s;
             }
-            if (type_of<E>::HALF) top_o = fmaxf(top_o, sum(n2));
+            if (type_of<E>::HALF) {
+                const int tok = (p0 + ROWS * k) / p.R;
+                n2 = sum(n2);
+                if (tok >= q_lo && tok < q_hi) top_o = fmaxf(top_o, n2);
+            }
         }
     }
     if (!type_of<E>::HALF) return;
-    const int n_v = p.T_k * p.G;
-    for (int64_t row = (int64_t) blockIdx.x * ROWS + sub; row < n_v; row += (int64_t) gridDim.x * ROWS) {
+    const int n_v = k_hi * p.G;
+    for (int64_t row = (int64_t) k_lo * p.G + (int64_t) blockIdx.x * ROWS + sub; row < n_v; row += (int64_t) gridDim.x * ROWS) {
         float n2 = 0.0f;
         if (cc * 8 < p.D) {
             const int tok = (int) row / p.G, g = (int) row % p.G;
@@ -927,6 +1071,25 @@ __device__ __forceinline__ void dq_tile(v16f (&dq)[DT], const typename type_of<E
     }
 }
 
+// P and dS of a pair and a key from the definition.
+struct weights {
+    float p, ds;
+};
+template <class E>
+__device__ __forceinline__ weights weights_of(const attn_p & p, const doc & c, int g, int pair, const char * k, const char * v) {
+    const int tok = pair / p.R, head = g * p.R + pair % p.R;
+    const int64_t row = ((int64_t) g * p.T_q + c.q0) * p.R + pair;
+    const char * q = p.q.data + (c.q0 + tok) * p.q.ts + head * p.q.hs, * d = p.dout.data + (c.q0 + tok) * p.dout.ts + head * p.dout.hs;
+    weights w;
+    w.p = __builtin_amdgcn_exp2f(dot<E>(q, k, p.D) * p.scale * LOG2E - (p.lse2[row] + (type_of<E>::HALF ? P_SHIFT : 0)));
+    w.ds = w.p * (dot<E>(d, v, p.D) + p.ndelta[row]);
+    return w;
+}
+template <class E, class K, class V>
+__device__ __forceinline__ void add_ds(float (&x)[2], const attn_p & p, const doc & c, int g, int pair, int lo, int hi, float * lds, K k_row, V v_row) {
+    add_rows<E>(x, lo, hi, p.D, lds, [&](int j) { return weights_of<E>(p, c, g, pair, k_row(j), v_row(j)).ds; }, k_row);
+}
+
 template <class E, int DT>
 __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
     constexpr int BM = 128, BN = 64, TILE = BN * SP<DT>;
@@ -979,11 +1142,24 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
     barrier();
     if (!active) return;
     E * tile = (wave < 2 ? sk[0] : sv[0]) + (wave & 1) * 32 * SP<DT>;
+    uint32_t bad = bad_columns<DT>(dq);
     store_columns<E, DT>(tile, dq, p.scale / ds_scale, p.D, [&](int r) -> char * {
         const int pr = pw + r;
         if (pr >= np) return nullptr;
         return p.dq.data + (int64_t) (c.q0 + pr / p.R) * p.dq.ts + (g * p.R + pr % p.R) * p.dq.hs;
     });
+    if (!bad) return;
+    auto k_row = [&](int j) { return p.k.data + (int64_t) (c.k0 + j) * p.k.ts + g * p.k.hs; };
+    auto v_row = [&](int j) { return p.v.data + (int64_t) (c.k0 + j) * p.v.ts + g * p.v.hs; };
+    if (!holds_bad<E>(j_lo * BN, min(all_lo, c.m), p.D, k_row) && !holds_bad<E>(max(all_hi, 0), min(j_hi * BN, c.m), p.D, k_row)) return;
+    for (; bad; bad &= bad - 1) {
+        const int pair = pw + __builtin_ctz(bad);
+        if (pair >= np) break;
+        float x[2] = {0.0f, 0.0f};
+        const int t = pair / p.R;
+        add_ds<E>(x, p, c, g, pair, key_lo(p, c, t), key_hi(p, c, t), reinterpret_cast<float *>(tile), k_row, v_row);
+        store_row<E>(p.dq.data + (int64_t) (c.q0 + t) * p.dq.ts + (g * p.R + pair % p.R) * p.dq.hs, x, p.scale, p.D);
+    }
 }
 
 // Ends a phase of N products of one LDS read each, with two reads ahead of the products: more would not
@@ -1177,9 +1353,28 @@ __global__ __launch_bounds__(256 * QG, 2) void attn_rows_dkv_kernel(attn_p p) {
     auto dst = [&](const rows & x) {
         return [&, x](int r) -> char * { return kw + r < c.m ? x.data + (int64_t) (c.k0 + kw + r) * x.ts + g * x.hs : nullptr; };
     };
+    uint32_t bad = bad_columns<DT>(dv) | bad_columns<DT>(dk);
     store_columns<E, DT>(tile, dv, type_of<E>::HALF ? 1.0f / (1 << P_SHIFT) : 1.0f, p.D, dst(p.dv));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     store_columns<E, DT>(tile, dk, p.scale / ds_scale, p.D, dst(p.dk));
+    if (!bad) return;
+    auto pair_row = [&](const rows & x) {
+        return [&, x](int pr) { return (const char *) x.data + (int64_t) (c.q0 + pr / p.R) * x.ts + (g * p.R + pr % p.R) * x.hs; };
+    };
+    const int a0 = j_lo * BQ, a1 = min(all_lo, np), b0 = max(all_hi, 0), b1 = min(j_hi * BQ, np);
+    if (!holds_bad<E>(a0, a1, p.D, pair_row(p.q)) && !holds_bad<E>(a0, a1, p.D, pair_row(p.dout)) &&
+        !holds_bad<E>(b0, b1, p.D, pair_row(p.q)) && !holds_bad<E>(b0, b1, p.D, pair_row(p.dout))) return;
+    for (; bad; bad &= bad - 1) {
+        const int j = kw + __builtin_ctz(bad);
+        if (j >= c.m) break;
+        const char * k_row = p.k.data + (int64_t) (c.k0 + j) * p.k.ts + g * p.k.hs, * v_row = p.v.data + (int64_t) (c.k0 + j) * p.v.ts + g * p.v.hs;
+        const int lo = tok_lo(p, c, j) * p.R, hi = tok_hi(p, c, j) * p.R;
+        float x[2] = {0.0f, 0.0f}, y[2] = {0.0f, 0.0f};
+        add_rows<E>(x, lo, hi, p.D, reinterpret_cast<float *>(tile), [&](int pr) { return weights_of<E>(p, c, g, pr, k_row, v_row).p; }, pair_row(p.dout));
+        add_rows<E>(y, lo, hi, p.D, reinterpret_cast<float *>(tile), [&](int pr) { return weights_of<E>(p, c, g, pr, k_row, v_row).ds; }, pair_row(p.q));
+        store_row<E>(p.dv.data + (int64_t) (c.k0 + j) * p.dv.ts + g * p.dv.hs, x, 1.0f, p.D);
+        store_row<E>(p.dk.data + (int64_t) (c.k0 + j) * p.dk.ts + g * p.dk.hs, y, p.scale, p.D);
+    }
 }
 
 // ---------------------------------------------------------------------------

@@ -255,3 +255,35 @@ def test_against_differences(nxg, torch, dev):
         bound = float((rows_ref.attention(q, k, v, cu, cu, 0.125, -1, 0, do)[("dq", "dk", "dv")[i]][1] * step.double().abs()).sum())
         # the difference's own third-order term: 2^-20 of the values here
         assert abs(diff - want) <= bound + 2.0 ** -16, (i, diff, want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,G,lens,at", [(4, 2, [70, 20], [69, 40]), (4, 2, [300], [0, 150, 299]), (16, 16, [2100], [1000, 2099])])
+def test_forward_leaves_out_what_is_not_seen(nxg, torch, dev, dtype, H, G, lens, at):
+    """NaN and infinities in keys and values: only the queries that see them feel them (few-pairs kernel,
+    and 128 pairs a workgroup)."""
+    say(f"attention_rows {dtype} {lens}: NaN and infinities at {at}")
+    dt = getattr(torch, dtype)
+    for left, right in ((-1, 0), (10, 0), (40, 40), (5, -1)):
+        q, k, v, _ = make(torch, dt, lens, lens, H, G, 64, 3)
+        for i, t in enumerate(at):
+            v[t, :, i::7] = math.inf if i % 2 else math.nan
+            if i % 2 == 0:
+                k[t, :, 5] = math.nan
+        run_and_check(nxg, torch, dt, lens, H=H, G=G, left=left, right=right, inputs=(q, k, v, None), grad=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", ["q", "k", "v", "dout"])
+def test_gradients_leave_out_what_is_not_seen(nxg, torch, dev, dtype, D, bad):
+    """A token's NaN (in one input) reaches the gradients of the tokens that it sees or that see it, and what
+    those touch, and no others."""
+    say(f"attention_rows_backward {dtype} D={D}: NaN in {bad}")
+    dt = getattr(torch, dtype)
+    lens = [150, 75]
+    for left, right in ((-1, 0), (7, 7), (12, 0), (0, 3)):
+        tensors = dict(zip(("q", "k", "v", "dout"), make(torch, dt, lens, lens, 4, 2, D, 5)))
+        for t in (100, 149, 160):
+            tensors[bad][t] = math.nan
+        run_and_check(nxg, torch, dt, lens, H=4, G=2, D=D, left=left, right=right, inputs=tuple(tensors.values()))
