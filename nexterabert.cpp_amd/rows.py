@@ -9,6 +9,7 @@ raises the errors that the package's other functions do, and keeps nothing betwe
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -34,7 +35,11 @@ class _AttentionParams(ctypes.Structure):
                 ("scale", ctypes.c_float)]
 
 
+# The checks below are most of what a call for a few rows costs (10 to 20 us in all), so they look at each
+# tensor once, and struct nxg_rows are made several at a time, as an array of their 64-bit words.
 _types = {}
+_words = {n: ctypes.c_int64 * (3 * n) for n in (2, 4, 8)}
+_ROWS_BYTES = ctypes.sizeof(_Rows)
 
 
 def _type_of(t, name, allowed=None):
@@ -47,39 +52,46 @@ def _type_of(t, name, allowed=None):
     return ty
 
 
-def _on_current_device(t, name):
-    if not t.is_cuda or t.device.index != _raw_device():
+def _device_of(t, name) -> int:
+    """The tensor's device, which must be the current one."""
+    dev = t.get_device() if t.is_cuda else -1
+    if dev < 0 or dev != _raw_device():
         raise ValueError(f"{name} must be a tensor on the current device")
-    return t
+    return dev
 
 
-def _head_rows(t, name, like=None, shape=None):
-    """A [T][n_head][head_dim] tensor as struct nxg_rows."""
-    _on_current_device(t, name)
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+def _head_rows(t, name, dev, dtype, shape=None):
+    """A [T][n_head][head_dim] tensor as the words of struct nxg_rows."""
+    if not t.is_cuda or t.get_device() != dev:
+        raise ValueError(f"{name} must be a tensor on the current device")
+    st = t.stride()
+    if len(st) != 3 or (st[2] != 1 and t.shape[2] > 1):
         raise ValueError(f"{name} must be [T][n_head][head_dim] with values next to each other")
-    if like is not None and t.dtype != like.dtype:
-        raise ValueError(f"{name} must have type {like.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must have type {dtype}")
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    return _Rows(t.data_ptr(), t.stride(0), t.stride(1))
+    return t.data_ptr(), st[0], st[1]
 
 
-def _vector(t, name, n, dtypes):
-    _on_current_device(t, name)
-    if t.dtype not in dtypes or tuple(t.shape) != (n,) or not t.is_contiguous():
+def _vector(t, name, n, dev, dtypes):
+    if not t.is_cuda or t.get_device() != dev:
+        raise ValueError(f"{name} must be a tensor on the current device")
+    if t.dtype not in dtypes or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor [{n}] of {' or '.join(map(str, dtypes))}")
     return t.data_ptr()
 
 
-def _plain_rows(t, name, like=None):
+def _plain_rows(t, name, dev, like=None):
     """A [T][C] tensor with values next to each other: (pointer, row stride)."""
-    _on_current_device(t, name)
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    if not t.is_cuda or t.get_device() != dev:
+        raise ValueError(f"{name} must be a tensor on the current device")
+    st = t.stride()
+    if len(st) != 2 or (st[1] != 1 and t.shape[1] > 1):
         raise ValueError(f"{name} must be [T][C] with values next to each other")
     if like is not None and (t.dtype != like.dtype or t.shape != like.shape):
         raise ValueError(f"{name} must have type {like.dtype} and shape {tuple(like.shape)}")
-    return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), st[0]
 
 
 # --- rotary positions --------------------------------------------------------------------------
@@ -106,40 +118,43 @@ def rope_rows(x, freq, cu_offsets=None, positions=None, layout: str = "half", ms
     call. out may be x."""
     torch = _torch()
     ty = _type_of(x, "x")
-    xr = _head_rows(x, "x")
+    dev = _device_of(x, "x")
+    xr = _head_rows(x, "x", dev, x.dtype)
     T, H, D = x.shape
-    n = 2 * freq.numel()
-    fp = _vector(freq, "freq", n // 2, (torch.float64,))
+    half = freq.numel()
+    fp = _vector(freq, "freq", half, dev, (torch.float64,))
     if layout not in ROPE_LAYOUTS:
         raise ValueError(f"layout must be one of {', '.join(ROPE_LAYOUTS)}")
     if (cu_offsets is None) == (positions is None):
         raise ValueError("give either cu_offsets or positions")
     cu = None
     if positions is not None:
-        pp, cp, n_seqs = _vector(positions, "positions", T, (torch.int32,)), None, 0
+        pp, cp, n_seqs = _vector(positions, "positions", T, dev, (torch.int32,)), None, 0
     else:
         cu = _device_offsets(cu_offsets, x.device)
         pp, cp, n_seqs = None, cu.data_ptr(), cu.numel() - 1
     if out is None:
-        out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
-    orows = _head_rows(out, "out", x, x.shape)
+        out = x.new_empty((T, H, D))
+    rows = _words[2](*xr, *_head_rows(out, "out", dev, x.dtype, x.shape))
+    at = ctypes.addressof(rows)
     _order_on(stream, cu, out)
-    _check(load_library().nxg_rope_rows(ty, ctypes.byref(xr), T, H, D, fp, n, ROPE_LAYOUTS[layout], float(mscale),
-                                        1 if inverse else 0, pp, cp, n_seqs, ctypes.byref(orows), _stream_ptr(stream)), "rope_rows")
+    _check(load_library().nxg_rope_rows(ty, at, T, H, D, fp, 2 * half, ROPE_LAYOUTS[layout], float(mscale), 1 if inverse else 0,
+                                        pp, cp, n_seqs, at + _ROWS_BYTES, _stream_ptr(stream)), "rope_rows")
     return out
 
 
 # --- layer norm --------------------------------------------------------------------------------
 
-def _norm_weights(x, w, b):
+def _norm_weights(x, w, b, dev):
     """(w pointer, b pointer, weight type)."""
-    torch = _torch()
-    given = [t for t in (w, b) if t is not None]
-    wt = _type_of(given[0], "w") if given else TYPE_F32
-    if given and given[-1].dtype != given[0].dtype:
-        raise ValueError("w and b must have one type")
-    ptr = [None if t is None else _vector(t, name, x.shape[1], (torch.float32, x.dtype)) for name, t in (("w", w), ("b", b))]
-    return ptr[0], ptr[1], wt
+    first = w if w is not None else b
+    if first is None:
+        return None, None, TYPE_F32
+    wt = _type_of(first, "w")
+    if wt != TYPE_F32 and first.dtype != x.dtype:
+        raise ValueError(f"w and b must be float32 or {x.dtype}")
+    n, dtypes = x.shape[1], (first.dtype,)
+    return (None if w is None else _vector(w, "w", n, dev, dtypes)), (None if b is None else _vector(b, "b", n, dev, dtypes)), wt
 
 
 def layer_norm_rows(x, w=None, b=None, eps: float = 1e-5, out=None, mean=None, rstd=None, stream=None):
@@ -148,21 +163,27 @@ def layer_norm_rows(x, w=None, b=None, eps: float = 1e-5, out=None, mean=None, r
     may be x."""
     torch = _torch()
     ty = _type_of(x, "x")
-    xp, xs = _plain_rows(x, "x")
+    dev = _device_of(x, "x")
+    xp, xs = _plain_rows(x, "x", dev)
     T, C = x.shape
-    wp, bp, wt = _norm_weights(x, w, b)
+    wp, bp, wt = _norm_weights(x, w, b, dev)
     if out is None:
-        out = torch.empty((T, C), dtype=x.dtype, device=x.device)
-    yp, ys = _plain_rows(out, "out", x)
-    mean = torch.empty(T, dtype=torch.float32, device=x.device) if mean is None else mean
-    rstd = torch.empty(T, dtype=torch.float32, device=x.device) if rstd is None else rstd
-    mp, rp = (_vector(t, name, T, (torch.float32,)) for name, t in (("mean", mean), ("rstd", rstd)))
+        out = x.new_empty((T, C))
+    yp, ys = _plain_rows(out, "out", dev, x)
+    f32 = torch.float32
+    if mean is None and rstd is None:
+        mean, rstd = x.new_empty((2, T), dtype=f32)
+    else:
+        mean = x.new_empty(T, dtype=f32) if mean is None else mean
+        rstd = x.new_empty(T, dtype=f32) if rstd is None else rstd
+    mp, rp = _vector(mean, "mean", T, dev, (f32,)), _vector(rstd, "rstd", T, dev, (f32,))
     _order_on(stream, out, mean, rstd)
     _check(load_library().nxg_layer_norm_rows(ty, xp, xs, wp, bp, wt, float(eps), T, C, yp, ys, mp, rp, _stream_ptr(stream)),
            "layer_norm_rows")
     return out, mean, rstd
 
 
+@functools.lru_cache(maxsize=256)
 def layer_norm_rows_workspace_bytes(T: int, C: int) -> int:
     """nxg_layer_norm_rows_workspace_bytes."""
     n = int(load_library().nxg_layer_norm_rows_workspace_bytes(T, C))
@@ -170,12 +191,13 @@ def layer_norm_rows_workspace_bytes(T: int, C: int) -> int:
     return n
 
 
-def _workspace(t, nbytes, device):
+def _workspace(t, nbytes, like):
     """The caller's workspace (a uint8 device tensor) or one made for the call."""
     torch = _torch()
     if t is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _on_current_device(t, "workspace")
+        return like.new_empty(nbytes, dtype=torch.uint8)
+    if not t.is_cuda or t.get_device() != like.get_device():
+        raise ValueError("workspace must be a tensor on the current device")
     if t.dtype != torch.uint8 or not t.is_contiguous():
         raise ValueError("workspace must be a contiguous uint8 device tensor")
     return t
@@ -186,19 +208,21 @@ def layer_norm_rows_backward(dy, x, mean, rstd, w=None, dx=None, dw=None, db=Non
     workspace: None (made for the call) or a uint8 device tensor of layer_norm_rows_workspace_bytes(T, C)."""
     torch = _torch()
     ty = _type_of(x, "x")
-    xp, xs = _plain_rows(x, "x")
-    gp, gs = _plain_rows(dy, "dy", x)
+    dev = _device_of(x, "x")
+    xp, xs = _plain_rows(x, "x", dev)
+    gp, gs = _plain_rows(dy, "dy", dev, x)
     T, C = x.shape
-    wp, _, wt = _norm_weights(x, w, None)
-    w_dtype = w.dtype if w is not None else torch.float32
-    mp, rp = (_vector(t, name, T, (torch.float32,)) for name, t in (("mean", mean), ("rstd", rstd)))
+    wp, _, wt = _norm_weights(x, w, None, dev)
+    f32 = (torch.float32,)
+    w_dtype = w.dtype if w is not None else f32[0]
+    mp, rp = _vector(mean, "mean", T, dev, f32), _vector(rstd, "rstd", T, dev, f32)
     if dx is None:
-        dx = torch.empty((T, C), dtype=x.dtype, device=x.device)
-    dxp, dxs = _plain_rows(dx, "dx", x)
-    dw = torch.empty(C, dtype=w_dtype, device=x.device) if dw is None else dw
-    db = torch.empty(C, dtype=w_dtype, device=x.device) if db is None else db
-    dwp, dbp = (_vector(t, name, C, (w_dtype,)) for name, t in (("dw", dw), ("db", db)))
-    ws = _workspace(workspace, layer_norm_rows_workspace_bytes(T, C), x.device)
+        dx = x.new_empty((T, C))
+    dxp, dxs = _plain_rows(dx, "dx", dev, x)
+    dw = x.new_empty(C, dtype=w_dtype) if dw is None else dw
+    db = x.new_empty(C, dtype=w_dtype) if db is None else db
+    dwp, dbp = _vector(dw, "dw", C, dev, (w_dtype,)), _vector(db, "db", C, dev, (w_dtype,))
+    ws = _workspace(workspace, layer_norm_rows_workspace_bytes(T, C), x)
     _order_on(stream, dx, dw, db, ws)
     _check(load_library().nxg_layer_norm_rows_backward(ty, gp, gs, xp, xs, mp, rp, wp, wt, T, C, dxp, dxs, dwp, dbp,
                                                        ws.data_ptr(), ws.numel(), _stream_ptr(stream)), "layer_norm_rows_backward")
@@ -207,19 +231,43 @@ def layer_norm_rows_backward(dy, x, mean, rstd, w=None, dx=None, dw=None, db=Non
 
 # --- attention ---------------------------------------------------------------------------------
 
-def _attention_params(q, k, v, cu_q, cu_k, left, right, scale):
+@functools.lru_cache(maxsize=256)
+def _attention_bytes(dev, ty, H, G, D, T, K, n_seqs, left, right):
+    """The workspaces of the two passes for these sizes on this device (the scale has no part in them)."""
+    L = load_library()
+    p = ctypes.byref(_AttentionParams(ty, H, G, D, T, K, n_seqs, None, None, left, right, 1.0))
+    n = int(L.nxg_attention_rows_workspace_bytes(p)), int(L.nxg_attention_rows_backward_workspace_bytes(p))
+    _check(-min(n) if min(n) < 0 else 0, "attention_rows")
+    return n
+
+
+def _attention_args(q, k, v, cu_q, cu_k, left, right, scale):
+    """(params, the words of q, k and v, workspaces, cu_q, cu_k, device)"""
     ty = _type_of(q, "q", (TYPE_F16, TYPE_BF16))
-    rows = [_head_rows(q, "q"), _head_rows(k, "k", q), _head_rows(v, "v", q, k.shape)]
+    dev, dtype = _device_of(q, "q"), q.dtype
+    words = _head_rows(q, "q", dev, dtype) + _head_rows(k, "k", dev, dtype) + _head_rows(v, "v", dev, dtype, k.shape)
     T, H, D = q.shape
-    if k.shape[2] != D:
+    K, G, Dk = k.shape
+    if Dk != D:
         raise ValueError(f"k and v must have heads of {D}")
     cu_q = _device_offsets(cu_q, q.device)
     cu_k = cu_q if cu_k is None else _device_offsets(cu_k, q.device)
-    if cu_q.numel() != cu_k.numel():
+    n = cu_q.numel()
+    if cu_k.numel() != n:
         raise ValueError("cu_q and cu_k must have the same number of documents")
-    p = _AttentionParams(ty, H, k.shape[1], D, T, k.shape[0], cu_q.numel() - 1, cu_q.data_ptr(), cu_k.data_ptr(), int(left),
-                         int(right), 1.0 / math.sqrt(D) if scale is None else float(scale))
-    return p, rows, cu_q, cu_k
+    left, right = int(left), int(right)
+    sizes = _attention_bytes(dev, ty, H, G, D, T, K, n - 1, left, right)
+    p = _AttentionParams(ty, H, G, D, T, K, n - 1, cu_q.data_ptr(), cu_k.data_ptr(), left, right,
+                         1.0 / math.sqrt(D) if scale is None else float(scale))
+    return p, words, sizes, cu_q, cu_k, dev
+
+
+def _lse_arg(lse, T, H, dev):
+    if not lse.is_cuda or lse.get_device() != dev:
+        raise ValueError("lse must be a tensor on the current device")
+    if lse.dtype != _torch().float32 or lse.shape != (T, H) or not lse.is_contiguous():
+        raise ValueError(f"lse must be a contiguous float32 tensor [{T}][{H}]")
+    return lse.data_ptr()
 
 
 def attention_rows(q, k, v, cu_q, cu_k=None, scale: Optional[float] = None, left: int = -1, right: int = -1, out=None, lse=None,
@@ -231,33 +279,26 @@ def attention_rows(q, k, v, cu_q, cu_k=None, scale: Optional[float] = None, left
     fp32 [T_q][n_head] log of each query's sum, as attention_rows_backward takes it. Queries without a key
     give 0 and -inf. workspace: None (made where the launch uses one) or a uint8 device tensor."""
     torch = _torch()
-    L = load_library()
-    p, (qr, kr, vr), cu_q, cu_k = _attention_params(q, k, v, cu_q, cu_k, left, right, scale)
-    T, H, D = q.shape
+    p, words, sizes, cu_q, cu_k, dev = _attention_args(q, k, v, cu_q, cu_k, left, right, scale)
+    T, H, _ = q.shape
     if out is None:
-        out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
-    orows = _head_rows(out, "out", q, q.shape)
+        out = q.new_empty(q.shape)
     if lse is None:
-        lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
-    elif lse.dtype != torch.float32 or tuple(lse.shape) != (T, H) or not lse.is_contiguous():
-        raise ValueError(f"lse must be a contiguous float32 tensor [{T}][{H}]")
-    _on_current_device(lse, "lse")
-    n = int(L.nxg_attention_rows_workspace_bytes(ctypes.byref(p)))
-    _check(-n if n < 0 else 0, "attention_rows")
-    ws = _workspace(workspace, n, q.device) if n or workspace is not None else None
+        lse = q.new_empty((T, H), dtype=torch.float32)
+    lp = _lse_arg(lse, T, H, dev)
+    rows = _words[4](*words, *_head_rows(out, "out", dev, q.dtype, q.shape))
+    at = ctypes.addressof(rows)
+    ws = _workspace(workspace, sizes[0], q) if sizes[0] or workspace is not None else None
+    n = 0 if ws is None else ws.numel()
     _order_on(stream, cu_q, cu_k, out, lse, ws)
-    _check(L.nxg_attention_rows(ctypes.byref(p), ctypes.byref(qr), ctypes.byref(kr), ctypes.byref(vr), ctypes.byref(orows),
-                                lse.data_ptr(), ws.data_ptr() if ws is not None and ws.numel() else None,
-                                ws.numel() if ws is not None else 0, _stream_ptr(stream)), "attention_rows")
+    _check(load_library().nxg_attention_rows(ctypes.byref(p), at, at + _ROWS_BYTES, at + 2 * _ROWS_BYTES, at + 3 * _ROWS_BYTES, lp,
+                                             ws.data_ptr() if n else None, n, _stream_ptr(stream)), "attention_rows")
     return out, lse
 
 
 def attention_rows_backward_workspace_bytes(q, k, v, cu_q, cu_k=None, scale: Optional[float] = None, left: int = -1, right: int = -1) -> int:
     """The workspace attention_rows_backward takes for these arguments."""
-    p = _attention_params(q, k, v, cu_q, cu_k, left, right, scale)[0]
-    n = int(load_library().nxg_attention_rows_backward_workspace_bytes(ctypes.byref(p)))
-    _check(-n if n < 0 else 0, "attention_rows_backward_workspace_bytes")
-    return n
+    return _attention_args(q, k, v, cu_q, cu_k, left, right, scale)[2][1]
 
 
 def attention_rows_backward(dout, q, k, v, out, lse, cu_q, cu_k=None, scale: Optional[float] = None, left: int = -1,
@@ -265,26 +306,19 @@ def attention_rows_backward(dout, q, k, v, out, lse, cu_q, cu_k=None, scale: Opt
     """The gradients of attention_rows: (dq, dk, dv), from dout, its inputs and what it returned (out, lse).
     Rows of no document are left as they were. workspace: None (made for the call) or a uint8 device tensor of
     attention_rows_backward_workspace_bytes."""
-    torch = _torch()
-    L = load_library()
-    p, (qr, kr, vr), cu_q, cu_k = _attention_params(q, k, v, cu_q, cu_k, left, right, scale)
-    T, H, D = q.shape
-    gr, orows = _head_rows(dout, "dout", q, q.shape), _head_rows(out, "out", q, q.shape)
-    _on_current_device(lse, "lse")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (T, H) or not lse.is_contiguous():
-        raise ValueError(f"lse must be a contiguous float32 tensor [{T}][{H}]")
-    made = []
-    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        made.append(torch.empty(like.shape, dtype=q.dtype, device=q.device) if t is None else t)
-        if t is not None:
-            _head_rows(t, name, q, like.shape)
-    dqr, dkr, dvr = (_Rows(t.data_ptr(), t.stride(0), t.stride(1)) for t in made)
-    n = int(L.nxg_attention_rows_backward_workspace_bytes(ctypes.byref(p)))
-    _check(-n if n < 0 else 0, "attention_rows_backward")
-    ws = _workspace(workspace, n, q.device)
-    _order_on(stream, cu_q, cu_k, *made, ws)
-    _check(L.nxg_attention_rows_backward(ctypes.byref(p), ctypes.byref(gr), ctypes.byref(qr), ctypes.byref(kr), ctypes.byref(vr),
-                                         ctypes.byref(orows), lse.data_ptr(), ctypes.byref(dqr), ctypes.byref(dkr),
-                                         ctypes.byref(dvr), ws.data_ptr(), ws.numel(), _stream_ptr(stream)),
-           "attention_rows_backward")
-    return tuple(made)
+    p, words, sizes, cu_q, cu_k, dev = _attention_args(q, k, v, cu_q, cu_k, left, right, scale)
+    T, H, _ = q.shape
+    dtype = q.dtype
+    lp = _lse_arg(lse, T, H, dev)
+    dq = q.new_empty(q.shape) if dq is None else dq
+    dk = q.new_empty(k.shape) if dk is None else dk
+    dv = q.new_empty(k.shape) if dv is None else dv
+    rows = _words[8](*words, *_head_rows(dout, "dout", dev, dtype, q.shape), *_head_rows(out, "out", dev, dtype, q.shape),
+                     *_head_rows(dq, "dq", dev, dtype, q.shape), *_head_rows(dk, "dk", dev, dtype, k.shape),
+                     *_head_rows(dv, "dv", dev, dtype, k.shape))
+    qa, ka, va, da, oa, dqa, dka, dva = range(ctypes.addressof(rows), ctypes.addressof(rows) + 8 * _ROWS_BYTES, _ROWS_BYTES)
+    ws = _workspace(workspace, sizes[1], q)
+    _order_on(stream, cu_q, cu_k, dq, dk, dv, ws)
+    _check(load_library().nxg_attention_rows_backward(ctypes.byref(p), da, qa, ka, va, oa, lp, dqa, dka, dva, ws.data_ptr(),
+                                                      ws.numel(), _stream_ptr(stream)), "attention_rows_backward")
+    return dq, dk, dv

@@ -110,9 +110,8 @@ def test_few_queries_split(nxg, torch, dev, dtype, D):
     dt = getattr(torch, dtype)
     q, k, v, _, out, lse = run_and_check(nxg, torch, dt, [1], [20000], H=4, G=2, D=D, seed=D, grad=False)
     import ctypes
-    p, rows, cu_q, cu_k = nxg.rows._attention_params(q, k, v, offsets([1]), offsets([20000]), -1, -1, None)
-    L = nxg.load_library()
-    assert L.nxg_attention_rows_workspace_bytes(ctypes.byref(p)) > 0, "this launch is to be split"
+    p = nxg.rows._AttentionParams(nxg.rows._type_of(q, "q"), 4, 2, D, 1, 20000, 1, None, None, -1, -1, 1.0)
+    assert nxg.load_library().nxg_attention_rows_workspace_bytes(ctypes.byref(p)) > 0, "this launch is to be split"
     small = torch.empty(16, dtype=torch.uint8, device="cuda")
     out2, lse2 = nxg.attention_rows(q, k, v, offsets([1]), offsets([20000]), workspace=small)
     ref = rows_ref.attention(q, k, v, offsets([1]), offsets([20000]), 1 / math.sqrt(D), -1, -1)
