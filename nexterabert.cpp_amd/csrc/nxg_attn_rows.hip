@@ -184,7 +184,7 @@ __device__ __forceinline__ job find_job(const attn_p & p, bool by_keys, int mul,
     r.tile = -1;
     const int32_t * cu = by_keys ? p.cu_k : p.cu_q;
     const int T = by_keys ? p.T_k : p.T_q;
-    if (order == BY_ROWS || p.n_seqs > 64) {
+    if (p.n_seqs > 64) {
         const int d = find_doc(cu, p.n_seqs, T, mul, size, slot);
         r.c = doc_of(p, d);
         const int64_t at = slot - slot_of(cu, d, T, mul, size);
@@ -192,10 +192,26 @@ __device__ __forceinline__ job find_job(const attn_p & p, bool by_keys, int mul,
         if (at >= 0 && at * size < len) r.tile = uni((int) (from_end ? (len + size - 1) / size - 1 - at : at));
         return r;
     }
+    // a document a lane, its offsets in one load each
     const int lane = threadIdx.x & 63, d = min(lane, p.n_seqs - 1);
     const int q0 = offset(p.cu_q, d, p.T_q), n = max(offset(p.cu_q, d + 1, p.T_q) - q0, 0);
     const int k0 = offset(p.cu_k, d, p.T_k), m = max(offset(p.cu_k, d + 1, p.T_k) - k0, 0);
     const int count = lane < p.n_seqs ? (int) (((int64_t) (by_keys ? m : n) * mul + size - 1) / size) : 0;
+    auto take = [&](int at, int tile) {
+        r.c.q0 = __builtin_amdgcn_readlane(q0, at);
+        r.c.n = __builtin_amdgcn_readlane(n, at);
+        r.c.k0 = __builtin_amdgcn_readlane(k0, at);
+        r.c.m = __builtin_amdgcn_readlane(m, at);
+        r.tile = uni(tile);
+    };
+    if (order == BY_ROWS) {
+        const int upto = scan64(count);
+        const uint64_t here = __ballot(slot < upto);
+        if (!here) return r;
+        const int at = __builtin_ctzll(here), left = __builtin_amdgcn_readlane(upto, at) - slot;
+        take(at, from_end ? left - 1 : __builtin_amdgcn_readlane(count, at) - left);
+        return r;
+    }
     int rank = 0;              // documents of more tiles, or as many and before this one
     for (int j = 0; j < p.n_seqs; ++j) {
         const int cj = __builtin_amdgcn_readlane(count, j);
@@ -223,11 +239,7 @@ __device__ __forceinline__ job find_job(const attn_p & p, bool by_keys, int mul,
     }
     const int at = __builtin_ctzll(__ballot(rank == doc_rank));
     if (from_end && order == BY_LEVEL) tile = __builtin_amdgcn_readlane(count, at) - 1 - tile;
-    r.c.q0 = __builtin_amdgcn_readlane(q0, at);
-    r.c.n = __builtin_amdgcn_readlane(n, at);
-    r.c.k0 = __builtin_amdgcn_readlane(k0, at);
-    r.c.m = __builtin_amdgcn_readlane(m, at);
-    r.tile = uni(tile);
+    take(at, tile);
     return r;
 }
 
@@ -442,16 +454,18 @@ __device__ __forceinline__ typename type_of<E>::v8 pack(const v16f & x, int a) {
     return o;
 }
 
-// The wave's own 32 rows of D values as an operand in registers, from src (this lane's row).
+// The wave's own 32 rows of D values as operands in registers, from src (this lane's row); one, or two at once.
 template <class E, int DT>
-__device__ __forceinline__ void load_operand(typename type_of<E>::v8 (&x)[2 * DT], const char * src, int D) {
+__device__ __forceinline__ void issue_operand(v4i (&z)[2 * DT], const char * src, int D) {
     const int h = (threadIdx.x & 63) >> 5;
-    v4i z[2 * DT];
 #pragma unroll
     for (int s = 0; s < 2 * DT; ++s) {
         z[s] = v4i{0, 0, 0, 0};
         if (16 * s + 8 * h < D) z[s] = *reinterpret_cast<const v4i *>(src + (16 * s + 8 * h) * 2);
     }
+}
+template <class E, int DT>
+__device__ __forceinline__ void take_operand(typename type_of<E>::v8 (&x)[2 * DT], v4i (&z)[2 * DT]) {
     // arrived here, not at their first use: that is in a loop, where the compiler would wait for the tiles
     // under way as well
 #pragma unroll
@@ -459,6 +473,21 @@ __device__ __forceinline__ void load_operand(typename type_of<E>::v8 (&x)[2 * DT
         asm volatile("" : "+v"(z[s]));
         __builtin_memcpy(&x[s], &z[s], 16);
     }
+}
+template <class E, int DT>
+__device__ __forceinline__ void load_operand(typename type_of<E>::v8 (&x)[2 * DT], const char * src, int D) {
+    v4i z[2 * DT];
+    issue_operand<E, DT>(z, src, D);
+    take_operand<E, DT>(x, z);
+}
+template <class E, int DT>
+__device__ __forceinline__ void load_operands(typename type_of<E>::v8 (&x)[2 * DT], const char * x_src, typename type_of<E>::v8 (&y)[2 * DT],
+                                              const char * y_src, int D) {
+    v4i zx[2 * DT], zy[2 * DT];
+    issue_operand<E, DT>(zx, x_src, D);
+    issue_operand<E, DT>(zy, y_src, D);
+    take_operand<E, DT>(x, zx);
+    take_operand<E, DT>(y, zy);
 }
 
 // The wave's 32 columns of DT 32x32 results as rows of D values in memory, scaled by f: through a tile
@@ -694,9 +723,6 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     const int pw = p0 + 32 * wave;
     const bool active = pw < np;
     const int pc = min(pw + (lane & 31), np - 1), tok = pc / p.R, head = g * p.R + pc % p.R;
-    typename type_of<E>::v8 q[2 * DT];
-    load_operand<E, DT>(q, p.q.data + (c.q0 + tok) * p.q.ts + head * p.q.hs, p.D);
-
     const int lo = key_lo(p, c, tok), hi = key_hi(p, c, tok);
     // keys of the workgroup, and of the wave: some pair's, and every pair's
     const int t_end = (min(p0 + BM, np) - 1) / p.R;
@@ -720,6 +746,10 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
         keys.first_k(lds_addr(sk[1]));
         keys.next_k(lds_addr(sk[0]));
         keys.next_v(lds_addr(sv[0]));
+    }
+    typename type_of<E>::v8 q[2 * DT];
+    load_operand<E, DT>(q, p.q.data + (c.q0 + tok) * p.q.ts + head * p.q.hs, p.D);
+    if (j_lo < j_hi) {
         wait_all();
         barrier();
         s0 = fwd_scores<E, DT>(q, lds_addr(sk[1]) + at.row, 32);
@@ -1105,13 +1135,6 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
     const int pw = p0 + 32 * wave;
     const bool active = pw < np;
     const int pc = min(pw + (lane & 31), np - 1), tok = pc / p.R, head = g * p.R + pc % p.R;
-    typename type_of<E>::v8 q[2 * DT], go[2 * DT];
-    load_operand<E, DT>(q, p.q.data + (c.q0 + tok) * p.q.ts + head * p.q.hs, p.D);
-    load_operand<E, DT>(go, p.dout.data + (c.q0 + tok) * p.dout.ts + head * p.dout.hs, p.D);
-    const int64_t row = ((int64_t) g * p.T_q + c.q0) * p.R + pc;
-    const float factor = ds_factor<E>(p), ds_scale = type_of<E>::HALF ? ldexpf(factor, P_SHIFT) : 1.0f;
-    float lse2 = p.lse2[row], ndelta = p.ndelta[row];
-    asm volatile("" : "+v"(lse2), "+v"(ndelta));
 
     const int lo = key_lo(p, c, tok), hi = key_hi(p, c, tok);
     const int t_end = (min(p0 + BM, np) - 1) / p.R;
@@ -1131,6 +1154,12 @@ __global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
     const float cs = p.scale * LOG2E;
     const lane_at at = lane_places<DT>();
     if (j_lo < j_hi) keys.next(lds_addr(sk[0]), lds_addr(sv[0]));
+    typename type_of<E>::v8 q[2 * DT], go[2 * DT];
+    load_operands<E, DT>(q, p.q.data + (c.q0 + tok) * p.q.ts + head * p.q.hs, go, p.dout.data + (c.q0 + tok) * p.dout.ts + head * p.dout.hs, p.D);
+    const int64_t row = ((int64_t) g * p.T_q + c.q0) * p.R + pc;
+    const float factor = ds_factor<E>(p), ds_scale = type_of<E>::HALF ? ldexpf(factor, P_SHIFT) : 1.0f;
+    float lse2 = p.lse2[row], ndelta = p.ndelta[row];
+    asm volatile("" : "+v"(lse2), "+v"(ndelta));
     for (int j = j_lo; j < j_hi; ++j) {
         const int buf = (j - j_lo) & 1, j0 = j * BN;
         wait_all();
@@ -1244,10 +1273,6 @@ __global__ __launch_bounds__(256 * QG, 2) void attn_rows_dkv_kernel(attn_p p) {
     const int kw = kb0 + 32 * wave;
     const bool active = kw < c.m;
     const int key = min(kw + (lane & 31), c.m - 1);
-    typename type_of<E>::v8 k[2 * DT], v[2 * DT];
-    load_operand<E, DT>(k, p.k.data + (int64_t) (c.k0 + key) * p.k.ts + g * p.k.hs, p.D);
-    load_operand<E, DT>(v, p.v.data + (int64_t) (c.k0 + key) * p.v.ts + g * p.v.hs, p.D);
-    const float factor = ds_factor<E>(p), ds_scale = type_of<E>::HALF ? ldexpf(factor, P_SHIFT) : 1.0f;
 
     const int k_end = min(kb0 + BK, c.m) - 1;
     const int j_lo = tok_lo(p, c, kb0) * p.R / BQ, j_hi = (tok_hi(p, c, k_end) * p.R + BQ - 1) / BQ;
@@ -1290,6 +1315,9 @@ __global__ __launch_bounds__(256 * QG, 2) void attn_rows_dkv_kernel(attn_p p) {
     const float cs = p.scale * LOG2E;
     const lane_at at = lane_places<DT>();
     if (j_lo < j_hi) load(j_lo, 0);
+    typename type_of<E>::v8 k[2 * DT], v[2 * DT];
+    load_operands<E, DT>(k, p.k.data + (int64_t) (c.k0 + key) * p.k.ts + g * p.k.hs, v, p.v.data + (int64_t) (c.k0 + key) * p.v.ts + g * p.v.hs, p.D);
+    const float factor = ds_factor<E>(p), ds_scale = type_of<E>::HALF ? ldexpf(factor, P_SHIFT) : 1.0f;
     for (int j = j_lo; j < j_hi; ++j) {
         const int buf = (j - j_lo) & 1, j0 = j * BQ;
         wait_all();

@@ -94,6 +94,15 @@ def _plain_rows(t, name, dev, like=None):
     return t.data_ptr(), st[0]
 
 
+def _offsets_arg(cu, like, dev):
+    """cu_offsets (host sequence or device int32 tensor) as a device int32 tensor."""
+    torch = _torch()
+    if isinstance(cu, torch.Tensor) and cu.is_cuda and cu.get_device() == dev and cu.dtype == torch.int32 and cu.dim() == 1 \
+            and cu.is_contiguous() and cu.numel() > 1:
+        return cu
+    return _device_offsets(cu, like.device)
+
+
 # --- rotary positions --------------------------------------------------------------------------
 
 def rope_frequencies(n_rot: int, base: float, scaling: str = "none", factor: float = 1.0, train_len: int = 0):
@@ -131,7 +140,7 @@ def rope_rows(x, freq, cu_offsets=None, positions=None, layout: str = "half", ms
     if positions is not None:
         pp, cp, n_seqs = _vector(positions, "positions", T, dev, (torch.int32,)), None, 0
     else:
-        cu = _device_offsets(cu_offsets, x.device)
+        cu = _offsets_arg(cu_offsets, x, dev)
         pp, cp, n_seqs = None, cu.data_ptr(), cu.numel() - 1
     if out is None:
         out = x.new_empty((T, H, D))
@@ -250,8 +259,8 @@ def _attention_args(q, k, v, cu_q, cu_k, left, right, scale):
     K, G, Dk = k.shape
     if Dk != D:
         raise ValueError(f"k and v must have heads of {D}")
-    cu_q = _device_offsets(cu_q, q.device)
-    cu_k = cu_q if cu_k is None else _device_offsets(cu_k, q.device)
+    cu_q = _offsets_arg(cu_q, q, dev)
+    cu_k = cu_q if cu_k is None else _offsets_arg(cu_k, q, dev)
     n = cu_q.numel()
     if cu_k.numel() != n:
         raise ValueError("cu_q and cu_k must have the same number of documents")
