@@ -917,36 +917,49 @@ v16f s = fwd_scores<E, DT>(q, lds_addr(lds[wave][buf][0]) + at.row, 0), w;
     }
 }
 
-// The splits' sums of a (token, head) row joined: 16 lanes a row, 8 values each.
-template <class E>
+// The splits' sums of a (token, head) row joined: a wave a row, L lanes for its values (8 each), 64 / L groups of them
+// for every 64 / L'th split, whose loads are independent; the groups' sums added at the end.
+template <class E, int L>
 __global__ __launch_bounds__(256) void attn_rows_join_kernel(attn_p p) {
-    const int64_t row = (int64_t) blockIdx.x * 16 + threadIdx.x / 16, n_rows = (int64_t) p.T_q * p.H;
-    const int cc = threadIdx.x % 16;
-    if (row >= n_rows || cc * 8 >= p.D) return;
+    const int64_t row = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6), n_rows = (int64_t) p.T_q * p.H;
+    const int lane = threadIdx.x & 63, cc = lane % L, first = lane / L;
+    if (row >= n_rows) return;
     const int tok = (int) (row / p.H), head = (int) (row % p.H);
     // rows of no document have no sums
-    const int end = offset(p.cu_q, p.n_seqs, p.T_q);
-    if (tok >= end || tok < offset(p.cu_q, 0, p.T_q)) return;
-    float m = -INFINITY, l = 0.0f, x[8] = {};
-    for (int s = 0; s < p.n_split; ++s) m = fmaxf(m, p.part[(s * n_rows + row) * (p.D + 8)]);
-    for (int s = 0; s < p.n_split; ++s) {
-        const float * o = p.part + (s * n_rows + row) * (p.D + 8);
-        if (o[0] == -INFINITY && o[1] == 0.0f) continue;
-        const float f = __builtin_amdgcn_exp2f(o[0] - m);
-        l += f * o[1];
-        const v4f a = *reinterpret_cast<const v4f *>(o + 8 + cc * 8), b = *reinterpret_cast<const v4f *>(o + 12 + cc * 8);
+    if (tok >= offset(p.cu_q, p.n_seqs, p.T_q) || tok < offset(p.cu_q, 0, p.T_q)) return;
+    const float * part = p.part + row * (p.D + 8);
+    const int64_t next = n_rows * (p.D + 8);
+    // m and l of split `lane` (64 at most); a share without keys has -inf and 0
+    const bool mine = lane < p.n_split;
+    const float m = mine ? part[lane * next] : -INFINITY, l = mine ? part[lane * next + 1] : 0.0f;
+    const float top = wave_max(m);
+    const float f = m == -INFINITY && l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    const float total = wave_sum(f * l);
+    float x[8] = {};
+#pragma unroll 4
+    for (int s0 = 0; s0 < p.n_split; s0 += 64 / L) {
+        const int s = s0 + first;
+        const float fs = __shfl(f, s);
+        if (s < p.n_split && cc * 8 < p.D && fs != 0.0f) {
+            const v4f a = *reinterpret_cast<const v4f *>(part + s * next + 8 + cc * 8), b = *reinterpret_cast<const v4f *>(part + s * next + 12 + cc * 8);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] += f * a[i];
-            x[4 + i] += f * b[i];
+            for (int i = 0; i < 4; ++i) {
+                x[i] += fs * a[i];
+                x[4 + i] += fs * b[i];
+            }
         }
     }
-    const float f = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+#pragma unroll
+    for (int k = L; k < 64; k *= 2)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += __shfl_xor(x[i], k);
+    if (lane == 0) p.lse[row] = top == -INFINITY && total == 0.0f ? -INFINITY : LN2 * (top + __builtin_amdgcn_logf(total));
+    if (lane >= L || cc * 8 >= p.D) return;
+    const float g = total > 0.0f ? 1.0f / total : (total == 0.0f ? 0.0f : total);
     typename type_of<E>::v8 e;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = (E) (x[i] * f);
+    for (int i = 0; i < 8; ++i) e[i] = (E) (x[i] * g);
     *reinterpret_cast<typename type_of<E>::v8 *>(p.out.data + (int64_t) tok * p.out.ts + head * p.out.hs + cc * 16) = e;
-    if (cc == 0) p.lse[row] = m == -INFINITY && l == 0.0f ? -INFINITY : LN2 * (m + __builtin_amdgcn_logf(l));
 }
 
 // ---------------------------------------------------------------------------
@@ -1507,8 +1520,9 @@ int work_order(const attn_p & p, int64_t workgroups) {
     return p.left < 0 && p.right < 0 ? BY_LENGTH : BY_LEVEL;
 }
 
-// The few-pairs kernel where tiles of 128 pairs would leave most CUs idle, its keys split until there are
-// two workgroups a CU, 256 keys of the average document at least to each.
+// The few-pairs kernel where tiles of 128 pairs would leave CUs idle, its keys split until there is a workgroup a CU
+// (more only add sums to join: 8 x 1 query over 8,192 keys of 128 values 50.0, 54.1 and 63.1 us with one, two and
+// four a CU), 256 keys of the average document at least to each.
 struct fwd_plan {
     bool few;
     int n_split;
@@ -1523,7 +1537,7 @@ fwd_plan plan_forward(const attn_p & p) {
     f.few = true;
     const int64_t wgs = slots(p.T_q, p.R, 32, p.n_seqs) * p.G;
     const int64_t keys = p.T_k / std::max(1, p.n_seqs);
-    f.n_split = (int) std::max<int64_t>(1, std::min({2 * cus / wgs, keys / 256, (int64_t) 64}));
+    f.n_split = (int) std::max<int64_t>(1, std::min({cus / wgs, keys / 256, (int64_t) 64}));
     return f;
 }
 
@@ -1569,9 +1583,14 @@ int32_t nxg_attention_rows(const nxg_attention_rows_params * a, const nxg_rows *
         NXG_BY_TYPE(a->type, p.D, (attn_rows_few_kernel<E, DT><<<grid, 256, 0, s>>>(p)));
         NXG_TRY(nxg_launch_check(what));
         if (p.n_split == 1) return NXG_OK;
-        const unsigned rows_grid = (unsigned) (((int64_t) p.T_q * p.H + 15) / 16);
-        if (a->type == NXG_TYPE_BF16) attn_rows_join_kernel<__bf16><<<rows_grid, 256, 0, s>>>(p);
-        else attn_rows_join_kernel<_Float16><<<rows_grid, 256, 0, s>>>(p);
+        const unsigned rows_grid = (unsigned) (((int64_t) p.T_q * p.H + 3) / 4);
+        if (a->type == NXG_TYPE_BF16) {
+            if (p.D <= 64) attn_rows_join_kernel<__bf16, 8><<<rows_grid, 256, 0, s>>>(p);
+            else attn_rows_join_kernel<__bf16, 16><<<rows_grid, 256, 0, s>>>(p);
+        } else {
+            if (p.D <= 64) attn_rows_join_kernel<_Float16, 8><<<rows_grid, 256, 0, s>>>(p);
+            else attn_rows_join_kernel<_Float16, 16><<<rows_grid, 256, 0, s>>>(p);
+        }
         return nxg_launch_check(what);
     }
     p.order = work_order(p, grid);

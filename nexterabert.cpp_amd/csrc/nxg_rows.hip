@@ -50,6 +50,7 @@ struct rope_p {
     const double * freq;
     const int32_t * positions, * cu;
     int32_t T, H, D, n, n_seqs, tb, hb;    // tokens of a workgroup, heads of one (grid.y)
+    uint32_t by_token, by_head, by_token_last;   // 2^32 / pieces of a token's heads, of a head, of a token in the last grid.y, rounded up
     float mscale, sign;
     bool copy;                             // out is not x: values behind n are written too
 };
@@ -90,8 +91,11 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(rope_p p) {
     const int pieces = half / V, per_head = pieces + (p.copy ? (p.D - p.n) / V : 0), per_token = per_head * heads;
     const E * x0 = (const E *) p.x;
     E * o0 = (E *) p.out;
+    const uint32_t by_token = heads == p.hb ? p.by_token : p.by_token_last;
     for (int k = threadIdx.x; k < tokens * per_token; k += 256) {
-        const int t = k / per_token, r = k - t * per_token, h = r / per_head, piece = r - h * per_head;
+        // k / per_token and r / per_head: exact while k * per_token < 2^32
+        const int t = by_token ? __umulhi(k, by_token) : k, r = k - t * per_token;
+        const int h = p.by_head ? __umulhi(r, p.by_head) : r, piece = r - h * per_head;
         const E * x = x0 + (t0 + t) * p.x_ts + (h0 + h) * p.x_hs;
         E * o = o0 + (t0 + t) * p.o_ts + (h0 + h) * p.o_hs;
         if (piece >= pieces) {
@@ -365,22 +369,24 @@ __global__ __launch_bounds__(256) void layer_norm_back_columns_kernel(norm_p p) 
     part[p.C + c] = db;
 }
 
-// The columns' sums of the n_part rows of `part`: 16 columns of dw or db a workgroup, 16 threads each,
-// every 16th row a thread, then the 16 in order.
+// The columns' sums of the n_part rows of `part`: 16 columns of dw or db a workgroup, 64 threads each, every 64th row
+// a thread (8 loads under way at a time), then the 64 in order.
 template <class W>
-__global__ __launch_bounds__(256) void norm_reduce_kernel(norm_p p) {
-    __shared__ float lds[16][17];
-    const int64_t col = (int64_t) blockIdx.x * 16 + threadIdx.x % 16;
+__global__ __launch_bounds__(1024) void norm_reduce_kernel(norm_p p) {
+    __shared__ float lds[64][17];
+    const int64_t col = (int64_t) blockIdx.x * 16 + threadIdx.x % 16, n = 2 * (int64_t) p.C;
     const int sub = threadIdx.x / 16;
     float s = 0.0f;
-    if (col < 2 * (int64_t) p.C)
-        for (int r = sub; r < p.n_part; r += 16) s += p.part[(int64_t) r * 2 * p.C + col];
+    if (col < n) {
+#pragma unroll 8
+        for (int r = sub; r < p.n_part; r += 64) s += p.part[r * n + col];
+    }
     lds[sub][threadIdx.x % 16] = s;
     __syncthreads();
-    if (sub || col >= 2 * (int64_t) p.C) return;
+    if (sub || col >= n) return;
     s = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) s += lds[k][threadIdx.x];
+#pragma unroll 16
+    for (int k = 0; k < 64; ++k) s += lds[k][threadIdx.x];
     if (col < p.C) {
         if (p.dw) ((W *) p.dw)[col] = (W) s;
     } else if (p.db) {
@@ -552,6 +558,14 @@ int32_t nxg_rope_rows(int32_t type, const nxg_rows * x, int32_t T, int32_t n_hea
     while (p.tb > 1 && (T + p.tb - 1) / p.tb < 2 * cus) p.tb /= 2;
     p.hb = n_head;
     while (p.hb > 1 && (int64_t) ((T + p.tb - 1) / p.tb) * ((n_head + p.hb - 1) / p.hb) < cus && p.hb * head_dim > 256 * (w ? V : 1)) p.hb = (p.hb + 1) / 2;
+    const int v = w ? V : 1, per_head = n_rot / 2 / v + (p.copy ? (head_dim - n_rot) / v : 0);
+    if (per_head == 0) return NXG_OK;
+    p.hb = std::min(p.hb, 65535 / per_head);
+    while (p.tb > 1 && (int64_t) p.tb * p.hb * per_head * p.hb * per_head > INT32_MAX) p.tb /= 2;
+    auto magic = [](int d) { return (uint32_t) (((1ull << 32) + d - 1) / d); };       // 0 for 1
+    p.by_head = magic(per_head);
+    p.by_token = magic(per_head * p.hb);
+    p.by_token_last = magic(per_head * ((n_head - 1) % p.hb + 1));
     const dim3 grid((unsigned) ((T + p.tb - 1) / p.tb), (unsigned) ((n_head + p.hb - 1) / p.hb));
     if (grid.y > 65535 || (int64_t) p.tb * p.hb * head_dim > INT32_MAX) return nxg_fail(NXG_EINVAL, "%s: n_head=%d", what, n_head);
     const size_t lds = (size_t) p.tb * (n_rot / 2) * sizeof(float2);
@@ -678,7 +692,7 @@ int32_t nxg_layer_norm_rows_backward(int32_t type, const void * dy, int64_t dy_s
     }
     if (!p.part) return NXG_OK;
     const unsigned grid = (unsigned) ((2 * (int64_t) C + 15) / 16);
-    by_types(type, w_type, [&](auto, auto we) { norm_reduce_kernel<decltype(we)><<<grid, 256, 0, s>>>(p); });
+    by_types(type, w_type, [&](auto, auto we) { norm_reduce_kernel<decltype(we)><<<grid, 1024, 0, s>>>(p); });
     return nxg_launch_check(what);
 }
 
