@@ -68,8 +68,8 @@ __device__ __forceinline__ int doc_of_row(const int32_t * cu, int n_seqs, int t)
 
 // A workgroup: tb tokens of hb heads. Their angles once, into LDS: position * frequency in 64 bits, as
 // turns less whole turns, then fp32 (error 2^-25 of a turn). Then the heads' rows as one run of
-// pieces, neighbouring lanes on neighbouring pieces: V pairs of a head (HALF: V values from i and V from
-// i + n / 2; else 2 V values in a row), or V values behind n to copy.
+// pieces, neighbouring lanes on neighbouring pieces: V values of a head from i and V from i + n / 2
+// (HALF), V values in a row (else; a pair of single values where V is 1), or V values behind n to copy.
 template <class E, int V, bool HALF>
 __global__ __launch_bounds__(256) void rope_rows_kernel(rope_p p) {
     extern __shared__ float2 turn[];       // [tb][n / 2]
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(rope_p p) {
     }
     __syncthreads();
     const int h0 = blockIdx.y * p.hb, heads = min(p.hb, p.H - h0);
-    const int pieces = half / V, per_head = pieces + (p.copy ? (p.D - p.n) / V : 0), per_token = per_head * heads;
+    const int pieces = HALF || V == 1 ? half / V : p.n / V, per_head = pieces + (p.copy ? (p.D - p.n) / V : 0), per_token = per_head * heads;
     const E * x0 = (const E *) p.x;
     E * o0 = (E *) p.out;
     const uint32_t by_token = heads == p.hb ? p.by_token : p.by_token_last;
@@ -105,30 +105,32 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(rope_p p) {
             store<E, V>(o + d, a);
             continue;
         }
-        const float2 * w = turn + t * half + piece * V;
-        const int da = HALF ? piece * V : 2 * piece * V, db = HALF ? half + piece * V : (2 * piece + 1) * V;
-        float a[V], b[V], y[V], z[V];
-        load<E, V>(a, x + da);
-        load<E, V>(b, x + db);
         if constexpr (HALF || V == 1) {
+            const float2 * w = turn + t * half + piece * V;
+            const int da = HALF ? piece * V : 2 * piece, db = HALF ? half + piece * V : 2 * piece + 1;
+            float a[V], b[V], y[V], z[V];
+            load<E, V>(a, x + da);
+            load<E, V>(b, x + db);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float c = w[i].x, s = w[i].y;
                 y[i] = a[i] * c - b[i] * s;
                 z[i] = a[i] * s + b[i] * c;
             }
+            store<E, V>(o + da, y);
+            store<E, V>(o + db, z);
         } else {
+            const float2 * w = turn + t * half + piece * (V / 2);
+            float a[V], y[V];
+            load<E, V>(a, x + piece * V);
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) {
-                const float c = w[i].x, s = w[i].y, c2 = w[V / 2 + i].x, s2 = w[V / 2 + i].y;
+                const float c = w[i].x, s = w[i].y;
                 y[2 * i] = a[2 * i] * c - a[2 * i + 1] * s;
                 y[2 * i + 1] = a[2 * i] * s + a[2 * i + 1] * c;
-                z[2 * i] = b[2 * i] * c2 - b[2 * i + 1] * s2;
-                z[2 * i + 1] = b[2 * i] * s2 + b[2 * i + 1] * c2;
             }
+            store<E, V>(o + piece * V, y);
         }
-        store<E, V>(o + da, y);
-        store<E, V>(o + db, z);
     }
 }
 
@@ -550,15 +552,16 @@ int32_t nxg_rope_rows(int32_t type, const nxg_rows * x, int32_t T, int32_t n_hea
     p.sign = inverse ? -1.0f : 1.0f;
     const int V = 16 / es;
     const bool w = wide(p.x, p.x_ts, es) && wide(p.x, p.x_hs, es) && wide(p.out, p.o_ts, es) && wide(p.out, p.o_hs, es) &&
-                   n_rot % (2 * V) == 0 && head_dim % V == 0;
-    // tokens of a workgroup: an angle a thread, fewer where that would leave CUs without work; heads in
-    // pieces too for the shortest
+                   n_rot % (layout == NXG_ROPE_HALF ? 2 * V : V) == 0 && head_dim % V == 0;
+    // tokens of a workgroup: at most an angle a thread, and about 12 KiB of rows (65,536 x 24 heads of 64: fp32 152 us
+    // with 12 KiB, 160 with 98; bf16 75 with 12, 80 with 24, 82 with 3), fewer where that would leave CUs without
+    // work; heads in pieces too for the shortest
     const int cus = nxg_device_cus();
-    p.tb = std::max(1, std::min(512 / n_rot, 64));
+    p.tb = std::max<int>(1, std::min<int64_t>(512 / n_rot, 12288 / ((int64_t) n_head * head_dim * es)));
     while (p.tb > 1 && (T + p.tb - 1) / p.tb < 2 * cus) p.tb /= 2;
     p.hb = n_head;
     while (p.hb > 1 && (int64_t) ((T + p.tb - 1) / p.tb) * ((n_head + p.hb - 1) / p.hb) < cus && p.hb * head_dim > 256 * (w ? V : 1)) p.hb = (p.hb + 1) / 2;
-    const int v = w ? V : 1, per_head = n_rot / 2 / v + (p.copy ? (head_dim - n_rot) / v : 0);
+    const int v = w ? V : 1, per_head = (layout == NXG_ROPE_HALF || v == 1 ? n_rot / 2 / v : n_rot / v) + (p.copy ? (head_dim - n_rot) / v : 0);
     if (per_head == 0) return NXG_OK;
     p.hb = std::min(p.hb, 65535 / per_head);
     while (p.tb > 1 && (int64_t) p.tb * p.hb * per_head * p.hb * per_head > INT32_MAX) p.tb /= 2;
