@@ -1134,12 +1134,16 @@ __device__ __forceinline__ void add_ds(float (&x)[2], const attn_p & p, const do
 }
 
 template <class E, int DT>
-__global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
-    constexpr int BM = 128, BN = 64, TILE = BN * SP<DT>;
-    __shared__ __align__(1024) E sk[2][TILE], sv[2][TILE];
-    __shared__ int s_job[8];
-    const int g = blockIdx.x % p.G;
-    const job todo = workgroup_job(p, false, p.R, BM, blockIdx.x / p.G, p.right >= 0 ? p.order == BY_ROWS : p.left >= 0 && p.order != BY_ROWS, s_job);
+struct dq_lds {
+    E sk[2][64 * SP<DT>], sv[2][64 * SP<DT>];
+};
+template <class E, int DT>
+__device__ __forceinline__ void dq_workgroup(const attn_p & p, int block, dq_lds<E, DT> & lds, int * s_job) {
+    constexpr int BM = 128, BN = 64;
+    auto & sk = lds.sk;
+    auto & sv = lds.sv;
+    const int g = block % p.G;
+    const job todo = workgroup_job(p, false, p.R, BM, block / p.G, p.right >= 0 ? p.order == BY_ROWS : p.left >= 0 && p.order != BY_ROWS, s_job);
     if (todo.tile < 0) return;
     const doc c = todo.c;
     const int np = c.n * p.R, p0 = todo.tile * BM;
@@ -1271,13 +1275,20 @@ __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const t
 // others. QG groups, one workgroup a CU: for launches that fit the CUs at once, where it would be a CU's longest
 // workgroup, alone at the end with a quarter of the waves, that takes the time.
 template <class E, int DT, int QG>
-__global__ __launch_bounds__(256 * QG, 2) void attn_rows_dkv_kernel(attn_p p) {
-    constexpr int BK = 128, SUB = QG == 1 ? 2 : 1, BQ = 32 * QG * SUB, TILE = BQ * SP<DT>;
-    __shared__ __align__(1024) E sq[2][TILE], so[2][TILE];
-    __shared__ __align__(16) float s_lse[2][128], s_delta[2][128];       // BQ of them used
-    __shared__ int s_job[8];
-    const int g = blockIdx.x % p.G;
-    const job todo = workgroup_job(p, true, 1, BK, blockIdx.x / p.G, p.right >= 0 && p.order != BY_ROWS, s_job);
+struct dkv_lds {
+    static constexpr int SUB = QG == 1 ? 2 : 1, BQ = 32 * QG * SUB;
+    E sq[2][BQ * SP<DT>], so[2][BQ * SP<DT>];
+    float s_lse[2][128], s_delta[2][128];       // BQ of them used
+};
+template <class E, int DT, int QG>
+__device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_lds<E, DT, QG> & lds, int * s_job) {
+    constexpr int BK = 128, SUB = dkv_lds<E, DT, QG>::SUB, BQ = dkv_lds<E, DT, QG>::BQ;
+    auto & sq = lds.sq;
+    auto & so = lds.so;
+    auto & s_lse = lds.s_lse;
+    auto & s_delta = lds.s_delta;
+    const int g = block % p.G;
+    const job todo = workgroup_job(p, true, 1, BK, block / p.G, p.right >= 0 && p.order != BY_ROWS, s_job);
     if (todo.tile < 0) return;
     const doc c = todo.c;
     const int np = c.n * p.R, kb0 = todo.tile * BK;
@@ -1416,6 +1427,35 @@ __global__ __launch_bounds__(256 * QG, 2) void attn_rows_dkv_kernel(attn_p p) {
         store_row<E>(p.dv.data + (int64_t) (c.k0 + j) * p.dv.ts + g * p.dv.hs, x, 1.0f, p.D);
         store_row<E>(p.dk.data + (int64_t) (c.k0 + j) * p.dk.ts + g * p.dk.hs, y, p.scale, p.D);
     }
+}
+
+// Both in one launch, dK and dV's workgroups first (they are the longer ones), so that the ends of the one
+// are filled by the others; or, where dK, dV take groups of waves, each by itself.
+template <class E, int DT>
+__global__ __launch_bounds__(256, 2) void attn_rows_grad_kernel(attn_p p, int n_dkv, int order_dq) {
+    __shared__ __align__(1024) union {
+        dq_lds<E, DT> dq;
+        dkv_lds<E, DT, 1> dkv;
+    } lds;
+    __shared__ int s_job[8];
+    if ((int) blockIdx.x < n_dkv) {
+        dkv_workgroup<E, DT, 1>(p, blockIdx.x, lds.dkv, s_job);
+    } else {
+        p.order = order_dq;
+        dq_workgroup<E, DT>(p, blockIdx.x - n_dkv, lds.dq, s_job);
+    }
+}
+template <class E, int DT>
+__global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
+    __shared__ __align__(1024) dq_lds<E, DT> lds;
+    __shared__ int s_job[8];
+    dq_workgroup<E, DT>(p, blockIdx.x, lds, s_job);
+}
+template <class E, int DT, int QG>
+__global__ __launch_bounds__(256 * QG, 2) void attn_rows_dkv_kernel(attn_p p) {
+    __shared__ __align__(1024) dkv_lds<E, DT, QG> lds;
+    __shared__ int s_job[8];
+    dkv_workgroup<E, DT, QG>(p, blockIdx.x, lds, s_job);
 }
 
 // ---------------------------------------------------------------------------
@@ -1646,23 +1686,28 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
             else attn_rows_delta_kernel<_Float16, 16><<<N_MAX, 1024, 0, s>>>(p);
         }
         NXG_TRY(nxg_launch_check(what));
-        p.n_slots = (int32_t) slots(p.T_q, p.R, 128, p.n_seqs);
-        p.order = work_order(p, (int64_t) p.n_slots * p.G);
-        NXG_BY_TYPE(a->type, p.D, (attn_rows_dq_kernel<E, DT><<<(unsigned) (p.n_slots * p.G), 256, 0, s>>>(p)));
-        NXG_TRY(nxg_launch_check(what));
     }
-    if (p.T_k > 0) {
-        p.n_slots = (int32_t) slots(p.T_k, 1, 128, p.n_seqs);
-        const unsigned grid = (unsigned) (p.n_slots * p.G);
-        p.order = work_order(p, grid);
-        // documents' ends differ in work where one side of the window is open and the other not
-        const bool uneven = (p.left < 0) != (p.right < 0);
-        const bool groups = grid <= (uneven ? 3u : 1u) * (unsigned) nxg_device_cus();
+    const unsigned n_dq = p.T_q > 0 ? (unsigned) (slots(p.T_q, p.R, 128, p.n_seqs) * p.G) : 0;
+    const unsigned n_dkv = p.T_k > 0 ? (unsigned) (slots(p.T_k, 1, 128, p.n_seqs) * p.G) : 0;
+    // documents' ends differ in work where one side of the window is open and the other not
+    const bool uneven = (p.left < 0) != (p.right < 0);
+    const bool groups = n_dkv <= (uneven ? 3u : 1u) * (unsigned) nxg_device_cus();
+    const int order_dq = work_order(p, n_dq);
+    p.order = work_order(p, n_dkv);
+    if (!groups) {
+        NXG_BY_TYPE(a->type, p.D, (attn_rows_grad_kernel<E, DT><<<n_dkv + n_dq, 256, 0, s>>>(p, (int) n_dkv, order_dq)));
+        return nxg_launch_check(what);
+    }
+    if (n_dkv > 0) {
         NXG_BY_TYPE(a->type, p.D, {
             constexpr int QG = DT <= 2 ? 3 : 2;
-            if (groups) attn_rows_dkv_kernel<E, DT, QG><<<grid, 256 * QG, 0, s>>>(p);
-            else attn_rows_dkv_kernel<E, DT, 1><<<grid, 256, 0, s>>>(p);
+            attn_rows_dkv_kernel<E, DT, QG><<<n_dkv, 256 * QG, 0, s>>>(p);
         });
+        NXG_TRY(nxg_launch_check(what));
+    }
+    if (n_dq > 0) {
+        p.order = order_dq;
+        NXG_BY_TYPE(a->type, p.D, (attn_rows_dq_kernel<E, DT><<<n_dq, 256, 0, s>>>(p)));
         NXG_TRY(nxg_launch_check(what));
     }
     return NXG_OK;
