@@ -841,7 +841,7 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
         wait_all();
         if (j + 4 < j_hi) keys.next(lds_addr(lds[wave][buf ^ 1][0]), lds_addr(lds[wave][buf ^ 1][1]));
         const int j0 = j * BN;
-v16f s = fwd_scores<E, DT>(q, lds_addr(lds[wave][buf][0]) + at.row, 0), w;
+        v16f s = fwd_scores<E, DT>(q, lds_addr(lds[wave][buf][0]) + at.row, 0), w;
         const int sides = (j0 < all_lo ? 1 : 0) | (j0 + BN > all_hi ? 2 : 0);
         if (sides) mask_rows(s, sides, lo - j0, hi - j0, -INFINITY);
         fwd_weights<DT>(w, s, st, cs);
@@ -1270,19 +1270,15 @@ __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const t
     }
 }
 
-// A workgroup: 128 keys, 4 waves of 32; QG groups of waves with the same keys take every QG'th 32 pairs and
-// add their sums at the end. One group, several workgroups a CU: a workgroup's start and end hide behind the
-// others. QG groups, one workgroup a CU: for launches that fit the CUs at once, where it would be a CU's longest
-// workgroup, alone at the end with a quarter of the waves, that takes the time.
-template <class E, int DT, int QG>
+// A workgroup: 128 keys, 4 waves of 32.
+template <class E, int DT>
 struct dkv_lds {
-    static constexpr int SUB = QG == 1 ? 2 : 1, BQ = 32 * QG * SUB;
-    E sq[2][BQ * SP<DT>], so[2][BQ * SP<DT>];
-    float s_lse[2][128], s_delta[2][128];       // BQ of them used
+    E sq[2][64 * SP<DT>], so[2][64 * SP<DT>];
+    float s_lse[2][64], s_delta[2][64];
 };
-template <class E, int DT, int QG>
-__device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_lds<E, DT, QG> & lds, int * s_job) {
-    constexpr int BK = 128, SUB = dkv_lds<E, DT, QG>::SUB, BQ = dkv_lds<E, DT, QG>::BQ;
+template <class E, int DT>
+__device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_lds<E, DT> & lds, int * s_job) {
+    constexpr int BK = 128, BQ = 64;
     auto & sq = lds.sq;
     auto & so = lds.so;
     auto & s_lse = lds.s_lse;
@@ -1293,7 +1289,7 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
     const doc c = todo.c;
     const int np = c.n * p.R, kb0 = todo.tile * BK;
 
-    const int wave = uni(threadIdx.x >> 6) % 4, group = uni(threadIdx.x >> 8), lane = threadIdx.x & 63;
+    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int kw = kb0 + 32 * wave;
     const bool active = kw < c.m;
     const int key = min(kw + (lane & 31), c.m - 1);
@@ -1304,12 +1300,12 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
     const int some_lo = tok_lo(p, c, ka) * p.R, some_hi = tok_hi(p, c, ke) * p.R;
     const int all_lo = tok_lo(p, c, ke) * p.R, all_hi = tok_hi(p, c, ka) * p.R;
 
-    tile_loader<DT, BQ, 256 * QG> lq(p.D), l_out(p.D);
+    tile_loader<DT, BQ, 256> lq(p.D), l_out(p.D);
     lq.pairs_at(p.R, p.q.ts, p.q.hs);
     l_out.pairs_at(p.R, p.dout.ts, p.dout.hs);
     if (p.D != 32 * DT) {
-        clear(sq, sizeof(sq), threadIdx.x, 256 * QG);
-        clear(so, sizeof(so), threadIdx.x, 256 * QG);
+        clear(sq, sizeof(sq), threadIdx.x, 256);
+        clear(so, sizeof(so), threadIdx.x, 256);
         barrier();
     }
     auto load = [&](int j, int buf) {
@@ -1325,12 +1321,12 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
             lq.load_each(lds_addr(sq[buf]), [&](int r) { return at(p.q, r); });
             l_out.load_each(lds_addr(so[buf]), [&](int r) { return at(p.dout, r); });
         }
-        // the pairs' sums, 64 a wave (behind the document: whatever is there, masked)
-        if (group == 0 && wave < 2 * ((BQ + 63) / 64)) {
+        // the pairs' sums, by waves 0 and 1 (behind the document: whatever is there, masked)
+        if (wave < 2) {
             int t = threadIdx.x;
             asm volatile("" : "+v"(t));
-            const float * from = (wave & 1 ? p.ndelta : p.lse2) + ((int64_t) g * p.T_q + c.q0) * p.R + j0 + (wave >> 1) * 64;
-            dma4s(uni((const char *) from), (t & 63) * 4, lds_addr((wave & 1 ? s_delta[buf] : s_lse[buf]) + (wave >> 1) * 64));
+            const float * from = (wave ? p.ndelta : p.lse2) + ((int64_t) g * p.T_q + c.q0) * p.R + j0;
+            dma4s(uni((const char *) from), (t & 63) * 4, lds_addr(wave ? s_delta[buf] : s_lse[buf]));
         }
     };
     v16f dk[DT], dv[DT];
@@ -1358,48 +1354,13 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
                 hi = tok_hi(p, c, j) * p.R - j0;
             }
 #pragma unroll 1
-            for (int a = 32 * SUB * group; a < 32 * SUB * (group + 1); a += 32) {
+            for (int a = 0; a < BQ; a += 32) {
                 dkv_tile<E, DT>(dk, dv, k, v, at, lds_addr(sq[buf]) + a * SP<DT> * 2, lds_addr(so[buf]) + a * SP<DT> * 2, lds_addr(s_lse[buf]) + 4 * a,
                                 lds_addr(s_delta[buf]) + 4 * a, cs, factor, sides, lo - a, hi - a);
             }
         }
     }
     barrier();
-    if constexpr (QG > 1) {
-        // the groups' sums one after another into the first's, through LDS
-        int t = threadIdx.x;
-        asm volatile("" : "+v"(t));            // not kept in a register over the loop
-        float * sums = reinterpret_cast<float *>(wave < 2 ? sq : so) + (wave & 1) * DT * 16 * 64 + (t & 63) * 4;
-        static_assert(2 * DT * 16 * 64 * 4 <= (int) sizeof(sq), "two waves' sums in half of the tiles");
-        auto join = [&](v16f (&x)[DT]) {
-#pragma unroll
-            for (int q = 1; q < QG; ++q) {
-                if (group == q) {
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            *reinterpret_cast<v4f *>(sums + (4 * d + i) * 256) = v4f{x[d][4 * i], x[d][4 * i + 1], x[d][4 * i + 2], x[d][4 * i + 3]};
-                }
-                barrier();
-                if (group == 0) {
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const v4f y = *reinterpret_cast<const v4f *>(sums + (4 * d + i) * 256);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) x[d][4 * i + k] += y[k];
-                            if (i & 1) __builtin_amdgcn_sched_barrier(0);      // not all reads at once: registers
-                        }
-                }
-                barrier();
-            }
-        };
-        join(dv);
-        join(dk);
-        if (group) return;
-    }
     if (!active) return;
     E * tile = (wave < 2 ? sq[0] : so[0]) + (wave & 1) * 32 * SP<DT>;
     auto dst = [&](const rows & x) {
@@ -1429,33 +1390,22 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
     }
 }
 
-// Both in one launch, dK and dV's workgroups first (they are the longer ones), so that the ends of the one
-// are filled by the others; or, where dK, dV take groups of waves, each by itself.
+// Both in one launch, dK and dV's workgroups first (they are the longer ones), so that the end of the one is
+// filled by the others: against a launch each, 8 x 1,024 tokens banded 71 -> 58 us, one document of 8,192 causal
+// 720 -> 535 us (64 values a head) and 1,176 -> 1,037 (128).
 template <class E, int DT>
 __global__ __launch_bounds__(256, 2) void attn_rows_grad_kernel(attn_p p, int n_dkv, int order_dq) {
     __shared__ __align__(1024) union {
         dq_lds<E, DT> dq;
-        dkv_lds<E, DT, 1> dkv;
+        dkv_lds<E, DT> dkv;
     } lds;
     __shared__ int s_job[8];
     if ((int) blockIdx.x < n_dkv) {
-        dkv_workgroup<E, DT, 1>(p, blockIdx.x, lds.dkv, s_job);
+        dkv_workgroup<E, DT>(p, blockIdx.x, lds.dkv, s_job);
     } else {
         p.order = order_dq;
         dq_workgroup<E, DT>(p, blockIdx.x - n_dkv, lds.dq, s_job);
     }
-}
-template <class E, int DT>
-__global__ __launch_bounds__(256, 2) void attn_rows_dq_kernel(attn_p p) {
-    __shared__ __align__(1024) dq_lds<E, DT> lds;
-    __shared__ int s_job[8];
-    dq_workgroup<E, DT>(p, blockIdx.x, lds, s_job);
-}
-template <class E, int DT, int QG>
-__global__ __launch_bounds__(256 * QG, 2) void attn_rows_dkv_kernel(attn_p p) {
-    __shared__ __align__(1024) dkv_lds<E, DT, QG> lds;
-    __shared__ int s_job[8];
-    dkv_workgroup<E, DT, QG>(p, blockIdx.x, lds, s_job);
 }
 
 // ---------------------------------------------------------------------------
@@ -1536,21 +1486,21 @@ int32_t check_rows(const char * what, const char * name, const nxg_rows * x, int
 #define NXG_TRY(call) do { const int32_t rc_ = (call); if (rc_) return rc_; } while (0)
 
 // Values of a row array of the backward pass: one a (token, head), and a tile's reach behind the last.
-int64_t row_values(const attn_p & p) { return (int64_t) p.T_q * p.H + 128; }
+int64_t row_values(const attn_p & p) { return (int64_t) p.T_q * p.H + 64; }
 int64_t backward_bytes(const attn_p & p) { return (2 * N_MAX + 2 * row_values(p)) * 4; }
 
 // Launches one of a kernel's instances by type and head size.
-#define NXG_BY_TYPE(type, D, ...)                                                  \
+#define NXG_BY_TYPE(type, D, LAUNCH)                                               \
     do {                                                                           \
-        if ((type) == NXG_TYPE_BF16) { typedef __bf16 E; NXG_BY_DIM(D, __VA_ARGS__); }  \
-        else { typedef _Float16 E; NXG_BY_DIM(D, __VA_ARGS__); }                   \
+        if ((type) == NXG_TYPE_BF16) { typedef __bf16 E; NXG_BY_DIM(D, LAUNCH); }  \
+        else { typedef _Float16 E; NXG_BY_DIM(D, LAUNCH); }                        \
     } while (0)
-#define NXG_BY_DIM(D, ...)                                                         \
+#define NXG_BY_DIM(D, LAUNCH)                                                      \
     do {                                                                           \
-        if ((D) <= 32) { constexpr int DT = 1; __VA_ARGS__; }                           \
-        else if ((D) <= 64) { constexpr int DT = 2; __VA_ARGS__; }                      \
-        else if ((D) <= 96) { constexpr int DT = 3; __VA_ARGS__; }                      \
-        else { constexpr int DT = 4; __VA_ARGS__; }                                     \
+        if ((D) <= 32) { constexpr int DT = 1; LAUNCH; }                           \
+        else if ((D) <= 64) { constexpr int DT = 2; LAUNCH; }                      \
+        else if ((D) <= 96) { constexpr int DT = 3; LAUNCH; }                      \
+        else { constexpr int DT = 4; LAUNCH; }                                     \
     } while (0)
 
 // Documents in the order of their rows where the workgroups fit the CUs at once, where there is one
@@ -1689,28 +1639,9 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
     }
     const unsigned n_dq = p.T_q > 0 ? (unsigned) (slots(p.T_q, p.R, 128, p.n_seqs) * p.G) : 0;
     const unsigned n_dkv = p.T_k > 0 ? (unsigned) (slots(p.T_k, 1, 128, p.n_seqs) * p.G) : 0;
-    // documents' ends differ in work where one side of the window is open and the other not
-    const bool uneven = (p.left < 0) != (p.right < 0);
-    const bool groups = n_dkv <= (uneven ? 3u : 1u) * (unsigned) nxg_device_cus();
-    const int order_dq = work_order(p, n_dq);
     p.order = work_order(p, n_dkv);
-    if (!groups) {
-        NXG_BY_TYPE(a->type, p.D, (attn_rows_grad_kernel<E, DT><<<n_dkv + n_dq, 256, 0, s>>>(p, (int) n_dkv, order_dq)));
-        return nxg_launch_check(what);
-    }
-    if (n_dkv > 0) {
-        NXG_BY_TYPE(a->type, p.D, {
-            constexpr int QG = DT <= 2 ? 3 : 2;
-            attn_rows_dkv_kernel<E, DT, QG><<<n_dkv, 256 * QG, 0, s>>>(p);
-        });
-        NXG_TRY(nxg_launch_check(what));
-    }
-    if (n_dq > 0) {
-        p.order = order_dq;
-        NXG_BY_TYPE(a->type, p.D, (attn_rows_dq_kernel<E, DT><<<n_dq, 256, 0, s>>>(p)));
-        NXG_TRY(nxg_launch_check(what));
-    }
-    return NXG_OK;
+    NXG_BY_TYPE(a->type, p.D, (attn_rows_grad_kernel<E, DT><<<n_dkv + n_dq, 256, 0, s>>>(p, (int) n_dkv, work_order(p, n_dq))));
+    return nxg_launch_check(what);
 }
 
 } // extern "C"

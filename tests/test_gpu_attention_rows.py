@@ -286,3 +286,62 @@ def test_gradients_leave_out_what_is_not_seen(nxg, torch, dev, dtype, D, bad):
         for t in (100, 149, 160):
             tensors[bad][t] = math.nan
         run_and_check(nxg, torch, dt, lens, H=4, G=2, D=D, left=left, right=right, inputs=tuple(tensors.values()))
+
+
+@pytest.mark.parametrize("left,right", [(-1, -1), (-1, 0), (7, -1), (70, 70)])
+@pytest.mark.parametrize("H,G,D,same", [(16, 16, 32, True), (32, 16, 64, False)])
+def test_documents_of_mixed_lengths(nxg, torch, dev, left, right, H, G, D, same):
+    """Documents enough for more workgroups than run at once, among them empty ones and many of one length:
+    every tile of every one is done once, in whatever order. More queries than keys, and fewer."""
+    say(f"attention_rows 61 documents H={H} G={G} D={D} window={left},{right}")
+    rng = np.random.default_rng(9)
+    lens = [0, 400, 1, 128, 128, 256, 0, 129, 127] + [int(n) for n in rng.integers(0, 200, 50)] + [300, 0]
+    keys = lens if same else [int(n) for n in rng.integers(0, 260, len(lens))]
+    run_and_check(nxg, torch, torch.bfloat16, lens, keys, H=H, G=G, D=D, left=left, right=right, seed=D)
+
+
+@pytest.mark.parametrize("n", [63, 64, 65, 130])
+def test_number_of_documents(nxg, torch, dev, n):
+    """About as many documents as a wave has lanes, and more."""
+    say(f"attention_rows {n} documents")
+    run_and_check(nxg, torch, torch.float16, [(37 * i) % 150 for i in range(n)], H=16, G=16, D=32, right=0, seed=n)
+
+
+@pytest.mark.parametrize("stride,lens", [(8_000_000, [250, 50]), (20_000_000, [130, 7])], ids=str)
+@pytest.mark.parametrize("H,G", [(4, 2), (128, 128), (128, 64), (96, 32)])
+def test_rows_far_apart(nxg, torch, dev, stride, lens, H, G):
+    """Rows over more than 4 GiB: a tile's own offsets fit 32 bits, or do not either."""
+    say(f"attention_rows H={H} G={G} rows {2 * stride} bytes apart")
+    T, D = sum(lens), 64
+    need = (T - 1) * stride + 4 * (H + G) * D
+    buf = torch.empty(need, dtype=torch.bfloat16, device="cuda")
+    at, views = 0, []
+    for n in (H, H, H, H, G, G, G, G):
+        views.append(buf.as_strided((T, n, D), (stride, D, 1), at))
+        at += n * D
+    q, do, out, dq, k, v, dk, dv = views
+    g = torch.Generator(device="cuda").manual_seed(H)
+    for t in (q, do, k, v):
+        t.copy_(torch.randn(t.shape, device="cuda", generator=g))
+    cu = offsets(lens)
+    ref = rows_ref.attention(q.contiguous(), k.contiguous(), v.contiguous(), cu, cu, 0.125, -1, 0, do.contiguous())
+    _, lse = nxg.attention_rows(q, k, v, cu, left=-1, right=0, out=out)
+    nxg.attention_rows_backward(do, q, k, v, out, lse, cu, left=-1, right=0, dq=dq, dk=dk, dv=dv)
+    for name, t in (("out", out), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
+        rows_ref.check(name, t, *ref[name])
+
+
+@pytest.mark.parametrize("n,stride", [(1, 8_000_000), (1, 20_000_000), (3, 20_000_000)])
+def test_few_queries_over_a_far_cache(nxg, torch, dev, n, stride):
+    say(f"attention_rows {n} queries over keys {2 * stride} bytes apart")
+    K, H, G, D = 600, 4, 2, 128
+    buf = torch.empty((K - 1) * stride + 2 * G * D, dtype=torch.bfloat16, device="cuda")
+    k, v = (buf.as_strided((K, G, D), (stride, D, 1), i * G * D) for i in range(2))
+    g = torch.Generator(device="cuda").manual_seed(n)
+    for t in (k, v):
+        t.copy_(torch.randn(t.shape, device="cuda", generator=g))
+    q = torch.randn(n, H, D, device="cuda", generator=g).bfloat16()
+    out, lse = nxg.attention_rows(q, k, v, [0, n], [0, K], right=0)
+    ref = rows_ref.attention(q, k.contiguous(), v.contiguous(), [0, n], [0, K], 1 / math.sqrt(D), -1, 0)
+    rows_ref.check("out", out, *ref["out"])
+    rows_ref.check("lse", lse, *ref["lse"])

@@ -221,3 +221,32 @@ def test_layer_norm_gradient_against_differences(nxg, torch, dev):
         want = float((grad.double() * step).sum())
         # fp32 roundings of the gradient (2^-18 of its size is far above them) and the third-order term
         assert abs(diff - want) <= 2.0 ** -18 * float((grad.double().abs() * step.abs()).sum()) + 2.0 ** -36, (i, diff, want)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rope_rows_far_apart(nxg, torch, dev, layout):
+    """Rows over more than 4 GiB, in and out."""
+    say(f"rope_rows {layout} far apart")
+    T, H, D, stride = 130, 5, 64, 20_000_000
+    buf = torch.empty((T - 1) * stride + 2 * H * D, dtype=torch.bfloat16, device="cuda")
+    x, out = (buf.as_strided((T, H, D), (stride, D, 1), i * H * D) for i in range(2))
+    x.copy_(randn(torch, 1, "bfloat16", T, H, D))
+    f = torch.from_numpy(nxg.rope_frequencies(D, 10000.0)[0]).cuda()
+    nxg.rope_rows(x, f, [0, 100, T], layout=layout, out=out)
+    rows_ref.check("y", out, *rows_ref.rope(x.contiguous(), f, torch.from_numpy(positions_of([100, 30])).cuda(), layout, 1.0, False))
+
+
+@pytest.mark.parametrize("C", [1024, 1000, 9000])
+def test_layer_norm_rows_far_apart(nxg, torch, dev, C):
+    say(f"layer_norm_rows far apart C={C}")
+    T, stride = 130, 20_000_000
+    buf = torch.empty((T - 1) * stride + 3 * C, dtype=torch.bfloat16, device="cuda")
+    x, dy, out = (buf.as_strided((T, C), (stride, 1), i * C) for i in range(3))
+    x.copy_(randn(torch, 3, "bfloat16", T, C))
+    dy.copy_(randn(torch, 4, "bfloat16", T, C))
+    w, b = randn(torch, 1, "float32", C), randn(torch, 2, "float32", C)
+    y, mean, rstd = nxg.layer_norm_rows(x, w, b, 1e-5, out=out)
+    rows_ref.check("y", y, *rows_ref.layer_norm(x.contiguous(), w, b, 1e-5)[0])
+    ref = rows_ref.layer_norm_back(dy.contiguous(), x.contiguous(), mean, rstd, w)
+    for name, t, r in zip(("dx", "dw", "db"), nxg.layer_norm_rows_backward(dy, x, mean, rstd, w, dx=out), ref):
+        rows_ref.check(name, t, *r)
