@@ -67,7 +67,8 @@ NXG_API int32_t nxg_rope_frequencies(int32_t n_rot, double base, int32_t scaling
  * it turns by -t: the gradient of the same call (with mscale as in the forward call), and the
  * sense in which the encoder's nxg_qk_prep turns. Angles are position * frequency in 64 bits, less
  * whole turns, so that far positions keep theirs.
- *   x, out     device rows of `type`, [T][n_head][head_dim]; out may be x (same strides)
+ *   x, out     device rows of `type`, [T][n_head][head_dim]; out may be x (same strides). Sizes that would take
+ *              2^24 workgroups of about 12 KiB of rows are refused
  *   freq       device double [n_rot / 2];  n_rot even, 0 < n_rot <= head_dim <= 1024
  *   positions  device int32 [T] (any value), or null: the row's place in its document by cu
  *   cu         device int32 [n_seqs + 1] (positions null); rows outside the documents count from the
@@ -82,7 +83,8 @@ NXG_API int32_t nxg_rope_rows(int32_t type, const nxg_rows * x, int32_t T, int32
  * ------------------------------------------------------------------------- */
 
 /* y = (x - mean) * rstd * w + b per row, rstd = 1 / sqrt(mean((x - mean)^2) + eps).
- *   x, y         device rows of `type`, T x C, x_stride and y_stride values apart (y may be x)
+ *   x, y         device rows of `type`, T x C, x_stride and y_stride values apart (y may be x, with its stride);
+ *                C at most 2^23, T below 2^24 (2^26 with C up to 1,024)
  *   w, b         device [C] of w_type (`type` or F32), or null: 1 and 0
  *   mean, rstd   device float [T], or null: what nxg_layer_norm_rows_backward takes */
 NXG_API int32_t nxg_layer_norm_rows(int32_t type, const void * x, int64_t x_stride, const void * w, const void * b,
@@ -94,7 +96,7 @@ NXG_API int32_t nxg_layer_norm_rows(int32_t type, const void * x, int64_t x_stri
  * The sums over rows are taken in a fixed order: the same call gives the same bits.
  *   dy, x        device rows of `type`;  mean, rstd  as nxg_layer_norm_rows left them
  *   w            device [C] of w_type, or null: 1
- *   dx           device rows of `type`, or null;  may be dy or x
+ *   dx           device rows of `type`, or null;  may be dy or x, with its stride
  *   dw, db       device [C] of w_type, or null;  T = 0 gives zeros
  *   workspace    device memory, 16-byte aligned, nxg_layer_norm_rows_workspace_bytes(T, C) bytes (none with dw and db null) */
 NXG_API int64_t nxg_layer_norm_rows_workspace_bytes(int32_t T, int32_t C);
@@ -114,7 +116,8 @@ NXG_API int32_t nxg_layer_norm_rows_backward(int32_t type, const void * dy, int6
 typedef struct nxg_attention_rows_params {
     int32_t type;              /* of every row: NXG_TYPE_F16 or NXG_TYPE_BF16 */
     int32_t n_head, n_kv_head, head_dim;   /* head_dim: a multiple of 8, at most 128 */
-    int32_t T_q, T_k;          /* rows of q and out, and of k and v */
+    int32_t T_q, T_k;          /* rows of q and out, and of k and v: up to 2^30, T_q * n_head and T_k * n_kv_head below 2^31,
+                                * and n_kv_head * 128-row tiles of both below 2^24 (a document more: a tile more) */
     int32_t n_seqs;
     const int32_t * cu_q;      /* device int32 [n_seqs + 1] */
     const int32_t * cu_k;

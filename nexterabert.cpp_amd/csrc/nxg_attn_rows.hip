@@ -1415,6 +1415,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_grad_kernel(attn_p p, int n_
 int64_t slots(int64_t T, int64_t mul, int64_t tile, int64_t n_seqs) { return T * mul / tile + n_seqs; }
 
 constexpr int64_t MAX_T = 1 << 30;
+constexpr int64_t MAX_GRID = (1 << 24) - 1;    // workgroups of a launch: less than 2^32 threads
 
 int32_t check_params(const char * what, const nxg_attention_rows_params * a, attn_p & p) {
     if (!a) return nxg_fail(NXG_EINVAL, "%s: null parameters", what);
@@ -1446,7 +1447,7 @@ int32_t check_params(const char * what, const nxg_attention_rows_params * a, att
     p.cu_q = a->cu_q;
     p.cu_k = a->cu_k;
     if ((int64_t) p.T_q * p.H > INT32_MAX - 256 || (int64_t) p.T_k * p.G > INT32_MAX ||
-        (slots(p.T_q, p.R, 32, p.n_seqs)) * p.G > INT32_MAX / 64 || slots(p.T_k, 1, 128, p.n_seqs) * p.G > INT32_MAX) {
+        (slots(p.T_q, p.R, 128, p.n_seqs) + slots(p.T_k, 1, 128, p.n_seqs)) * p.G > MAX_GRID) {
         return nxg_fail(NXG_EINVAL, "%s: T_q=%d T_k=%d of %d heads is too large", what, p.T_q, p.T_k, p.H);
     }
     p.n_split = 1;

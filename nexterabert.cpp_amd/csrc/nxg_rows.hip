@@ -424,10 +424,13 @@ constexpr int NORM_PARTS = 512;        // workgroups of the gradients' kernels: 
 bool wide(const void * p, int64_t stride, int es) { return ((uintptr_t) p & 15) == 0 && stride * es % 16 == 0; }
 bool aligned(const void * p, int es) { return ((uintptr_t) p & (es - 1)) == 0; }
 
+constexpr int MAX_GRID = (1 << 24) - 1;        // workgroups of a launch: less than 2^32 threads
+constexpr int MAX_C = 1 << 23;
 int32_t check_norm(const char * what, int32_t type, int32_t w_type, int32_t T, int32_t C) {
     if (!size_of(type)) return nxg_fail(NXG_EINVAL, "%s: type %d (F32, F16 or BF16)", what, type);
     if (w_type != type && w_type != NXG_TYPE_F32) return nxg_fail(NXG_EINVAL, "%s: weight type %d (the rows' or F32)", what, w_type);
     if (T < 0 || C < 1) return nxg_fail(NXG_EINVAL, "%s: T=%d C=%d", what, T, C);
+    if (C > MAX_C || T > (C <= 1024 ? 4 : 1) * MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d C=%d is too large", what, T, C);
     return NXG_OK;
 }
 int32_t check_norm_rows(const char * what, const char * name, const void * p, int64_t stride, int32_t T, int32_t C, int es, bool written) {
@@ -538,7 +541,6 @@ int32_t nxg_rope_rows(int32_t type, const nxg_rows * x, int32_t T, int32_t n_hea
     p.o_ts = T > 1 ? out->token_stride : 0;
     p.o_hs = n_head > 1 ? out->head_stride : 0;
     if (p.x == p.out && (p.x_ts != p.o_ts || p.x_hs != p.o_hs)) return nxg_fail(NXG_EINVAL, "%s: out is x with other strides", what);
-    NXG_TRY(nxg_check_device());
     p.copy = p.x != p.out;
     p.freq = freq;
     p.positions = positions;
@@ -558,9 +560,9 @@ int32_t nxg_rope_rows(int32_t type, const nxg_rows * x, int32_t T, int32_t n_hea
     // work; heads in pieces too for the shortest
     const int cus = nxg_device_cus();
     p.tb = std::max<int>(1, std::min<int64_t>(512 / n_rot, 12288 / ((int64_t) n_head * head_dim * es)));
-    while (p.tb > 1 && (T + p.tb - 1) / p.tb < 2 * cus) p.tb /= 2;
+    while (p.tb > 1 && ((int64_t) T + p.tb - 1) / p.tb < 2 * cus) p.tb /= 2;
     p.hb = n_head;
-    while (p.hb > 1 && (int64_t) ((T + p.tb - 1) / p.tb) * ((n_head + p.hb - 1) / p.hb) < cus && p.hb * head_dim > 256 * (w ? V : 1)) p.hb = (p.hb + 1) / 2;
+    while (p.hb > 1 && ((int64_t) T + p.tb - 1) / p.tb * ((n_head + p.hb - 1) / p.hb) < cus && p.hb * head_dim > 256 * (w ? V : 1)) p.hb = (p.hb + 1) / 2;
     const int v = w ? V : 1, per_head = (layout == NXG_ROPE_HALF || v == 1 ? n_rot / 2 / v : n_rot / v) + (p.copy ? (head_dim - n_rot) / v : 0);
     if (per_head == 0) return NXG_OK;
     p.hb = std::min(p.hb, 65535 / per_head);
@@ -569,8 +571,11 @@ int32_t nxg_rope_rows(int32_t type, const nxg_rows * x, int32_t T, int32_t n_hea
     p.by_head = magic(per_head);
     p.by_token = magic(per_head * p.hb);
     p.by_token_last = magic(per_head * ((n_head - 1) % p.hb + 1));
-    const dim3 grid((unsigned) ((T + p.tb - 1) / p.tb), (unsigned) ((n_head + p.hb - 1) / p.hb));
-    if (grid.y > 65535 || (int64_t) p.tb * p.hb * head_dim > INT32_MAX) return nxg_fail(NXG_EINVAL, "%s: n_head=%d", what, n_head);
+    const dim3 grid((unsigned) (((int64_t) T + p.tb - 1) / p.tb), (unsigned) (((int64_t) n_head + p.hb - 1) / p.hb));
+    if (grid.y > 65535 || (int64_t) grid.x * grid.y > MAX_GRID) {
+        return nxg_fail(NXG_EINVAL, "%s: T=%d n_head=%d is too large", what, T, n_head);
+    }
+    NXG_TRY(nxg_check_device());
     const size_t lds = (size_t) p.tb * (n_rot / 2) * sizeof(float2);
     hipStream_t s = (hipStream_t) stream;
     by_type(type, [&](auto e) {
@@ -597,6 +602,7 @@ int32_t nxg_layer_norm_rows(int32_t type, const void * x, int64_t x_stride, cons
     NXG_TRY(check_norm_rows(what, "x", x, x_stride, T, C, es, false));
     NXG_TRY(check_norm_rows(what, "y", y, y_stride, T, C, es, true));
     if ((w && !aligned(w, ws)) || (b && !aligned(b, ws))) return nxg_fail(NXG_EINVAL, "%s: w or b is not aligned to its type", what);
+    if (x == y && T > 1 && x_stride != y_stride) return nxg_fail(NXG_EINVAL, "%s: y is x with another stride", what);
     NXG_TRY(nxg_check_device());
     norm_p p = {};
     p.x = x;
@@ -627,7 +633,8 @@ int32_t nxg_layer_norm_rows(int32_t type, const void * x, int64_t x_stride, cons
 }
 
 int64_t nxg_layer_norm_rows_workspace_bytes(int32_t T, int32_t C) {
-    if (T < 0 || C < 1) return -nxg_fail(NXG_EINVAL, "layer_norm_rows_workspace_bytes: T=%d C=%d", T, C);
+    const int32_t rc = check_norm("layer_norm_rows_workspace_bytes", NXG_TYPE_F32, NXG_TYPE_F32, T, C);
+    if (rc) return -rc;
     return (int64_t) norm_parts(T, C) * 2 * C * 4;
 }
 
@@ -647,6 +654,9 @@ int32_t nxg_layer_norm_rows_backward(int32_t type, const void * dy, int64_t dy_s
         NXG_TRY(check_norm_rows(what, "x", x, x_stride, T, C, es, false));
         if (dx) NXG_TRY(check_norm_rows(what, "dx", dx, dx_stride, T, C, es, true));
         if (!mean || !rstd) return nxg_fail(NXG_EINVAL, "%s: null mean or rstd", what);
+        if (dx && T > 1 && ((dx == dy && dx_stride != dy_stride) || (dx == x && dx_stride != x_stride))) {
+            return nxg_fail(NXG_EINVAL, "%s: dx is dy or x with another stride", what);
+        }
     }
     norm_p p = {};
     p.n_part = T > 0 ? norm_parts(T, C) : 0;
@@ -686,10 +696,11 @@ int32_t nxg_layer_norm_rows_backward(int32_t type, const void * dy, int64_t dy_s
                 }
             });
             if (done) return;
-            if (dx) layer_norm_back_long_kernel<E, W><<<(unsigned) T, 256, 0, s>>>(p);
+            // the columns first: dx may be dy or x
             if (p.part) {
                 layer_norm_back_columns_kernel<E><<<dim3((unsigned) p.n_part, (unsigned) ((C + 255) / 256)), 256, 0, s>>>(p);
             }
+            if (dx) layer_norm_back_long_kernel<E, W><<<(unsigned) T, 256, 0, s>>>(p);
         });
         NXG_TRY(nxg_launch_check(what));
     }

@@ -250,3 +250,18 @@ def test_layer_norm_rows_far_apart(nxg, torch, dev, C):
     ref = rows_ref.layer_norm_back(dy.contiguous(), x.contiguous(), mean, rstd, w)
     for name, t, r in zip(("dx", "dw", "db"), nxg.layer_norm_rows_backward(dy, x, mean, rstd, w, dx=out), ref):
         rows_ref.check(name, t, *r)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [64, 1000, 4096, 9000])
+@pytest.mark.parametrize("into", ["dy", "x"])
+def test_layer_norm_gradients_in_place(nxg, torch, dev, dtype, C, into):
+    """dx over dy or over x: the weights' gradients are those of the rows as they were."""
+    say(f"layer_norm_rows_backward {dtype} C={C} dx over {into}")
+    T = 600
+    x, dy, w = randn(torch, 1, dtype, T, C), randn(torch, 2, dtype, T, C), randn(torch, 3, "float32", C)
+    _, mean, rstd = nxg.layer_norm_rows(x, w)
+    want = nxg.layer_norm_rows_backward(dy, x, mean, rstd, w)
+    got = nxg.layer_norm_rows_backward(dy, x, mean, rstd, w, dx=dy if into == "dy" else x)
+    for name, a, b in zip(("dx", "dw", "db"), got, want):
+        assert torch.equal(a, b), name

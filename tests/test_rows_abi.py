@@ -199,3 +199,22 @@ def test_host_tensors_refused(nxg):
         nxg.attention_rows(q.float(), q.float(), q.float(), [0, 4])
     with pytest.raises(ValueError, match="does not take"):
         nxg.layer_norm_rows(x.double())
+
+
+def test_sizes_past_a_launch_refused(nxg, L):
+    """More workgroups than a launch has: said before any device work."""
+    for kw in ({"T_q": 1 << 30, "n_head": 1, "n_kv_head": 1, "T_k": 1 << 30}, {"n_seqs": 1 << 24}, {"T_k": 1 << 29, "n_kv_head": 4}):
+        refused(nxg, L, forward(nxg, L, params(nxg, **kw)), "too large")
+    x, n = ctypes.byref(rows(nxg, ts=64)), 1 << 25
+    refused(nxg, L, L.nxg_rope_rows(nxg.TYPE_F32, x, n, 100, 64, P16, 64, 0, 1.0, 0, None, P16, 1, ctypes.byref(rows(nxg, data=2 * P16, ts=6400)), None), "too large")
+    for T, C in ((1 << 24, 1025), (1 << 26, 1024), (4, (1 << 23) + 1)):
+        refused(nxg, L, L.nxg_layer_norm_rows(nxg.TYPE_F32, P16, C, None, None, nxg.TYPE_F32, 1e-5, T, C, P16, C, None, None, None), "too large")
+        assert L.nxg_layer_norm_rows_workspace_bytes(T, C) == -nxg.NXG_EINVAL
+
+
+def test_layer_norm_in_place_with_another_stride_refused(nxg, L):
+    f32 = nxg.TYPE_F32
+    refused(nxg, L, L.nxg_layer_norm_rows(f32, P16, 128, None, None, f32, 1e-5, 4, 64, P16, 64, None, None, None), "another stride")
+    for dys, xs, dx in ((128, 64, P16), (64, 128, 2 * P16)):
+        refused(nxg, L, L.nxg_layer_norm_rows_backward(f32, P16, dys, 2 * P16, xs, P16, P16, None, f32, 4, 64, dx, 64, None, None, None, 0, None),
+                "another stride")
