@@ -73,10 +73,13 @@ struct attn_p {
     float * lse2, * ndelta;    // for the backward pass, a KV head's pairs one after another ([G][T_q R]): log2 of the sums, -delta
     float * maxima;            // [N_MAX][2]: largest |dout row|^2 and |v row|^2 (fp16)
     float * part;              // partial sums of the split forward pass
+    float * part_q, * part_kv; // partial gradients: [split_q][G][T_q R][D], [split_kv][dK, dV][G][T_k][D]
     const int32_t * cu_q, * cu_k;
-    int32_t n_seqs, T_q, T_k, H, G, R, D, left, right, n_slots, n_split, order;
+    int32_t n_seqs, T_q, T_k, H, G, R, D, left, right, n_slots, n_split, split_q, split_kv, order;
     float scale;
-    bool near_k, near_q;       // a tile's rows are within 32-bit offsets of its first (of q and dout: and lie alike in every tile)
+    uint32_t by_R;             // 2^22 / R, rounded up
+    bool near_k, near_q;       // a tile's rows are within 32-bit offsets of its first
+    bool even_q;               // pairs lie alike in every tile
 };
 
 // ---------------------------------------------------------------------------
@@ -330,6 +333,18 @@ struct tile_loader {
             if (c * 8 < D) dma16s(base + k * step, off + c * 16, lds + wave_at + k * NT * 16);
         }
     }
+    // Pairs from the r0'th of the base's token on, any R (their places differ from tile to tile); by_R = 2^22 / R, rounded up: exact
+    // for (64 + R) R < 2^22.
+    __device__ __forceinline__ void load_pairs(const char * base, int r0, int R, uint32_t by_R, uint32_t ts, uint32_t hs, uint32_t lds) const {
+        int t = threadIdx.x;
+        asm volatile("" : "+v"(t));
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const uint32_t x = r0 + row_of(t) + k * STEP, token = x * by_R >> 22;
+            const int c = chunk_of(t, k);
+            if (c * 8 < D) dma16s(base, token * ts + (x - token * R) * hs + c * 16, lds + wave_at + k * NT * 16);
+        }
+    }
     // row r from src(r), zeros where that is null
     template <class Src>
     __device__ __forceinline__ void load_each(uint32_t lds, Src src) const {
@@ -518,6 +533,31 @@ __device__ __forceinline__ void store_columns(E * tile, const v16f (&acc)[DT], f
         const v4i x = *reinterpret_cast<const v4i *>(tile + r * SP<DT> + (c ^ swz<DT>(r)) * 8);
         if (o && c * 8 < D) *reinterpret_cast<v4i *>(o + c * 16) = x;
     }
+}
+
+// The same as rows of D floats in memory, one after another, the first n of them: a split's share of a sum.
+template <int DT>
+__device__ __forceinline__ void store_partial(const v16f (&acc)[DT], float f, int D, int n, float * to) {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    if ((lane & 31) >= n) return;
+    float * o = to + (lane & 31) * D + 4 * (lane >> 5);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (32 * d + 8 * k < D) *reinterpret_cast<v4f *>(o + 32 * d + 8 * k) = v4f{acc[d][4 * k], acc[d][4 * k + 1], acc[d][4 * k + 2], acc[d][4 * k + 3]} * f;
+}
+
+// The part of the tiles lo .. hi - 1 that a split takes, every split but the last as many; those behind the last tile
+// take none.
+struct span {
+    int lo, hi;
+};
+__device__ __forceinline__ int share_of(span x, int n_split) { return (max(x.hi - x.lo, 0) + n_split - 1) / n_split; }
+__device__ __forceinline__ span split_of(span x, int n_split, int split) {
+    const int share = share_of(x, n_split);
+    return {x.lo + split * share, min(x.lo + (split + 1) * share, x.hi)};
 }
 
 // ---------------------------------------------------------------------------
@@ -1133,6 +1173,16 @@ __device__ __forceinline__ void add_ds(float (&x)[2], const attn_p & p, const do
     add_rows<E>(x, lo, hi, p.D, lds, [&](int j) { return weights_of<E>(p, c, g, pair, k_row(j), v_row(j)).ds; }, k_row);
 }
 
+// The tiles of 64 keys that the 128 pairs from p0 see some of, and of 64 pairs that see some of the 128 keys from kb0.
+__device__ __forceinline__ span keys_of(const attn_p & p, const doc & c, int p0) {
+    const int t_end = (min(p0 + 128, c.n * p.R) - 1) / p.R;
+    return {key_lo(p, c, p0 / p.R) / 64, (key_hi(p, c, t_end) + 63) / 64};
+}
+__device__ __forceinline__ span pairs_of(const attn_p & p, const doc & c, int kb0) {
+    const int k_end = min(kb0 + 128, c.m) - 1;
+    return {tok_lo(p, c, kb0) * p.R / 64, (tok_hi(p, c, k_end) * p.R + 63) / 64};
+}
+
 template <class E, int DT>
 struct dq_lds {
     E sk[2][64 * SP<DT>], sv[2][64 * SP<DT>];
@@ -1142,8 +1192,8 @@ __device__ __forceinline__ void dq_workgroup(const attn_p & p, int block, dq_lds
     constexpr int BM = 128, BN = 64;
     auto & sk = lds.sk;
     auto & sv = lds.sv;
-    const int g = block % p.G;
-    const job todo = workgroup_job(p, false, p.R, BM, block / p.G, p.right >= 0 ? p.order == BY_ROWS : p.left >= 0 && p.order != BY_ROWS, s_job);
+    const int g = block % p.G, split = block / p.G % p.split_q;
+    const job todo = workgroup_job(p, false, p.R, BM, block / (p.G * p.split_q), p.right >= 0 ? p.order == BY_ROWS : p.left >= 0 && p.order != BY_ROWS, s_job);
     if (todo.tile < 0) return;
     const doc c = todo.c;
     const int np = c.n * p.R, p0 = todo.tile * BM;
@@ -1154,8 +1204,9 @@ __device__ __forceinline__ void dq_workgroup(const attn_p & p, int block, dq_lds
     const int pc = min(pw + (lane & 31), np - 1), tok = pc / p.R, head = g * p.R + pc % p.R;
 
     const int lo = key_lo(p, c, tok), hi = key_hi(p, c, tok);
-    const int t_end = (min(p0 + BM, np) - 1) / p.R;
-    const int j_lo = key_lo(p, c, p0 / p.R) / BN, j_hi = (key_hi(p, c, t_end) + BN - 1) / BN;
+    const span mine = split_of(keys_of(p, c, p0), p.split_q, split);
+    const int j_lo = uni(mine.lo), j_hi = uni(mine.hi);
+    if (p.split_q > 1 && j_lo >= j_hi) return;
     const int ta = uni(min(pw, np - 1) / p.R), tb = uni(min(pw + 31, np - 1) / p.R);
     const int some_lo = key_lo(p, c, ta), some_hi = key_hi(p, c, tb), all_lo = key_lo(p, c, tb), all_hi = key_hi(p, c, ta);
 
@@ -1189,11 +1240,16 @@ __device__ __forceinline__ void dq_workgroup(const attn_p & p, int block, dq_lds
     if (!active) return;
     E * tile = (wave < 2 ? sk[0] : sv[0]) + (wave & 1) * 32 * SP<DT>;
     uint32_t bad = bad_columns<DT>(dq);
-    store_columns<E, DT>(tile, dq, p.scale / ds_scale, p.D, [&](int r) -> char * {
-        const int pr = pw + r;
-        if (pr >= np) return nullptr;
-        return p.dq.data + (int64_t) (c.q0 + pr / p.R) * p.dq.ts + (g * p.R + pr % p.R) * p.dq.hs;
-    });
+    float * part = p.part_q + (((int64_t) split * p.G + g) * p.T_q + c.q0) * p.R * p.D;
+    if (p.split_q > 1) {
+        store_partial<DT>(dq, p.scale / ds_scale, p.D, np - pw, part + (int64_t) pw * p.D);
+    } else {
+        store_columns<E, DT>(tile, dq, p.scale / ds_scale, p.D, [&](int r) -> char * {
+            const int pr = pw + r;
+            if (pr >= np) return nullptr;
+            return p.dq.data + (int64_t) (c.q0 + pr / p.R) * p.dq.ts + (g * p.R + pr % p.R) * p.dq.hs;
+        });
+    }
     if (!bad) return;
     auto k_row = [&](int j) { return p.k.data + (int64_t) (c.k0 + j) * p.k.ts + g * p.k.hs; };
     auto v_row = [&](int j) { return p.v.data + (int64_t) (c.k0 + j) * p.v.ts + g * p.v.hs; };
@@ -1203,8 +1259,9 @@ __device__ __forceinline__ void dq_workgroup(const attn_p & p, int block, dq_lds
         if (pair >= np) break;
         float x[2] = {0.0f, 0.0f};
         const int t = pair / p.R;
-        add_ds<E>(x, p, c, g, pair, key_lo(p, c, t), key_hi(p, c, t), reinterpret_cast<float *>(tile), k_row, v_row);
-        store_row<E>(p.dq.data + (int64_t) (c.q0 + t) * p.dq.ts + (g * p.R + pair % p.R) * p.dq.hs, x, p.scale, p.D);
+        add_ds<E>(x, p, c, g, pair, max(key_lo(p, c, t), j_lo * BN), min(key_hi(p, c, t), j_hi * BN), reinterpret_cast<float *>(tile), k_row, v_row);
+        if (p.split_q > 1) store_row<float>((char *) (part + (int64_t) pair * p.D), x, p.scale, p.D);
+        else store_row<E>(p.dq.data + (int64_t) (c.q0 + t) * p.dq.ts + (g * p.R + pair % p.R) * p.dq.hs, x, p.scale, p.D);
     }
 }
 
@@ -1283,8 +1340,8 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
     auto & so = lds.so;
     auto & s_lse = lds.s_lse;
     auto & s_delta = lds.s_delta;
-    const int g = block % p.G;
-    const job todo = workgroup_job(p, true, 1, BK, block / p.G, p.right >= 0 && p.order != BY_ROWS, s_job);
+    const int g = block % p.G, split = block / p.G % p.split_kv;
+    const job todo = workgroup_job(p, true, 1, BK, block / (p.G * p.split_kv), p.right >= 0 && p.order != BY_ROWS, s_job);
     if (todo.tile < 0) return;
     const doc c = todo.c;
     const int np = c.n * p.R, kb0 = todo.tile * BK;
@@ -1294,8 +1351,9 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
     const bool active = kw < c.m;
     const int key = min(kw + (lane & 31), c.m - 1);
 
-    const int k_end = min(kb0 + BK, c.m) - 1;
-    const int j_lo = tok_lo(p, c, kb0) * p.R / BQ, j_hi = (tok_hi(p, c, k_end) * p.R + BQ - 1) / BQ;
+    const span mine = split_of(pairs_of(p, c, kb0), p.split_kv, split);
+    const int j_lo = uni(mine.lo), j_hi = uni(mine.hi);
+    if (p.split_kv > 1 && j_lo >= j_hi) return;
     const int ka = uni(min(kw, c.m - 1)), ke = uni(min(kw + 31, c.m - 1));
     const int some_lo = tok_lo(p, c, ka) * p.R, some_hi = tok_hi(p, c, ke) * p.R;
     const int all_lo = tok_lo(p, c, ke) * p.R, all_hi = tok_hi(p, c, ka) * p.R;
@@ -1310,7 +1368,11 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
     }
     auto load = [&](int j, int buf) {
         const int j0 = j * BQ;
-        if (p.near_q && j0 + BQ <= np) {
+        if (p.near_q && !p.even_q && j0 + BQ <= np) {
+            const int t0 = j0 / p.R, r0 = j0 - t0 * p.R;
+            lq.load_pairs(uni(p.q.data + (int64_t) (c.q0 + t0) * p.q.ts + g * p.R * p.q.hs), r0, p.R, p.by_R, (uint32_t) p.q.ts, (uint32_t) p.q.hs, lds_addr(sq[buf]));
+            l_out.load_pairs(uni(p.dout.data + (int64_t) (c.q0 + t0) * p.dout.ts + g * p.R * p.dout.hs), r0, p.R, p.by_R, (uint32_t) p.dout.ts, (uint32_t) p.dout.hs, lds_addr(so[buf]));
+        } else if (p.near_q && j0 + BQ <= np) {
             lq.load(uni(p.q.data + (int64_t) (c.q0 + j0 / p.R) * p.q.ts + g * p.R * p.q.hs), lds_addr(sq[buf]));
             l_out.load(uni(p.dout.data + (int64_t) (c.q0 + j0 / p.R) * p.dout.ts + g * p.R * p.dout.hs), lds_addr(so[buf]));
         } else {
@@ -1367,9 +1429,16 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
         return [&, x](int r) -> char * { return kw + r < c.m ? x.data + (int64_t) (c.k0 + kw + r) * x.ts + g * x.hs : nullptr; };
     };
     uint32_t bad = bad_columns<DT>(dv) | bad_columns<DT>(dk);
-    store_columns<E, DT>(tile, dv, type_of<E>::HALF ? 1.0f / (1 << P_SHIFT) : 1.0f, p.D, dst(p.dv));
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    store_columns<E, DT>(tile, dk, p.scale / ds_scale, p.D, dst(p.dk));
+    const int64_t part_v = (int64_t) p.G * p.T_k * p.D;
+    float * part = p.part_kv + 2 * split * part_v + ((int64_t) g * p.T_k + c.k0) * p.D;
+    if (p.split_kv > 1) {
+        store_partial<DT>(dv, type_of<E>::HALF ? 1.0f / (1 << P_SHIFT) : 1.0f, p.D, c.m - kw, part + part_v + (int64_t) kw * p.D);
+        store_partial<DT>(dk, p.scale / ds_scale, p.D, c.m - kw, part + (int64_t) kw * p.D);
+    } else {
+        store_columns<E, DT>(tile, dv, type_of<E>::HALF ? 1.0f / (1 << P_SHIFT) : 1.0f, p.D, dst(p.dv));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        store_columns<E, DT>(tile, dk, p.scale / ds_scale, p.D, dst(p.dk));
+    }
     if (!bad) return;
     auto pair_row = [&](const rows & x) {
         return [&, x](int pr) { return (const char *) x.data + (int64_t) (c.q0 + pr / p.R) * x.ts + (g * p.R + pr % p.R) * x.hs; };
@@ -1381,12 +1450,17 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
         const int j = kw + __builtin_ctz(bad);
         if (j >= c.m) break;
         const char * k_row = p.k.data + (int64_t) (c.k0 + j) * p.k.ts + g * p.k.hs, * v_row = p.v.data + (int64_t) (c.k0 + j) * p.v.ts + g * p.v.hs;
-        const int lo = tok_lo(p, c, j) * p.R, hi = tok_hi(p, c, j) * p.R;
+        const int lo = max(tok_lo(p, c, j) * p.R, j_lo * BQ), hi = min(tok_hi(p, c, j) * p.R, j_hi * BQ);
         float x[2] = {0.0f, 0.0f}, y[2] = {0.0f, 0.0f};
         add_rows<E>(x, lo, hi, p.D, reinterpret_cast<float *>(tile), [&](int pr) { return weights_of<E>(p, c, g, pr, k_row, v_row).p; }, pair_row(p.dout));
         add_rows<E>(y, lo, hi, p.D, reinterpret_cast<float *>(tile), [&](int pr) { return weights_of<E>(p, c, g, pr, k_row, v_row).ds; }, pair_row(p.q));
-        store_row<E>(p.dv.data + (int64_t) (c.k0 + j) * p.dv.ts + g * p.dv.hs, x, 1.0f, p.D);
-        store_row<E>(p.dk.data + (int64_t) (c.k0 + j) * p.dk.ts + g * p.dk.hs, y, p.scale, p.D);
+        if (p.split_kv > 1) {
+            store_row<float>((char *) (part + part_v + (int64_t) j * p.D), x, 1.0f, p.D);
+            store_row<float>((char *) (part + (int64_t) j * p.D), y, p.scale, p.D);
+        } else {
+            store_row<E>(p.dv.data + (int64_t) (c.k0 + j) * p.dv.ts + g * p.dv.hs, x, 1.0f, p.D);
+            store_row<E>(p.dk.data + (int64_t) (c.k0 + j) * p.dk.ts + g * p.dk.hs, y, p.scale, p.D);
+        }
     }
 }
 
@@ -1405,6 +1479,52 @@ __global__ __launch_bounds__(256, 2) void attn_rows_grad_kernel(attn_p p, int n_
     } else {
         p.order = order_dq;
         dq_workgroup<E, DT>(p, blockIdx.x - n_dkv, lds.dq, s_job);
+    }
+}
+
+// The splits' shares of the gradients joined, a workgroup a tile of them: the first n_kv workgroups dK and dV, the
+// others dQ. Summed in the splits' order.
+template <class E>
+__global__ __launch_bounds__(1024) void attn_rows_grad_join_kernel(attn_p p, int n_kv) {
+    const int chunks = p.D / 8;
+    auto sum = [&](const float * from, int64_t step, int n, char * to) {
+        float x[8] = {};
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+            const v4f a = *reinterpret_cast<const v4f *>(from + k * step), b = *reinterpret_cast<const v4f *>(from + k * step + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] += a[i];
+                x[4 + i] += b[i];
+            }
+        }
+        typename type_of<E>::v8 e;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = (E) x[i];
+        *reinterpret_cast<typename type_of<E>::v8 *>(to) = e;
+    };
+    const bool kv = (int) blockIdx.x < n_kv;
+    const int block = kv ? blockIdx.x : blockIdx.x - n_kv, g = block % p.G;
+    const job todo = find_job(p, kv, kv ? 1 : p.R, 128, block / p.G, BY_ROWS, false);
+    if (todo.tile < 0) return;
+    const doc c = todo.c;
+    const int first = todo.tile * 128, rows_here = min(128, (kv ? c.m : c.n * p.R) - first), n_split = kv ? p.split_kv : p.split_q;
+    const span all = kv ? pairs_of(p, c, first) : keys_of(p, c, first);
+    const int share = share_of(all, n_split), n = share ? (all.hi - all.lo + share - 1) / share : 0;
+    if (kv) {
+        const int64_t part_v = (int64_t) p.G * p.T_k * p.D;
+        for (int i = threadIdx.x; i < 2 * rows_here * chunks; i += 1024) {
+            const int which = i >= rows_here * chunks, at = i - which * rows_here * chunks, row = c.k0 + first + at / chunks, d = at % chunks * 8;
+            const rows & to = which ? p.dv : p.dk;
+            sum(p.part_kv + which * part_v + ((int64_t) g * p.T_k + row) * p.D + d, 2 * part_v, n, to.data + row * to.ts + g * to.hs + 2 * d);
+        }
+    } else {
+        const int64_t part_g = (int64_t) p.T_q * p.R * p.D;
+        for (int i = threadIdx.x; i < rows_here * chunks; i += 1024) {
+            const int pair = first + i / chunks, d = i % chunks * 8;
+            sum(p.part_q + g * part_g + ((int64_t) c.q0 * p.R + pair) * p.D + d, p.G * part_g, n,
+                p.dq.data + (int64_t) (c.q0 + pair / p.R) * p.dq.ts + (g * p.R + pair % p.R) * p.dq.hs + 2 * d);
+        }
     }
 }
 
@@ -1454,11 +1574,10 @@ int32_t check_params(const char * what, const nxg_attention_rows_params * a, att
     return NXG_OK;
 }
 
-// Whether 64 rows' offsets from the first fit 32 bits: keys one after another, and pairs, whose places
-// repeat from tile to tile where R divides the rows of a thread's step (16).
+// Whether 64 rows' offsets from the first fit 32 bits: keys one after another, and pairs.
 bool near_rows(const rows & x) { return x.ts <= (INT32_MAX - 4096) / 64; }
 bool near_pairs(const rows & x, int R) {
-    return 16 % R == 0 && x.ts <= (INT32_MAX - 4096) / 128 && x.hs <= (INT32_MAX - 4096) / 2 / R;
+    return R <= 1024 && x.ts <= (INT32_MAX - 4096) / 128 && x.hs <= (INT32_MAX - 4096) / 2 / R;
 }
 
 int32_t check_rows(const char * what, const char * name, const nxg_rows * x, int64_t T, int n_head, int D, bool written, rows & r) {
@@ -1487,8 +1606,26 @@ int32_t check_rows(const char * what, const char * name, const nxg_rows * x, int
 #define NXG_TRY(call) do { const int32_t rc_ = (call); if (rc_) return rc_; } while (0)
 
 // Values of a row array of the backward pass: one a (token, head), and a tile's reach behind the last.
-int64_t row_values(const attn_p & p) { return (int64_t) p.T_q * p.H + 64; }
-int64_t backward_bytes(const attn_p & p) { return (2 * N_MAX + 2 * row_values(p)) * 4; }
+int64_t row_values(const attn_p & p) { return ((int64_t) p.T_q * p.H + 67) / 4 * 4; }
+int64_t part_q_values(const attn_p & p) { return p.split_q > 1 ? (int64_t) p.split_q * p.T_q * p.H * p.D : 0; }
+int64_t part_kv_values(const attn_p & p) { return p.split_kv > 1 ? (int64_t) p.split_kv * 2 * p.T_k * p.G * p.D : 0; }
+int64_t backward_bytes(const attn_p & p) { return (2 * N_MAX + 2 * row_values(p) + part_q_values(p) + part_kv_values(p)) * 4; }
+
+// Where there are few tiles of keys or of pairs, what each goes over is split until there are two workgroups a CU, at
+// least MIN_SHARE tiles of 64 for each in a document of twice the average length.
+constexpr int MIN_SHARE = 4;
+void plan_backward(attn_p & p) {
+    const int64_t cus = nxg_device_cus(), docs = (p.n_seqs + 1) / 2;
+    const int64_t window = p.left >= 0 && p.right >= 0 ? (int64_t) p.left + p.right + 1 : INT32_MAX;
+    p.split_q = p.split_kv = 1;
+    if (docs == 0) return;
+    const int64_t pairs = std::min(p.T_q / docs, window + 128) * p.R, keys = std::min(p.T_k / docs, window + 128 / p.R + 1);
+    auto split = [&](int64_t workgroups, int64_t rows) {
+        return (int) std::max<int64_t>(1, std::min({2 * cus / workgroups, rows / (64 * MIN_SHARE), (int64_t) 64}));
+    };
+    p.split_kv = split(slots(p.T_k, 1, 128, p.n_seqs) * p.G, pairs);
+    p.split_q = split(slots(p.T_q, p.R, 128, p.n_seqs) * p.G, keys);
+}
 
 // Launches one of a kernel's instances by type and head size.
 #define NXG_BY_TYPE(type, D, LAUNCH)                                               \
@@ -1593,6 +1730,7 @@ int64_t nxg_attention_rows_backward_workspace_bytes(const nxg_attention_rows_par
     attn_p p;
     const int32_t rc = check_params("attention_rows_backward_workspace_bytes", a, p);
     if (rc) return -rc;
+    plan_backward(p);
     return backward_bytes(p);
 }
 
@@ -1613,6 +1751,7 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
     NXG_TRY(check_rows(what, "dv", dv, p.T_k, p.G, p.D, true, p.dv));
     if (p.n_seqs == 0 || (p.T_q == 0 && p.T_k == 0)) return NXG_OK;
     if (!p.cu_q || !p.cu_k || (p.T_q > 0 && !lse)) return nxg_fail(NXG_EINVAL, "%s: cu_q, cu_k or lse is null", what);
+    plan_backward(p);
     if (!workspace || ((uintptr_t) workspace & 15) || workspace_bytes < backward_bytes(p)) {
         return nxg_fail(NXG_EINVAL, "%s: workspace must be 16-byte aligned memory of %lld bytes", what,
                         (long long) backward_bytes(p));
@@ -1621,9 +1760,13 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
     p.lse = (float *) lse;
     p.near_k = near_rows(p.k) && near_rows(p.v);
     p.near_q = near_pairs(p.q, p.R) && near_pairs(p.dout, p.R);
+    p.even_q = 16 % p.R == 0;              // the rows of a thread's step
+    p.by_R = ((1u << 22) + p.R - 1) / p.R;
     p.maxima = (float *) workspace;
     p.lse2 = p.maxima + 2 * N_MAX;
     p.ndelta = p.lse2 + row_values(p);
+    p.part_q = p.ndelta + row_values(p);
+    p.part_kv = p.part_q + part_q_values(p);
     hipStream_t s = (hipStream_t) stream;
     if (p.T_q > 0) {
         const int L = p.D <= 64 ? 8 : 16;
@@ -1641,7 +1784,13 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
     const unsigned n_dq = p.T_q > 0 ? (unsigned) (slots(p.T_q, p.R, 128, p.n_seqs) * p.G) : 0;
     const unsigned n_dkv = p.T_k > 0 ? (unsigned) (slots(p.T_k, 1, 128, p.n_seqs) * p.G) : 0;
     p.order = work_order(p, n_dkv);
-    NXG_BY_TYPE(a->type, p.D, (attn_rows_grad_kernel<E, DT><<<n_dkv + n_dq, 256, 0, s>>>(p, (int) n_dkv, work_order(p, n_dq))));
+    const unsigned wgs_dkv = n_dkv * p.split_kv, wgs = wgs_dkv + n_dq * p.split_q;
+    NXG_BY_TYPE(a->type, p.D, (attn_rows_grad_kernel<E, DT><<<wgs, 256, 0, s>>>(p, (int) wgs_dkv, work_order(p, n_dq))));
+    const unsigned join_kv = p.split_kv > 1 ? n_dkv : 0, joins = join_kv + (p.split_q > 1 ? n_dq : 0);
+    if (joins == 0) return nxg_launch_check(what);
+    NXG_TRY(nxg_launch_check(what));
+    if (a->type == NXG_TYPE_BF16) attn_rows_grad_join_kernel<__bf16><<<joins, 1024, 0, s>>>(p, (int) join_kv);
+    else attn_rows_grad_join_kernel<_Float16><<<joins, 1024, 0, s>>>(p, (int) join_kv);
     return nxg_launch_check(what);
 }
 

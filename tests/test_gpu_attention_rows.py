@@ -345,3 +345,29 @@ def test_few_queries_over_a_far_cache(nxg, torch, dev, n, stride):
     ref = rows_ref.attention(q, k.contiguous(), v.contiguous(), [0, n], [0, K], 1 / math.sqrt(D), -1, 0)
     rows_ref.check("out", out, *ref["out"])
     rows_ref.check("lse", lse, *ref["lse"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,G,D", [(8, 1, 96), (6, 2, 64), (5, 1, 128), (7, 1, 32)])
+@pytest.mark.parametrize("lens,keys", [([900, 40, 0, 333], None), ([34, 1], [3000, 200]), ([1100, 9], [70, 0])], ids=str)
+@pytest.mark.parametrize("left,right", [(-1, 0), (-1, -1), (200, 100)])
+def test_gradients_of_few_long_documents(nxg, torch, dev, dtype, H, G, D, lens, keys, left, right):
+    """Few tiles, each with much to go over: shared out over workgroups, for queries and for keys, documents of
+    other lengths and shares that are empty among them."""
+    say(f"attention_rows {dtype} H={H} G={G} D={D} lens={lens} keys={keys} window={left},{right}")
+    run_and_check(nxg, torch, getattr(torch, dtype), lens, keys, H=H, G=G, D=D, left=left, right=right, seed=D)
+
+
+def test_split_gradients_need_their_workspace(nxg, torch, dev):
+    say("attention_rows_backward workspace of shares")
+    q, k, v, do = make(torch, torch.bfloat16, [2000], [2000], 4, 1, 64, 3)
+    n = nxg.rows.attention_rows_backward_workspace_bytes(q, k, v, [0, 2000], right=0)
+    assert n > 4 * 2 * 2000 * 4 + 4 * 2 * 2000 * 64, "shares are left in the workspace"
+    out, lse = nxg.attention_rows(q, k, v, [0, 2000], right=0)
+    with pytest.raises(ValueError, match="workspace"):
+        nxg.attention_rows_backward(do, q, k, v, out, lse, [0, 2000], right=0, workspace=torch.empty(n - 1, dtype=torch.uint8, device="cuda"))
+    big = torch.full((n + 256,), 7, dtype=torch.uint8, device="cuda")
+    a = nxg.attention_rows_backward(do, q, k, v, out, lse, [0, 2000], right=0, workspace=big[:n])
+    assert (big[n:] == 7).all()
+    b = nxg.attention_rows_backward(do, q, k, v, out, lse, [0, 2000], right=0)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
