@@ -1611,17 +1611,32 @@ int64_t part_q_values(const attn_p & p) { return p.split_q > 1 ? (int64_t) p.spl
 int64_t part_kv_values(const attn_p & p) { return p.split_kv > 1 ? (int64_t) p.split_kv * 2 * p.T_k * p.G * p.D : 0; }
 int64_t backward_bytes(const attn_p & p) { return (2 * N_MAX + 2 * row_values(p) + part_q_values(p) + part_kv_values(p)) * 4; }
 
-// Where there are few tiles of keys or of pairs, what each goes over is split until there are two workgroups a CU, at
-// least MIN_SHARE tiles of 64 for each in a document of twice the average length.
-constexpr int MIN_SHARE = 4;
+// The length that a split is reckoned for, of which only the sum is known here: one document's, two's average, twice
+// that of more (mixed lengths: with the average 17 documents of 5 queries over 405 keys take 32 us, so 25).
+int64_t long_document(int64_t T, int n_seqs) { return n_seqs <= 2 ? T / std::max(1, n_seqs) : 2 * T / n_seqs; }
+
+// Keys that a window leaves of them for `tokens` queries next to each other, and the other way round.
+int64_t within_window(const attn_p & p, int64_t length, int64_t tokens) {
+    return p.left >= 0 && p.right >= 0 ? std::min(length, (int64_t) p.left + p.right + tokens) : length;
+}
+
+// Where there are few tiles of keys, or of pairs, what each goes over is split until there are two workgroups a CU
+// (2,048 tokens causal 107 -> 59 us; four a CU cost more in the join: 2 documents of 1,840 tokens, 32 heads of 128 on 4:
+// 200 us with two, 241 with four). Where there are up to two a CU anyhow but documents of mixed lengths, and windows that
+// leave their tiles mixed work, in two: the longest document's would be the launch's last (17 documents of 3,700 tokens,
+// the longest of 1,700: 204 -> 147 us; not for 11 documents of 260, 45 -> 57). A share is two tiles of 64 at least (a
+// document of 750 tokens, 8 heads on one: 104 us with 4, 87 with 2), and fewer than 6 tiles are not shared out
+// (5 documents of 410 in a window of 16: 50 -> 56 us).
+constexpr int MAX_SPLIT = 16;
 void plan_backward(attn_p & p) {
-    const int64_t cus = nxg_device_cus(), docs = (p.n_seqs + 1) / 2;
-    const int64_t window = p.left >= 0 && p.right >= 0 ? (int64_t) p.left + p.right + 1 : INT32_MAX;
-    p.split_q = p.split_kv = 1;
-    if (docs == 0) return;
-    const int64_t pairs = std::min(p.T_q / docs, window + 128) * p.R, keys = std::min(p.T_k / docs, window + 128 / p.R + 1);
+    const int64_t cus = nxg_device_cus(), pairs = within_window(p, long_document(p.T_q, p.n_seqs), 128) * p.R,
+                  keys = within_window(p, long_document(p.T_k, p.n_seqs), (128 + p.R - 1) / p.R);
+    const bool mixed = p.n_seqs > 1 && (p.left < 0 || p.right < 0);
     auto split = [&](int64_t workgroups, int64_t rows) {
-        return (int) std::max<int64_t>(1, std::min({2 * cus / workgroups, rows / (64 * MIN_SHARE), (int64_t) 64}));
+        const int64_t tiles = rows / 64;
+        int64_t n = 2 * cus / std::max<int64_t>(1, workgroups);
+        if (n == 1 && mixed && tiles >= 24) n = 2;
+        return tiles < 6 ? 1 : (int) std::max<int64_t>(1, std::min({n, tiles / 2, (int64_t) MAX_SPLIT}));
     };
     p.split_kv = split(slots(p.T_k, 1, 128, p.n_seqs) * p.G, pairs);
     p.split_q = split(slots(p.T_q, p.R, 128, p.n_seqs) * p.G, keys);
@@ -1648,23 +1663,21 @@ int work_order(const attn_p & p, int64_t workgroups) {
     return p.left < 0 && p.right < 0 ? BY_LENGTH : BY_LEVEL;
 }
 
-// The few-pairs kernel where tiles of 128 pairs would leave CUs idle, its keys split until there is a workgroup a CU
-// (more only add sums to join: 8 x 1 query over 8,192 keys of 128 values 50.0, 54.1 and 63.1 us with one, two and
-// four a CU), 256 keys of the average document at least to each.
+// The few-pairs kernel where tiles of 128 pairs would be nearly empty, or would leave CUs idle and tiles of 32 run in
+// one round (two workgroups a CU by LDS with up to 64 values a head, else one: 4 documents of 766 tokens, 8 heads of 96 on
+// one, 45 us in three rounds, 19 with tiles of 128; 3 documents of 339 tokens of 64 values, 12 us in one, and 14). Its keys are split until there is a workgroup a CU (more only add sums to join: 8 x 1
+// query over 8,192 keys of 128 values 50.0, 54.1 and 63.1 us with one, two and four a CU), 256 keys to each at least.
 struct fwd_plan {
     bool few;
     int n_split;
 };
 fwd_plan plan_forward(const attn_p & p) {
-    const int64_t cus = nxg_device_cus();
+    const int64_t cus = nxg_device_cus(), wgs = slots(p.T_q, p.R, 32, p.n_seqs) * p.G;
     fwd_plan f{false, 1};
-    if (slots(p.T_q, p.R, 128, p.n_seqs) * p.G >= cus) {
-        // documents of few pairs each: tiles of 128 would be nearly empty
-        if ((int64_t) p.T_q * p.R > 32LL * p.n_seqs) return f;
-    }
+    const bool empty_tiles = (int64_t) p.T_q * p.R <= 32LL * p.n_seqs, idle = slots(p.T_q, p.R, 128, p.n_seqs) * p.G < cus;
+    if (!empty_tiles && !(idle && wgs <= cus * (p.D <= 64 ? 2 : 1))) return f;
     f.few = true;
-    const int64_t wgs = slots(p.T_q, p.R, 32, p.n_seqs) * p.G;
-    const int64_t keys = p.T_k / std::max(1, p.n_seqs);
+    const int64_t keys = within_window(p, long_document(p.T_k, p.n_seqs), (32 + p.R - 1) / p.R);
     f.n_split = (int) std::max<int64_t>(1, std::min({cus / wgs, keys / 256, (int64_t) 64}));
     return f;
 }
