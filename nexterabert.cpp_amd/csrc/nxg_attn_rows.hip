@@ -748,6 +748,12 @@ __device__ __forceinline__ void fwd_again(const attn_p & p, const doc & c, int g
 // the next 32 keys are computed beside the exponentials of these, which take about as long as both products:
 // K's tiles start 32 keys behind V's. Every wave takes every tile of the workgroup (the windows of its 128 pairs
 // differ by few keys), so that the loop has no branches between the products.
+//
+// Bound by the matrix units, and by the power that they and the exponentials beside them draw together: 65,536 tokens,
+// 16 heads of 64 on 8, bf16, full: 17.1 ms, 1,030 TFLOP/s (a library product of 8,192^3 reaches 1,138); the LDS copies cost
+// 7 to 9% of it, the exponentials 7%. 32 documents of 32,900 tokens, causal: 135 us, 680 TFLOP/s, the rest the masked
+// halves of tiles on the diagonal and the first tiles' latency. With 128 values a head 8,192 tokens full take 510 us,
+// 1,078 TFLOP/s; 8 x 1,024 tokens in a band of 257 keys 24 us, 6 tiles a workgroup, bound by their latency.
 template <class E, int DT>
 __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     constexpr int BM = 128, BN = 64, TILE = BN * SP<DT>;
@@ -843,6 +849,10 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
 // Few pairs: a workgroup takes 32 of them, its four waves every fourth 32 keys of the split's share, each through
 // LDS of its own; the waves' sums are joined in LDS. With n_split > 1 the shares of a document's keys go to
 // different workgroups, which leave sums (o, m, l) that attn_rows_join_kernel joins.
+//
+// A wave's tiles are its own so that it waits for its own loads alone, no barrier in the loop. Bound by HBM where the cache is
+// long (one query over 65,536 keys, 16 heads of 64 on 8: 134 MB in 25 us, 5.4 TB/s, and 4 us of joining), else by the
+// chain of loads, products and the join (32 queries over 16 to 2,048 keys, 68 MB: 20 us; 4 texts of 125 tokens: 7 us).
 template <class E, int DT>
 __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
     constexpr int BM = 32, BN = 32, TILE = BN * SP<DT>;
@@ -958,7 +968,8 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
 }
 
 // The splits' sums of a (token, head) row joined: a wave a row, L lanes for its values (8 each), 64 / L groups of them
-// for every 64 / L'th split, whose loads are independent; the groups' sums added at the end.
+// for every 64 / L'th split, whose loads are independent; the groups' sums added at the end. 4.4 us for 16 rows of 64 values
+// in 32 shares: a launch and two rounds of loads.
 template <class E, int L>
 __global__ __launch_bounds__(256) void attn_rows_join_kernel(attn_p p) {
     const int64_t row = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6), n_rows = (int64_t) p.T_q * p.H;
@@ -1006,9 +1017,44 @@ __global__ __launch_bounds__(256) void attn_rows_join_kernel(attn_p p) {
 // backward
 // ---------------------------------------------------------------------------
 
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float dot8(v8b a, v8b b) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2_f32_bf16(v2b{a[i], a[i + 1]}, v2b{b[i], b[i + 1]}, s, false);
+    return s;
+}
+__device__ __forceinline__ float dot8(v8h a, v8h b) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2(v2h{a[i], a[i + 1]}, v2h{b[i], b[i + 1]}, s, false);
+    return s;
+}
+
+// A query of at most EXACT_KEYS keys takes delta from the definition, the sum of P dP over them, not from `out`, whose rounding
+// would stay in its gradients: dS = P (dP - delta) cancels the more, the fewer the keys (nothing is left of one), and few
+// keys make the largest dS. With 3 keys a query dQ and dK are off by 0.0024 of their norm so, by 0.0032 from out (bf16, of which
+// the rounding of dS and of the result make 0.0024); with 17 by 0.0024 and 0.0025. It costs 2 us of 8 with 8 x 1,024 tokens
+// in a band, 4 of 28 with 32 documents, where the queries of more keys only have their documents looked up.
+constexpr int EXACT_KEYS = 16;
+// Documents whose offsets the delta kernel's workgroups hold; those of more are looked up in memory.
+constexpr int DELTA_DOCS = 256;
+
+// The largest d with cu[d] <= t.
+__device__ __forceinline__ int doc_of_token(const int32_t * cu, int n_seqs, int T, int t) {
+    int lo = 0, hi = n_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (offset(cu, mid, T) <= t) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
 // -delta = -sum(dout out) and log2 of the sums of each (token, head) row; for fp16 the largest squared norms of dout's and v's
 // rows, from which the gradients' kernels take the power of two that dS is carried with. L lanes a row (8 for heads of
-// up to 64).
+// up to 64). Bound by HBM: 32,900 tokens of 16 heads of 64, 135 MB, 33 us, 4.1 TB/s (28.5 without the look-up).
 template <class E, int L>
 __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
     typedef typename type_of<E>::v8 v8;
@@ -1023,11 +1069,39 @@ __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
     // the largest norms: of documents' rows alone
     const int q_lo = offset(p.cu_q, 0, p.T_q), q_hi = offset(p.cu_q, p.n_seqs, p.T_q);
     const int k_lo = offset(p.cu_k, 0, p.T_k), k_hi = offset(p.cu_k, p.n_seqs, p.T_k);
+    __shared__ int32_t s_cu[2][DELTA_DOCS + 1];
+    const bool held = p.n_seqs <= DELTA_DOCS;
+    if (held) {
+        for (int i = threadIdx.x; i <= p.n_seqs; i += 1024) {
+            s_cu[0][i] = p.cu_q[i];
+            s_cu[1][i] = p.cu_k[i];
+        }
+        __syncthreads();
+    }
+    const int32_t * cu_q = held ? s_cu[0] : p.cu_q, * cu_k = held ? s_cu[1] : p.cu_k;
+    const float cs = p.scale * LOG2E;
+    // up to 63 documents' offsets a lane each: may a query of the tokens ta .. tb have few keys? (Their number rises, stays
+    // and falls over a document, so that its ends tell.)
+    const int lane = threadIdx.x & 63;
+    const int lane_q = held ? offset(cu_q, min(lane, p.n_seqs), p.T_q) : 0, lane_k = held ? offset(cu_k, min(lane, p.n_seqs), p.T_k) : 0;
+    auto few_keys = [&](int ta, int tb) {
+        if (p.n_seqs > 63) return true;
+        const int d = __popcll(__ballot(lane <= p.n_seqs && lane_q <= ta)) - 1;
+        if (d < 0 || d >= p.n_seqs) return true;
+        doc c;
+        c.q0 = __builtin_amdgcn_readlane(lane_q, d);
+        c.n = __builtin_amdgcn_readlane(lane_q, d + 1) - c.q0;
+        c.k0 = __builtin_amdgcn_readlane(lane_k, d);
+        c.m = max(__builtin_amdgcn_readlane(lane_k, d + 1) - c.k0, 0);
+        if (tb >= c.q0 + c.n) return true;
+        const int a = ta - c.q0, b = tb - c.q0;
+        return min(key_hi(p, c, a) - key_lo(p, c, a), key_hi(p, c, b) - key_lo(p, c, b)) <= EXACT_KEYS;
+    };
     // in the order of lse2 and ndelta, a KV head's pairs one after another; two rows at a time under way
     const int n_pairs = p.T_q * p.R, all = p.G * ((n_pairs + 2 * ROWS - 1) / (2 * ROWS));
     for (int w = blockIdx.x; w < all; w += gridDim.x) {
         const int g = w % p.G, p0 = w / p.G * (2 * ROWS) + sub;
-        v8 a[2], b[2];
+        v8 a[2] = {}, b[2] = {};
         int64_t at[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -1043,6 +1117,8 @@ __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
+            const int pw = uni(p0 + ROWS * k);
+            const bool few = pw < n_pairs && few_keys(pw / p.R, (min(pw + 64 / L, n_pairs) - 1) / p.R);
             if (at[k] < 0) continue;          // a row's lanes alike
             float s = 0.0f, n2 = 0.0f;
             if (cc * 8 < p.D) {
@@ -1053,13 +1129,46 @@ __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
                 }
             }
             s = sum(s);
+            const int tok = (p0 + ROWS * k) / p.R;
+            const float lse2 = p.lse[at[k]] * LOG2E;
+            if (few && tok >= q_lo && tok < q_hi) {
+                const int d = doc_of_token(cu_q, p.n_seqs, p.T_q, tok);
+                doc c;
+                c.q0 = offset(cu_q, d, p.T_q);
+                c.n = max(offset(cu_q, d + 1, p.T_q) - c.q0, 0);
+                c.k0 = offset(cu_k, d, p.T_k);
+                c.m = max(offset(cu_k, d + 1, p.T_k) - c.k0, 0);
+                const int lo = key_lo(p, c, tok - c.q0), hi = key_hi(p, c, tok - c.q0);
+                if (hi > lo && hi - lo <= EXACT_KEYS) {
+                    const int head = (int) (at[k] - (int64_t) tok * p.H);
+                    v8 x = {};
+                    if (cc * 8 < p.D) x = *reinterpret_cast<const v8 *>(p.q.data + (int64_t) tok * p.q.ts + head * p.q.hs + cc * 16);
+                    s = 0.0f;
+                    constexpr int AT = 2;                 // keys whose loads are under way together
+                    for (int j = lo; j < hi; j += AT) {
+                        v8 y[AT] = {}, z[AT] = {};
+                        if (cc * 8 < p.D) {
+#pragma unroll
+                            for (int i = 0; i < AT; ++i) {
+                                const int64_t key = c.k0 + min(j + i, hi - 1);
+                                y[i] = *reinterpret_cast<const v8 *>(p.k.data + key * p.k.ts + g * p.k.hs + cc * 16);
+                                z[i] = *reinterpret_cast<const v8 *>(p.v.data + key * p.v.ts + g * p.v.hs + cc * 16);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < AT; ++i) {
+                            const float t = __builtin_amdgcn_exp2f(__builtin_fmaf(sum(dot8(x, y[i])), cs, -lse2)) * sum(dot8(a[k], z[i]));
+                            if (j + i < hi) s += t;
+                        }
+                    }
+                }
+            }
             if (cc == 0) {
                 const int64_t row = (int64_t) g * n_pairs + p0 + ROWS * k;
-                p.lse2[row] = p.lse[at[k]] * LOG2E - (type_of<E>::HALF ? P_SHIFT : 0);
+                p.lse2[row] = lse2 - (type_of<E>::HALF ? P_SHIFT : 0);
                 p.ndelta[row] = -s;
             }
             if (type_of<E>::HALF) {
-                const int tok = (p0 + ROWS * k) / p.R;
                 n2 = sum(n2);
                 if (tok >= q_lo && tok < q_hi) top_o = fmaxf(top_o, n2);
             }
@@ -1183,6 +1292,9 @@ __device__ __forceinline__ span pairs_of(const attn_p & p, const doc & c, int kb
     return {tok_lo(p, c, kb0) * p.R / 64, (tok_hi(p, c, k_end) * p.R + 63) / 64};
 }
 
+// dQ: a workgroup has 128 pairs, a wave 32 of them with q and dout in registers, and goes over the keys that they see, 64 at a
+// time: S^T = K Q^T and dP^T = V dO^T from the tiles' rows, dQ^T += K^T dS^T from K's columns. P and dS are computed here again
+// rather than shared with dK and dV, whose sums over pairs would need atomics, in no fixed order.
 template <class E, int DT>
 struct dq_lds {
     E sk[2][64 * SP<DT>], sv[2][64 * SP<DT>];
@@ -1327,7 +1439,8 @@ __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const t
     }
 }
 
-// A workgroup: 128 keys, 4 waves of 32.
+// A workgroup: 128 keys, 4 waves of 32 with k and v in registers; tiles of q and dout are read in rows for S and dP, in columns for
+// dV += dO^T P and dK += Q^T dS: four products a tile, the other operand of each matrix instruction read from LDS.
 template <class E, int DT>
 struct dkv_lds {
     E sq[2][64 * SP<DT>], so[2][64 * SP<DT>];
@@ -1467,6 +1580,12 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
 // Both in one launch, dK and dV's workgroups first (they are the longer ones), so that the end of the one is
 // filled by the others: against a launch each, 8 x 1,024 tokens banded 71 -> 58 us, one document of 8,192 causal
 // 720 -> 535 us (64 values a head) and 1,176 -> 1,037 (128).
+//
+// Bound by the matrix units with the exponentials and the LDS reads between them (the products of one wave wait for
+// each other; two workgroups' waves a CU fill part of that): of the five products that the gradients need (seven are
+// taken, S and dP on both sides), 8,192 tokens full, 16 heads of 64 on 8: 975 us, 705 TFLOP/s, 987 with the two taken twice;
+// 128 values a head 1,715 us, 802. Taking P for the next tile beside dP of this (841 against 759 us), V's tile in LDS, and
+// other priorities of the waves were no faster.
 template <class E, int DT>
 __global__ __launch_bounds__(256, 2) void attn_rows_grad_kernel(attn_p p, int n_dkv, int order_dq) {
     __shared__ __align__(1024) union {
@@ -1483,7 +1602,8 @@ __global__ __launch_bounds__(256, 2) void attn_rows_grad_kernel(attn_p p, int n_
 }
 
 // The splits' shares of the gradients joined, a workgroup a tile of them: the first n_kv workgroups dK and dV, the
-// others dQ. Summed in the splits' order.
+// others dQ. Summed in the splits' order. Bound by the shares' reads: 2,048 tokens, 16 heads of 64 on 8, in three and two
+// shares 6.6 us.
 template <class E>
 __global__ __launch_bounds__(1024) void attn_rows_grad_join_kernel(attn_p p, int n_kv) {
     const int chunks = p.D / 8;

@@ -70,6 +70,9 @@ __device__ __forceinline__ int doc_of_row(const int32_t * cu, int n_seqs, int t)
 // turns less whole turns, then fp32 (error 2^-25 of a turn). Then the heads' rows as one run of
 // pieces, neighbouring lanes on neighbouring pieces: V values of a head from i and V from i + n / 2
 // (HALF), V values in a row (else; a pair of single values where V is 1), or V values behind n to copy.
+// Bound by HBM: 65,536 tokens of 24 heads of 64 in a fused projection's rows, fp32, 805 MB in 153 us, 5.3 TB/s (a large copy
+// reaches 5.1 to 5.5); loads and stores past the caches take 246 to 261. Divisions are multiplications by a 32-bit
+// reciprocal, exact for the numbers of a workgroup.
 template <class E, int V, bool HALF>
 __global__ __launch_bounds__(256) void rope_rows_kernel(rope_p p) {
     extern __shared__ float2 turn[];       // [tb][n / 2]
@@ -159,7 +162,8 @@ struct norm_p {
 };
 
 // A row by TPR threads (a wave, or the workgroup), held in registers as NC pieces of V values a thread: one
-// read, the mean, then the squares of what is left.
+// read, the mean, then the squares of what is left. Bound by HBM: 65,536 rows of 1,024 bf16 values, 269 MB in 41 to 43 us,
+// 6.3 TB/s (part of the output stays in the last cache); 8,192 rows of 8,192 in 45 us.
 template <class E, class W, int V, int NC, int TPR>
 __global__ __launch_bounds__(256) void layer_norm_rows_kernel(norm_p p) {
     __shared__ float lds[4];
@@ -214,7 +218,9 @@ __global__ __launch_bounds__(256) void layer_norm_rows_kernel(norm_p p) {
     }
 }
 
-// Rows too long for registers: read three times by a workgroup.
+// Rows too long for registers: read three times by a workgroup, from HBM once, a value a lane in the order that rows off 16 bytes
+// need too, so that both give the same bits. 8,192 rows of 9,000 bf16 values 162 us, 1.8 TB/s of HBM: bound by the loads'
+// number.
 template <class E, class W>
 __global__ __launch_bounds__(256) void layer_norm_long_kernel(norm_p p) {
     __shared__ float lds[4];
@@ -241,7 +247,8 @@ __global__ __launch_bounds__(256) void layer_norm_long_kernel(norm_p p) {
 }
 
 // Gradients: the rows of a workgroup (every gridDim.x'th group of 256 / TPR) one after another, dw and db of
-// its rows in registers, left at the end as one row of `part` each; norm_reduce_kernel sums those.
+// its rows in registers, left at the end as one row of `part` each; norm_reduce_kernel sums those. Bound by HBM: 32,900 rows
+// of 1,024 bf16 values, 203 MB in 38.5 us, 5.3 TB/s, with 4.2 us of norm_reduce_kernel.
 template <class E, class W, int V, int NC, int TPR>
 __global__ __launch_bounds__(256) void layer_norm_back_kernel(norm_p p) {
     __shared__ float lds[4];
@@ -334,7 +341,8 @@ __global__ __launch_bounds__(256) void layer_norm_back_kernel(norm_p p) {
     }
 }
 
-// Rows too long for registers: dx by a workgroup a row, and the rows' sums by columns.
+// Rows too long for registers: dx by a workgroup a row (8,192 rows of 9,000 bf16 values 170 us), and the rows' sums by columns,
+// which read the rows once more (88 us, 3.4 TB/s).
 template <class E, class W>
 __global__ __launch_bounds__(256) void layer_norm_back_long_kernel(norm_p p) {
     __shared__ float lds[4];

@@ -371,3 +371,28 @@ def test_split_gradients_need_their_workspace(nxg, torch, dev):
     assert (big[n:] == 7).all()
     b = nxg.attention_rows_backward(do, q, k, v, out, lse, [0, 2000], right=0)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 80])
+@pytest.mark.parametrize("n_docs", [40, 300])
+def test_gradients_of_single_keys_cancel(nxg, torch, dev, dtype, D, n_docs):
+    """A query of one key: dS = P (dP - delta) is 0, so that dQ and dK are what fp32 leaves of it, not what the rounding of
+    `out` would. dP and delta: D products and sums each, off by D + 8 half steps of the sum of their sizes; P, whose
+    exponent is rounded at up to 8 (2^-20 of it) and again by exp2, by 2^-18 at most, in both."""
+    say(f"attention_rows {dtype} single keys D={D} {n_docs} documents")
+    dt, H, G = getattr(torch, dtype), 4, 2
+    for lens, keys, left, right in (([1] * n_docs, [1] * n_docs, -1, -1), ([3] * n_docs, [1] * n_docs, -1, -1), ([5] * n_docs, [5] * n_docs, 0, 0)):
+        q, k, v, do = make(torch, dt, lens, keys, H, G, D, n_docs)
+        cu_q, cu_k = offsets(lens), offsets(keys)
+        out, lse = nxg.attention_rows(q, k, v, cu_q, cu_k, left=left, right=right)
+        dq, dk, _ = nxg.attention_rows_backward(do, q, k, v, out, lse, cu_q, cu_k, left=left, right=right)
+        at = torch.arange(len(q), device="cuda") if left == 0 else torch.arange(n_docs, device="cuda").repeat_interleave(lens[0])
+        K, V = (t.double().repeat_interleave(H // G, 1)[at] for t in (k, v))      # of each query
+        dO = do.double()
+        e = 2.0 ** -17 * (dO * V).sum(2).abs() + 2 * (D + 8) * 2.0 ** -24 * (dO * V).abs().sum(2)
+        least = rows_ref.least_step(dt)
+        e = e[:, :, None] * 1.02 * D ** -0.5
+        assert (dq.double().abs() <= e * K.abs() + least).all()
+        b = torch.zeros(len(k), H, D, dtype=torch.float64, device="cuda").index_add_(0, at, e * q.double().abs())
+        assert (dk.double().abs() <= b.reshape(len(k), G, H // G, D).sum(2) + least).all()
