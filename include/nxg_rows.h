@@ -22,9 +22,9 @@
  * projection's rows, or head after head. A stride of 0 repeats a row (inputs only).
  *
  * Packed documents: cu is device int32, n_seqs + 1 offsets, from 0 and not decreasing (an empty
- * document is allowed). Rows that no document covers are neither read nor written by
- * nxg_attention_rows and its gradient. Other offsets give unspecified rows but no access out
- * of bounds.
+ * document is allowed). Rows that no document covers have no part in a result of
+ * nxg_attention_rows and its gradient, and are not written. Other offsets give unspecified rows but
+ * no access out of bounds.
  */
 #ifndef NXG_ROWS_H
 #define NXG_ROWS_H

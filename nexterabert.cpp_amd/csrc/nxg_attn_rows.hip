@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <type_traits>
 
 #include "nxg_rows.h"
@@ -1039,7 +1040,7 @@ __device__ __forceinline__ float dot8(v8h a, v8h b) {
 // in a band, 4 of 28 with 32 documents, where the queries of more keys only have their documents looked up.
 constexpr int EXACT_KEYS = 16;
 // Documents whose offsets the delta kernel's workgroups hold; those of more are looked up in memory.
-constexpr int DELTA_DOCS = 256;
+constexpr int DELTA_DOCS = 1024;
 
 // The largest d with cu[d] <= t.
 __device__ __forceinline__ int doc_of_token(const int32_t * cu, int n_seqs, int T, int t) {
@@ -1725,6 +1726,14 @@ int32_t check_rows(const char * what, const char * name, const nxg_rows * x, int
 
 #define NXG_TRY(call) do { const int32_t rc_ = (call); if (rc_) return rc_; } while (0)
 
+// Refuses an output that is another row array of the call.
+int32_t check_apart(const char * what, const char * name, const rows & out, std::initializer_list<const rows *> others) {
+    for (const rows * r : others) {
+        if (out.data && out.data == r->data) return nxg_fail(NXG_EINVAL, "%s: %s is another tensor of the call too", what, name);
+    }
+    return NXG_OK;
+}
+
 // Values of a row array of the backward pass: one a (token, head), and a tile's reach behind the last.
 int64_t row_values(const attn_p & p) { return ((int64_t) p.T_q * p.H + 67) / 4 * 4; }
 int64_t part_q_values(const attn_p & p) { return p.split_q > 1 ? (int64_t) p.split_q * p.T_q * p.H * p.D : 0; }
@@ -1829,6 +1838,7 @@ int32_t nxg_attention_rows(const nxg_attention_rows_params * a, const nxg_rows *
     }
     if (p.T_q == 0 || p.n_seqs == 0) return NXG_OK;
     if (!p.cu_q || !p.cu_k || !lse) return nxg_fail(NXG_EINVAL, "%s: cu_q, cu_k or lse is null", what);
+    NXG_TRY(check_apart(what, "out", p.out, {&p.q, &p.k, &p.v}));
     NXG_TRY(nxg_check_device());
     p.lse = lse;
     p.near_k = near_rows(p.k) && near_rows(p.v);
@@ -1889,6 +1899,9 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
         return nxg_fail(NXG_EINVAL, "%s: workspace must be 16-byte aligned memory of %lld bytes", what,
                         (long long) backward_bytes(p));
     }
+    NXG_TRY(check_apart(what, "dq", p.dq, {&p.dout, &p.q, &p.k, &p.v, &p.out}));
+    NXG_TRY(check_apart(what, "dk", p.dk, {&p.dout, &p.q, &p.k, &p.v, &p.out, &p.dq}));
+    NXG_TRY(check_apart(what, "dv", p.dv, {&p.dout, &p.q, &p.k, &p.v, &p.out, &p.dq, &p.dk}));
     NXG_TRY(nxg_check_device());
     p.lse = (float *) lse;
     p.near_k = near_rows(p.k) && near_rows(p.v);

@@ -218,3 +218,19 @@ def test_layer_norm_in_place_with_another_stride_refused(nxg, L):
     for dys, xs, dx in ((128, 64, P16), (64, 128, 2 * P16)):
         refused(nxg, L, L.nxg_layer_norm_rows_backward(f32, P16, dys, 2 * P16, xs, P16, P16, None, f32, 4, 64, dx, 64, None, None, None, 0, None),
                 "another stride")
+
+
+def test_outputs_over_other_tensors_refused(nxg, L):
+    p = params(nxg, T_q=12)
+    for name in ("q", "k", "v"):
+        at = {n: rows(nxg, data=(2 + i) * P16) for i, n in enumerate(("q", "k", "v"))}
+        at["out"] = rows(nxg, data=at[name].data)
+        refused(nxg, L, forward(nxg, L, p, **at), "out is another tensor")
+    names = ["dout", "q", "k", "v", "out", "dq", "dk", "dv"]
+    need = L.nxg_attention_rows_backward_workspace_bytes(ctypes.byref(p))
+    for i, name in enumerate(names[5:], 5):
+        for other in names[:i]:
+            at = {n: rows(nxg, data=(2 + k) * P16) for k, n in enumerate(names)}
+            at[name] = rows(nxg, data=at[other].data)
+            a = [ctypes.byref(at[n]) for n in names]
+            refused(nxg, L, L.nxg_attention_rows_backward(ctypes.byref(p), *a[:5], P16, *a[5:], P16, need, None), f"{name} is another tensor")
