@@ -232,7 +232,8 @@ __device__ __forceinline__ job find_job(const attn_p & p, bool by_keys, int mul,
         tile = slot - (__builtin_amdgcn_readlane(upto, doc_rank) - __builtin_amdgcn_readlane(c, doc_rank));
     } else {
         // tiles of the first r + 1 documents above the next one's count
-        const int next = lane < 63 ? __shfl_down(c, 1) : 0;
+        // (every lane takes part in the move: what a lane that is switched off holds reads as 0)
+        const int down = __shfl_down(c, 1), next = lane < 63 ? down : 0;
         const int above = upto - (lane + 1) * next;
         const uint64_t here = __ballot(slot < above);
         if (!here) return r;
