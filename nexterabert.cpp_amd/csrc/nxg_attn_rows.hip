@@ -45,7 +45,10 @@ constexpr float LN2 = 0.69314718055994530942f;
 // fp16 alone: P is carried as 2^15 P in the backward pass (P <= 1, fp16 ends at 65504), so that weights
 // down to 2^-29 keep all their bits
 constexpr int P_SHIFT = 15;
-constexpr int N_MAX = 256;     // workgroups of the delta kernel, and row maxima they leave for fp16
+// ... and dS as f 2^15 P (dP - delta), a power of two f for each row that a lane sums up (dQ: a pair, dK: a key). It starts at
+// DS_START, for dS down to 2^-74, and is lowered to where the largest value is in 2^9 .. 2^10 whenever one is past DS_TOP.
+constexpr float DS_START = 0x1p45f, DS_TOP = 32768.0f;
+constexpr int DS_PLACE = 10;
 
 template <class E> struct type_of;
 template <> struct type_of<__bf16> {
@@ -72,7 +75,6 @@ struct attn_p {
     rows q, k, v, out, dout, dq, dk, dv;
     float * lse;               // [T_q][H]
     float * lse2, * ndelta;    // for the backward pass, a KV head's pairs one after another ([G][T_q R]): log2 of the sums, -delta
-    float * maxima;            // [N_MAX][2]: largest |dout row|^2 and |v row|^2 (fp16)
     float * part;              // partial sums of the split forward pass
     float * part_q, * part_kv; // partial gradients: [split_q][G][T_q R][D], [split_kv][dK, dV][G][T_k][D]
     const int32_t * cu_q, * cu_k;
@@ -1054,23 +1056,19 @@ __device__ __forceinline__ int doc_of_token(const int32_t * cu, int n_seqs, int 
     return lo;
 }
 
-// -delta = -sum(dout out) and log2 of the sums of each (token, head) row; for fp16 the largest squared norms of dout's and v's
-// rows, from which the gradients' kernels take the power of two that dS is carried with. L lanes a row (8 for heads of
-// up to 64). Bound by HBM: 32,900 tokens of 16 heads of 64, 135 MB, 33 us, 4.1 TB/s (28.5 without the look-up).
+// -delta = -sum(dout out) and log2 of the sums of each (token, head) row. L lanes a row (8 for heads of up to 64). Bound by
+// HBM: 32,900 tokens of 16 heads of 64, 135 MB, 33 us, 4.1 TB/s (28.5 without the look-up).
 template <class E, int L>
 __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
     typedef typename type_of<E>::v8 v8;
     constexpr int ROWS = 1024 / L;
     const int cc = threadIdx.x % L, sub = threadIdx.x / L;
-    float top_o = 0.0f, top_v = 0.0f;
     auto sum = [](float x) {
 #pragma unroll
         for (int k = L / 2; k; k >>= 1) x += __shfl_xor(x, k, L);
         return x;
     };
-    // the largest norms: of documents' rows alone
     const int q_lo = offset(p.cu_q, 0, p.T_q), q_hi = offset(p.cu_q, p.n_seqs, p.T_q);
-    const int k_lo = offset(p.cu_k, 0, p.T_k), k_hi = offset(p.cu_k, p.n_seqs, p.T_k);
     __shared__ int32_t s_cu[2][DELTA_DOCS + 1];
     const bool held = p.n_seqs <= DELTA_DOCS;
     if (held) {
@@ -1122,13 +1120,10 @@ __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
             const int pw = uni(p0 + ROWS * k);
             const bool few = pw < n_pairs && few_keys(pw / p.R, (min(pw + 64 / L, n_pairs) - 1) / p.R);
             if (at[k] < 0) continue;          // a row's lanes alike
-            float s = 0.0f, n2 = 0.0f;
+            float s = 0.0f;
             if (cc * 8 < p.D) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    s += (float) a[k][i] * (float) b[k][i];
-                    n2 += (float) a[k][i] * (float) a[k][i];
-                }
+                for (int i = 0; i < 8; ++i) s += (float) a[k][i] * (float) b[k][i];
             }
             s = sum(s);
             const int tok = (p0 + ROWS * k) / p.R;
@@ -1170,77 +1165,46 @@ __global__ __launch_bounds__(1024) void attn_rows_delta_kernel(attn_p p) {
                 p.lse2[row] = lse2 - (type_of<E>::HALF ? P_SHIFT : 0);
                 p.ndelta[row] = -s;
             }
-            if (type_of<E>::HALF) {
-                n2 = sum(n2);
-                if (tok >= q_lo && tok < q_hi) top_o = fmaxf(top_o, n2);
-            }
-        }
-    }
-    if (!type_of<E>::HALF) return;
-    const int n_v = k_hi * p.G;
-    for (int64_t row = (int64_t) k_lo * p.G + (int64_t) blockIdx.x * ROWS + sub; row < n_v; row += (int64_t) gridDim.x * ROWS) {
-        float n2 = 0.0f;
-        if (cc * 8 < p.D) {
-            const int tok = (int) row / p.G, g = (int) row % p.G;
-            const v8 a = *reinterpret_cast<const v8 *>(p.v.data + tok * p.v.ts + g * p.v.hs + cc * 16);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) n2 += (float) a[i] * (float) a[i];
-        }
-        top_v = fmaxf(top_v, sum(n2));
-    }
-    __shared__ float so[ROWS], sv[ROWS];
-    if (cc == 0) {
-        so[sub] = top_o;
-        sv[sub] = top_v;
-    }
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        float a = so[threadIdx.x], b = sv[threadIdx.x];
-        if (ROWS > 64) {
-            a = fmaxf(a, so[threadIdx.x + ROWS - 64]);
-            b = fmaxf(b, sv[threadIdx.x + ROWS - 64]);
-        }
-#pragma unroll
-        for (int k = 32; k; k >>= 1) {
-            a = fmaxf(a, __shfl_xor(a, k));
-            b = fmaxf(b, __shfl_xor(b, k));
-        }
-        if (threadIdx.x == 0) {
-            p.maxima[2 * blockIdx.x] = a;
-            p.maxima[2 * blockIdx.x + 1] = b;
         }
     }
 }
 
-// fp16: the factor from (2^15 P) (dP - delta) to dS as it is carried, 2^k dS with |dS| 2^k <= 2^15: |dP - delta| is at
-// most twice the product of the largest norms of dout's and v's rows, and P is at most 1. k = 0 where the
-// norms are no help.
-template <class E>
-__device__ __forceinline__ float ds_factor(const attn_p & p) {
-    if constexpr (!type_of<E>::HALF) return 1.0f;
-    const int lane = threadIdx.x & 63;
-    float a = 0.0f, b = 0.0f;
-    for (int i = lane; i < N_MAX; i += 64) {
-        a = fmaxf(a, p.maxima[2 * i]);
-        b = fmaxf(b, p.maxima[2 * i + 1]);
-    }
+// fp16: takes 2^15 dS to what is carried, f times that, within the type: where the lane's largest value is past DS_TOP, f and the
+// sum so far are lowered by a power of two, for both half waves of the column alike. So a row's small dS lose bits only
+// beside its own large ones (2^-34 of the largest at most), whatever other rows hold. Values that are not finite stay as
+// they are. Against one power of two for the launch, from the largest norms: 32 documents full 781 -> 818 us, 8,192 tokens causal
+// of 128 values a head 1,038 -> 1,045, 64 documents of 100 tokens 55 -> 50 (no norms to take).
+template <int DT>
+__device__ __forceinline__ void place_ds(v16f & ds, float & f, v16f (&sum)[DT]) {
+    float m = 0.0f;
 #pragma unroll
-    for (int k = 32; k; k >>= 1) {
-        a = fmaxf(a, __shfl_xor(a, k));
-        b = fmaxf(b, __shfl_xor(b, k));
+    for (int i = 0; i < 16; ++i) {
+        ds[i] *= f;
+        m = fmaxf(m, fabsf(ds[i]));
     }
-    const float bound = 2.0f * sqrtf(a) * sqrtf(b);
-    if (!(bound > 0.0f) || !(bound < INFINITY)) return ldexpf(1.0f, -P_SHIFT);
-    int e;
-    (void) frexpf(bound, &e);                        // bound < 2^e
-    return ldexpf(1.0f, min(max(15 - e, -30), 60) - P_SHIFT);
+    if (!__any(!(m <= DS_TOP))) return;
+    m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(ds[i]) < INFINITY ? fabsf(ds[i]) : 0.0f);
+    m = half_max(m);
+    const float lower = m > DS_TOP ? ldexpf(1.0f, DS_PLACE - __builtin_amdgcn_frexp_expf(m)) : 1.0f;
+    f *= lower;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ds[i] *= lower;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[d][i] *= lower;
 }
+// What turns a sum of carried dS into one of dS.
+template <class E>
+__device__ __forceinline__ float ds_unit(float f) { return type_of<E>::HALF ? 1.0f / ldexpf(f, P_SHIFT) : 1.0f; }
 
 // dQ: the forward pass's tiling. dQ^T = scale K^T dS^T.
 template <class E, int DT>
 __device__ __forceinline__ void dq_tile(v16f (&dq)[DT], const typename type_of<E>::v8 (&q)[2 * DT],
                                         const typename type_of<E>::v8 (&go)[2 * DT], lane_at at, uint32_t kt, uint32_t vt, float c,
-                                        float lse2, float ndelta, float factor, int sides, int lo, int hi) {
+                                        float lse2, float ndelta, float & f, int sides, int lo, int hi) {
     typedef type_of<E> TY;
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
@@ -1253,9 +1217,9 @@ __device__ __forceinline__ void dq_tile(v16f (&dq)[DT], const typename type_of<E
         for (int i = 0; i < 16; ++i) {
             const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2));
             s[i] = pr * (dp[i] + ndelta);
-            if (TY::HALF) s[i] *= factor;
         }
         if (sides) mask_rows(s, sides, lo - 32 * a, hi - 32 * a, 0.0f);
+        if constexpr (TY::HALF) place_ds<DT>(s, f, dq);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const typename TY::v8 ds = pack<E>(s, b);
@@ -1339,7 +1303,7 @@ __device__ __forceinline__ void dq_workgroup(const attn_p & p, int block, dq_lds
     typename type_of<E>::v8 q[2 * DT], go[2 * DT];
     load_operands<E, DT>(q, p.q.data + (c.q0 + tok) * p.q.ts + head * p.q.hs, go, p.dout.data + (c.q0 + tok) * p.dout.ts + head * p.dout.hs, p.D);
     const int64_t row = ((int64_t) g * p.T_q + c.q0) * p.R + pc;
-    const float factor = ds_factor<E>(p), ds_scale = type_of<E>::HALF ? ldexpf(factor, P_SHIFT) : 1.0f;
+    float f = DS_START;
     float lse2 = p.lse2[row], ndelta = p.ndelta[row];
     asm volatile("" : "+v"(lse2), "+v"(ndelta));
     for (int j = j_lo; j < j_hi; ++j) {
@@ -1348,7 +1312,7 @@ __device__ __forceinline__ void dq_workgroup(const attn_p & p, int block, dq_lds
         barrier();
         if (j + 1 < j_hi) keys.next(lds_addr(sk[buf ^ 1]), lds_addr(sv[buf ^ 1]));
         if (!active || j0 >= some_hi || j0 + BN <= some_lo) continue;
-        dq_tile<E, DT>(dq, q, go, at, lds_addr(sk[buf]), lds_addr(sv[buf]), cs, lse2, ndelta, factor, (j0 < all_lo ? 1 : 0) | (j0 + BN > all_hi ? 2 : 0), lo - j0, hi - j0);
+        dq_tile<E, DT>(dq, q, go, at, lds_addr(sk[buf]), lds_addr(sv[buf]), cs, lse2, ndelta, f, (j0 < all_lo ? 1 : 0) | (j0 + BN > all_hi ? 2 : 0), lo - j0, hi - j0);
     }
     barrier();
     if (!active) return;
@@ -1356,9 +1320,9 @@ __device__ __forceinline__ void dq_workgroup(const attn_p & p, int block, dq_lds
     uint32_t bad = bad_columns<DT>(dq);
     float * part = p.part_q + (((int64_t) split * p.G + g) * p.T_q + c.q0) * p.R * p.D;
     if (p.split_q > 1) {
-        store_partial<DT>(dq, p.scale / ds_scale, p.D, np - pw, part + (int64_t) pw * p.D);
+        store_partial<DT>(dq, p.scale * ds_unit<E>(f), p.D, np - pw, part + (int64_t) pw * p.D);
     } else {
-        store_columns<E, DT>(tile, dq, p.scale / ds_scale, p.D, [&](int r) -> char * {
+        store_columns<E, DT>(tile, dq, p.scale * ds_unit<E>(f), p.D, [&](int r) -> char * {
             const int pr = pw + r;
             if (pr >= np) return nullptr;
             return p.dq.data + (int64_t) (c.q0 + pr / p.R) * p.dq.ts + (g * p.R + pr % p.R) * p.dq.hs;
@@ -1398,7 +1362,7 @@ __device__ __forceinline__ void reads_ahead() {
 template <class E, int DT>
 __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const typename type_of<E>::v8 (&k)[2 * DT],
                                          const typename type_of<E>::v8 (&v)[2 * DT], lane_at at, uint32_t qt, uint32_t ot,
-                                         uint32_t lse2, uint32_t ndelta, float c, float factor, int sides, int lo, int hi) {
+                                         uint32_t lse2, uint32_t ndelta, float c, float & f, int sides, int lo, int hi) {
     typedef type_of<E> TY;
     typedef __attribute__((address_space(3))) v4f lds_v4f;
     const uint32_t h16 = (threadIdx.x & 32) >> 1;      // 4 values for the second half wave
@@ -1423,13 +1387,13 @@ __device__ __forceinline__ void dkv_tile(v16f (&dk)[DT], v16f (&dv)[DT], const t
             const int i = 4 * i4 + j;
             s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[j]));
             dp[i] *= s[i];
-            if (TY::HALF) dp[i] *= factor;
         }
     }
     if (sides) {
         mask_rows(s, sides, lo, hi, 0.0f);
         mask_rows(dp, sides, lo, hi, 0.0f);
     }
+    if constexpr (TY::HALF) place_ds<DT>(dp, f, dk);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
         const typename TY::v8 pp = pack<E>(s, b), ds = pack<E>(dp, b);
@@ -1514,7 +1478,7 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
     if (j_lo < j_hi) load(j_lo, 0);
     typename type_of<E>::v8 k[2 * DT], v[2 * DT];
     load_operands<E, DT>(k, p.k.data + (int64_t) (c.k0 + key) * p.k.ts + g * p.k.hs, v, p.v.data + (int64_t) (c.k0 + key) * p.v.ts + g * p.v.hs, p.D);
-    const float factor = ds_factor<E>(p), ds_scale = type_of<E>::HALF ? ldexpf(factor, P_SHIFT) : 1.0f;
+    float f = DS_START;
     for (int j = j_lo; j < j_hi; ++j) {
         const int buf = (j - j_lo) & 1, j0 = j * BQ;
         wait_all();
@@ -1533,7 +1497,7 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
 #pragma unroll 1
             for (int a = 0; a < BQ; a += 32) {
                 dkv_tile<E, DT>(dk, dv, k, v, at, lds_addr(sq[buf]) + a * SP<DT> * 2, lds_addr(so[buf]) + a * SP<DT> * 2, lds_addr(s_lse[buf]) + 4 * a,
-                                lds_addr(s_delta[buf]) + 4 * a, cs, factor, sides, lo - a, hi - a);
+                                lds_addr(s_delta[buf]) + 4 * a, cs, f, sides, lo - a, hi - a);
             }
         }
     }
@@ -1548,11 +1512,11 @@ __device__ __forceinline__ void dkv_workgroup(const attn_p & p, int block, dkv_l
     float * part = p.part_kv + 2 * split * part_v + ((int64_t) g * p.T_k + c.k0) * p.D;
     if (p.split_kv > 1) {
         store_partial<DT>(dv, type_of<E>::HALF ? 1.0f / (1 << P_SHIFT) : 1.0f, p.D, c.m - kw, part + part_v + (int64_t) kw * p.D);
-        store_partial<DT>(dk, p.scale / ds_scale, p.D, c.m - kw, part + (int64_t) kw * p.D);
+        store_partial<DT>(dk, p.scale * ds_unit<E>(f), p.D, c.m - kw, part + (int64_t) kw * p.D);
     } else {
         store_columns<E, DT>(tile, dv, type_of<E>::HALF ? 1.0f / (1 << P_SHIFT) : 1.0f, p.D, dst(p.dv));
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        store_columns<E, DT>(tile, dk, p.scale / ds_scale, p.D, dst(p.dk));
+        store_columns<E, DT>(tile, dk, p.scale * ds_unit<E>(f), p.D, dst(p.dk));
     }
     if (!bad) return;
     auto pair_row = [&](const rows & x) {
@@ -1739,7 +1703,7 @@ int32_t check_apart(const char * what, const char * name, const rows & out, std:
 int64_t row_values(const attn_p & p) { return ((int64_t) p.T_q * p.H + 67) / 4 * 4; }
 int64_t part_q_values(const attn_p & p) { return p.split_q > 1 ? (int64_t) p.split_q * p.T_q * p.H * p.D : 0; }
 int64_t part_kv_values(const attn_p & p) { return p.split_kv > 1 ? (int64_t) p.split_kv * 2 * p.T_k * p.G * p.D : 0; }
-int64_t backward_bytes(const attn_p & p) { return (2 * N_MAX + 2 * row_values(p) + part_q_values(p) + part_kv_values(p)) * 4; }
+int64_t backward_bytes(const attn_p & p) { return (2 * row_values(p) + part_q_values(p) + part_kv_values(p)) * 4; }
 
 // The length that a split is reckoned for, of which only the sum is known here: one document's, two's average, twice
 // that of more (mixed lengths: with the average 17 documents of 5 queries over 405 keys take 32 us, so 25).
@@ -1909,8 +1873,7 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
     p.near_q = near_pairs(p.q, p.R) && near_pairs(p.dout, p.R);
     p.even_q = 16 % p.R == 0;              // the rows of a thread's step
     p.by_R = ((1u << 22) + p.R - 1) / p.R;
-    p.maxima = (float *) workspace;
-    p.lse2 = p.maxima + 2 * N_MAX;
+    p.lse2 = (float *) workspace;
     p.ndelta = p.lse2 + row_values(p);
     p.part_q = p.ndelta + row_values(p);
     p.part_kv = p.part_q + part_q_values(p);
@@ -1918,13 +1881,13 @@ int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * a, const n
     if (p.T_q > 0) {
         const int L = p.D <= 64 ? 8 : 16;
         const int64_t n = ((int64_t) p.T_q * p.R + 2048 / L - 1) / (2048 / L) * p.G;
+        const unsigned grid = (unsigned) std::min<int64_t>(n, 1024);
         if (a->type == NXG_TYPE_BF16) {
-            const unsigned grid = (unsigned) std::min<int64_t>(n, 4 * N_MAX);
             if (L == 8) attn_rows_delta_kernel<__bf16, 8><<<grid, 1024, 0, s>>>(p);
             else attn_rows_delta_kernel<__bf16, 16><<<grid, 1024, 0, s>>>(p);
         } else {
-            if (L == 8) attn_rows_delta_kernel<_Float16, 8><<<N_MAX, 1024, 0, s>>>(p);
-            else attn_rows_delta_kernel<_Float16, 16><<<N_MAX, 1024, 0, s>>>(p);
+            if (L == 8) attn_rows_delta_kernel<_Float16, 8><<<grid, 1024, 0, s>>>(p);
+            else attn_rows_delta_kernel<_Float16, 16><<<grid, 1024, 0, s>>>(p);
         }
         NXG_TRY(nxg_launch_check(what));
     }
