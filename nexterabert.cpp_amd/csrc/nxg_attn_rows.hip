@@ -667,8 +667,12 @@ struct fwd_state {
 };
 
 // A sum of weights past which the reference is raised: P stays in either type's range, and the largest score is
-// looked for in few tiles, the first and some after it.
-constexpr float RAISE = 16384.0f;
+// looked for in few tiles, the first and some after it. A raise leaves the largest weight at 2^TOP: bf16 has fp32's exponents,
+// fp16 would lose weights below 2^-24, of which a long document's sum has many (one key 17.3 above 65,536 others alike:
+// their sum, 0.002 of all, as 0), and so loses those below 2^-34 of the largest.
+template <class E> struct reference {
+    static constexpr float RAISE = type_of<E>::HALF ? 60000.0f : 16384.0f, TOP = type_of<E>::HALF ? 10.0f : 0.0f;
+};
 
 // Scores of the wave's pairs with the 32 keys from row r0 of the tile.
 template <class E, int DT>
@@ -690,15 +694,15 @@ __device__ __forceinline__ float fwd_exp(v16f & w, const v16f & s, float c, floa
 }
 
 // The weights of 32 keys from their scores, with a new reference where the old one is passed: the largest
-// score so far.
-template <int DT>
+// score so far (fp16: 2^10 below it).
+template <class E, int DT>
 __device__ __forceinline__ void fwd_weights(v16f & w, const v16f & s, fwd_state<DT> & st, float c) {
     float t = fwd_exp(w, s, c, st.mc);
-    if (__any(!(t <= RAISE))) {
+    if (__any(!(t <= reference<E>::RAISE))) {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-        const float mc = fmaxf(st.mc, half_max(mx) * c);
+        const float mc = fmaxf(st.mc, half_max(mx) * c - reference<E>::TOP);
         const float f = st.mc == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.mc - mc);
         st.mc = mc;
         st.l *= f;
@@ -816,11 +820,11 @@ __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
         }
         if (sides) mask_rows(s0, sides, lo - j0, hi - j0, -INFINITY);
         s1 = fwd_scores<E, DT>(q, kt, 0);
-        fwd_weights<DT>(w, s0, st, cs);
+        fwd_weights<E, DT>(w, s0, st, cs);
         fwd_values<E, DT>(st, w, vt, 0);
         if (sides) mask_rows(s1, sides, lo - j0 - 32, hi - j0 - 32, -INFINITY);
         s0 = fwd_scores<E, DT>(q, kt, 32);             // of the next tile's first keys
-        fwd_weights<DT>(w, s1, st, cs);
+        fwd_weights<E, DT>(w, s1, st, cs);
         fwd_values<E, DT>(st, w, vt, 32);
     }
     barrier();
@@ -898,7 +902,7 @@ __global__ __launch_bounds__(256) void attn_rows_few_kernel(attn_p p) {
         v16f s = fwd_scores<E, DT>(q, lds_addr(lds[wave][buf][0]) + at.row, 0), w;
         const int sides = (j0 < all_lo ? 1 : 0) | (j0 + BN > all_hi ? 2 : 0);
         if (sides) mask_rows(s, sides, lo - j0, hi - j0, -INFINITY);
-        fwd_weights<DT>(w, s, st, cs);
+        fwd_weights<E, DT>(w, s, st, cs);
         fwd_values<E, DT>(st, w, lds_addr(lds[wave][buf][1]) + at.col, 0);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next load writes it
     }

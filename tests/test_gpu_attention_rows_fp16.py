@@ -171,3 +171,59 @@ def test_a_document_alone_and_in_a_batch(nxg, torch, dev):
     print("attention_rows fp16: twelve documents, one of them changed", flush=True)
     for a, b in zip(plain, run(nxg, q, k, v, do, cu, -1, 0)):
         assert torch.equal(a[:512], b[:512]) and torch.equal(a[1024:], b[1024:])
+
+
+def forward(torch, q, k, v, n, m, left, right, u, step):
+    """One document's (out, bound), as rows_ref's, where a carried weight is off by u of it, or by `step` of the largest."""
+    H, G, D = q.shape[1], k.shape[1], q.shape[2]
+    value, bound = (torch.zeros(n, H, D, dtype=torch.float64, device=q.device) for _ in range(2))
+    seen = rows_ref.window(n, m, left, right, q.device)
+    zero = torch.zeros((), dtype=torch.float64, device=q.device)
+    for h in range(H):
+        Q, K, V = q[:, h].double(), k[:, h // (H // G)].double(), v[:, h // (H // G)].double()
+        S = torch.where(seen, (Q @ K.t()) / math.sqrt(D), -math.inf)
+        es = torch.where(seen, (D + 8) * F32 / math.sqrt(D) * (Q.abs() @ K.abs().t()), zero).amax(1, keepdim=True)
+        # a sum takes 16 keys at once, with 4 roundings at most
+        ep = 2 * es + 8 * F32 * (torch.where(seen, S.abs(), zero).amax(1, keepdim=True) + 1) + (m / 4 + 64) * F32
+        P = torch.exp(S - torch.logsumexp(S, 1, keepdim=True))
+        value[:, h] = P @ V
+        bound[:, h] = (1.01 * u + 2 * ep) * (P @ V.abs()) + u * value[:, h].abs() + step * (seen.double() @ V.abs()) + rows_ref.least_step(q.dtype)
+    return value, bound
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 96])
+@pytest.mark.parametrize("n,m,H,G", [(1, 65536, 4, 2), (3, 30000, 2, 1), (700, 16384, 4, 4), (1, 1 << 20, 1, 1)])
+@pytest.mark.parametrize("above", [12.0, 14.0, 17.3, 21.0])
+@pytest.mark.parametrize("at", [0, 0.4, 1.0])
+def test_many_small_weights_beside_a_large_one(nxg, torch, dev, at, above, n, m, H, G, D, dtype):
+    """One key so far above all others (in nats) that each of them alone would be lost, but not their sum. A weight is carried with
+    the largest at 2^10 at least when it came, so that fp16's half step of 2^-25 is 2^-35 of it."""
+    print(f"attention_rows {dtype} {n} queries over {m} keys, one of them {above} above", flush=True)
+    dt = getattr(torch, dtype)
+    g = torch.Generator(device="cuda").manual_seed(m)
+    q = torch.zeros(n, H, D, device="cuda")
+    q[:, :, 0] = 1
+    k = torch.zeros(m, G, D, device="cuda")
+    k[int(at * (m - 1)), :, 0] = above * math.sqrt(D)
+    v = 1 + 0.25 * torch.randn(m, G, D, device="cuda", generator=g)
+    v[int(at * (m - 1))] = -0.01
+    q, k, v = q.to(dt), k.to(dt), v.to(dt)
+    out, _ = nxg.attention_rows(q, k, v, [0, n], [0, m])
+    step = 2.0 ** -35 if dt == torch.float16 else 0.0
+    rows_ref.check("out", out, *forward(torch, q, k, v, n, m, -1, -1, rows_ref.half_step(dt), step))
+
+
+@pytest.mark.parametrize("size", [0.5, 3.0, 10.0, 60.0])
+@pytest.mark.parametrize("n,m,H,G,left,right", [(1, 20000, 4, 2, -1, -1), (1500, 1500, 4, 2, -1, 0), (900, 900, 8, 8, 100, 100), (40, 3000, 2, 2, -1, 0)])
+def test_scores_of_all_sizes(nxg, torch, dev, n, m, H, G, left, right, size):
+    """Scores spread by `size`, rising along the keys too, so that the reference is raised now and then, or in every tile."""
+    print(f"attention_rows fp16 {n} over {m} keys, scores of +-{size}", flush=True)
+    D, dt = 64, torch.float16
+    g = torch.Generator(device="cuda").manual_seed(n)
+    q, k, v = (torch.randn(x, y, D, device="cuda", generator=g) for x, y in ((n, H), (m, G), (m, G)))
+    for ramp in (torch.ones(m, device="cuda"), torch.linspace(0.02, 1, m, device="cuda")):
+        a, b, c = (q * size).to(dt), (k * ramp[:, None, None]).to(dt), v.to(dt)
+        out, lse = nxg.attention_rows(a, b, c, [0, n], [0, m], left=left, right=right)
+        rows_ref.check("out", out, *forward(torch, a, b, c, n, m, left, right, rows_ref.half_step(dt), 2.0 ** -35))
+        rows_ref.check("lse", lse, *rows_ref.attention(a, b, c, [0, n], [0, m], 1 / math.sqrt(D), left, right)["lse"])
