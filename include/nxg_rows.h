@@ -131,7 +131,7 @@ typedef struct nxg_attention_rows_params {
  *   q, out     T_q rows of n_head heads;  k, v  T_k rows of n_kv_head heads (data 16-byte aligned, strides
  *              multiples of 8). out may not overlap an input
  *   lse        device float [T_q][n_head]
- *   workspace  device memory, 16-byte aligned, or null: nxg_attention_rows_workspace_bytes gives the size (0 for
+ *   workspace  device memory, 16-byte aligned, or null: nxg_attention_rows_workspace_bytes gives the size on the current device (0 for
  *              all but launches of few queries over many keys, which share a document's keys out over
  *              workgroups; with less they share less) */
 NXG_API int64_t nxg_attention_rows_workspace_bytes(const nxg_attention_rows_params * params);
@@ -144,7 +144,7 @@ NXG_API int32_t nxg_attention_rows(const nxg_attention_rows_params * params, con
  *   dout       T_q rows of n_head heads;  q, k, v, out, lse  as the forward call had and left them
  *   dq, dk, dv rows as q, k and v (written for every row of a document; keys that no query sees get zeros).
  *              They may not overlap an input or each other
- *   workspace  device memory, 16-byte aligned, nxg_attention_rows_backward_workspace_bytes bytes */
+ *   workspace  device memory, 16-byte aligned, nxg_attention_rows_backward_workspace_bytes (on the current device) bytes */
 NXG_API int64_t nxg_attention_rows_backward_workspace_bytes(const nxg_attention_rows_params * params);
 NXG_API int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * params, const nxg_rows * dout,
                                             const nxg_rows * q, const nxg_rows * k, const nxg_rows * v,

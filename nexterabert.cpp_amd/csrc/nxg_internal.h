@@ -19,7 +19,8 @@ int nxg_fail(int code, const char * fmt, ...) __attribute__((format(printf, 2, 3
 // NXG_OK if the current device is a gfx950 GPU.
 int nxg_check_device(void);
 
-// Compute units of the device that nxg_check_device last saw on this thread (256 before its first call).
+// Compute units of the current device (256 without a gfx950 GPU): the same on every thread, so that a workspace's size
+// and the call that uses it have one plan.
 int nxg_device_cus(void);
 
 // NXG_OK, or NXG_EDEVICE with the error of the launch just made.

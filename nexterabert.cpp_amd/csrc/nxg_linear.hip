@@ -3894,7 +3894,7 @@ int nxg_fail(int code, const char * fmt, ...) {
 }
 
 int nxg_check_device(void) { return check_device(); }
-int nxg_device_cus(void) { return device_cus(); }
+int nxg_device_cus(void) { return check_device() == NXG_OK ? device_cus() : 256; }
 int nxg_launch_check(const char * what) { return launch_check(what); }
 
 struct nxg_weight {
