@@ -42,6 +42,20 @@ _words = {n: ctypes.c_int64 * (3 * n) for n in (2, 4, 8)}
 _ROWS_BYTES = ctypes.sizeof(_Rows)
 
 
+_INT32 = (1 << 31) - 1
+
+
+def _sizes(*sizes):
+    """Refuses sizes that the C functions' int32 would take modulo 2^32."""
+    if max(sizes) > _INT32:
+        raise ValueError(f"sizes {', '.join(map(str, sizes))}: too large")
+
+
+def _side(n):
+    """A window's side as an int32: past it there is no more to see."""
+    return max(min(int(n), _INT32), -_INT32)
+
+
 def _type_of(t, name, allowed=None):
     if not _types:
         torch = _torch()
@@ -111,6 +125,7 @@ def rope_frequencies(n_rot: int, base: float, scaling: str = "none", factor: flo
     "by_parts" (each frequency by its turns over train_len positions)."""
     if scaling not in ROPE_SCALINGS:
         raise ValueError(f"scaling must be one of {', '.join(ROPE_SCALINGS)}")
+    _sizes(n_rot, train_len)
     freq = np.empty(max(n_rot, 0) // 2, np.float64)
     mscale = ctypes.c_float()
     _check(load_library().nxg_rope_frequencies(n_rot, float(base), ROPE_SCALINGS[scaling], float(factor), int(train_len),
@@ -131,6 +146,7 @@ def rope_rows(x, freq, cu_offsets=None, positions=None, layout: str = "half", ms
     xr = _head_rows(x, "x", dev, x.dtype)
     T, H, D = x.shape
     half = freq.numel()
+    _sizes(T, H, D, half)
     fp = _vector(freq, "freq", half, dev, (torch.float64,))
     if layout not in ROPE_LAYOUTS:
         raise ValueError(f"layout must be one of {', '.join(ROPE_LAYOUTS)}")
@@ -175,6 +191,7 @@ def layer_norm_rows(x, w=None, b=None, eps: float = 1e-5, out=None, mean=None, r
     dev = _device_of(x, "x")
     xp, xs = _plain_rows(x, "x", dev)
     T, C = x.shape
+    _sizes(T, C)
     wp, bp, wt = _norm_weights(x, w, b, dev)
     if out is None:
         out = x.new_empty((T, C))
@@ -195,6 +212,7 @@ def layer_norm_rows(x, w=None, b=None, eps: float = 1e-5, out=None, mean=None, r
 @functools.lru_cache(maxsize=256)
 def layer_norm_rows_workspace_bytes(T: int, C: int) -> int:
     """nxg_layer_norm_rows_workspace_bytes."""
+    _sizes(T, C)
     n = int(load_library().nxg_layer_norm_rows_workspace_bytes(T, C))
     _check(-n if n < 0 else 0, "layer_norm_rows_workspace_bytes")
     return n
@@ -221,6 +239,7 @@ def layer_norm_rows_backward(dy, x, mean, rstd, w=None, dx=None, dw=None, db=Non
     xp, xs = _plain_rows(x, "x", dev)
     gp, gs = _plain_rows(dy, "dy", dev, x)
     T, C = x.shape
+    _sizes(T, C)
     wp, _, wt = _norm_weights(x, w, None, dev)
     f32 = (torch.float32,)
     w_dtype = w.dtype if w is not None else f32[0]
@@ -259,12 +278,13 @@ def _attention_args(q, k, v, cu_q, cu_k, left, right, scale):
     K, G, Dk = k.shape
     if Dk != D:
         raise ValueError(f"k and v must have heads of {D}")
+    _sizes(T, H, K, G, D)
     cu_q = _offsets_arg(cu_q, q, dev)
     cu_k = cu_q if cu_k is None else _offsets_arg(cu_k, q, dev)
     n = cu_q.numel()
     if cu_k.numel() != n:
         raise ValueError("cu_q and cu_k must have the same number of documents")
-    left, right = int(left), int(right)
+    left, right = _side(left), _side(right)
     sizes = _attention_bytes(dev, ty, H, G, D, T, K, n - 1, left, right)
     p = _AttentionParams(ty, H, G, D, T, K, n - 1, cu_q.data_ptr(), cu_k.data_ptr(), left, right,
                          1.0 / math.sqrt(D) if scale is None else float(scale))
