@@ -115,7 +115,7 @@ NXG_API int32_t nxg_layer_norm_rows_backward(int32_t type, const void * dy, int6
  * h reads KV head h / (n_head / n_kv_head). */
 typedef struct nxg_attention_rows_params {
     int32_t type;              /* of every row: NXG_TYPE_F16 or NXG_TYPE_BF16 */
-    int32_t n_head, n_kv_head, head_dim;   /* head_dim: a multiple of 8, at most 128 */
+    int32_t n_head, n_kv_head, head_dim;   /* n_head: 1 to 65,536 times n_kv_head; head_dim: a multiple of 8, at most 128 */
     int32_t T_q, T_k;          /* rows of q and out, and of k and v: up to 2^30, T_q * n_head and T_k * n_kv_head below 2^31,
                                 * and n_kv_head * 128-row tiles of both below 2^24 (a document more: a tile more) */
     int32_t n_seqs;

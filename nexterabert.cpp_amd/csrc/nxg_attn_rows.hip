@@ -1625,6 +1625,7 @@ __global__ __launch_bounds__(1024) void attn_rows_grad_join_kernel(attn_p p, int
 int64_t slots(int64_t T, int64_t mul, int64_t tile, int64_t n_seqs) { return T * mul / tile + n_seqs; }
 
 constexpr int64_t MAX_T = 1 << 30;
+constexpr int MAX_R = 1 << 16;                 // the pieces of 128 tokens' pairs fit 32 bits
 constexpr int64_t MAX_GRID = (1 << 24) - 1;    // workgroups of a launch: less than 2^32 threads
 
 int32_t check_params(const char * what, const nxg_attention_rows_params * a, attn_p & p) {
@@ -1638,6 +1639,7 @@ int32_t check_params(const char * what, const nxg_attention_rows_params * a, att
     if (a->n_head < 1 || a->n_kv_head < 1 || a->n_head % a->n_kv_head) {
         return nxg_fail(NXG_EINVAL, "%s: n_head=%d n_kv_head=%d", what, a->n_head, a->n_kv_head);
     }
+    if (a->n_head / a->n_kv_head > MAX_R) return nxg_fail(NXG_EINVAL, "%s: n_head=%d n_kv_head=%d (up to %d to one)", what, a->n_head, a->n_kv_head, MAX_R);
     if (a->T_q < 0 || a->T_k < 0 || a->n_seqs < 0 || a->T_q > MAX_T || a->T_k > MAX_T) {
         return nxg_fail(NXG_EINVAL, "%s: T_q=%d T_k=%d n_seqs=%d", what, a->T_q, a->T_k, a->n_seqs);
     }

@@ -1,14 +1,17 @@
 """CPU: how a call of the row operators is shared out goes by the current device alone: not by the thread that asks, nor by
 what that thread called before. The device is a stand-in for the HIP runtime's two queries (in a process of its own); no call
-here gets as far as a launch."""
+here gets as far as a launch. And what sizes are refused."""
 from __future__ import annotations
 
+import ctypes
 import json
 import subprocess
 import sys
 from pathlib import Path
 
 import pytest
+
+from test_rows_abi import forward, params, refused
 
 ROOT = Path(__file__).resolve().parent.parent
 
@@ -98,3 +101,12 @@ def test_plans_go_by_the_device(tmp_path, nxg, before):
         assert rc == nxg.NXG_EINVAL and f"of {backward} bytes" in refusal
         got[cus] = forward, backward
     assert got[32][0] < got[256][0] and got[32][1] < got[256][1], "fewer CUs, fewer shares"
+
+
+def test_heads_of_a_kv_head(nxg):
+    """A tile's reach over 128 tokens is counted in 32 bits: 128 * 65,536 heads * 16 pieces of a head are 2^27."""
+    L = nxg.load_library()
+    for f in (L.nxg_attention_rows_workspace_bytes, L.nxg_attention_rows_backward_workspace_bytes):
+        assert f(ctypes.byref(params(nxg, n_head=1 << 16, n_kv_head=1))) >= 0
+        assert f(ctypes.byref(params(nxg, n_head=(1 << 16) + 1, n_kv_head=1))) == -nxg.NXG_EINVAL
+    refused(nxg, L, forward(nxg, L, params(nxg, n_head=1 << 20, n_kv_head=1, T_q=128)), "n_head=1048576")
