@@ -227,3 +227,27 @@ def test_scores_of_all_sizes(nxg, torch, dev, n, m, H, G, left, right, size):
         out, lse = nxg.attention_rows(a, b, c, [0, n], [0, m], left=left, right=right)
         rows_ref.check("out", out, *forward(torch, a, b, c, n, m, left, right, rows_ref.half_step(dt), 2.0 ** -35))
         rows_ref.check("lse", lse, *rows_ref.attention(a, b, c, [0, n], [0, m], 1 / math.sqrt(D), left, right)["lse"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("left,right", [(-1, 0), (7, 7), (12, 0), (0, 3), (40, -1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_infinities_inside_a_document(nxg, torch, dev, D, left, right, bad, dtype):
+    """Infinities of either sign in some tokens of one input: whatever does not depend on them (what stays finite in 64 bits with
+    NaN in their place) is as without. What does is not defined: a softmax of infinite scores, sums of both signs."""
+    print(f"attention_rows_backward {dtype} D={D} window={left},{right}: infinities in {bad}", flush=True)
+    dt = getattr(torch, dtype)
+    lens = [150, 75]
+    tensors = dict(zip(("q", "k", "v", "dout"), make(torch, dt, sum(lens), 4, 2, D, 5, 0.1)))
+    for i, t in enumerate((100, 149, 160)):
+        tensors[bad][t, i % 2, 3 * i] = math.inf if i % 2 else -math.inf
+    q, k, v, do = tensors.values()
+    got = run(nxg, q, k, v, do, offsets(lens), left, right)
+    q, k, v, do = (torch.where(torch.isinf(t), torch.full_like(t, math.nan), t) for t in (q, k, v, do))
+    ref = rows_ref.attention(q, k, v, offsets(lens), offsets(lens), 1 / math.sqrt(D), left, right, do)
+    for name, t in zip(("out", "lse", "dq", "dk", "dv"), got):
+        value, bound = ref[name]
+        exact, zero = torch.isfinite(value), torch.zeros((), dtype=torch.float64, device=t.device)
+        assert bool(exact.any())
+        rows_ref.check(name, torch.where(exact, t.double(), zero), torch.where(exact, value, zero), torch.where(exact, bound, zero))
