@@ -78,7 +78,7 @@ struct attn_p {
     float * part;              // partial sums of the split forward pass
     float * part_q, * part_kv; // partial gradients: [split_q][G][T_q R][D], [split_kv][dK, dV][G][T_k][D]
     const int32_t * cu_q, * cu_k;
-    int32_t n_seqs, T_q, T_k, H, G, R, D, left, right, n_slots, n_split, split_q, split_kv, order;
+    int32_t n_seqs, T_q, T_k, H, G, R, D, left, right, n_split, split_q, split_kv, order;
     float scale;
     uint32_t by_R;             // 2^22 / R, rounded up
     bool near_k, near_q;       // a tile's rows are within 32-bit offsets of its first
@@ -1819,8 +1819,7 @@ int32_t nxg_attention_rows(const nxg_attention_rows_params * a, const nxg_rows *
     p.n_split = f.n_split;
     p.part = (float *) workspace;
     hipStream_t s = (hipStream_t) stream;
-    p.n_slots = (int32_t) slots(p.T_q, p.R, f.few ? 32 : 128, p.n_seqs);
-    const unsigned grid = (unsigned) ((int64_t) p.n_slots * p.G * p.n_split);
+    const unsigned grid = (unsigned) (slots(p.T_q, p.R, f.few ? 32 : 128, p.n_seqs) * p.G * p.n_split);
     if (f.few) {
         NXG_BY_TYPE(a->type, p.D, (attn_rows_few_kernel<E, DT><<<grid, 256, 0, s>>>(p)));
         NXG_TRY(nxg_launch_check(what));

@@ -53,7 +53,8 @@ def _sizes(*sizes):
 
 def _side(n):
     """A window's side as an int32: past it there is no more to see."""
-    return max(min(int(n), _INT32), -_INT32)
+    n = int(n)
+    return n if -_INT32 <= n <= _INT32 else _INT32 if n > 0 else -_INT32
 
 
 def _type_of(t, name, allowed=None):
