@@ -759,9 +759,9 @@ __device__ __forceinline__ void fwd_again(const attn_p & p, const doc & c, int g
 //
 // Bound by the matrix units, and by the power that they and the exponentials beside them draw together: 65,536 tokens,
 // 16 heads of 64 on 8, bf16, full: 17.1 ms, 1,030 TFLOP/s (a library product of 8,192^3 reaches 1,138); the LDS copies cost
-// 7 to 9% of it, the exponentials 7%. 32 documents of 32,900 tokens, causal: 135 us, 680 TFLOP/s, the rest the masked
-// halves of tiles on the diagonal and the first tiles' latency. With 128 values a head 8,192 tokens full take 510 us,
-// 1,078 TFLOP/s; 8 x 1,024 tokens in a band of 257 keys 24 us, 6 tiles a workgroup, bound by their latency.
+// 7 to 9% of it, the exponentials 7%. 32 documents of 32,900 tokens, causal: 135 us, 680 TFLOP/s, the rest the starts
+// and ends of 4,248 workgroups of 11 tiles (9% of the tiles' pairs are masked). With 128 values a head 8,192 tokens full take 510 us,
+// 1,078 TFLOP/s; 8 x 1,024 tokens in a band of 257 keys 24 us, 5 tiles a workgroup, bound by their latency.
 template <class E, int DT>
 __global__ __launch_bounds__(256, 2) void attn_rows_fwd_kernel(attn_p p) {
     constexpr int BM = 128, BN = 64, TILE = BN * SP<DT>;

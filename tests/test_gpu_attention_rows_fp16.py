@@ -1,5 +1,5 @@
-"""GPU: attention_rows_backward in fp16, whose range dS leaves: each row's gradients are as exact as its own values allow,
-whatever other documents, or other tokens of its document, hold (bf16 with them, which has no such limits)."""
+"""GPU: attention_rows and its gradients in fp16, whose range P and dS leave: each row's results are as exact as its own values
+allow, whatever other documents, or other tokens of its document, hold (and bf16, which has no such limits)."""
 from __future__ import annotations
 
 import math
@@ -54,11 +54,10 @@ def check_documents(torch, got, q, k, v, do, lens, left, right, which):
 TYPES = ["float16", "bfloat16"]
 
 
-@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dtype,size", [("float16", (100.0, 30.0)), ("float16", (8000.0, 1000.0)), ("bfloat16", (8000.0, 1000.0))], ids=str)
 @pytest.mark.parametrize("lens", [[200, 70, 33], [1000, 300, 64]], ids=str)
-@pytest.mark.parametrize("size", [(100.0, 30.0), (1000.0, 100.0), (8000.0, 1000.0)], ids=str)
 @pytest.mark.parametrize("H,G,D", [(4, 2, 64), (2, 1, 128)])
-def test_another_documents_sizes(nxg, torch, dev, H, G, D, size, lens, dtype):
+def test_another_documents_sizes(nxg, torch, dev, H, G, D, lens, dtype, size):
     """dout and v of one document up to 2^23 and 2^10 times another's."""
     print(f"attention_rows {dtype} H={H} D={D} {lens}: a document of {size}", flush=True)
     q, k, v, do = make(torch, getattr(torch, dtype), sum(lens), H, G, D, 1)
@@ -72,13 +71,12 @@ def test_another_documents_sizes(nxg, torch, dev, H, G, D, size, lens, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bad", ["dout", "v", "both"])
-@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
-@pytest.mark.parametrize("grad", [1e-3, 1e-4])
-def test_another_documents_infinities(nxg, torch, dev, grad, value, bad, dtype):
+@pytest.mark.parametrize("value", [-math.inf, math.nan])
+def test_another_documents_infinities(nxg, torch, dev, value, bad, dtype):
     """One value of another document that is not finite."""
-    print(f"attention_rows {dtype} {value} in another document's {bad}, dout of {grad}", flush=True)
+    print(f"attention_rows {dtype} {value} in another document's {bad}", flush=True)
     lens = [500, 40, 90]
-    q, k, v, do = make(torch, getattr(torch, dtype), sum(lens), 4, 2, 64, 2, grad)
+    q, k, v, do = make(torch, getattr(torch, dtype), sum(lens), 4, 2, 64, 2, 1e-4)
     if bad != "v":
         do[510, 1, 3] = value
     if bad != "dout":
@@ -131,8 +129,7 @@ def gradients(torch, q, k, v, do, left, right, u, out_bound):
     return res
 
 
-@pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("H,G,D,n", [(4, 2, 64, 300), (2, 1, 64, 1500), (2, 2, 128, 700), (6, 2, 40, 260)])
+@pytest.mark.parametrize("H,G,D,n,dtype", [(4, 2, 64, 300, "float16"), (2, 1, 64, 1500, "float16"), (2, 2, 128, 700, "float16"), (6, 2, 40, 260, "bfloat16")])
 @pytest.mark.parametrize("left,right", [(-1, 0), (30, 30), (-1, -1)])
 @pytest.mark.parametrize("what", ["dout", "v", "both"])
 def test_tokens_of_other_sizes(nxg, torch, dev, what, left, right, H, G, D, n, dtype):
@@ -191,11 +188,10 @@ def forward(torch, q, k, v, n, m, left, right, u, step):
     return value, bound
 
 
-@pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("D", [64, 96])
-@pytest.mark.parametrize("n,m,H,G", [(1, 65536, 4, 2), (3, 30000, 2, 1), (700, 16384, 4, 4), (1, 1 << 20, 1, 1)])
-@pytest.mark.parametrize("above", [12.0, 14.0, 17.3, 21.0])
-@pytest.mark.parametrize("at", [0, 0.4, 1.0])
+@pytest.mark.parametrize("n,m,H,G,D,dtype", [(1, 65536, 4, 2, 64, "float16"), (3, 30000, 2, 1, 96, "float16"), (700, 16384, 4, 4, 64, "float16"),
+                                             (700, 16384, 4, 4, 96, "float16"), (700, 16384, 4, 4, 64, "bfloat16"), (1, 1 << 20, 1, 1, 64, "float16")])
+@pytest.mark.parametrize("above", [14.0, 17.3])
+@pytest.mark.parametrize("at", [0, 0.4])
 def test_many_small_weights_beside_a_large_one(nxg, torch, dev, at, above, n, m, H, G, D, dtype):
     """One key so far above all others (in nats) that each of them alone would be lost, but not their sum. A weight is carried with
     the largest at 2^10 at least when it came, so that fp16's half step of 2^-25 is 2^-35 of it."""
@@ -231,9 +227,8 @@ def test_scores_of_all_sizes(nxg, torch, dev, n, m, H, G, left, right, size):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bad", ["q", "k", "v", "dout"])
-@pytest.mark.parametrize("left,right", [(-1, 0), (7, 7), (12, 0), (0, 3), (40, -1)])
-@pytest.mark.parametrize("D", [64, 128])
-def test_infinities_inside_a_document(nxg, torch, dev, D, left, right, bad, dtype):
+@pytest.mark.parametrize("left,right,D", [(-1, 0, 64), (7, 7, 128), (40, -1, 64)])
+def test_infinities_inside_a_document(nxg, torch, dev, left, right, D, bad, dtype):
     """Infinities of either sign in some tokens of one input: whatever does not depend on them (what stays finite in 64 bits with
     NaN in their place) is as without. What does is not defined: a softmax of infinite scores, sums of both signs."""
     print(f"attention_rows_backward {dtype} D={D} window={left},{right}: infinities in {bad}", flush=True)
