@@ -12,7 +12,8 @@
  * are nxg_linear.h's: device pointers on the current device, `stream` a hipStream_t, NXG_OK or an
  * NXG_E* code with nxg_last_error(), calls return without waiting. Nothing is allocated and nothing
  * kept between calls, so calls on different streams may overlap as long as they share no output
- * and no workspace. Every call can be captured into a HIP graph.
+ * and no workspace. Every call can be captured into a HIP graph. An output shares no memory with
+ * another array of its call, except where it may be that array itself.
  *
  * Types are nxg_type's numbers: NXG_TYPE_F32, NXG_TYPE_F16, NXG_TYPE_BF16. Sums, statistics and
  * products are fp32 or wider whatever the rows' type; a result is rounded to it once.
