@@ -7,6 +7,9 @@
  *   nxg_rope_rows        rotary positions                     (beside nxg_qk_prep)
  *   nxg_layer_norm_rows  layer norm, forward and backward     (beside nxg_layer_norm)
  *   nxg_attention_rows   attention, forward and backward      (beside nxg_attention)
+ *   nxg_qk_norm_rope_rows  norms of queries and keys for each head, then their rotation, forward and backward (beside nxg_qk_prep)
+ *   nxg_dropout_rows     dropout whose mask is drawn again where it is needed
+ *   nxg_adapter_rows     low-rank adapters of many requests, forward and backward (beside nxg_linear_i8)
  *
  * They have no counterpart in the reference (NexteraBERT.cpp), which only infers. Conventions
  * are nxg_linear.h's: device pointers on the current device, `stream` a hipStream_t, NXG_OK or an
@@ -152,6 +155,100 @@ NXG_API int32_t nxg_attention_rows_backward(const nxg_attention_rows_params * pa
                                             const nxg_rows * out, const float * lse, const nxg_rows * dq,
                                             const nxg_rows * dk, const nxg_rows * dv, void * workspace,
                                             int64_t workspace_bytes, void * stream);
+
+/* ---------------------------------------------------------------------------
+ * Norms of queries and keys, and their rotation
+ * ------------------------------------------------------------------------- */
+
+/* What both directions take. Per head of a token: y = turn(x * rstd * w), rstd = 1 / sqrt(mean(x^2) + eps) over the
+ * head's values, turn as nxg_rope_rows with the same freq, n_rot, layout, mscale, positions and cu. */
+typedef struct nxg_qk_norm_rope_params {
+    int32_t type;              /* of every row */
+    int32_t T, n_head, n_kv_head, head_dim;    /* queries have n_head heads, keys n_kv_head; head_dim up to 1024 */
+    const void * wq, * wk;     /* device [head_dim] of w_type */
+    int32_t w_type;            /* `type` or F32 */
+    float   eps;
+    const double * freq;       /* as nxg_rope_rows */
+    int32_t n_rot, layout;
+    float   mscale;
+    const int32_t * positions, * cu;
+    int32_t n_seqs;
+} nxg_qk_norm_rope_params;
+
+/* Both in one launch. q_out and k_out may be q and k (same strides); k and k_out null: queries alone (n_kv_head 0). Sizes that
+ * would take 2^24 workgroups of about 12 KiB of rows are refused. */
+NXG_API int32_t nxg_qk_norm_rope_rows(const nxg_qk_norm_rope_params * params, const nxg_rows * q, const nxg_rows * k,
+                                      const nxg_rows * q_out, const nxg_rows * k_out, void * stream);
+
+/* The gradients, with u = the turn back of dy (times mscale), h = x * rstd, g = u * w:
+ *   dx = rstd * (g - h * mean(g * h)),  dw = sum over tokens and heads of u * h
+ * The sums are taken in a fixed order: the same call gives the same bits.
+ *   dq_out, dk_out  gradients of q_out and k_out;  q, k  the forward call's inputs
+ *   dq, dk          may be dq_out or q, dk_out or k, with their strides
+ *   dwq, dwk        device [head_dim] of w_type;  T = 0 gives zeros
+ *   workspace       device memory, 16-byte aligned, nxg_qk_norm_rope_rows_workspace_bytes(params) bytes */
+NXG_API int64_t nxg_qk_norm_rope_rows_workspace_bytes(const nxg_qk_norm_rope_params * params);
+NXG_API int32_t nxg_qk_norm_rope_rows_backward(const nxg_qk_norm_rope_params * params, const nxg_rows * dq_out,
+                                               const nxg_rows * dk_out, const nxg_rows * q, const nxg_rows * k,
+                                               const nxg_rows * dq, const nxg_rows * dk, void * dwq, void * dwk,
+                                               void * workspace, int64_t workspace_bytes, void * stream);
+
+/* ---------------------------------------------------------------------------
+ * Dropout
+ * ------------------------------------------------------------------------- */
+
+/* out = residual + (kept ? x / (1 - p) : 0), p rounded to a multiple of 2^-16. Whether value (t, c) is kept is drawn again by
+ * every call from (seed, offset, t, c) alone, whatever the strides and types: the same call on the gradient of out, without the
+ * residual, gives the gradient of x. The generator is Philox 4x32-10 (Salmon, Moraes, Dror and Shaw, 2011): key = seed's low and
+ * high 32 bits, counter = (c / 8, t, offset's low and high 32 bits); value c takes the 16 bits 16 (c % 2) of result word
+ * (c % 8) / 2 and is dropped where they are below p 2^16.
+ *   x, residual, out  device rows of `type`, T x C (C up to 2^30), their strides in values; residual may be null; out may be x or residual,
+ *                     with its stride
+ *   p        0 up to 65535 / 65536
+ *   offset   another for every mask of a seed;  step  device int64 [1] that is added to it, or null: read when the call
+ *            runs, so that replays of a captured graph draw new masks */
+NXG_API int32_t nxg_dropout_rows(int32_t type, const void * x, int64_t x_stride, const void * residual, int64_t residual_stride,
+                                 int32_t T, int32_t C, double p, uint64_t seed, uint64_t offset, const int64_t * step,
+                                 void * out, int64_t out_stride, void * stream);
+
+/* ---------------------------------------------------------------------------
+ * Low-rank adapters
+ * ------------------------------------------------------------------------- */
+
+/* Document d has adapter i = ids[d], or none (an id that is not in 0 .. n_adapters - 1). */
+typedef struct nxg_adapter_rows_params {
+    int32_t type;              /* of the rows */
+    int32_t w_type;            /* of a and b: `type`; F32 rows take F32, F16 or BF16 */
+    int32_t T, n_in, n_out;    /* T below 2^24; n_in, n_out up to 2^20 */
+    int32_t rank;              /* 1 to 128 */
+    int32_t n_adapters;        /* n_adapters * rank * n_in and * n_out below 2^31, * (n_in + n_out) below 2^30 */
+    int32_t n_seqs;            /* below 2^22 */
+    const int32_t * cu;        /* device int32 [n_seqs + 1] */
+    const int32_t * ids;       /* device int32 [n_seqs] */
+    const void * a;            /* device [n_adapters][rank][n_in] */
+    const void * b;            /* device [n_adapters][n_out][rank] */
+    float   scale;             /* of every adapter's share, finite */
+} nxg_adapter_rows_params;
+
+/* s = x a_i^T,  y = base + scale * s b_i^T  per row of a document; rows of a document without an adapter get base, and 0 as s. A row
+ * of x or base that holds an infinity or a NaN may give NaN where it would give an infinity; it has no part in other rows.
+ *   x      device rows of n_in values, base, y  of n_out (their strides in values); base may be null: 0. y may be base, with its stride
+ *   s      device float [T][rank]: what nxg_adapter_rows_backward takes */
+NXG_API int32_t nxg_adapter_rows(const nxg_adapter_rows_params * params, const void * x, int64_t x_stride, const void * base,
+                                 int64_t base_stride, void * y, int64_t y_stride, float * s, void * stream);
+
+/* The gradients, with g = scale * dy b_i:
+ *   dx = base + g a_i,  da_i = sum of g^T x,  db_i = scale * sum of dy^T s  over the rows of the documents with adapter i
+ * The sums are taken in a fixed order: the same call gives the same bits.
+ *   dy       device rows of n_out values;  x, s  as the forward call had and left them
+ *   base     rows of n_in values (the shared projection's part of dx), or null: 0;  dx  rows, or null; may be base, with its stride
+ *   da, db   device, as a and b, or null; zeros for an adapter that no row has
+ *   workspace  device memory, 16-byte aligned, nxg_adapter_rows_backward_workspace_bytes (on the current device) bytes */
+NXG_API int64_t nxg_adapter_rows_backward_workspace_bytes(const nxg_adapter_rows_params * params);
+NXG_API int32_t nxg_adapter_rows_backward(const nxg_adapter_rows_params * params, const void * dy, int64_t dy_stride, const void * x,
+                                          int64_t x_stride, const float * s, const void * base, int64_t base_stride, void * dx,
+                                          int64_t dx_stride, void * da, void * db, void * workspace, int64_t workspace_bytes,
+                                          void * stream);
 
 #ifdef __cplusplus
 }

@@ -11,7 +11,7 @@ stream as the HIP stream:
   Builder.linear(name, x, residual)         builder::linear        src/nexterabert.cpp:1121-1143
 
 and, with no counterpart in the reference, floating-point row operators with their gradients (rows.py,
-include/nxg_rows.h): rope_rows, layer_norm_rows, attention_rows.
+include/nxg_rows.h): rope_rows, layer_norm_rows, attention_rows, qk_norm_rope_rows, dropout_rows, adapter_rows.
 
 Errors follow the reference: bad input raises ValueError (rc 1), allocation
 MemoryError (rc 2), device failures RuntimeError (rc 3). There is no CPU
@@ -137,6 +137,13 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
         "nxg_attention_rows": ([P, P, P, P, P, P, P, i64, P], i32),
         "nxg_attention_rows_backward_workspace_bytes": ([P], i64),
         "nxg_attention_rows_backward": ([P, P, P, P, P, P, P, P, P, P, P, i64, P], i32),
+        "nxg_qk_norm_rope_rows": ([P, P, P, P, P, P], i32),
+        "nxg_qk_norm_rope_rows_workspace_bytes": ([P], i64),
+        "nxg_qk_norm_rope_rows_backward": ([P, P, P, P, P, P, P, P, P, P, i64, P], i32),
+        "nxg_dropout_rows": ([i32, P, i64, P, i64, i32, i32, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, P, P, i64, P], i32),
+        "nxg_adapter_rows": ([P, P, i64, P, i64, P, i64, P, P], i32),
+        "nxg_adapter_rows_backward_workspace_bytes": ([P], i64),
+        "nxg_adapter_rows_backward": ([P, P, i64, P, i64, P, P, i64, P, i64, P, P, P, i64, P], i32),
         "nxg_gemm_kernel_name": ([i32, i32, i32, i32, i32], ctypes.c_char_p),
         # include/nxg_gguf.h
         "nxg_gguf_open": ([ctypes.c_char_p, ctypes.POINTER(P)], i32),
@@ -1277,5 +1284,7 @@ class Builder:
         self.qcache.clear()
 
 
-from .rows import (attention_rows, attention_rows_backward, attention_rows_backward_workspace_bytes,  # noqa: E402
-                   layer_norm_rows, layer_norm_rows_backward, layer_norm_rows_workspace_bytes, rope_frequencies, rope_rows)
+from .rows import (adapter_rows, adapter_rows_backward, adapter_rows_backward_workspace_bytes, attention_rows,  # noqa: E402
+                   attention_rows_backward, attention_rows_backward_workspace_bytes, dropout_rows, layer_norm_rows,
+                   layer_norm_rows_backward, layer_norm_rows_workspace_bytes, qk_norm_rope_rows, qk_norm_rope_rows_backward,
+                   qk_norm_rope_rows_workspace_bytes, rope_frequencies, rope_rows)

@@ -88,7 +88,8 @@ def build(verbose: bool = False) -> Path:
     rows_common = ["-ffp-contract=fast" if c == "-ffp-contract=off" else c for c in common] + ["-Wno-inline-asm"]
     cmds = [[str(c) for c in (_hipcc(), *hip_only, *flags, "-Rpass-analysis=kernel-resource-usage",
                               "-c", CSRC / f"{src}.hip", "-o", OBJ / f"{src}.o")]
-            for src, flags in (("nxg_linear", common), ("nxg_rows", rows_common), ("nxg_attn_rows", rows_common))]
+            for src, flags in (("nxg_linear", common), ("nxg_rows", rows_common), ("nxg_attn_rows", rows_common),
+                              ("nxg_adapter_rows", rows_common))]
     runs = []
     for cmd in cmds:
         if verbose:
@@ -102,7 +103,8 @@ def build(verbose: bool = False) -> Path:
     (OBJ / "kernel_resources.txt").write_text("\n".join(map(_check_resources, errs)) + "\n")
     tmp = LIB.with_suffix(".so.tmp")
     _run([_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-pthread",
-          OBJ / "nxg_linear.o", OBJ / "nxg_rows.o", OBJ / "nxg_attn_rows.o", OBJ / "nxg_host.o", OBJ / "nxg_gguf.o", OBJ / "nxg_encoder.o", "-o", tmp], verbose)
+          OBJ / "nxg_linear.o", OBJ / "nxg_rows.o", OBJ / "nxg_attn_rows.o", OBJ / "nxg_adapter_rows.o",
+          OBJ / "nxg_host.o", OBJ / "nxg_gguf.o", OBJ / "nxg_encoder.o", "-o", tmp], verbose)
     os.replace(tmp, LIB)
     tmp = API_LIB.with_suffix(".so.tmp")
     _run(["g++", "-O2", "-fPIC", "-std=c++17", "-Wall", "-fvisibility=hidden", "-DNEXTERA_SHARED", "-DNEXTERA_BUILD",

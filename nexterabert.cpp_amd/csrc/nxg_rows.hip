@@ -1,5 +1,5 @@
-// nxg_rows.hip -- gfx950 kernels over packed floating-point rows: rotary positions and layer norm with its
-// gradients, and their C ABI (include/nxg_rows.h). All of them are bound by HBM: rows are read and written
+// nxg_rows.hip -- gfx950 kernels over packed floating-point rows: rotary positions, layer norm, head norms with rotary positions (both
+// with their gradients) and dropout, and their C ABI (include/nxg_rows.h). All of them are bound by HBM: rows are read and written
 // 16 bytes per lane, once.
 
 #include <hip/hip_runtime.h>
@@ -66,6 +66,21 @@ __device__ __forceinline__ int doc_of_row(const int32_t * cu, int n_seqs, int t)
     return lo;
 }
 
+// The turns of `tokens` rows from t0, [tokens][half], as (cos, sin) times the factor on the result, by the 256 threads of a workgroup.
+template <class P>
+__device__ __forceinline__ void find_turns(float2 * turn, const P & p, int t0, int tokens, int half) {
+    for (int k = threadIdx.x; k < tokens * half; k += 256) {
+        const int t = t0 + k / half, i = k % half;
+        int pos;
+        if (p.positions) pos = p.positions[t];
+        else pos = t - p.cu[doc_of_row(p.cu, p.n_seqs, t)];
+        const double turns = (double) pos * p.freq[i] * 0.15915494309189533577;   // 1 / (2 pi)
+        float s, c;
+        sincospif(2.0f * (float) (turns - rint(turns)), &s, &c);
+        turn[k] = make_float2(c * p.mscale, s * p.mscale * p.sign);
+    }
+}
+
 // A workgroup: tb tokens of hb heads. Their angles once, into LDS: position * frequency in 64 bits, as
 // turns less whole turns, then fp32 (error 2^-25 of a turn). Then the heads' rows as one run of
 // pieces, neighbouring lanes on neighbouring pieces: V values of a head from i and V from i + n / 2
@@ -79,16 +94,7 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(rope_p p) {
     const int half = p.n / 2;
     const int64_t t0 = (int64_t) blockIdx.x * p.tb;
     const int tokens = (int) min((int64_t) p.tb, p.T - t0);
-    for (int k = threadIdx.x; k < tokens * half; k += 256) {
-        const int t = (int) t0 + k / half, i = k % half;
-        int pos;
-        if (p.positions) pos = p.positions[t];
-        else pos = t - p.cu[doc_of_row(p.cu, p.n_seqs, t)];
-        const double turns = (double) pos * p.freq[i] * 0.15915494309189533577;   // 1 / (2 pi)
-        float s, c;
-        sincospif(2.0f * (float) (turns - rint(turns)), &s, &c);
-        turn[k] = make_float2(c * p.mscale, s * p.mscale * p.sign);
-    }
+    find_turns(turn, p, (int) t0, tokens, half);
     __syncthreads();
     const int h0 = blockIdx.y * p.hb, heads = min(p.hb, p.H - h0);
     const int pieces = HALF || V == 1 ? half / V : p.n / V, per_head = pieces + (p.copy ? (p.D - p.n) / V : 0), per_token = per_head * heads;
@@ -405,6 +411,335 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(norm_p p) {
 }
 
 // ---------------------------------------------------------------------------
+// norms of queries and keys, and their rotation
+// ---------------------------------------------------------------------------
+
+struct qk_rows {
+    const void * x, * dy;
+    void * out;                            // y, or dx
+    const void * w;
+    int64_t x_ts, x_hs, dy_ts, dy_hs, o_ts, o_hs;
+    int32_t H;
+};
+struct qk_p {
+    qk_rows of[2];                         // queries, keys
+    const double * freq;
+    const int32_t * positions, * cu;
+    float * part;                          // [workgroups][2][D]
+    int32_t T, D, n, n_seqs, tb, lanes;    // tokens of a workgroup at a time, lanes of a head (a power of two)
+    float mscale, sign, eps;
+    int32_t w_type;
+};
+
+// Where a head's values lie in its lanes: slot j (lane j % lanes, its j / lanes'th) has V values from d[0] and V from d[1]. A pair that is
+// turned is within a slot: values i of both pieces (HALF, and single values), or neighbours in one piece. A piece behind the head's
+// end has d = -1; turn: the first angle of the slot, or of the piece, or -1 where nothing is turned.
+struct qk_slot {
+    int d[2], turn[2];
+};
+template <int V, bool HALF>
+__device__ __forceinline__ qk_slot qk_slot_of(int j, int n, int D) {
+    qk_slot s;
+    const int half = n / 2;
+    if (HALF && j < half / V) {
+        s.d[0] = j * V;
+        s.d[1] = half + j * V;
+        s.turn[0] = s.turn[1] = j * V;
+        return s;
+    }
+    s.d[0] = HALF ? n + 2 * V * (j - half / V) : 2 * V * j;
+    s.d[1] = s.d[0] + V;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        s.turn[k] = !HALF && s.d[k] < n ? s.d[k] / 2 : -1;
+        if (s.d[k] >= D) s.d[k] = -1;
+    }
+    return s;
+}
+
+// A slot's values turned by the token's turns w.
+template <int V, bool HALF>
+__device__ __forceinline__ void qk_turn(float (&x)[2][V], const qk_slot & s, const float2 * w) {
+    if constexpr (HALF || V == 1) {
+        if (s.turn[0] < 0) return;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float c = w[s.turn[0] + i].x, z = w[s.turn[0] + i].y, a = x[0][i], b = x[1][i];
+            x[0][i] = a * c - b * z;
+            x[1][i] = a * z + b * c;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (s.turn[k] < 0) continue;
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float c = w[s.turn[k] + i].x, z = w[s.turn[k] + i].y, a = x[k][2 * i], b = x[k][2 * i + 1];
+                x[k][2 * i] = a * c - b * z;
+                x[k][2 * i + 1] = a * z + b * c;
+            }
+        }
+    }
+}
+
+template <class E, int V>
+__device__ __forceinline__ void qk_load(float (&x)[2][V], const E * row, const qk_slot & s) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[k][i] = 0.0f;
+        if (s.d[k] >= 0) load<E, V>(x[k], row + s.d[k]);
+    }
+}
+template <class E, int V>
+__device__ __forceinline__ void qk_store(E * row, const float (&x)[2][V], const qk_slot & s) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (s.d[k] >= 0) store<E, V>(row + s.d[k], x[k]);
+}
+
+// Sum over the lanes of a head.
+__device__ __forceinline__ float head_sum(float x, int lanes) {
+    for (int k = lanes / 2; k; k >>= 1) x += __shfl_xor(x, k);
+    return x;
+}
+
+// The weights as fp32 in LDS, and the turns of a workgroup's tokens; both before a barrier.
+__device__ __forceinline__ void qk_weights(float * w, const qk_p & p) {
+    for (int k = threadIdx.x; k < 2 * p.D; k += 256) {
+        const int i = k % p.D;
+        const void * from = p.of[k / p.D].w;
+        float x = 0.0f;
+        if (from) x = p.w_type == NXG_TYPE_F32 ? static_cast<const float *>(from)[i] : p.w_type == NXG_TYPE_F16 ? (float) static_cast<const _Float16 *>(from)[i]
+                                                                                                            : (float) static_cast<const __bf16 *>(from)[i];
+        w[k] = x;
+    }
+}
+
+// A workgroup: tb tokens, their turns and the weights once in LDS, then their heads, `lanes` lanes a head, P slots a lane: one
+// read, one write.
+template <class E, int V, bool HALF, int P>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(qk_p p) {
+    extern __shared__ float lds[];
+    const int half = p.n / 2;
+    float * w = lds;                                       // [2][D]
+    float2 * turn = reinterpret_cast<float2 *>(lds + 2 * p.D);
+    const int64_t t0 = (int64_t) blockIdx.x * p.tb;
+    const int tokens = (int) min((int64_t) p.tb, p.T - t0);
+    qk_weights(w, p);
+    find_turns(turn, p, (int) t0, tokens, half);
+    __syncthreads();
+    const int lane = threadIdx.x % p.lanes, first = threadIdx.x / p.lanes, step = 256 / p.lanes, heads = p.of[0].H + p.of[1].H;
+    qk_slot at[P];
+#pragma unroll
+    for (int s = 0; s < P; ++s) at[s] = qk_slot_of<V, HALF>(lane + s * p.lanes, p.n, p.D);
+    const float inv = 1.0f / (float) p.D;
+    for (int u = first; u < tokens * heads; u += step) {
+        const int t = u / heads, hh = u - t * heads, key = hh >= p.of[0].H;
+        const qk_rows & r = p.of[key];
+        const int h = key ? hh - p.of[0].H : hh;
+        const E * x = static_cast<const E *>(r.x) + (t0 + t) * r.x_ts + h * r.x_hs;
+        E * o = static_cast<E *>(r.out) + (t0 + t) * r.o_ts + h * r.o_hs;
+        float v[P][2][V], ss = 0.0f;
+#pragma unroll
+        for (int s = 0; s < P; ++s) qk_load<E, V>(v[s], x, at[s]);
+#pragma unroll
+        for (int s = 0; s < P; ++s)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) ss += v[s][k][i] * v[s][k][i];
+        const float rstd = 1.0f / sqrtf(head_sum(ss, p.lanes) * inv + p.eps);
+#pragma unroll
+        for (int s = 0; s < P; ++s) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[s][k][i] *= rstd * (at[s].d[k] >= 0 ? w[key * p.D + at[s].d[k] + i] : 0.0f);
+            qk_turn<V, HALF>(v[s], at[s], turn + t * half);
+            qk_store<E, V>(o, v[s], at[s]);
+        }
+    }
+}
+
+// Gradients: a workgroup's groups of tb tokens (every gridDim.x'th) one after another, the weights' sums of its heads in registers, left
+// as one row of `part`, which norm_reduce_kernel sums in order.
+template <class E, int V, bool HALF, int P>
+__global__ __launch_bounds__(256) void qk_norm_rope_back_kernel(qk_p p) {
+    extern __shared__ float lds[];
+    const int half = p.n / 2;
+    float * w = lds;                                       // [2][D]
+    float2 * turn = reinterpret_cast<float2 *>(lds + 2 * p.D);
+    const int lane = threadIdx.x % p.lanes, first = threadIdx.x / p.lanes, step = 256 / p.lanes;
+    qk_weights(w, p);
+    qk_slot at[P];
+    float dw[2][P][2][V];
+#pragma unroll
+    for (int s = 0; s < P; ++s) {
+        at[s] = qk_slot_of<V, HALF>(lane + s * p.lanes, p.n, p.D);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) dw[0][s][k][i] = dw[1][s][k][i] = 0.0f;
+    }
+    const float inv = 1.0f / (float) p.D;
+    for (int64_t t0 = (int64_t) blockIdx.x * p.tb; t0 < p.T; t0 += (int64_t) gridDim.x * p.tb) {
+        const int tokens = (int) min((int64_t) p.tb, p.T - t0);
+        __syncthreads();
+        find_turns(turn, p, (int) t0, tokens, half);
+        __syncthreads();
+#pragma unroll
+        for (int key = 0; key < 2; ++key) {
+            const qk_rows & r = p.of[key];
+            for (int u = first; u < tokens * r.H; u += step) {
+                const int t = u / r.H, h = u - t * r.H;
+                const E * x = static_cast<const E *>(r.x) + (t0 + t) * r.x_ts + h * r.x_hs;
+                const E * dy = static_cast<const E *>(r.dy) + (t0 + t) * r.dy_ts + h * r.dy_hs;
+                E * o = static_cast<E *>(r.out) + (t0 + t) * r.o_ts + h * r.o_hs;
+                float v[P][2][V], g[P][2][V], ss = 0.0f, gx = 0.0f;
+#pragma unroll
+                for (int s = 0; s < P; ++s) {
+                    qk_load<E, V>(v[s], x, at[s]);
+                    qk_load<E, V>(g[s], dy, at[s]);
+                }
+#pragma unroll
+                for (int s = 0; s < P; ++s)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) ss += v[s][k][i] * v[s][k][i];
+                const float rstd = 1.0f / sqrtf(head_sum(ss, p.lanes) * inv + p.eps);
+#pragma unroll
+                for (int s = 0; s < P; ++s) {
+                    qk_turn<V, HALF>(g[s], at[s], turn + t * half);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            v[s][k][i] *= rstd;
+                            dw[key][s][k][i] += g[s][k][i] * v[s][k][i];
+                            g[s][k][i] *= at[s].d[k] >= 0 ? w[key * p.D + at[s].d[k] + i] : 0.0f;
+                            gx += g[s][k][i] * v[s][k][i];
+                        }
+                }
+                gx = head_sum(gx, p.lanes) * inv;
+#pragma unroll
+                for (int s = 0; s < P; ++s) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) g[s][k][i] = rstd * (g[s][k][i] - v[s][k][i] * gx);
+                    qk_store<E, V>(o, g[s], at[s]);
+                }
+            }
+        }
+    }
+    // the heads' lanes that have the same slots, one group after another
+    float * sums = lds;                                    // [2][D], over the weights
+    for (int turn_of = 0; turn_of < step; ++turn_of) {
+        __syncthreads();
+        if (first != turn_of) continue;
+#pragma unroll
+        for (int key = 0; key < 2; ++key)
+#pragma unroll
+            for (int s = 0; s < P; ++s)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (at[s].d[k] >= 0) {
+                            float * to = sums + key * p.D + at[s].d[k] + i;
+                            *to = turn_of ? *to + dw[key][s][k][i] : dw[key][s][k][i];
+                        }
+    }
+    __syncthreads();
+    float * part = p.part + (int64_t) blockIdx.x * 2 * p.D;
+    for (int c = threadIdx.x; c < 2 * p.D; c += 256) part[c] = sums[c];
+}
+
+// ---------------------------------------------------------------------------
+// dropout
+// ---------------------------------------------------------------------------
+
+struct dropout_p {
+    const void * x, * residual;
+    void * out;
+    int64_t x_s, r_s, o_s;
+    const int64_t * step;
+    uint64_t seed, offset;
+    int32_t T, C, groups;                  // groups of 8 values of a row
+    uint32_t by_groups;                    // 2^32 / groups, rounded up; 0 for 1
+    uint32_t least;                        // the least 16 bits that keep a value
+    float scale;
+};
+
+// Philox 4x32-10: ten rounds of two 32 x 32-bit products on the counter, with a key that goes on by two constants.
+__device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+        const uint64_t a = (uint64_t) c[0] * 0xD2511F53u, b = (uint64_t) c[2] * 0xCD9E8D57u;
+        c[0] = (uint32_t) (b >> 32) ^ c[1] ^ k0;
+        c[1] = (uint32_t) b;
+        c[2] = (uint32_t) (a >> 32) ^ c[3] ^ k1;
+        c[3] = (uint32_t) a;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+}
+
+constexpr int DROP_GROUPS = 4;             // of a thread, whose loads are under way together
+
+// A thread: DROP_GROUPS groups of 8 values of a row, 256 apart, of the rows' groups one after another. The mask's bits are made while
+// the loads are under way.
+template <class E, bool WIDE>
+__global__ __launch_bounds__(256) void dropout_rows_kernel(dropout_p p) {
+    constexpr int V = WIDE ? 16 / (int) sizeof(E) : 1, N = 8 / V;
+    const uint64_t first = (uint64_t) blockIdx.x * 256 * DROP_GROUPS;
+    const uint32_t row0 = (uint32_t) (first / (uint32_t) p.groups), group0 = (uint32_t) (first % (uint32_t) p.groups);
+    const uint64_t offset = p.offset + (p.step ? (uint64_t) *p.step : 0);
+    const E * x = static_cast<const E *>(p.x), * residual = static_cast<const E *>(p.residual);
+    E * out = static_cast<E *>(p.out);
+    float v[DROP_GROUPS][N][V], r[DROP_GROUPS][N][V];
+    uint32_t row[DROP_GROUPS], group[DROP_GROUPS];
+#pragma unroll
+    for (int k = 0; k < DROP_GROUPS; ++k) {
+        // groups behind the first of row0: below 2^11 past a row's, or past one row at most
+        const uint32_t at = group0 + threadIdx.x + 256 * k, groups = p.groups;
+        const uint32_t rows = groups >= 256 * DROP_GROUPS ? at >= groups : p.by_groups ? __umulhi(at, p.by_groups) : at;
+        row[k] = row0 + rows;
+        group[k] = at - rows * groups;
+        const bool some = row[k] < (uint32_t) p.T;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int c = 8 * (int) group[k] + j * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[k][j][i] = r[k][j][i] = 0.0f;
+            if (some && c < p.C) {
+                load<E, V>(v[k][j], x + (int64_t) row[k] * p.x_s + c);
+                if (residual) load<E, V>(r[k][j], residual + (int64_t) row[k] * p.r_s + c);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < DROP_GROUPS; ++k) {
+        uint32_t bits[4] = {group[k], row[k], (uint32_t) offset, (uint32_t) (offset >> 32)};
+        philox(bits, (uint32_t) p.seed, (uint32_t) (p.seed >> 32));
+        if (row[k] >= (uint32_t) p.T) continue;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int c = 8 * (int) group[k] + j * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int e = j * V + i;
+                const uint32_t u = bits[e / 2] >> (16 * (e % 2)) & 0xffffu;
+                v[k][j][i] = (u >= p.least ? v[k][j][i] * p.scale : 0.0f) + r[k][j][i];
+            }
+            if (c < p.C) store<E, V>(out + (int64_t) row[k] * p.o_s + c, v[k][j]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 
@@ -485,6 +820,131 @@ bool by_row(int C, int es, bool wide, F f) {
 int norm_parts(int32_t T, int32_t C) {
     const int rows = C <= 1024 ? 4 : 1;          // of a workgroup at a time, at least
     return (int) std::max<int64_t>(1, std::min<int64_t>(NORM_PARTS, ((int64_t) T + rows - 1) / rows));
+}
+
+// Strides of rows of n_head heads that one call may read; of an output's, that no two of its rows overlap.
+int32_t check_heads(const char * what, const char * name, const nxg_rows * r, int32_t T, int32_t n_head, int32_t D, int es, bool written) {
+    if (!r || !r->data) return nxg_fail(NXG_EINVAL, "%s: %s is null", what, name);
+    const int64_t most = INT64_MAX / 16, ts = T > 1 ? r->token_stride : 0, hs = n_head > 1 ? r->head_stride : 0;
+    if (!aligned(r->data, es) || ts < 0 || hs < 0 || ts > most / T || hs > most / n_head) {
+        return nxg_fail(NXG_EINVAL, "%s: %s is not aligned to its type, or has strides %lld, %lld", what, name, (long long) ts, (long long) hs);
+    }
+    if (written) {
+        const bool heads_in = hs <= ts || T == 1;
+        const int64_t in_n = heads_in ? n_head : T, in_s = heads_in ? hs : ts, out_n = heads_in ? T : n_head, out_s = heads_in ? ts : hs;
+        if ((in_n > 1 && in_s < D) || (out_n > 1 && out_s < (in_n - 1) * in_s + D)) {
+            return nxg_fail(NXG_EINVAL, "%s: rows of %s overlap (strides %lld, %lld)", what, name, (long long) ts, (long long) hs);
+        }
+    }
+    return NXG_OK;
+}
+
+int32_t check_qk(const char * what, const nxg_qk_norm_rope_params * p) {
+    if (!p) return nxg_fail(NXG_EINVAL, "%s: null params", what);
+    if (!size_of(p->type)) return nxg_fail(NXG_EINVAL, "%s: type %d (F32, F16 or BF16)", what, p->type);
+    if (p->w_type != p->type && p->w_type != NXG_TYPE_F32) return nxg_fail(NXG_EINVAL, "%s: weight type %d (the rows' or F32)", what, p->w_type);
+    if (p->T < 0 || p->n_head < 1 || p->n_kv_head < 0 || p->head_dim < 2 || p->head_dim > 1024 || p->n_head > 65536 || p->n_kv_head > 65536) {
+        return nxg_fail(NXG_EINVAL, "%s: T=%d n_head=%d n_kv_head=%d head_dim=%d", what, p->T, p->n_head, p->n_kv_head, p->head_dim);
+    }
+    if (!(p->eps >= 0.0f) || !std::isfinite(p->eps)) return nxg_fail(NXG_EINVAL, "%s: eps=%g", what, p->eps);
+    if (p->n_rot < 2 || p->n_rot % 2 || p->n_rot > p->head_dim) return nxg_fail(NXG_EINVAL, "%s: n_rot=%d of head_dim=%d", what, p->n_rot, p->head_dim);
+    if (p->layout != NXG_ROPE_HALF && p->layout != NXG_ROPE_INTERLEAVED) return nxg_fail(NXG_EINVAL, "%s: layout %d", what, p->layout);
+    return NXG_OK;
+}
+
+// The rows of one operand pair (queries, or keys) into p, checked. out: y, or dx.
+int32_t take_qk(const char * what, const nxg_qk_norm_rope_params & a, qk_rows & r, bool keys, const nxg_rows * x, const nxg_rows * dy,
+                const nxg_rows * out, bool back) {
+    const int es = size_of(a.type);
+    const char * x_name = keys ? "k" : "q", * dy_name = keys ? "dk_out" : "dq_out", * out_name = back ? (keys ? "dk" : "dq") : keys ? "k_out" : "q_out";
+    r.H = keys ? a.n_kv_head : a.n_head;
+    r.w = keys ? a.wk : a.wq;
+    if (!r.w || !aligned(r.w, size_of(a.w_type))) return nxg_fail(NXG_EINVAL, "%s: %s is null or not aligned to its type", what, keys ? "wk" : "wq");
+    NXG_TRY(check_heads(what, x_name, x, a.T, r.H, a.head_dim, es, false));
+    if (back) NXG_TRY(check_heads(what, dy_name, dy, a.T, r.H, a.head_dim, es, false));
+    NXG_TRY(check_heads(what, out_name, out, a.T, r.H, a.head_dim, es, true));
+    auto ts = [&](const nxg_rows * v) { return a.T > 1 ? v->token_stride : 0; };
+    auto hs = [&](const nxg_rows * v) { return r.H > 1 ? v->head_stride : 0; };
+    for (const nxg_rows * v : {x, back ? dy : x}) {
+        if (v->data == out->data && (ts(v) != ts(out) || hs(v) != hs(out))) {
+            return nxg_fail(NXG_EINVAL, "%s: %s is an input with other strides", what, out_name);
+        }
+    }
+    r.x = x->data;
+    r.x_ts = ts(x);
+    r.x_hs = hs(x);
+    r.dy = back ? dy->data : nullptr;
+    r.dy_ts = back ? ts(dy) : 0;
+    r.dy_hs = back ? hs(dy) : 0;
+    r.out = out->data;
+    r.o_ts = ts(out);
+    r.o_hs = hs(out);
+    return NXG_OK;
+}
+
+// Both directions' plan: tokens of a workgroup, lanes of a head, and the instance f(V, HALF, P).
+struct qk_plan {
+    bool wide;
+    int slots, per_lane;
+    size_t lds;
+};
+qk_plan plan_qk(const nxg_qk_norm_rope_params & a, qk_p & p) {
+    qk_plan l;
+    const int es = size_of(a.type), V = 16 / es;
+    l.wide = a.n_rot % (a.layout == NXG_ROPE_HALF ? 2 * V : V) == 0 && a.head_dim % V == 0;
+    for (const qk_rows & r : p.of) {
+        if (r.H == 0) continue;
+        l.wide = l.wide && wide(r.x, r.x_ts, es) && wide(r.x, r.x_hs, es) && wide(r.out, r.o_ts, es) && wide(r.out, r.o_hs, es) &&
+                 wide(r.dy, r.dy_ts, es) && wide(r.dy, r.dy_hs, es);
+    }
+    const int v = l.wide ? V : 1;
+    l.slots = a.layout == NXG_ROPE_HALF ? a.n_rot / 2 / v + (a.head_dim - a.n_rot + 2 * v - 1) / (2 * v) : (a.head_dim + 2 * v - 1) / (2 * v);
+    p.lanes = 1;
+    while (p.lanes < 64 && p.lanes < l.slots) p.lanes *= 2;
+    l.per_lane = (l.slots + p.lanes - 1) / p.lanes;
+    // tokens: about 12 KiB of rows, an angle a thread at most, fewer where that would leave CUs without work
+    const int64_t row = (int64_t) (a.n_head + a.n_kv_head) * a.head_dim * es;
+    p.tb = std::max<int>(1, std::min<int64_t>(512 / a.n_rot, 12288 / row));
+    while (p.tb > 1 && ((int64_t) a.T + p.tb - 1) / p.tb < 2 * nxg_device_cus()) p.tb /= 2;
+    l.lds = (size_t) 2 * a.head_dim * sizeof(float) + (size_t) p.tb * (a.n_rot / 2) * sizeof(float2);
+    p.freq = a.freq;
+    p.positions = a.positions;
+    p.cu = a.cu;
+    p.n_seqs = a.n_seqs;
+    p.T = a.T;
+    p.D = a.head_dim;
+    p.n = a.n_rot;
+    p.eps = a.eps;
+    p.mscale = a.mscale;
+    p.w_type = a.w_type;
+    return l;
+}
+// A lane has one slot of 16-byte pieces, or two of fp32 heads over 512 values; up to 8 of single values.
+template <class F>
+void by_qk(const nxg_qk_norm_rope_params & a, const qk_plan & l, F f) {
+    by_type(a.type, [&](auto e) {
+        constexpr int V = 16 / (int) sizeof(e);
+        auto by_lane = [&](auto half) {
+            if (l.wide) {
+                if constexpr (V == 4) {
+                    if (l.per_lane > 1) return f(e, num<V>(), half, num<2>());
+                }
+                f(e, num<V>(), half, num<1>());
+            } else if (l.per_lane <= 1) {
+                f(e, num<1>(), half, num<1>());
+            } else {
+                f(e, num<1>(), half, num<8>());
+            }
+        };
+        if (a.layout == NXG_ROPE_HALF) by_lane(std::true_type());
+        else by_lane(std::false_type());
+    });
+}
+
+int32_t check_positions(const char * what, const nxg_qk_norm_rope_params & a) {
+    if (!a.freq || (!a.positions && !a.cu)) return nxg_fail(NXG_EINVAL, "%s: null freq, or neither positions nor cu", what);
+    if (!a.positions && a.n_seqs < 1) return nxg_fail(NXG_EINVAL, "%s: n_seqs=%d", what, a.n_seqs);
+    return NXG_OK;
 }
 
 } // namespace
@@ -715,6 +1175,131 @@ int32_t nxg_layer_norm_rows_backward(int32_t type, const void * dy, int64_t dy_s
     if (!p.part) return NXG_OK;
     const unsigned grid = (unsigned) ((2 * (int64_t) C + 15) / 16);
     by_types(type, w_type, [&](auto, auto we) { norm_reduce_kernel<decltype(we)><<<grid, 1024, 0, s>>>(p); });
+    return nxg_launch_check(what);
+}
+
+int32_t nxg_qk_norm_rope_rows(const nxg_qk_norm_rope_params * params, const nxg_rows * q, const nxg_rows * k, const nxg_rows * q_out,
+                              const nxg_rows * k_out, void * stream) {
+    const char * what = "qk_norm_rope_rows";
+    NXG_TRY(check_qk(what, params));
+    const nxg_qk_norm_rope_params & a = *params;
+    if (a.T == 0) return NXG_OK;
+    NXG_TRY(check_positions(what, a));
+    qk_p p = {};
+    NXG_TRY(take_qk(what, a, p.of[0], false, q, nullptr, q_out, false));
+    if (a.n_kv_head) {
+        NXG_TRY(take_qk(what, a, p.of[1], true, k, nullptr, k_out, false));
+        if (q_out->data == k_out->data || q_out->data == k->data || k_out->data == q->data) {
+            return nxg_fail(NXG_EINVAL, "%s: an output is another tensor of the call", what);
+        }
+    }
+    const qk_plan l = plan_qk(a, p);
+    p.sign = 1.0f;
+    const int64_t grid = ((int64_t) a.T + p.tb - 1) / p.tb;
+    if (grid > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d is too large", what, a.T);
+    NXG_TRY(nxg_check_device());
+    by_qk(a, l, [&](auto e, auto V, auto half, auto P) {
+        qk_norm_rope_kernel<decltype(e), V(), half(), P()><<<(unsigned) grid, 256, l.lds, (hipStream_t) stream>>>(p);
+    });
+    return nxg_launch_check(what);
+}
+
+int64_t nxg_qk_norm_rope_rows_workspace_bytes(const nxg_qk_norm_rope_params * params) {
+    const int32_t rc = check_qk("qk_norm_rope_rows_workspace_bytes", params);
+    return rc ? -rc : (int64_t) NORM_PARTS * 2 * params->head_dim * 4;
+}
+
+int32_t nxg_qk_norm_rope_rows_backward(const nxg_qk_norm_rope_params * params, const nxg_rows * dq_out, const nxg_rows * dk_out,
+                                       const nxg_rows * q, const nxg_rows * k, const nxg_rows * dq, const nxg_rows * dk, void * dwq,
+                                       void * dwk, void * workspace, int64_t workspace_bytes, void * stream) {
+    const char * what = "qk_norm_rope_rows_backward";
+    NXG_TRY(check_qk(what, params));
+    const nxg_qk_norm_rope_params & a = *params;
+    const int ws = size_of(a.w_type);
+    if (!dwq || !aligned(dwq, ws) || (a.n_kv_head && (!dwk || !aligned(dwk, ws)))) {
+        return nxg_fail(NXG_EINVAL, "%s: dwq or dwk is null or not aligned to its type", what);
+    }
+    if (!workspace || ((uintptr_t) workspace & 15) || workspace_bytes < (int64_t) NORM_PARTS * 2 * a.head_dim * 4) {
+        return nxg_fail(NXG_EINVAL, "%s: workspace must be 16-byte aligned memory of %lld bytes", what,
+                        (long long) nxg_qk_norm_rope_rows_workspace_bytes(params));
+    }
+    qk_p p = {};
+    int64_t grid = 0;
+    hipStream_t s = (hipStream_t) stream;
+    if (a.T > 0) {
+        NXG_TRY(check_positions(what, a));
+        NXG_TRY(take_qk(what, a, p.of[0], false, q, dq_out, dq, true));
+        if (a.n_kv_head) {
+            NXG_TRY(take_qk(what, a, p.of[1], true, k, dk_out, dk, true));
+            for (const nxg_rows * o : {dq, dk}) {
+                const nxg_rows * other[] = {o == dq ? k : q, o == dq ? dk_out : dq_out, o == dq ? dk : dq};
+                for (const nxg_rows * r : other)
+                    if (o->data == r->data) return nxg_fail(NXG_EINVAL, "%s: an output is another tensor of the call", what);
+            }
+        }
+        const qk_plan l = plan_qk(a, p);
+        p.sign = -1.0f;
+        p.part = static_cast<float *>(workspace);
+        grid = std::min<int64_t>(NORM_PARTS, ((int64_t) a.T + p.tb - 1) / p.tb);
+        NXG_TRY(nxg_check_device());
+        by_qk(a, l, [&](auto e, auto V, auto half, auto P) {
+            qk_norm_rope_back_kernel<decltype(e), V(), half(), P()><<<(unsigned) grid, 256, l.lds, s>>>(p);
+        });
+        NXG_TRY(nxg_launch_check(what));
+    } else {
+        NXG_TRY(nxg_check_device());
+    }
+    // dw and db of the norm's sums are here dwq and dwk
+    norm_p n = {};
+    n.part = static_cast<float *>(workspace);
+    n.n_part = (int32_t) grid;
+    n.C = a.head_dim;
+    n.dw = dwq;
+    n.db = a.n_kv_head ? dwk : nullptr;
+    by_types(a.type, a.w_type, [&](auto, auto we) { norm_reduce_kernel<decltype(we)><<<(2 * a.head_dim + 15) / 16, 1024, 0, s>>>(n); });
+    return nxg_launch_check(what);
+}
+
+int32_t nxg_dropout_rows(int32_t type, const void * x, int64_t x_stride, const void * residual, int64_t residual_stride, int32_t T,
+                         int32_t C, double drop, uint64_t seed, uint64_t offset, const int64_t * step, void * out,
+                         int64_t out_stride, void * stream) {
+    const char * what = "dropout_rows";
+    const int es = size_of(type);
+    if (!es) return nxg_fail(NXG_EINVAL, "%s: type %d (F32, F16 or BF16)", what, type);
+    if (T < 0 || C < 1 || C > 1 << 30) return nxg_fail(NXG_EINVAL, "%s: T=%d C=%d", what, T, C);
+    if (!(drop >= 0.0) || !(drop < 1.0) || std::nearbyint(drop * 65536.0) > 65535.0) return nxg_fail(NXG_EINVAL, "%s: p=%g (0 to 65535 / 65536)", what, drop);
+    if (T == 0) return NXG_OK;
+    NXG_TRY(check_norm_rows(what, "x", x, x_stride, T, C, es, false));
+    if (residual) NXG_TRY(check_norm_rows(what, "residual", residual, residual_stride, T, C, es, false));
+    NXG_TRY(check_norm_rows(what, "out", out, out_stride, T, C, es, true));
+    if (step && !aligned(step, 8)) return nxg_fail(NXG_EINVAL, "%s: step is not aligned to its type", what);
+    if (T > 1 && ((out == x && out_stride != x_stride) || (out == residual && out_stride != residual_stride))) {
+        return nxg_fail(NXG_EINVAL, "%s: out is x or residual with another stride", what);
+    }
+    dropout_p p = {};
+    p.x = x;
+    p.residual = residual;
+    p.out = out;
+    p.x_s = T > 1 ? x_stride : 0;
+    p.r_s = T > 1 ? residual_stride : 0;
+    p.o_s = T > 1 ? out_stride : 0;
+    p.step = step;
+    p.seed = seed;
+    p.offset = offset;
+    p.T = T;
+    p.C = C;
+    p.groups = (C + 7) / 8;
+    p.by_groups = (uint32_t) (((1ull << 32) + p.groups - 1) / p.groups);
+    p.least = (uint32_t) std::nearbyint(drop * 65536.0);
+    p.scale = 65536.0f / (float) (65536 - p.least);
+    const int64_t grid = ((int64_t) T * p.groups + 256 * DROP_GROUPS - 1) / (256 * DROP_GROUPS);
+    if (grid > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d C=%d is too large", what, T, C);
+    NXG_TRY(nxg_check_device());
+    const bool w = wide(x, p.x_s, es) && (!residual || wide(residual, p.r_s, es)) && wide(out, p.o_s, es) && C % (16 / es) == 0;
+    by_type(type, [&](auto e) {
+        if (w) dropout_rows_kernel<decltype(e), true><<<(unsigned) grid, 256, 0, (hipStream_t) stream>>>(p);
+        else dropout_rows_kernel<decltype(e), false><<<(unsigned) grid, 256, 0, (hipStream_t) stream>>>(p);
+    });
     return nxg_launch_check(what);
 }
 

@@ -1,5 +1,6 @@
 """Floating-point operators over packed rows, with their gradients (include/nxg_rows.h): rotary
-positions, layer norm and attention, in 16-bit types (rope and norm in fp32 too).
+positions, layer norm, attention, head norms with rotation, dropout and low-rank adapters, in 16-bit types (all but
+attention in fp32 too).
 
 Rows of several heads are tensors [T][n_head][head_dim] with any strides whose last is 1 (a slice of a
 fused projection, or head-major storage as a transposed view). Documents are given by cu_offsets, a host
@@ -16,7 +17,7 @@ from typing import Optional
 import numpy as np
 
 from . import (TYPE_BF16, TYPE_F16, TYPE_F32, _check, _device_offsets, _np_ptr, _order_on, _raw_device, _stream_ptr, _torch,
-               load_library)
+               _uploaded, load_library)
 
 ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "by_parts": 3}
 ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
@@ -35,10 +36,26 @@ class _AttentionParams(ctypes.Structure):
                 ("scale", ctypes.c_float)]
 
 
+class _QkNormRopeParams(ctypes.Structure):
+    """struct nxg_qk_norm_rope_params."""
+    _fields_ = [("type", ctypes.c_int32), ("T", ctypes.c_int32), ("n_head", ctypes.c_int32), ("n_kv_head", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("wq", ctypes.c_void_p), ("wk", ctypes.c_void_p), ("w_type", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("freq", ctypes.c_void_p), ("n_rot", ctypes.c_int32), ("layout", ctypes.c_int32),
+                ("mscale", ctypes.c_float), ("positions", ctypes.c_void_p), ("cu", ctypes.c_void_p), ("n_seqs", ctypes.c_int32)]
+
+
+class _AdapterParams(ctypes.Structure):
+    """struct nxg_adapter_rows_params."""
+    _fields_ = [("type", ctypes.c_int32), ("w_type", ctypes.c_int32), ("T", ctypes.c_int32), ("n_in", ctypes.c_int32),
+                ("n_out", ctypes.c_int32), ("rank", ctypes.c_int32), ("n_adapters", ctypes.c_int32), ("n_seqs", ctypes.c_int32),
+                ("cu", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
+                ("scale", ctypes.c_float)]
+
+
 # The checks below are most of what a call for a few rows costs (10 to 20 us in all), so they look at each
 # tensor once, and struct nxg_rows are made several at a time, as an array of their 64-bit words.
 _types = {}
-_words = {n: ctypes.c_int64 * (3 * n) for n in (2, 4, 8)}
+_words = {n: ctypes.c_int64 * (3 * n) for n in (2, 4, 6, 8)}
 _ROWS_BYTES = ctypes.sizeof(_Rows)
 
 
@@ -352,3 +369,249 @@ def attention_rows_backward(dout, q, k, v, out, lse, cu_q, cu_k=None, scale: Opt
     _check(load_library().nxg_attention_rows_backward(ctypes.byref(p), da, qa, ka, va, oa, lp, dqa, dka, dva, ws.data_ptr(),
                                                       ws.numel(), _stream_ptr(stream)), "attention_rows_backward")
     return dq, dk, dv
+
+
+# --- norms of queries and keys, and their rotation -----------------------------------------------
+
+def _qk_args(q, k, wq, wk, freq, cu_offsets, positions, eps, layout, mscale):
+    """(params, the words of q and k, cu, device)"""
+    torch = _torch()
+    ty = _type_of(q, "q")
+    dev, dtype = _device_of(q, "q"), q.dtype
+    T, H, D = q.shape if q.dim() == 3 else (0, 0, 0)
+    words = _head_rows(q, "q", dev, dtype)
+    half = freq.numel()
+    if (k is None) != (wk is None):
+        raise ValueError("give k and wk together")
+    if k is None:
+        G, kw = 0, None
+    else:
+        G = k.shape[1] if k.dim() == 3 else 0
+        words += _head_rows(k, "k", dev, dtype, torch.Size((T, G, D)))
+        if G == 0:
+            raise ValueError("k has no heads")
+    _sizes(T, H, G, D, half)
+    wt = _type_of(wq, "wq")
+    if wt != TYPE_F32 and wq.dtype != dtype:
+        raise ValueError(f"wq and wk must be float32 or {dtype}")
+    qw = _vector(wq, "wq", D, dev, (wq.dtype,))
+    if k is not None:
+        kw = _vector(wk, "wk", D, dev, (wq.dtype,))
+    fp = _vector(freq, "freq", half, dev, (torch.float64,))
+    if layout not in ROPE_LAYOUTS:
+        raise ValueError(f"layout must be one of {', '.join(ROPE_LAYOUTS)}")
+    if (cu_offsets is None) == (positions is None):
+        raise ValueError("give either cu_offsets or positions")
+    cu = None
+    if positions is not None:
+        pp, cp, n_seqs = _vector(positions, "positions", T, dev, (torch.int32,)), None, 0
+    else:
+        cu = _offsets_arg(cu_offsets, q, dev)
+        pp, cp, n_seqs = None, cu.data_ptr(), cu.numel() - 1
+    p = _QkNormRopeParams(ty, T, H, G, D, qw, kw, wt, float(eps), fp, 2 * half, ROPE_LAYOUTS[layout], float(mscale), pp, cp, n_seqs)
+    return p, words, cu, dev
+
+
+def qk_norm_rope_rows(q, k, wq, wk, freq, cu_offsets=None, positions=None, eps: float = 1e-6, layout: str = "half",
+                      mscale: float = 1.0, q_out=None, k_out=None, stream=None):
+    """The RMS norm of every head of q [T][n_head][head_dim] and k [T][n_kv_head][head_dim] (fp32, fp16 or bf16), times wq or
+    wk [head_dim] (of their type or fp32), then rotary positions as rope_rows turns them. k and wk may both be None. Returns
+    (q_out, k_out), which may be q and k."""
+    p, words, cu, dev = _qk_args(q, k, wq, wk, freq, cu_offsets, positions, eps, layout, mscale)
+    if q_out is None:
+        q_out = q.new_empty(q.shape)
+    words += _head_rows(q_out, "q_out", dev, q.dtype, q.shape)
+    if k is not None:
+        if k_out is None:
+            k_out = q.new_empty(k.shape)
+        words += _head_rows(k_out, "k_out", dev, q.dtype, k.shape)
+        rows = _words[4](*words)
+        qa, ka, qo, ko = range(ctypes.addressof(rows), ctypes.addressof(rows) + 4 * _ROWS_BYTES, _ROWS_BYTES)
+    else:
+        rows = _words[2](*words)
+        qa, ka, qo, ko = ctypes.addressof(rows), None, ctypes.addressof(rows) + _ROWS_BYTES, None
+    _order_on(stream, cu, q_out, k_out)
+    _check(load_library().nxg_qk_norm_rope_rows(ctypes.byref(p), qa, ka, qo, ko, _stream_ptr(stream)), "qk_norm_rope_rows")
+    return q_out, k_out
+
+
+@functools.lru_cache(maxsize=256)
+def qk_norm_rope_rows_workspace_bytes(head_dim: int) -> int:
+    """The workspace qk_norm_rope_rows_backward takes for heads of this size."""
+    _sizes(head_dim)
+    p = _QkNormRopeParams(TYPE_F32, 0, 1, 0, head_dim, None, None, TYPE_F32, 0.0, None, 2, 0, 1.0, None, None, 0)
+    n = int(load_library().nxg_qk_norm_rope_rows_workspace_bytes(ctypes.byref(p)))
+    _check(-n if n < 0 else 0, "qk_norm_rope_rows_workspace_bytes")
+    return n
+
+
+def qk_norm_rope_rows_backward(dq_out, dk_out, q, k, wq, wk, freq, cu_offsets=None, positions=None, eps: float = 1e-6,
+                               layout: str = "half", mscale: float = 1.0, dq=None, dk=None, dwq=None, dwk=None, workspace=None,
+                               stream=None):
+    """The gradients of qk_norm_rope_rows: (dq, dk, dwq, dwk), from the gradients of its outputs and its inputs; dwq and dwk of
+    wq's type. dq may be dq_out or q, dk dk_out or k. Without k and wk: dk and dwk are None. workspace: None (made for the
+    call) or a uint8 device tensor of qk_norm_rope_rows_workspace_bytes(head_dim)."""
+    p, words, cu, dev = _qk_args(q, k, wq, wk, freq, cu_offsets, positions, eps, layout, mscale)
+    dtype, D = q.dtype, q.shape[2]
+    dq = q.new_empty(q.shape) if dq is None else dq
+    words += _head_rows(dq_out, "dq_out", dev, dtype, q.shape) + _head_rows(dq, "dq", dev, dtype, q.shape)
+    dwq = q.new_empty(D, dtype=wq.dtype) if dwq is None else dwq
+    wqp, wkp = _vector(dwq, "dwq", D, dev, (wq.dtype,)), None
+    if k is not None:
+        dk = q.new_empty(k.shape) if dk is None else dk
+        words += _head_rows(dk_out, "dk_out", dev, dtype, k.shape) + _head_rows(dk, "dk", dev, dtype, k.shape)
+        dwk = q.new_empty(D, dtype=wq.dtype) if dwk is None else dwk
+        wkp = _vector(dwk, "dwk", D, dev, (wq.dtype,))
+        rows = _words[6](*words)
+        qa, ka, dqo, dqa, dko, dka = range(ctypes.addressof(rows), ctypes.addressof(rows) + 6 * _ROWS_BYTES, _ROWS_BYTES)
+    else:
+        dk = dwk = None
+        rows = _words[4](*words, 0, 0, 0)
+        at = ctypes.addressof(rows)
+        qa, ka, dqo, dqa, dko, dka = at, None, at + _ROWS_BYTES, at + 2 * _ROWS_BYTES, None, None
+    ws = _workspace(workspace, qk_norm_rope_rows_workspace_bytes(D), q)
+    _order_on(stream, cu, dq, dk, dwq, dwk, ws)
+    _check(load_library().nxg_qk_norm_rope_rows_backward(ctypes.byref(p), dqo, dko, qa, ka, dqa, dka, wqp, wkp, ws.data_ptr(), ws.numel(),
+                                                         _stream_ptr(stream)), "qk_norm_rope_rows_backward")
+    return dq, dk, dwq, dwk
+
+
+# --- dropout -------------------------------------------------------------------------------------
+
+def dropout_rows(x, p: float, seed: int, offset: int = 0, step=None, residual=None, out=None, stream=None):
+    """residual + dropout(x) of rows x [T][C] (fp32, fp16 or bf16); residual None: dropout alone. Which values are kept is drawn
+    again by every call from (seed, offset, row, column): dropout_rows(dout, p, seed, offset) is the gradient of x. Kept values are
+    divided by 1 - p (p a multiple of 2^-16, or rounded to one). seed and offset: 0 .. 2^64 - 1; step: a device int64 [1] that is added to offset when the call
+    runs (new masks in the replays of a graph). out may be x or residual."""
+    ty = _type_of(x, "x")
+    dev = _device_of(x, "x")
+    xp, xs = _plain_rows(x, "x", dev)
+    T, C = x.shape
+    _sizes(T, C)
+    rp, rs = (None, 0) if residual is None else _plain_rows(residual, "residual", dev, x)
+    if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
+        raise ValueError("seed and offset must be 64-bit numbers")
+    sp = None if step is None else _vector(step, "step", 1, dev, (_torch().int64,))
+    if out is None:
+        out = x.new_empty((T, C))
+    op, os_ = _plain_rows(out, "out", dev, x)
+    _order_on(stream, out)
+    _check(load_library().nxg_dropout_rows(ty, xp, xs, rp, rs, T, C, float(p), seed, offset, sp, op, os_, _stream_ptr(stream)),
+           "dropout_rows")
+    return out
+
+
+# --- low-rank adapters -----------------------------------------------------------------------------
+
+@functools.lru_cache(maxsize=256)
+def _adapter_bytes(dev, ty, wt, T, K, N, r, n, n_seqs):
+    """The backward pass's workspace for these sizes on this device."""
+    p = _AdapterParams(ty, wt, T, K, N, r, n, n_seqs, None, None, None, None, 1.0)
+    b = int(load_library().nxg_adapter_rows_backward_workspace_bytes(ctypes.byref(p)))
+    _check(-b if b < 0 else 0, "adapter_rows_backward")
+    return b
+
+
+def _ids_arg(ids, n_seqs, like, dev):
+    """ids (host sequence or device int32 tensor) as a device int32 tensor [n_seqs]."""
+    torch = _torch()
+    if not isinstance(ids, torch.Tensor):
+        host = np.ascontiguousarray(ids)
+        if host.ndim == 1 and host.shape[0] == n_seqs and host.dtype.kind in "iu":
+            return _uploaded(np.clip(host, -1, _INT32).astype(np.int32), like.device)
+    elif ids.is_cuda and ids.get_device() == dev and ids.dtype == torch.int32 and ids.dim() == 1 and ids.shape[0] == n_seqs \
+            and ids.is_contiguous():
+        return ids
+    raise ValueError(f"ids must be {n_seqs} whole numbers: a host sequence, or a contiguous int32 tensor on the current device")
+
+
+def _adapter_args(x, a, b, cu_offsets, ids, scale):
+    """(params, cu, ids, workspace bytes, device)"""
+    ty = _type_of(x, "x")
+    dev = _device_of(x, "x")
+    wt = _type_of(a, "a")
+    if wt != ty and ty != TYPE_F32:
+        raise ValueError(f"a and b must have type {x.dtype}")
+    for t, name in ((a, "a"), (b, "b")):
+        if not t.is_cuda or t.get_device() != dev:
+            raise ValueError(f"{name} must be a tensor on the current device")
+        if t.dtype != a.dtype or t.dim() != 3 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous tensor of 3 dimensions and type {a.dtype}")
+    n, r, K = a.shape
+    N = b.shape[1]
+    if b.shape[0] != n or b.shape[2] != r or x.dim() != 2 or x.shape[1] != K:
+        raise ValueError("x [T][n_in], a [n_adapters][rank][n_in] and b [n_adapters][n_out][rank] do not fit")
+    T = x.shape[0]
+    _sizes(T, K, N, r, n)
+    cu = _offsets_arg(cu_offsets, x, dev)
+    n_seqs = cu.numel() - 1
+    ids = _ids_arg(ids, n_seqs, x, dev)
+    p = _AdapterParams(ty, wt, T, K, N, r, n, n_seqs, cu.data_ptr(), ids.data_ptr(), a.data_ptr(), b.data_ptr(), float(scale))
+    return p, cu, ids, dev
+
+
+def _s_arg(s, T, r, dev):
+    if not s.is_cuda or s.get_device() != dev:
+        raise ValueError("s must be a tensor on the current device")
+    if s.dtype != _torch().float32 or s.shape != (T, r) or not s.is_contiguous():
+        raise ValueError(f"s must be a contiguous float32 tensor [{T}][{r}]")
+    return s.data_ptr()
+
+
+def _rows_of_width(t, name, dev, dtype, T, C):
+    if t.dtype != dtype or t.shape != (T, C):
+        raise ValueError(f"{name} must have type {dtype} and shape ({T}, {C})")
+    return _plain_rows(t, name, dev)
+
+
+def adapter_rows(x, a, b, cu_offsets, ids, scale: float = 1.0, base=None, out=None, s=None, stream=None):
+    """Low-rank adapters of many requests: document d's rows of x [T][n_in] through adapter i = ids[d], base + scale * (x a_i^T)
+    b_i^T, a [n_adapters][rank][n_in] and b [n_adapters][n_out][rank] of x's type (fp32 rows, as the int8 linears leave them: of any
+    type). base [T][n_out]: the shared projection's rows, or None. An id that is no adapter leaves base as it is (0 without).
+    Returns (out, s), s the fp32 [T][rank] rows x a_i^T, as adapter_rows_backward takes them. out may be base."""
+    p, cu, ids, dev = _adapter_args(x, a, b, cu_offsets, ids, scale)
+    T, N, r = p.T, p.n_out, p.rank
+    xp, xs = _plain_rows(x, "x", dev)
+    bp, bs = (None, 0) if base is None else _rows_of_width(base, "base", dev, x.dtype, T, N)
+    if out is None:
+        out = x.new_empty((T, N))
+    op, os_ = _rows_of_width(out, "out", dev, x.dtype, T, N)
+    if s is None:
+        s = x.new_empty((T, r), dtype=_torch().float32)
+    sp = _s_arg(s, T, r, dev)
+    _order_on(stream, cu, ids, out, s)
+    _check(load_library().nxg_adapter_rows(ctypes.byref(p), xp, xs, bp, bs, op, os_, sp, _stream_ptr(stream)), "adapter_rows")
+    return out, s
+
+
+def adapter_rows_backward_workspace_bytes(x, a, b, cu_offsets, ids) -> int:
+    """The workspace adapter_rows_backward takes for these arguments."""
+    p, _, _, dev = _adapter_args(x, a, b, cu_offsets, ids, 1.0)
+    return _adapter_bytes(dev, p.type, p.w_type, p.T, p.n_in, p.n_out, p.rank, p.n_adapters, p.n_seqs)
+
+
+def adapter_rows_backward(dout, x, a, b, s, cu_offsets, ids, scale: float = 1.0, base=None, dx=None, da=None, db=None, workspace=None,
+                          stream=None):
+    """The gradients of adapter_rows: (dx, da, db), from dout [T][n_out], its inputs and the s that it returned. base [T][n_in]: what
+    dx is added to (the shared projection's part), or None; dx may be base. da and db as a and b, zeros for adapters
+    that no row has. workspace: None (made for the call) or a uint8 device tensor of adapter_rows_backward_workspace_bytes."""
+    p, cu, ids, dev = _adapter_args(x, a, b, cu_offsets, ids, scale)
+    T, K, N = p.T, p.n_in, p.n_out
+    xp, xs = _plain_rows(x, "x", dev)
+    gp, gs = _rows_of_width(dout, "dout", dev, x.dtype, T, N)
+    sp = _s_arg(s, T, p.rank, dev)
+    bp, bs = (None, 0) if base is None else _rows_of_width(base, "base", dev, x.dtype, T, K)
+    dx = x.new_empty((T, K)) if dx is None else dx
+    dp, ds = _rows_of_width(dx, "dx", dev, x.dtype, T, K)
+    da = a.new_empty(a.shape) if da is None else da
+    db = b.new_empty(b.shape) if db is None else db
+    for t, like, name in ((da, a, "da"), (db, b, "db")):
+        if not t.is_cuda or t.get_device() != dev:
+            raise ValueError(f"{name} must be a tensor on the current device")
+        if t.dtype != like.dtype or t.shape != like.shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous tensor of type {like.dtype} and shape {tuple(like.shape)}")
+    ws = _workspace(workspace, _adapter_bytes(dev, p.type, p.w_type, T, K, N, p.rank, p.n_adapters, p.n_seqs), x)
+    _order_on(stream, cu, ids, dx, da, db, ws)
+    _check(load_library().nxg_adapter_rows_backward(ctypes.byref(p), gp, gs, xp, xs, sp, bp, bs, dp, ds, da.data_ptr(), db.data_ptr(),
+                                                    ws.data_ptr(), ws.numel(), _stream_ptr(stream)), "adapter_rows_backward")
+    return dx, da, db
