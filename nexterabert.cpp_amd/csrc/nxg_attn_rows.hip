@@ -140,7 +140,7 @@ __device__ __forceinline__ int find_doc(const int32_t * cu, int n_seqs, int T, i
         const int step = (n + 63) >> 6;
         const int d = lo + lane * step;
         const bool at = lane * step < n && slot_of(cu, d, T, mul, tile) <= slot;
-        const int last = max(__popcll(__ballot(at)) - 1, 0);
+        const int last = max((int) __popcll(__ballot(at)) - 1, 0);       // none: the first (the count is unsigned)
         n = min(step, n - last * step);
         lo += last * step;
     }

@@ -1,0 +1,41 @@
+"""GPU: device offsets that do not start at 0 give unspecified rows but no access out of bounds."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as t
+    assert t.cuda.is_available(), "no GPU"
+    return t
+
+
+@pytest.fixture(scope="module")
+def dev(torch, nxg):
+    nxg.init()
+    return torch.device("cuda:0")
+
+
+@pytest.mark.parametrize("first", [4000, 6000])
+def test_attention_rows_many_documents(nxg, torch, dev, first):
+    """More documents than a wave has lanes, the first of them behind a slot's: looked for by their offsets."""
+    print(f"attention_rows, 100 documents from row {first}", flush=True)
+    T = 6000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, dout = (torch.randn(T, n, 64, device="cuda", generator=g).to(torch.bfloat16) for n in (4, 2, 2, 4))
+    cu = torch.tensor(np.linspace(first, T, 101).astype(np.int32), device="cuda")
+    for right in (-1, 0):
+        out = torch.full((T + 2, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        _, lse = nxg.attention_rows(q, k, v, cu, right=right, out=out[1:T + 1])
+        grads = nxg.attention_rows_backward(dout, q, k, v, out[1:T + 1], lse, cu, right=right)
+        torch.cuda.synchronize()
+        assert (out[0] == 7).all() and (out[T + 1] == 7).all() and grads[0].shape == q.shape
+    # the same offsets from 0, with the rows in front as a document of their own: its neighbours' results
+    if first < T:
+        whole = torch.cat([torch.zeros(1, dtype=torch.int32, device="cuda"), cu])
+        want = nxg.attention_rows(q, k, v, whole, right=0)[0]
+        assert torch.isfinite(want).all()
