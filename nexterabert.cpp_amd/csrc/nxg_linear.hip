@@ -1020,7 +1020,7 @@ __device__ __forceinline__ doc_rows doc_of_wave(const int32_t * cu, int n, int t
         a += skip;
         len = min(step, len - skip);
     }
-    a += max(__popcll(__ballot(lane < len && cu[a + min(lane, len - 1)] <= t0)) - 1, 0);
+    a += max((int) __popcll(__ballot(lane < len && cu[a + min(lane, len - 1)] <= t0)) - 1, 0);       // none: the first (the count is unsigned)
     while (a + 1 < n && cu[a + 1] <= t) ++a;
     doc_rows r;
     r.d = a;

@@ -39,3 +39,16 @@ def test_attention_rows_many_documents(nxg, torch, dev, first):
         whole = torch.cat([torch.zeros(1, dtype=torch.int32, device="cuda"), cu])
         want = nxg.attention_rows(q, k, v, whole, right=0)[0]
         assert torch.isfinite(want).all()
+
+
+@pytest.mark.parametrize("docs", [1, 40, 70])
+def test_lily_state_many_rows(nxg, torch, dev, docs):
+    """The kernel for many rows, whose first rows lie in front of every document."""
+    print(f"lily state, {docs} documents from row 20,000", flush=True)
+    T, C = 22001, 1024
+    g = torch.Generator(device="cuda").manual_seed(1)
+    a, x, b = (torch.randn(T, C, device="cuda", generator=g) for _ in range(3))
+    cu = torch.tensor(np.linspace(20000, T, docs + 1).astype(np.int32), device="cuda")
+    qa = nxg.lily_state_quantize_rows(a, x, b, torch.randn(2, C, device="cuda", generator=g), cu)
+    torch.cuda.synchronize()
+    assert qa.T == T
