@@ -52,16 +52,14 @@ template <> struct operand<float> {
     }
 };
 
-// Values k .. k + V - 1 of a row of n values, zeros behind its end. WIDE: 16 bytes of the row at once (n and k multiples of V).
-template <class E, class S, bool WIDE>
+// Values k .. k + V - 1 of a row of n values, zeros behind its end: 16 bytes (of E) at once (n and k multiples of V), or one by one.
+template <class E, bool WIDE, class S>
 __device__ __forceinline__ typename operand<E>::vec fetch(const S * row, int k, int n) {
     constexpr int V = operand<E>::V;
     typename operand<E>::vec v;
     if constexpr (WIDE) {
         typedef S svec __attribute__((ext_vector_type(V)));
-        svec x;
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = (S) 0.0f;
+        svec x = {};
         if (k < n) x = *reinterpret_cast<const svec *>(row + k);
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = (E) x[i];
@@ -71,6 +69,21 @@ __device__ __forceinline__ typename operand<E>::vec fetch(const S * row, int k, 
     }
     return v;
 }
+// The V values of type S at p as an operand of type E, or zeros.
+template <class E, class S>
+__device__ __forceinline__ typename operand<E>::vec taken(const char * p, bool some) {
+    constexpr int V = operand<E>::V;
+    typedef S svec __attribute__((ext_vector_type(V)));
+    const svec x = *reinterpret_cast<const svec *>(p);
+    typename operand<E>::vec v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = some ? (E) x[i] : (E) 0.0f;
+    return v;
+}
+// Before a wave reads what its other lanes left in LDS, and after: LDS takes a wave's instructions in their order, and so must the compiler.
+__device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
+// A barrier for LDS alone: loads from memory stay under way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // x as the sum of two bf16 values: itself rounded, and what is left.
 __device__ __forceinline__ void split(const float (&x)[8], v8b & hi, v8b & lo) {
@@ -128,186 +141,491 @@ __device__ __forceinline__ tile find_tile(const adapter_p & p, int size, int slo
     return t;
 }
 
-// A workgroup: 16 MT rows of one document. Its four waves share the contracted index of x A^T out, a line of 128 bytes of every
-// row at a time, so that the weights are read once per workgroup; their sums are joined in LDS, in a fixed order. Then they
-// share out the columns of s B^T, taken as (B s^T): a lane has V columns next to each other of one row, 16 bytes, from
-// V / 4 results whose rows of B are picked for that.
-template <class E, class W, int MT, int RT, bool WIDE>
-__global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
-    constexpr bool F32 = std::is_same<E, float>::value, F16 = std::is_same<E, _Float16>::value;
-    constexpr int V = operand<E>::V, BM = 16 * MT, RP = 16 * RT, LD = RP + 4;
-    typedef typename operand<E>::vec vec;
-    __shared__ __align__(16) float lds[2][BM][LD];
-    const tile c = find_tile(p, BM, blockIdx.x);
-    if (c.len <= 0) return;
-    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+// s beside rows of type E, 16 RT ranks of it: operands of 16 ranks each (fp32, and RT 1 with both parts of s side by side), else 32.
+template <class E, int RT> struct ranks {
+    static constexpr bool F32 = std::is_same<E, float>::value;
+    static constexpr int Q = F32 ? RT : RT == 1 ? 1 : RT / 2, SV = F32 || RT == 1 ? 1 : 2;
+    typedef typename std::conditional<F32, v4f, v8b>::type vec;
 
-    if (c.id < 0) {                // no adapter: base as it is, s = 0
-        if (blockIdx.y) return;
-        for (int i = threadIdx.x; i < c.len * p.r; i += 256) p.s[(int64_t) c.row * p.r + i] = 0.0f;
-        if (!p.y || p.y == p.base) return;
-        for (int t = wave; t < c.len; t += 4) {
-            const E * from = reinterpret_cast<const E *>(p.base + (c.row + (int64_t) t) * p.base_s);
-            E * to = reinterpret_cast<E *>(p.y + (c.row + (int64_t) t) * p.y_s);
-            for (int k = lane; k < p.N; k += 64) to[k] = p.base ? from[k] : (E) 0.0f;
+    // the first rank of a lane's values of operand q
+    static __device__ __forceinline__ int first(int q, int g) { return F32 ? 16 * q + 4 * g : RT == 1 ? 8 * (g & 1) : 32 * q + 8 * g; }
+    // from a token's row of s in LDS
+    static __device__ __forceinline__ void operands(vec (&s)[Q][SV], const float * row, int g) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            if constexpr (F32) {
+                s[q][0] = *reinterpret_cast<const v4f *>(row + first(q, g));
+            } else {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = row[first(q, g) + i];
+                v8b hi, lo;
+                split(x, hi, lo);
+                if constexpr (RT == 1) {
+                    s[q][0] = g < 2 ? hi : lo;
+                } else {
+                    s[q][0] = hi;
+                    s[q][1] = lo;
+                }
+            }
         }
+    }
+    // up += operand q of B times s
+    static __device__ __forceinline__ void multiply(v4f & up, const typename operand<E>::vec & b, const vec (&s)[SV]) {
+        if constexpr (F32) {
+            up = operand<float>::mul(b, s[0], up);
+        } else {
+            v8b hi, lo;
+            if constexpr (std::is_same<E, _Float16>::value) split(b, hi, lo);
+            else hi = b;
+#pragma unroll
+            for (int k = 0; k < SV; ++k) up = operand<__bf16>::mul(hi, s[k], up);
+            if constexpr (std::is_same<E, _Float16>::value) up = operand<__bf16>::mul(lo, s[0], up);
+        }
+    }
+};
+
+// The rows of a document without an adapter: base as it is, s = 0. By a workgroup, V values at a time.
+template <class E, int V>
+__device__ __forceinline__ void copy_rows(const adapter_p & p, const tile & c) {
+    typedef E vec __attribute__((ext_vector_type(V)));
+    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    for (int i = threadIdx.x; i < c.len * p.r; i += 256) p.s[(int64_t) c.row * p.r + i] = 0.0f;
+    if (!p.y || p.y == p.base) return;
+    for (int t = wave; t < c.len; t += 4) {
+        const E * from = reinterpret_cast<const E *>(p.base + (c.row + (int64_t) t) * p.base_s);
+        E * to = reinterpret_cast<E *>(p.y + (c.row + (int64_t) t) * p.y_s);
+#pragma unroll 4
+        for (int k = lane * V; k < p.N; k += 64 * V) {
+            vec x = {};
+            if (p.base) x = *reinterpret_cast<const vec *>(from + k);
+            *reinterpret_cast<vec *>(to + k) = x;
+        }
+    }
+}
+
+// A workgroup: 16 rows of one document. Its four waves share the contracted index of x A^T out, 128 bytes of every row a step, so
+// that the weights are read once per workgroup; their sums are joined in LDS, in a fixed order. Then they share out the columns of
+// s B^T, taken as (B s^T), 128 bytes of every row a block: of a result, a lane has V columns next to each other of one row.
+//
+// THROUGH_LDS: everything comes from memory 8 lanes to 128 bytes of a row, a step or block ahead, and goes to the operands' lanes (16 of
+// them 16 rows) through LDS that a wave has to itself; results go the same way back. A wave's load of 16 bytes from each of 64 places
+// takes the first cache four times as long as one of 16 runs of 64 bytes, and bound this kernel before (32,935 rows of fp32, rank 16:
+// 181 us with 64 rows a workgroup, 110 with 16). WIDE: operands straight from memory, 16 bytes a lane, for calls of few workgroups,
+// which wait for their own chain of loads alone. BY_VALUE: rows off 16 bytes.
+enum { THROUGH_LDS, WIDE, BY_VALUE };
+template <class E, class W, int RT, int HOW>
+__global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
+    constexpr int V = operand<E>::V, RP = 16 * RT, LD = RP + 4;
+    constexpr int WV = 16 / (int) sizeof(W), A_ROW = 8 * V * (int) sizeof(W);      // weights of 16 bytes; bytes of a rank's step
+    constexpr int A_LOADS = RP * A_ROW / 1024;             // 16-byte loads of a step's, or a block's, weights: 64 lanes each
+    constexpr int OUT = 8 * V * 4 + 16;                    // bytes of a row of results in LDS
+    constexpr int X_BYTES = 16 * OUT, A_BYTES = RP * A_ROW + 8 * V * 16;
+    constexpr int SUMS = 2 * 16 * LD * 4, LDS = HOW == THROUGH_LDS ? std::max(4 * (X_BYTES + A_BYTES), SUMS) : SUMS;
+    typedef typename operand<E>::vec vec;
+    __shared__ __align__(16) char lds[LDS];
+    const tile c = find_tile(p, 16, blockIdx.x);
+    if (c.len <= 0) return;
+    if (c.id < 0) {
+        if (blockIdx.y == 0) copy_rows<E, HOW == BY_VALUE ? 1 : V>(p, c);
         return;
     }
+    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    char * xs = lds + wave * (X_BYTES + A_BYTES), * as = xs + X_BYTES;     // the wave's own
+    const int row8 = lane >> 3, at8 = lane & 7;                            // 8 lanes a row
 
     // s, ranks as rows and tokens as columns
-    v4f acc[MT][RT];
+    v4f acc[RT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int j = 0; j < RT; ++j) acc[j] = v4f{};
+    const W * a = static_cast<const W *>(p.a) + (int64_t) c.id * p.r * p.K;
+    constexpr int STEP = 32 * V;
+    int k0 = wave * 8 * V;
+    if constexpr (HOW == THROUGH_LDS) {
+        // 16-byte chunk i of row r is at chunk i ^ (r / 2) % 8 of it (rows of 64 bytes: i ^ (r / 4) % 4): 16 rows' same chunk fill the banks
+        struct step {
+            v4i x[2], a[A_LOADS];
+        };
+        const char * x[2];
+        int ar[A_LOADS];
 #pragma unroll
-        for (int j = 0; j < RT; ++j) acc[m][j] = v4f{};
-    {
-        const E * x[MT];
+        for (int i = 0; i < 2; ++i) x[i] = p.x + (c.row + (int64_t) min(8 * i + row8, c.len - 1)) * p.x_s;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) x[m] = reinterpret_cast<const E *>(p.x + (c.row + (int64_t) min(16 * m + col, c.len - 1)) * p.x_s);
-        const W * a = static_cast<const W *>(p.a) + (int64_t) c.id * p.r * p.K;
-#pragma unroll 1
-        for (int k0 = wave * 8 * V; k0 < p.K; k0 += 32 * V) {
-            vec xf[2][MT], af[2][RT];
+        for (int i = 0; i < A_LOADS; ++i) ar[i] = min(A_ROW == 128 ? 8 * i + row8 : 16 * i + (lane >> 2), p.r - 1) * p.K;
+        auto load = [&](step & s, int k0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s.x[i] = *reinterpret_cast<const v4i *>(x[i] + min(k0 + at8 * V, p.K - V) * (int) sizeof(E));
+#pragma unroll
+            for (int i = 0; i < A_LOADS; ++i) s.a[i] = *reinterpret_cast<const v4i *>(a + ar[i] + min(k0 + (A_ROW == 128 ? at8 : lane & 3) * WV, p.K - WV));
+        };
+        auto use = [&](const step & s, int k0) {
+            in_order();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) *reinterpret_cast<v4i *>(xs + (8 * i + row8) * 128 + ((at8 ^ ((4 * i + (lane >> 4)) & 7)) << 4)) = s.x[i];
+#pragma unroll
+            for (int i = 0; i < A_LOADS; ++i) {
+                if constexpr (A_ROW == 128) *reinterpret_cast<v4i *>(as + (8 * i + row8) * 128 + ((at8 ^ ((4 * i + (lane >> 4)) & 7)) << 4)) = s.a[i];
+                else *reinterpret_cast<v4i *>(as + (16 * i + (lane >> 2)) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) << 4)) = s.a[i];
+            }
+            in_order();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int k = k0 + (2 * g + h) * V;
+                const int k = k0 + (4 * h + g) * V, sw = (4 * h + g) ^ (col >> 1);
+                const vec xf = taken<E, E>(xs + col * 128 + (sw << 4), true);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) xf[h][m] = fetch<E, E, WIDE>(x[m], k, p.K);
+                for (int j = 0; j < RT; ++j) {
+                    const char * from = A_ROW == 128 ? as + (16 * j + col) * 128 + (sw << 4)
+                                                     : as + (16 * j + col) * 64 + (((2 * h + (g >> 1)) ^ (col >> 2)) << 4) + (g & 1) * 8;
+                    acc[j] = operand<E>::mul(taken<E, W>(from, k < p.K && 16 * j + col < p.r), xf, acc[j]);
+                }
+            }
+        };
+        step s0, s1;
+        if (k0 < p.K) load(s0, k0);
+        for (; k0 < p.K; k0 += 2 * STEP) {
+            if (k0 + STEP < p.K) load(s1, k0 + STEP);
+            use(s0, k0);
+            if (k0 + STEP >= p.K) break;
+            if (k0 + 2 * STEP < p.K) load(s0, k0 + 2 * STEP);
+            use(s1, k0 + STEP);
+        }
+    } else {
+        const E * x = reinterpret_cast<const E *>(p.x + (c.row + (int64_t) min(col, c.len - 1)) * p.x_s);
+        for (; k0 < p.K; k0 += STEP) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = k0 + (4 * h + g) * V;
+                const vec xf = fetch<E, HOW == WIDE>(x, k, p.K);
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
                     const int r = 16 * j + col;
-                    af[h][j] = fetch<E, W, WIDE>(a + (int64_t) r * p.K, r < p.r ? k : p.K, p.K);
+                    acc[j] = operand<E>::mul(fetch<E, HOW == WIDE>(a + (int64_t) r * p.K, r < p.r ? k : p.K, p.K), xf, acc[j]);
                 }
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int j = 0; j < RT; ++j) acc[m][j] = operand<E>::mul(af[h][j], xf[h][m], acc[m][j]);
         }
     }
     // the waves' sums: 0 + 2 and 1 + 3, then both
+    typedef float row_sums[16][LD];
+    row_sums * sums = reinterpret_cast<row_sums *>(lds);
+    if (HOW == THROUGH_LDS) __syncthreads();
     for (int turn = 0; turn < 2; ++turn) {
         if ((wave >> 1) == turn) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int j = 0; j < RT; ++j) {
-                    v4f * to = reinterpret_cast<v4f *>(&lds[wave & 1][16 * m + col][16 * j + 4 * g]);
-                    *to = turn ? *to + acc[m][j] : acc[m][j];
-                }
+            for (int j = 0; j < RT; ++j) {
+                v4f * to = reinterpret_cast<v4f *>(&sums[wave & 1][col][16 * j + 4 * g]);
+                *to = turn ? *to + acc[j] : acc[j];
+            }
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < BM * RP; i += 256) {
+    for (int i = threadIdx.x; i < 16 * RP; i += 256) {
         const int t = i / RP, r = i % RP;
-        const float x = (lds[0][t][r] + lds[1][t][r]) * p.pre;
-        lds[0][t][r] = x;
+        const float x = (sums[0][t][r] + sums[1][t][r]) * p.pre;
+        sums[0][t][r] = x;
         if (blockIdx.y == 0 && t < c.len && r < p.r) p.s[(c.row + (int64_t) t) * p.r + r] = x;
     }
     if (!p.y) return;
     __syncthreads();
 
-    // s as operands
-    constexpr int Q = F32 ? RT : RT == 1 ? 1 : RT / 2;      // ranks of one: 16 (fp32, and RT 1 with both parts side by side), else 32
-    constexpr int SV = F32 || RT == 1 ? 1 : 2;              // operands for them
-    typedef typename std::conditional<F32, v4f, v8b>::type svec;
-    svec s[MT][Q][SV];
+    constexpr int Q = ranks<E, RT>::Q, M = V / 4;          // M results make up a lane's V columns
+    typename ranks<E, RT>::vec s[Q][ranks<E, RT>::SV];
+    ranks<E, RT>::operands(s, sums[0][col], g);
+    if (HOW == THROUGH_LDS) __syncthreads();
+
+    const W * b = static_cast<const W *>(p.b) + (int64_t) c.id * p.N * p.r;
+    // row of B for a lane of result i of columns 4 V h .. of a block; its first rank of operand q
+    auto b_row = [&](int h, int i) { return 4 * V * h + V * (col >> 2) + 4 * i + (col & 3); };
+    auto b_rank = [&](int q) { return ranks<E, RT>::first(q, g); };
+    const int step = 32 * V * (int) gridDim.y;
+    int n0 = (blockIdx.y * 4 + wave) * 8 * V;
+    if constexpr (HOW == THROUGH_LDS) {
+        struct block {
+            v4i before[2], b[A_LOADS];
+        };
+        // B's rows of a block lie one after another; in LDS they are 16 bytes apart, where they are whole chunks
+        const int row_bytes = p.r * (int) sizeof(W), chunks = 8 * V * row_bytes / 16;
+        const bool whole = row_bytes % 16 == 0, aligned = p.r % V == 0;
+        const int stride = row_bytes + (whole ? 16 : 0);
+        int at[A_LOADS];                                   // the lane's chunks' places
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const float * row = lds[0][16 * m + col];
+        for (int i = 0; i < A_LOADS; ++i) {
+            const int q = 64 * i + lane;
+            at[i] = q >= chunks ? -1 : 16 * (whole ? q + q / (row_bytes / 16) : q);
+        }
+        auto load = [&](block & k, int n0) {
+            const char * from = reinterpret_cast<const char *>(b + (int64_t) n0 * p.r);
+            const int last = min(chunks, (p.N - n0) * row_bytes / 16) - 1;
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            if constexpr (F32) {
-                s[m][q][0] = *reinterpret_cast<const v4f *>(row + 16 * q + 4 * g);
-            } else {
-                const float * f = row + (RT == 1 ? 8 * (g & 1) : 32 * q + 8 * g);
-                float x[8];
+            for (int i = 0; i < A_LOADS; ++i) k.b[i] = *reinterpret_cast<const v4i *>(from + min(64 * i + lane, last) * 16);
+            if (p.base) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = f[i];
-                v8b hi, lo;
-                split(x, hi, lo);
-                if constexpr (RT == 1) {
-                    s[m][q][0] = g < 2 ? hi : lo;
+                for (int i = 0; i < 2; ++i) {
+                    const char * row = p.base + (c.row + (int64_t) min(8 * i + row8, c.len - 1)) * p.base_s;
+                    k.before[i] = *reinterpret_cast<const v4i *>(row + min(n0 + at8 * V, p.N - V) * (int) sizeof(E));
+                }
+            }
+        };
+        auto use = [&](const block & k, int n0) {
+            in_order();
+#pragma unroll
+            for (int i = 0; i < A_LOADS; ++i)
+                if (at[i] >= 0) *reinterpret_cast<v4i *>(as + at[i]) = k.b[i];
+            in_order();
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < M; ++i) {
+                    const char * row = as + b_row(h, i) * stride;
+                    v4f up = {};
+#pragma unroll
+                    for (int q = 0; q < Q; ++q) {
+                        vec bf;
+                        if (aligned) bf = taken<E, W>(row + b_rank(q) * (int) sizeof(W), b_rank(q) < p.r);
+                        else bf = fetch<E, false>(reinterpret_cast<const W *>(row), b_rank(q), p.r);
+                        ranks<E, RT>::multiply(up, bf, s[q]);
+                    }
+                    *reinterpret_cast<v4f *>(xs + col * OUT + (4 * V * h + V * g + 4 * i) * 4) = up;
+                }
+            in_order();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = 8 * i + row8, n = n0 + at8 * V;
+                const float * up = reinterpret_cast<const float *>(xs + t * OUT) + at8 * V;
+                vec before, out;
+                __builtin_memcpy(&before, &k.before[i], 16);
+#pragma unroll
+                for (int e = 0; e < V; ++e) out[e] = (E) __builtin_fmaf(up[e], p.post, p.base ? (float) before[e] : 0.0f);
+                if (t < c.len && n < p.N) *reinterpret_cast<vec *>(p.y + (c.row + (int64_t) t) * p.y_s + (int64_t) n * (int) sizeof(E)) = out;
+            }
+        };
+        block b0, b1;
+        if (n0 < p.N) load(b0, n0);
+        for (; n0 < p.N; n0 += 2 * step) {
+            if (n0 + step < p.N) load(b1, n0 + step);
+            use(b0, n0);
+            if (n0 + step >= p.N) break;
+            if (n0 + 2 * step < p.N) load(b0, n0 + 2 * step);
+            use(b1, n0 + step);
+        }
+    } else {
+        const bool whole = HOW == WIDE && p.r % V == 0;
+        const E * from = reinterpret_cast<const E *>(p.base + (c.row + (int64_t) col) * p.base_s);
+        E * to = reinterpret_cast<E *>(p.y + (c.row + (int64_t) col) * p.y_s);
+        for (; n0 < p.N; n0 += step) {
+            vec before[2], bf[2][M][Q];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                before[h] = fetch<E, HOW == WIDE>(from, p.base && col < c.len ? n0 + 4 * V * h + V * g : p.N, p.N);
+#pragma unroll
+                for (int i = 0; i < M; ++i) {
+                    const W * row = b + (int64_t) min(n0 + b_row(h, i), p.N - 1) * p.r;
+#pragma unroll
+                    for (int q = 0; q < Q; ++q) bf[h][i][q] = whole ? fetch<E, true>(row, b_rank(q), p.r) : fetch<E, false>(row, b_rank(q), p.r);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int n = n0 + 4 * V * h + V * g;
+                vec out;
+#pragma unroll
+                for (int i = 0; i < M; ++i) {
+                    v4f up = {};
+#pragma unroll
+                    for (int q = 0; q < Q; ++q) ranks<E, RT>::multiply(up, bf[h][i][q], s[q]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[4 * i + e] = (E) __builtin_fmaf(up[e], p.post, (float) before[h][4 * i + e]);
+                }
+                if (col >= c.len) continue;
+                if constexpr (HOW == WIDE) {
+                    if (n < p.N) *reinterpret_cast<vec *>(to + n) = out;
                 } else {
-                    s[m][q][0] = hi;
-                    s[m][q][1] = lo;
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (n + e < p.N) to[n + e] = out[e];
                 }
             }
         }
     }
+}
 
-    constexpr int M = V / 4;       // results that make up a lane's 16 bytes
+// The same for larger ranks and many rows: a workgroup takes 64 MT rows, a wave 16 MT of them for itself, and its four waves share
+// the weights, which they bring to LDS together, a step or block at a time (two in turn, so that one barrier a step does). That reads
+// the weights a fourth as often as above, and leaves a wave the registers of few loads.
+template <class E, class W, int MT, int RT>
+__global__ __launch_bounds__(256, 2) void adapter_rows_tall_kernel(adapter_p p) {
+    constexpr int V = operand<E>::V, RP = 16 * RT, LD = RP + 4;
+    constexpr int WV = 16 / (int) sizeof(W), A_ROW = 8 * V * (int) sizeof(W);
+    constexpr int A_LOADS = (RP * A_ROW / 1024 + 3) / 4;   // of a wave
+    constexpr int OUT = 8 * V * 4 + 16;
+    constexpr int X_BYTES = std::max(std::max(16 * MT * 128, 16 * OUT), 16 * LD * 4), A_BYTES = RP * A_ROW + 8 * V * 16;
+    typedef typename operand<E>::vec vec;
+    __shared__ __align__(16) char lds[4 * X_BYTES + 2 * A_BYTES];
+    const tile c = find_tile(p, 64 * MT, blockIdx.x);
+    if (c.len <= 0) return;
+    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int row8 = lane >> 3, at8 = lane & 7;
+    char * xs = lds + wave * X_BYTES, * const as = lds + 4 * X_BYTES;
+    const int t0 = 16 * MT * wave;                         // the wave's first row
+
+    if (c.id < 0) return copy_rows<E, V>(p, c);
+
+    v4f acc[MT][RT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[m][j] = v4f{};
+    const W * a = static_cast<const W *>(p.a) + (int64_t) c.id * p.r * p.K;
+    {
+        struct step {
+            v4i x[2 * MT], a[A_LOADS];
+        };
+        const char * x[2 * MT];
+        int ar[A_LOADS], rank[A_LOADS];
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) x[i] = p.x + (c.row + (int64_t) min(t0 + 8 * i + row8, c.len - 1)) * p.x_s;
+#pragma unroll
+        for (int i = 0; i < A_LOADS; ++i) {
+            rank[i] = A_ROW == 128 ? 8 * (4 * i + wave) + row8 : 16 * (4 * i + wave) + (lane >> 2);
+            ar[i] = min(rank[i], p.r - 1) * p.K;
+        }
+        auto load = [&](step & s, int k0) {
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i) s.x[i] = *reinterpret_cast<const v4i *>(x[i] + min(k0 + at8 * V, p.K - V) * (int) sizeof(E));
+#pragma unroll
+            for (int i = 0; i < A_LOADS; ++i) s.a[i] = *reinterpret_cast<const v4i *>(a + ar[i] + min(k0 + (A_ROW == 128 ? at8 : lane & 3) * WV, p.K - WV));
+        };
+        auto use = [&](step & s, int k0, char * buf, bool more) {
+            in_order();
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i) *reinterpret_cast<v4i *>(xs + (8 * i + row8) * 128 + ((at8 ^ ((4 * i + (lane >> 4)) & 7)) << 4)) = s.x[i];
+#pragma unroll
+            for (int i = 0; i < A_LOADS; ++i) {
+                if (rank[i] >= RP) continue;               // a wave without a share (few ranks)
+                if constexpr (A_ROW == 128) *reinterpret_cast<v4i *>(buf + rank[i] * 128 + ((at8 ^ ((rank[i] >> 1) & 7)) << 4)) = s.a[i];
+                else *reinterpret_cast<v4i *>(buf + rank[i] * 64 + (((lane & 3) ^ ((rank[i] >> 2) & 3)) << 4)) = s.a[i];
+            }
+            if (more) load(s, k0 + 16 * V);
+            lds_barrier();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = k0 + (4 * h + g) * V, sw = (4 * h + g) ^ (col >> 1);
+                vec xf[MT];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) xf[m] = taken<E, E>(xs + (16 * m + col) * 128 + (sw << 4), true);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                    const char * from = A_ROW == 128 ? buf + (16 * j + col) * 128 + (sw << 4)
+                                                     : buf + (16 * j + col) * 64 + (((2 * h + (g >> 1)) ^ (col >> 2)) << 4) + (g & 1) * 8;
+                    const vec af = taken<E, W>(from, k < p.K && 16 * j + col < p.r);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) acc[m][j] = operand<E>::mul(af, xf[m], acc[m][j]);
+                }
+            }
+        };
+        step s0, s1;
+        load(s0, 0);
+        if (8 * V < p.K) load(s1, 8 * V);
+        for (int k0 = 0; k0 < p.K; k0 += 16 * V) {
+            use(s0, k0, as, k0 + 16 * V < p.K);
+            if (k0 + 8 * V < p.K) use(s1, k0 + 8 * V, as + A_BYTES, k0 + 24 * V < p.K);
+        }
+    }
+    // s of 16 rows at a time through LDS: its rows to memory, and the next product's operands
+    constexpr int Q = ranks<E, RT>::Q;
+    typename ranks<E, RT>::vec s[MT][Q][ranks<E, RT>::SV];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        float * rows = reinterpret_cast<float *>(xs);
+        in_order();
+#pragma unroll
+        for (int j = 0; j < RT; ++j) *reinterpret_cast<v4f *>(rows + col * LD + 16 * j + 4 * g) = acc[m][j] * p.pre;
+        in_order();
+#pragma unroll
+        for (int i = 0; i < RP / 4; ++i) {
+            const int t = (64 * i + lane) / RP, r = (64 * i + lane) % RP;
+            if (t0 + 16 * m + t < c.len && r < p.r) p.s[(c.row + (int64_t) t0 + 16 * m + t) * p.r + r] = rows[t * LD + r];
+        }
+        ranks<E, RT>::operands(s[m], rows + col * LD, g);
+    }
+    if (!p.y) return;
+    lds_barrier();
+
+    constexpr int M = V / 4;
     const W * b = static_cast<const W *>(p.b) + (int64_t) c.id * p.N * p.r;
-    const bool whole = p.r % V == 0;
-    for (int n0 = (blockIdx.y * 4 + wave) * 8 * V; n0 < p.N; n0 += 32 * V * (int) gridDim.y) {
-        // two groups of 4 V columns: 128 bytes of a row
-        vec before[2][MT];
+    struct block {
+        v4i before[2 * MT], b[A_LOADS];
+    };
+    const int row_bytes = p.r * (int) sizeof(W), chunks = 8 * V * row_bytes / 16;
+    const bool whole = row_bytes % 16 == 0, aligned = p.r % V == 0;
+    const int stride = row_bytes + (whole ? 16 : 0);
+    int at[A_LOADS], from_q[A_LOADS];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+    for (int i = 0; i < A_LOADS; ++i) {
+        const int q = 64 * (4 * i + wave) + lane;
+        from_q[i] = q;
+        at[i] = q >= chunks ? -1 : 16 * (whole ? q + q / (row_bytes / 16) : q);
+    }
+    auto load = [&](block & k, int n0) {
+        const char * from = reinterpret_cast<const char *>(b + (int64_t) n0 * p.r);
+        const int last = min(chunks, (p.N - n0) * row_bytes / 16) - 1;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const int n = n0 + 4 * V * h + V * g, t = 16 * m + col;
-                const E * from = reinterpret_cast<const E *>(p.base + (c.row + (int64_t) t) * p.base_s);
-                before[h][m] = fetch<E, E, WIDE>(from, p.base && t < c.len ? n : p.N, p.N);
-            }
-        vec bf[2][M][Q];
+        for (int i = 0; i < A_LOADS; ++i) k.b[i] = *reinterpret_cast<const v4i *>(from + min(from_q[i], last) * 16);
+        if (p.base) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < M; ++i) {
-                const W * row = b + (int64_t) min(n0 + 4 * V * h + V * (col >> 2) + 4 * i + (col & 3), p.N - 1) * p.r;
-#pragma unroll
-                for (int q = 0; q < Q; ++q) {
-                    const int r = F32 ? 16 * q + 4 * g : RT == 1 ? 8 * (g & 1) : 32 * q + 8 * g;
-                    if (whole) bf[h][i][q] = fetch<E, W, true>(row, r, p.r);
-                    else bf[h][i][q] = fetch<E, W, false>(row, r, p.r);
-                }
-            }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            v4f up[M][MT];
-#pragma unroll
-            for (int i = 0; i < M; ++i) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m) up[i][m] = v4f{};
-#pragma unroll
-                for (int q = 0; q < Q; ++q) {
-                    if constexpr (F32) {
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) up[i][m] = operand<float>::mul(bf[h][i][q], s[m][q][0], up[i][m]);
-                    } else {
-                        v8b hi, lo;
-                        if constexpr (F16) split(bf[h][i][q], hi, lo);
-                        else hi = bf[h][i][q];
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-#pragma unroll
-                            for (int k = 0; k < SV; ++k) up[i][m] = operand<__bf16>::mul(hi, s[m][q][k], up[i][m]);
-                            if constexpr (F16) up[i][m] = operand<__bf16>::mul(lo, s[m][q][0], up[i][m]);
-                        }
-                    }
-                }
-            }
-            const int n = n0 + 4 * V * h + V * g;
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const int t = 16 * m + col;
-                vec out;
-#pragma unroll
-                for (int i = 0; i < V; ++i) out[i] = (E) __builtin_fmaf(up[i / 4][m][i % 4], p.post, (float) before[h][m][i]);
-                if (t >= c.len) continue;
-                E * to = reinterpret_cast<E *>(p.y + (c.row + (int64_t) t) * p.y_s);
-                if constexpr (WIDE) {
-                    if (n < p.N) *reinterpret_cast<vec *>(to + n) = out;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (n + i < p.N) to[n + i] = out[i];
-                }
+            for (int i = 0; i < 2 * MT; ++i) {
+                const char * row = p.base + (c.row + (int64_t) min(t0 + 8 * i + row8, c.len - 1)) * p.base_s;
+                k.before[i] = *reinterpret_cast<const v4i *>(row + min(n0 + at8 * V, p.N - V) * (int) sizeof(E));
             }
         }
+    };
+    auto use = [&](block & k, int n0, char * buf, bool more) {
+        in_order();
+#pragma unroll
+        for (int i = 0; i < A_LOADS; ++i)
+            if (at[i] >= 0) *reinterpret_cast<v4i *>(buf + at[i]) = k.b[i];
+        v4i before[2 * MT];
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) before[i] = k.before[i];
+        if (more) load(k, n0 + 16 * V);
+        lds_barrier();
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            in_order();
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < M; ++i) {
+                    const int n = 4 * V * h + V * (col >> 2) + 4 * i + (col & 3);
+                    v4f up = {};
+#pragma unroll
+                    for (int q = 0; q < Q; ++q) {
+                        const int r = ranks<E, RT>::first(q, g);
+                        vec bf;
+                        if (aligned) bf = taken<E, W>(buf + n * stride + r * (int) sizeof(W), r < p.r);
+                        else bf = fetch<E, false>(reinterpret_cast<const W *>(buf + n * stride), r, p.r);
+                        ranks<E, RT>::multiply(up, bf, s[m][q]);
+                    }
+                    *reinterpret_cast<v4f *>(xs + col * OUT + (4 * V * h + V * g + 4 * i) * 4) = up;
+                }
+            in_order();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = t0 + 16 * m + 8 * i + row8, n = n0 + at8 * V;
+                const float * up = reinterpret_cast<const float *>(xs + (8 * i + row8) * OUT) + at8 * V;
+                vec old, out;
+                __builtin_memcpy(&old, &before[2 * m + i], 16);
+#pragma unroll
+                for (int e = 0; e < V; ++e) out[e] = (E) __builtin_fmaf(up[e], p.post, p.base ? (float) old[e] : 0.0f);
+                if (t < c.len && n < p.N) *reinterpret_cast<vec *>(p.y + (c.row + (int64_t) t) * p.y_s + (int64_t) n * (int) sizeof(E)) = out;
+            }
+        }
+    };
+    block b0, b1;
+    load(b0, 0);
+    if (8 * V < p.N) load(b1, 8 * V);
+    for (int n0 = 0; n0 < p.N; n0 += 16 * V) {
+        use(b0, n0, as, n0 + 16 * V < p.N);
+        if (n0 + 8 * V < p.N) use(b1, n0 + 8 * V, as + A_BYTES, n0 + 24 * V < p.N);
     }
 }
 
@@ -458,26 +776,33 @@ __device__ __forceinline__ void put(void * to, int64_t i, float x, int32_t type)
     else static_cast<__bf16 *>(to)[i] = (__bf16) x;
 }
 
-// The sum over a chunk's rows of u^T z, r x 16 V columns: u = g, z = x (dA), or u = s, z = dy (dB). A wave takes every
-// fourth 32 rows: a lane loads 16 bytes of 8 rows, whose values of one column, next to each other after a
-// permutation of bytes, are the operand as it is (its 16 lanes' columns are V apart). The waves' sums are joined in LDS, in order.
-constexpr int CHUNK = 1024;        // rows of a chunk, at most
+// The sum over a chunk's rows of u^T z, r x 64 V columns: u = g, z = x (dA), or u = s, z = dy (dB), 32 rows a step. A wave has 16 V columns:
+// a lane loads 16 bytes of 8 rows, whose values of one column, next to each other after a permutation of bytes, are the
+// operand as it is (its 16 lanes' columns are V apart). u is brought to LDS once for the four waves, turned round and as operands
+// (two steps' in turn). The next step's loads are under way beside a step's products.
+constexpr int CHUNK = 2048;        // rows of a chunk, at most
 template <class E, int RT, int V, bool WIDE>
 __global__ __launch_bounds__(256) void adapter_grads_kernel(grads_p p) {
     constexpr bool F32 = std::is_same<E, float>::value, F16 = std::is_same<E, _Float16>::value;
-    constexpr int RP = 16 * RT, CW = 16 * V;
+    constexpr int RP = 16 * RT, CW = 64 * V, TP = RP / 8;      // TP: tokens of u of a thread
+    constexpr int U_ROW = F32 ? 32 * 4 + 16 : 32 * 2 + 16;     // bytes of a rank's 32 rows (of one part)
+    constexpr int PARTS = F32 ? 1 : 2, U_BYTES = RP * U_ROW;
     typedef E evec __attribute__((ext_vector_type(V)));
+    typedef typename std::conditional<F32, float, __bf16>::type U;
+    typedef U uvec __attribute__((ext_vector_type(TP)));
     __shared__ __align__(16) int rows[CHUNK];
-    __shared__ __align__(16) float sum[RP][CW + 4];
+    __shared__ __align__(16) char us[2][PARTS][U_BYTES];
     const int slabs = p.slabs_a + p.slabs_b, slab = blockIdx.x % slabs;
     const chunk c = p.slots[blockIdx.x / slabs];
     if (c.id < 0) return;
     const bool down = slab < p.slabs_a;
-    const int C = down ? p.K : p.N, c0 = (down ? slab : slab - p.slabs_a) * CW;
-    const char * z = down ? p.x : p.dy;
+    const int C = down ? p.K : p.N;
     const int64_t z_s = down ? p.x_s : p.dy_s;
-    const float * u = down ? p.g : p.s;
     const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int c0 = (down ? slab : slab - p.slabs_a) * CW + wave * 16 * V;      // the wave's first column
+    const char * z = (down ? p.x : p.dy) + (int64_t) min(c0 + V * col, WIDE ? C - V : C - 1) * (int) sizeof(E);
+    const int rank = threadIdx.x % RP, tok = threadIdx.x / RP * TP;            // of u
+    const float * u = (down ? p.g : p.s) + min(rank, p.r - 1);
 
     const int doc = p.of[c.id].doc, docs = p.of[c.id].docs;
     for (int i = threadIdx.x; i < c.count; i += 256) {
@@ -496,38 +821,66 @@ __global__ __launch_bounds__(256) void adapter_grads_kernel(grads_p p) {
     for (int v = 0; v < V; ++v)
 #pragma unroll
         for (int j = 0; j < RT; ++j) acc[v][j] = v4f{};
-    for (int t0 = wave * 32; t0 < c.count; t0 += 128) {
-        evec zv[8];
-        float uv[RT][8];
+    struct step {
+        evec z[8];
+        float u[TP];
+    };
+    const bool mine = c0 < C;
+    auto load = [&](step & s, int t0) {
+#pragma unroll
+        for (int k = 0; k < TP; ++k) s.u[k] = u[(int64_t) rows[min(t0 + tok + k, c.count - 1)] * p.r];
+        if (!mine) return;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const int t = t0 + 8 * g + k;
-            const bool some = t < c.count;
-            const int64_t row = some ? rows[t] : 0;
-            const E * from = reinterpret_cast<const E *>(z + row * z_s) + c0 + V * col;
-#pragma unroll
-            for (int v = 0; v < V; ++v) zv[k][v] = (E) 0.0f;
+            const char * from = z + rows[min(t0 + 8 * g + k, c.count - 1)] * z_s;
             if constexpr (WIDE) {
-                if (some && c0 + V * col < C) zv[k] = *reinterpret_cast<const evec *>(from);
+                s.z[k] = *reinterpret_cast<const evec *>(from);
             } else {
 #pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (some && c0 + V * col + v < C) zv[k][v] = from[v];
+                for (int v = 0; v < V; ++v) s.z[k][v] = c0 + V * col + v < C ? reinterpret_cast<const E *>(from)[v] : (E) 0.0f;
             }
-#pragma unroll
-            for (int j = 0; j < RT; ++j) uv[j][k] = some && 16 * j + col < p.r ? u[row * p.r + 16 * j + col] : 0.0f;
         }
+    };
+    auto use = [&](step & s, int t0, int buf, int next) {
+        // rows behind the chunk's end, and ranks behind the last, are zeros, in both operands
+        uvec hi;
+#pragma unroll
+        for (int k = 0; k < TP; ++k) hi[k] = (U) (s.u[k] = t0 + tok + k < c.count && rank < p.r ? s.u[k] : 0.0f);
+        *reinterpret_cast<uvec *>(us[buf][0] + rank * U_ROW + tok * (int) sizeof(U)) = hi;
+        if constexpr (!F32) {
+            uvec lo;
+#pragma unroll
+            for (int k = 0; k < TP; ++k) lo[k] = (U) (s.u[k] - (float) hi[k]);
+            *reinterpret_cast<uvec *>(us[buf][1] + rank * U_ROW + tok * (int) sizeof(U)) = lo;
+        }
+        evec zv[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            zv[k] = s.z[k];
+            if (t0 + 32 > c.count && t0 + 8 * g + k >= c.count) zv[k] = evec{};
+        }
+        if (next < c.count) load(s, next);
+        lds_barrier();
+        if (!mine) return;
         if constexpr (F32) {
+            v4f uv[RT][2];
+#pragma unroll
+            for (int j = 0; j < RT; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) uv[j][i] = *reinterpret_cast<const v4f *>(us[buf][0] + (16 * j + col) * U_ROW + 32 * g + 16 * i);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
 #pragma unroll
                 for (int v = 0; v < V; ++v)
 #pragma unroll
-                    for (int j = 0; j < RT; ++j) acc[v][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(uv[j][k], zv[k][v], acc[v][j], 0, 0, 0);
+                    for (int j = 0; j < RT; ++j) acc[v][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(uv[j][k / 4][k % 4], zv[k][v], acc[v][j], 0, 0, 0);
         } else {
-            v8b hi[RT], lo[RT];
+            v8b uh[RT], ul[RT];
 #pragma unroll
-            for (int j = 0; j < RT; ++j) split(uv[j], hi[j], lo[j]);
+            for (int j = 0; j < RT; ++j) {
+                uh[j] = *reinterpret_cast<const v8b *>(us[buf][0] + (16 * j + col) * U_ROW + 16 * g);
+                ul[j] = *reinterpret_cast<const v8b *>(us[buf][1] + (16 * j + col) * U_ROW + 16 * g);
+            }
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 typename operand<E>::vec zc;
@@ -538,40 +891,45 @@ __global__ __launch_bounds__(256) void adapter_grads_kernel(grads_p p) {
                 else zh = zc;
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
-                    acc[v][j] = operand<__bf16>::mul(hi[j], zh, acc[v][j]);
-                    acc[v][j] = operand<__bf16>::mul(lo[j], zh, acc[v][j]);
-                    if constexpr (F16) acc[v][j] = operand<__bf16>::mul(hi[j], zl, acc[v][j]);
+                    acc[v][j] = operand<__bf16>::mul(uh[j], zh, acc[v][j]);
+                    acc[v][j] = operand<__bf16>::mul(ul[j], zh, acc[v][j]);
+                    if constexpr (F16) acc[v][j] = operand<__bf16>::mul(uh[j], zl, acc[v][j]);
                 }
             }
         }
+    };
+    step s0, s1;
+    if (0 < c.count) load(s0, 0);
+    if (32 < c.count) load(s1, 32);
+    for (int t0 = 0; t0 < c.count; t0 += 64) {
+        use(s0, t0, 0, t0 + 64);
+        if (t0 + 32 < c.count) use(s1, t0 + 32, 1, t0 + 96);
     }
-    for (int turn = 0; turn < 4; ++turn) {
-        if (wave == turn) {
-#pragma unroll
-            for (int j = 0; j < RT; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int v = 0; v < V; v += 4) {
-                        v4f * to = reinterpret_cast<v4f *>(&sum[16 * j + 4 * g + i][V * col + v]);
-                        const v4f x = {acc[v][j][i], acc[v + 1][j][i], acc[v + 2][j][i], acc[v + 3][j][i]};
-                        *to = turn ? *to + x : x;
-                    }
-        }
-        __syncthreads();
-    }
-    const int cols = min(CW, C - c0);
+    if (!mine) return;
     const float f = down ? 1.0f : p.scale;
-    if (c.part >= 0) {
-        float * to = (down ? p.part_a : p.part_b) + (int64_t) c.part * p.r * C + c0;
-        for (int i = threadIdx.x; i < p.r * CW; i += 256)
-            if (i % CW < cols) to[(int64_t) (i / CW) * C + i % CW] = sum[i / CW][i % CW] * f;
-    } else if (down) {
-        for (int i = threadIdx.x; i < p.r * CW; i += 256)
-            if (i % CW < cols) put(p.da, ((int64_t) c.id * p.r + i / CW) * C + c0 + i % CW, sum[i / CW][i % CW], p.w_type);
-    } else {
-        for (int i = threadIdx.x; i < p.r * cols; i += 256) put(p.db, ((int64_t) c.id * C + c0) * p.r + i, sum[i % p.r][i / p.r] * f, p.w_type);
-    }
+    float * part = c.part < 0 ? nullptr : (down ? p.part_a : p.part_b) + (int64_t) c.part * p.r * C;
+    const int n = c0 + V * col;
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 16 * j + 4 * g + i;
+            if (r >= p.r || n >= C) continue;
+            if (part && WIDE) {
+#pragma unroll
+                for (int v = 0; v < V; v += 4)
+                    *reinterpret_cast<v4f *>(part + (int64_t) r * C + n + v) = v4f{acc[v][j][i], acc[v + 1][j][i], acc[v + 2][j][i], acc[v + 3][j][i]} * f;
+                continue;
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (n + v >= C) continue;
+                const float x = acc[v][j][i] * f;
+                if (part) part[(int64_t) r * C + n + v] = x;
+                else if (down) put(p.da, ((int64_t) c.id * p.r + r) * C + n + v, x, p.w_type);
+                else put(p.db, ((int64_t) c.id * C + n + v) * p.r + r, x, p.w_type);
+            }
+        }
 }
 
 // The chunks' sums of the adapters that have several, in order: a value a lane, its four waves every fourth chunk.
@@ -667,23 +1025,43 @@ bool wide(const void * p, int64_t stride_bytes) { return (((uintptr_t) p | (uint
 // The kernel of both directions: K values of x down to s, up to N values of y.
 int32_t launch_rows(const char * what, adapter_p & p, int32_t type, int32_t w_type, void * stream) {
     const int V = 16 / size_of(type), cus = nxg_device_cus();
-    const bool w = wide(p.x, p.x_s) && (!p.base || wide(p.base, p.base_s)) && wide(p.y, p.y ? p.y_s : 0) && p.K % V == 0 && p.N % V == 0;
-    // 64 rows a workgroup read the weights a quarter as often as 16, where that leaves work for every CU
-    const bool tall = w && p.T / 64 >= 2 * cus;
-    const int64_t slots = p.T / (tall ? 64 : 16) + (int64_t) p.n_seqs;
+    const bool w = wide(p.x, p.x_s) && (!p.base || wide(p.base, p.base_s)) && wide(p.y, p.y ? p.y_s : 0) && p.K % V == 0 && p.N % V == 0 &&
+                   p.K * (int64_t) size_of(w_type) % 16 == 0 && p.N * (int64_t) p.r * size_of(w_type) % 16 == 0;
+    // Which kernel, and rows of a workgroup: the larger ones read the weights less often, where that leaves work for every CU
+    // (32,768 rows of 1,024 to 1,024: bf16 rank 64 49 us with 64 rows, 70 with 16, rank 32 37 and 40; 16,384 rows of rank 64 43 and
+    // 40, of rank 128 64 and 97; fp32 rank 64 118 and 139, rank 32 110 and 92; 65,536 rows of rank 128 120 with 128 rows, 147
+    // with 64). Straight from memory: one row bf16 rank 16 5.3 us, through LDS 6.2; 8,192 rows 14.0 and 15.3; 16,384 rows 22.5
+    // and 20.6; rank 64 and fp32 are faster through LDS from one row on.
+    const bool f32 = type == NXG_TYPE_F32;
+    int rows = 16;
+    if (w && p.r > (f32 ? 32 : 16)) {
+        if (p.r > 64 && p.T / 128 >= 2 * cus) rows = 128;
+        else if (p.T / 64 >= (p.r > 64 && !f32 ? 1 : 2) * cus) rows = 64;
+    }
+    const int64_t slots = p.T / rows + (int64_t) p.n_seqs;
     if (slots > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d n_seqs=%d is too large", what, p.T, p.n_seqs);
+    const bool direct = !f32 && p.r <= 32 && slots < 4 * cus;
     // few rows: several workgroups share out the columns, each with the down product of its own
     int parts = 1;
-    while (p.y && !tall && slots * parts * 2 <= cus && p.N > 32 * V * parts) parts *= 2;
+    while (p.y && rows == 16 && slots * parts * 2 <= cus && p.N > 32 * V * parts) parts *= 2;
     const dim3 grid((unsigned) slots, (unsigned) parts);
     hipStream_t s = (hipStream_t) stream;
     by_types(type, w_type, [&](auto e, auto we) {
         typedef decltype(e) E;
         typedef decltype(we) W;
         by_rank(p.r, [&](auto rt) {
-            if (tall) adapter_rows_kernel<E, W, 4, rt(), true><<<grid, 256, 0, s>>>(p);
-            else if (w) adapter_rows_kernel<E, W, 1, rt(), true><<<grid, 256, 0, s>>>(p);
-            else adapter_rows_kernel<E, W, 1, rt(), false><<<grid, 256, 0, s>>>(p);
+            constexpr bool F32 = std::is_same<E, float>::value;
+            if (!w) return adapter_rows_kernel<E, W, rt(), BY_VALUE><<<grid, 256, 0, s>>>(p);
+            if constexpr (!F32 && rt() <= 2) {
+                if (direct) return adapter_rows_kernel<E, W, rt(), WIDE><<<grid, 256, 0, s>>>(p);
+            }
+            if constexpr (rt() == 8) {
+                if (rows == 128) return adapter_rows_tall_kernel<E, W, 2, rt()><<<grid, 256, 0, s>>>(p);
+            }
+            if constexpr (rt() > (F32 ? 2 : 1)) {
+                if (rows == 64) return adapter_rows_tall_kernel<E, W, 1, rt()><<<grid, 256, 0, s>>>(p);
+            }
+            adapter_rows_kernel<E, W, rt(), THROUGH_LDS><<<grid, 256, 0, s>>>(p);
         });
     });
     return nxg_launch_check(what);
@@ -698,11 +1076,12 @@ struct layout {
 layout plan_backward(const nxg_adapter_rows_params & p) {
     layout l;
     const int es = size_of(p.type), ws = size_of(p.w_type);
-    l.cw = es == 4 || p.rank > 64 ? 64 : 128;
+    l.cw = es == 4 || p.rank > 64 ? 256 : 512;
     const int64_t slabs = (p.n_in + l.cw - 1) / l.cw + (p.n_out + l.cw - 1) / l.cw;
-    // rows of a chunk: as many as leave about four workgroups a CU
-    l.size = CHUNK;
-    while (l.size > 128 && p.T / l.size * slabs < 4 * nxg_device_cus()) l.size /= 2;
+    // rows of a chunk: so that the workgroups, one more chunk an adapter counted in, are one a CU (32 documents of 4 adapters 30 us; a
+    // few more than that many take 42); at most twice as many with many adapters
+    const int64_t cus = nxg_device_cus(), room = std::max(cus - p.n_adapters * slabs, cus / 2);
+    l.size = (int) std::min<int64_t>(CHUNK, std::max<int64_t>(64, (p.T * slabs / room + 32) / 32 * 32));
     l.n_slots = p.T / l.size + (int64_t) p.n_adapters;
     l.n_parts = 2 * (int64_t) p.T / l.size;            // adapters of more rows than a chunk have less than twice as many chunks as whole ones
     int64_t at = 0;
