@@ -55,13 +55,14 @@ struct rope_p {
     bool copy;                             // out is not x: values behind n are written too
 };
 
-// The largest d with cu[d] <= t (0 if none): the row's document.
-__device__ __forceinline__ int doc_of_row(const int32_t * cu, int n_seqs, int t) {
-    int lo = 0, hi = n_seqs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (cu[mid] <= t) lo = mid;
-        else hi = mid - 1;
+// The largest d with cu[d] <= t (0 if none), t's document: for all lanes of a wave, 64 documents at a time.
+__device__ __forceinline__ int doc_of_rows(const int32_t * cu, int n_seqs, int t) {
+    int lo = 0, n = n_seqs;
+    while (n > 1) {
+        const int step = (n + 63) >> 6, k = (threadIdx.x & 63) * step;
+        const int last = max((int) __popcll(__ballot(k < n && cu[lo + k] <= t)) - 1, 0);
+        n = min(step, n - last * step);
+        lo += last * step;
     }
     return lo;
 }
@@ -69,12 +70,19 @@ __device__ __forceinline__ int doc_of_row(const int32_t * cu, int n_seqs, int t)
 // The turns of `tokens` rows from t0, [tokens][half], as (cos, sin) times the factor on the result, by the 256 threads of a workgroup.
 template <class P>
 __device__ __forceinline__ void find_turns(float2 * turn, const P & p, int t0, int tokens, int half) {
+    const int first = p.positions ? 0 : doc_of_rows(p.cu, p.n_seqs, t0);
     for (int k = threadIdx.x; k < tokens * half; k += 256) {
         const int t = t0 + k / half, i = k % half;
+        const double f = p.freq[i];
         int pos;
-        if (p.positions) pos = p.positions[t];
-        else pos = t - p.cu[doc_of_row(p.cu, p.n_seqs, t)];
-        const double turns = (double) pos * p.freq[i] * 0.15915494309189533577;   // 1 / (2 pi)
+        if (p.positions) {
+            pos = p.positions[t];
+        } else {
+            int d = first;
+            while (d + 1 < p.n_seqs && p.cu[d + 1] <= t) ++d;
+            pos = t - p.cu[d];
+        }
+        const double turns = (double) pos * f * 0.15915494309189533577;   // 1 / (2 pi)
         float s, c;
         sincospif(2.0f * (float) (turns - rint(turns)), &s, &c);
         turn[k] = make_float2(c * p.mscale, s * p.mscale * p.sign);
@@ -425,10 +433,12 @@ struct qk_p {
     qk_rows of[2];                         // queries, keys
     const double * freq;
     const int32_t * positions, * cu;
-    float * part;                          // [workgroups][2][D]
+    float * part;                          // [workgroups][D], the queries' first
     int32_t T, D, n, n_seqs, tb, lanes;    // tokens of a workgroup at a time, lanes of a head (a power of two)
+    int32_t n_q;                           // workgroups of the queries (gradients)
     float mscale, sign, eps;
     int32_t w_type;
+    void * dw[2];
 };
 
 // Where a head's values lie in its lanes: slot j (lane j % lanes, its j / lanes'th) has V values from d[0] and V from d[1]. A pair that is
@@ -482,14 +492,25 @@ __device__ __forceinline__ void qk_turn(float (&x)[2][V], const qk_slot & s, con
     }
 }
 
+// A slot's values as they are in memory, and as fp32.
+template <class E, int V> using qk_piece = E __attribute__((ext_vector_type(V == 1 ? 2 : V)));
 template <class E, int V>
-__device__ __forceinline__ void qk_load(float (&x)[2][V], const E * row, const qk_slot & s) {
+__device__ __forceinline__ void qk_load(qk_piece<E, V> (&x)[2], const E * row, const qk_slot & s) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[k][i] = 0.0f;
-        if (s.d[k] >= 0) load<E, V>(x[k], row + s.d[k]);
+        x[k] = qk_piece<E, V>{};
+        if (s.d[k] >= 0) {
+            if constexpr (V == 1) x[k][0] = row[s.d[k]];
+            else x[k] = *reinterpret_cast<const qk_piece<E, V> *>(row + s.d[k]);
+        }
     }
+}
+template <class E, int V>
+__device__ __forceinline__ void qk_take(float (&x)[2][V], const qk_piece<E, V> (&from)[2]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[k][i] = (float) from[k][i];
 }
 template <class E, int V>
 __device__ __forceinline__ void qk_store(E * row, const float (&x)[2][V], const qk_slot & s) {
@@ -498,26 +519,49 @@ __device__ __forceinline__ void qk_store(E * row, const float (&x)[2][V], const 
         if (s.d[k] >= 0) store<E, V>(row + s.d[k], x[k]);
 }
 
-// Sum over the lanes of a head.
+// Sum over the lanes of a head, the same bits in each: neighbours, pairs, fours and eights mirrored, then rows of 16.
 __device__ __forceinline__ float head_sum(float x, int lanes) {
-    for (int k = lanes / 2; k; k >>= 1) x += __shfl_xor(x, k);
+    auto add = [](float x, auto ctrl) {
+        return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), ctrl(), 0xf, 0xf, false));
+    };
+    if (lanes > 1) x = add(x, std::integral_constant<int, 0xb1>());
+    if (lanes > 2) x = add(x, std::integral_constant<int, 0x4e>());
+    if (lanes > 4) x = add(x, std::integral_constant<int, 0x141>());
+    if (lanes > 8) x = add(x, std::integral_constant<int, 0x140>());
+    if (lanes > 16) x += __shfl_xor(x, 16);
+    if (lanes > 32) x += __shfl_xor(x, 32);
     return x;
 }
 
-// The weights as fp32 in LDS, and the turns of a workgroup's tokens; both before a barrier.
+__device__ __forceinline__ float qk_weight(const void * w, int i, int32_t type) {
+    if (type == NXG_TYPE_F32) return static_cast<const float *>(w)[i];
+    return type == NXG_TYPE_F16 ? (float) static_cast<const _Float16 *>(w)[i] : (float) static_cast<const __bf16 *>(w)[i];
+}
+// Both weights as fp32 in LDS.
 __device__ __forceinline__ void qk_weights(float * w, const qk_p & p) {
     for (int k = threadIdx.x; k < 2 * p.D; k += 256) {
-        const int i = k % p.D;
         const void * from = p.of[k / p.D].w;
-        float x = 0.0f;
-        if (from) x = p.w_type == NXG_TYPE_F32 ? static_cast<const float *>(from)[i] : p.w_type == NXG_TYPE_F16 ? (float) static_cast<const _Float16 *>(from)[i]
-                                                                                                            : (float) static_cast<const __bf16 *>(from)[i];
-        w[k] = x;
+        w[k] = from ? qk_weight(from, k % p.D, p.w_type) : 0.0f;
     }
 }
 
+// The heads of a run of tokens, one after another, `step` apart.
+struct qk_walk {
+    int t, h, step_t, step_h, heads;
+    __device__ __forceinline__ qk_walk(int first, int step, int heads_)
+        : t(first / heads_), h(first % heads_), step_t(step / heads_), step_h(step % heads_), heads(heads_) {}
+    __device__ __forceinline__ void next() {
+        t += step_t;
+        h += step_h;
+        if (h >= heads) {
+            h -= heads;
+            ++t;
+        }
+    }
+};
+
 // A workgroup: tb tokens, their turns and the weights once in LDS, then their heads, `lanes` lanes a head, P slots a lane: one
-// read, one write.
+// read, one write. The first heads' rows are under way while the turns are made, each next while one is turned.
 template <class E, int V, bool HALF, int P>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(qk_p p) {
     extern __shared__ float lds[];
@@ -526,135 +570,181 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(qk_p p) {
     float2 * turn = reinterpret_cast<float2 *>(lds + 2 * p.D);
     const int64_t t0 = (int64_t) blockIdx.x * p.tb;
     const int tokens = (int) min((int64_t) p.tb, p.T - t0);
-    qk_weights(w, p);
-    find_turns(turn, p, (int) t0, tokens, half);
-    __syncthreads();
     const int lane = threadIdx.x % p.lanes, first = threadIdx.x / p.lanes, step = 256 / p.lanes, heads = p.of[0].H + p.of[1].H;
     qk_slot at[P];
 #pragma unroll
     for (int s = 0; s < P; ++s) at[s] = qk_slot_of<V, HALF>(lane + s * p.lanes, p.n, p.D);
-    const float inv = 1.0f / (float) p.D;
-    for (int u = first; u < tokens * heads; u += step) {
-        const int t = u / heads, hh = u - t * heads, key = hh >= p.of[0].H;
+    qk_walk u(first, step, heads);
+    qk_piece<E, V> raw[P][2];
+    auto load = [&](const qk_walk & u) {
+        const int key = u.h >= p.of[0].H;
         const qk_rows & r = p.of[key];
-        const int h = key ? hh - p.of[0].H : hh;
-        const E * x = static_cast<const E *>(r.x) + (t0 + t) * r.x_ts + h * r.x_hs;
+        const E * x = static_cast<const E *>(r.x) + (t0 + u.t) * r.x_ts + (u.h - (key ? p.of[0].H : 0)) * r.x_hs;
+#pragma unroll
+        for (int s = 0; s < P; ++s) qk_load<E, V>(raw[s], x, at[s]);
+    };
+    if (u.t < tokens) load(u);
+    qk_weights(w, p);
+    find_turns(turn, p, (int) t0, tokens, half);
+    __syncthreads();
+    const float inv = 1.0f / (float) p.D;
+    while (u.t < tokens) {
+        const int t = u.t, key = u.h >= p.of[0].H, h = u.h - (key ? p.of[0].H : 0);
+        const qk_rows & r = p.of[key];
         E * o = static_cast<E *>(r.out) + (t0 + t) * r.o_ts + h * r.o_hs;
         float v[P][2][V], ss = 0.0f;
 #pragma unroll
-        for (int s = 0; s < P; ++s) qk_load<E, V>(v[s], x, at[s]);
-#pragma unroll
-        for (int s = 0; s < P; ++s)
+        for (int s = 0; s < P; ++s) {
+            qk_take<E, V>(v[s], raw[s]);
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int i = 0; i < V; ++i) ss += v[s][k][i] * v[s][k][i];
+        }
+        u.next();
+        if (u.t < tokens) load(u);
         const float rstd = 1.0f / sqrtf(head_sum(ss, p.lanes) * inv + p.eps);
 #pragma unroll
         for (int s = 0; s < P; ++s) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int k = 0; k < 2; ++k) {
+                const float * wk = w + key * p.D + max(at[s].d[k], 0);
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[s][k][i] *= rstd * (at[s].d[k] >= 0 ? w[key * p.D + at[s].d[k] + i] : 0.0f);
+                for (int i = 0; i < V; ++i) v[s][k][i] *= rstd * wk[i];
+            }
             qk_turn<V, HALF>(v[s], at[s], turn + t * half);
             qk_store<E, V>(o, v[s], at[s]);
         }
     }
 }
 
-// Gradients: a workgroup's groups of tb tokens (every gridDim.x'th) one after another, the weights' sums of its heads in registers, left
-// as one row of `part`, which norm_reduce_kernel sums in order.
+// Gradients: a workgroup has queries or keys alone, a run of tokens in groups of tb one after another, the weights' sums of
+// its heads in registers, left at the end as a row of `part`. The next group's turns are made into the other half of the LDS, so that
+// a barrier a group does; the next heads' rows are under way while one head's are worked on.
 template <class E, int V, bool HALF, int P>
 __global__ __launch_bounds__(256) void qk_norm_rope_back_kernel(qk_p p) {
-    extern __shared__ float lds[];
-    const int half = p.n / 2;
-    float * w = lds;                                       // [2][D]
-    float2 * turn = reinterpret_cast<float2 *>(lds + 2 * p.D);
+    extern __shared__ float lds[];                         // weights [D], turns [2][tb][n / 2]; then sums [256 / lanes][D]
+    const int half = p.n / 2, key = (int) blockIdx.x >= p.n_q;
     const int lane = threadIdx.x % p.lanes, first = threadIdx.x / p.lanes, step = 256 / p.lanes;
-    qk_weights(w, p);
+    const int64_t parts = key ? (int) gridDim.x - p.n_q : p.n_q, part = (int) blockIdx.x - (key ? p.n_q : 0);
+    const int64_t end = p.T * (part + 1) / parts;          // of the workgroup's tokens
+    int64_t t0 = p.T * part / parts;
+    const qk_rows & r = p.of[key];
     qk_slot at[P];
-    float dw[2][P][2][V];
+    float dw[P][2][V];
 #pragma unroll
     for (int s = 0; s < P; ++s) {
         at[s] = qk_slot_of<V, HALF>(lane + s * p.lanes, p.n, p.D);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int i = 0; i < V; ++i) dw[0][s][k][i] = dw[1][s][k][i] = 0.0f;
+            for (int i = 0; i < V; ++i) dw[s][k][i] = 0.0f;
     }
     const float inv = 1.0f / (float) p.D;
-    for (int64_t t0 = (int64_t) blockIdx.x * p.tb; t0 < p.T; t0 += (int64_t) gridDim.x * p.tb) {
-        const int tokens = (int) min((int64_t) p.tb, p.T - t0);
-        __syncthreads();
-        find_turns(turn, p, (int) t0, tokens, half);
-        __syncthreads();
+    auto tokens_of = [&](int64_t t0) { return (int) min((int64_t) p.tb, end - t0); };
+    qk_piece<E, V> rx[P][2], rg[P][2];
+    auto load = [&](int64_t t0, const qk_walk & u) {
+        const E * x = static_cast<const E *>(r.x) + (t0 + u.t) * r.x_ts + u.h * r.x_hs;
+        const E * dy = static_cast<const E *>(r.dy) + (t0 + u.t) * r.dy_ts + u.h * r.dy_hs;
 #pragma unroll
-        for (int key = 0; key < 2; ++key) {
-            const qk_rows & r = p.of[key];
-            for (int u = first; u < tokens * r.H; u += step) {
-                const int t = u / r.H, h = u - t * r.H;
-                const E * x = static_cast<const E *>(r.x) + (t0 + t) * r.x_ts + h * r.x_hs;
-                const E * dy = static_cast<const E *>(r.dy) + (t0 + t) * r.dy_ts + h * r.dy_hs;
-                E * o = static_cast<E *>(r.out) + (t0 + t) * r.o_ts + h * r.o_hs;
-                float v[P][2][V], g[P][2][V], ss = 0.0f, gx = 0.0f;
-#pragma unroll
-                for (int s = 0; s < P; ++s) {
-                    qk_load<E, V>(v[s], x, at[s]);
-                    qk_load<E, V>(g[s], dy, at[s]);
-                }
-#pragma unroll
-                for (int s = 0; s < P; ++s)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int i = 0; i < V; ++i) ss += v[s][k][i] * v[s][k][i];
-                const float rstd = 1.0f / sqrtf(head_sum(ss, p.lanes) * inv + p.eps);
-#pragma unroll
-                for (int s = 0; s < P; ++s) {
-                    qk_turn<V, HALF>(g[s], at[s], turn + t * half);
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            v[s][k][i] *= rstd;
-                            dw[key][s][k][i] += g[s][k][i] * v[s][k][i];
-                            g[s][k][i] *= at[s].d[k] >= 0 ? w[key * p.D + at[s].d[k] + i] : 0.0f;
-                            gx += g[s][k][i] * v[s][k][i];
-                        }
-                }
-                gx = head_sum(gx, p.lanes) * inv;
-#pragma unroll
-                for (int s = 0; s < P; ++s) {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int i = 0; i < V; ++i) g[s][k][i] = rstd * (g[s][k][i] - v[s][k][i] * gx);
-                    qk_store<E, V>(o, g[s], at[s]);
-                }
-            }
+        for (int s = 0; s < P; ++s) {
+            qk_load<E, V>(rx[s], x, at[s]);
+            qk_load<E, V>(rg[s], dy, at[s]);
         }
-    }
-    // the heads' lanes that have the same slots, one group after another
-    float * sums = lds;                                    // [2][D], over the weights
-    for (int turn_of = 0; turn_of < step; ++turn_of) {
+    };
+    const qk_walk begin(first, step, r.H);
+    float2 * turn = reinterpret_cast<float2 *>(lds + (p.D + 3) / 4 * 4), * other = turn + p.tb * half;
+    if (begin.t < tokens_of(t0)) load(t0, begin);
+    for (int k = threadIdx.x; k < p.D; k += 256) lds[k] = qk_weight(r.w, k, p.w_type);
+    find_turns(turn, p, (int) t0, tokens_of(t0), half);
+    for (; t0 < end; t0 += p.tb) {
+        const int tokens = tokens_of(t0);
         __syncthreads();
-        if (first != turn_of) continue;
+        const bool more = t0 + p.tb < end;
+        qk_walk u = begin;
+        while (u.t < tokens) {
+            E * o = static_cast<E *>(r.out) + (t0 + u.t) * r.o_ts + u.h * r.o_hs;
+            const float2 * turns = turn + u.t * half;
+            float v[P][2][V], g[P][2][V], ss = 0.0f, gx = 0.0f;
 #pragma unroll
-        for (int key = 0; key < 2; ++key)
-#pragma unroll
-            for (int s = 0; s < P; ++s)
+            for (int s = 0; s < P; ++s) {
+                qk_take<E, V>(v[s], rx[s]);
+                qk_take<E, V>(g[s], rg[s]);
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (at[s].d[k] >= 0) {
-                            float * to = sums + key * p.D + at[s].d[k] + i;
-                            *to = turn_of ? *to + dw[key][s][k][i] : dw[key][s][k][i];
-                        }
+                    for (int i = 0; i < V; ++i) ss += v[s][k][i] * v[s][k][i];
+            }
+            u.next();
+            if (u.t < tokens) load(t0, u);
+            else if (more && begin.t < tokens_of(t0 + p.tb)) load(t0 + p.tb, begin);
+            const float rstd = 1.0f / sqrtf(head_sum(ss, p.lanes) * inv + p.eps);
+#pragma unroll
+            for (int s = 0; s < P; ++s) {
+                qk_turn<V, HALF>(g[s], at[s], turns);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float * w = lds + max(at[s].d[k], 0);        // values behind a head's end are zeros
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        v[s][k][i] *= rstd;
+                        dw[s][k][i] += g[s][k][i] * v[s][k][i];
+                        g[s][k][i] *= w[i];
+                        gx += g[s][k][i] * v[s][k][i];
+                    }
+                }
+            }
+            gx = head_sum(gx, p.lanes) * inv;
+#pragma unroll
+            for (int s = 0; s < P; ++s) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) g[s][k][i] = rstd * (g[s][k][i] - v[s][k][i] * gx);
+                qk_store<E, V>(o, g[s], at[s]);
+            }
+        }
+        if (more) find_turns(other, p, (int) (t0 + p.tb), tokens_of(t0 + p.tb), half);
+        float2 * const swap = turn;
+        turn = other;
+        other = swap;
     }
     __syncthreads();
-    float * part = p.part + (int64_t) blockIdx.x * 2 * p.D;
-    for (int c = threadIdx.x; c < 2 * p.D; c += 256) part[c] = sums[c];
+#pragma unroll
+    for (int s = 0; s < P; ++s)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (at[s].d[k] >= 0) lds[first * p.D + at[s].d[k] + i] = dw[s][k][i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.D; c += 256) {
+        float x = 0.0f;
+        for (int k = 0; k < step; ++k) x += lds[k * p.D + c];
+        p.part[(int64_t) blockIdx.x * p.D + c] = x;
+    }
+}
+
+// The workgroups' rows of `part` summed up in order: 16 columns of dwq or dwk a workgroup, 64 threads each, every 64th row a thread (8
+// loads under way at a time), then the 64 in order.
+template <class W>
+__global__ __launch_bounds__(1024) void qk_reduce_kernel(qk_p p, int n_all) {
+    __shared__ float lds[64][17];
+    const int blocks = (p.D + 15) / 16, key = (int) blockIdx.x >= blocks;
+    const int col = ((int) blockIdx.x - (key ? blocks : 0)) * 16 + threadIdx.x % 16, sub = threadIdx.x / 16;
+    const int r0 = key ? p.n_q : 0, r1 = key ? n_all : p.n_q;
+    float s = 0.0f;
+    if (col < p.D) {
+#pragma unroll 8
+        for (int r = r0 + sub; r < r1; r += 64) s += p.part[(int64_t) r * p.D + col];
+    }
+    lds[sub][threadIdx.x % 16] = s;
+    __syncthreads();
+    if (sub || col >= p.D) return;
+    s = 0.0f;
+#pragma unroll 16
+    for (int k = 0; k < 64; ++k) s += lds[k][threadIdx.x];
+    static_cast<W *>(p.dw[key])[col] = (W) s;
 }
 
 // ---------------------------------------------------------------------------
@@ -882,13 +972,15 @@ int32_t take_qk(const char * what, const nxg_qk_norm_rope_params & a, qk_rows & 
     return NXG_OK;
 }
 
+constexpr int QK_PARTS = 768;          // workgroups of the gradients' kernel: three a CU, as many as its registers leave at once
+
 // Both directions' plan: tokens of a workgroup, lanes of a head, and the instance f(V, HALF, P).
 struct qk_plan {
     bool wide;
     int slots, per_lane;
     size_t lds;
 };
-qk_plan plan_qk(const nxg_qk_norm_rope_params & a, qk_p & p) {
+qk_plan plan_qk(const nxg_qk_norm_rope_params & a, qk_p & p, bool back) {
     qk_plan l;
     const int es = size_of(a.type), V = 16 / es;
     l.wide = a.n_rot % (a.layout == NXG_ROPE_HALF ? 2 * V : V) == 0 && a.head_dim % V == 0;
@@ -902,11 +994,13 @@ qk_plan plan_qk(const nxg_qk_norm_rope_params & a, qk_p & p) {
     p.lanes = 1;
     while (p.lanes < 64 && p.lanes < l.slots) p.lanes *= 2;
     l.per_lane = (l.slots + p.lanes - 1) / p.lanes;
-    // tokens: about 12 KiB of rows, an angle a thread at most, fewer where that would leave CUs without work
+    // tokens: about 24 KiB of rows and an angle a thread, so that the heads fill a few whole rounds of the workgroup (16 and 8 heads of 64
+    // bf16 values: 3); gradients, whose workgroups stay, two angles a thread. Fewer where that would leave CUs without work
     const int64_t row = (int64_t) (a.n_head + a.n_kv_head) * a.head_dim * es;
-    p.tb = std::max<int>(1, std::min<int64_t>(512 / a.n_rot, 12288 / row));
-    while (p.tb > 1 && ((int64_t) a.T + p.tb - 1) / p.tb < 2 * nxg_device_cus()) p.tb /= 2;
-    l.lds = (size_t) 2 * a.head_dim * sizeof(float) + (size_t) p.tb * (a.n_rot / 2) * sizeof(float2);
+    p.tb = std::max<int>(1, back ? std::min<int64_t>(1024 / a.n_rot, 65536 / row) : std::min<int64_t>(512 / a.n_rot, 24576 / row));
+    while (p.tb > 1 && ((int64_t) a.T + p.tb - 1) / p.tb < (back ? QK_PARTS : 2 * nxg_device_cus())) p.tb /= 2;
+    const size_t turns = (size_t) p.tb * (a.n_rot / 2) * sizeof(float2);
+    l.lds = back ? std::max<size_t>((a.head_dim + 3) / 4 * 4 * sizeof(float) + 2 * turns, (size_t) (256 / p.lanes) * a.head_dim * sizeof(float)) : 2 * a.head_dim * sizeof(float) + turns;
     p.freq = a.freq;
     p.positions = a.positions;
     p.cu = a.cu;
@@ -1193,7 +1287,7 @@ int32_t nxg_qk_norm_rope_rows(const nxg_qk_norm_rope_params * params, const nxg_
             return nxg_fail(NXG_EINVAL, "%s: an output is another tensor of the call", what);
         }
     }
-    const qk_plan l = plan_qk(a, p);
+    const qk_plan l = plan_qk(a, p, false);
     p.sign = 1.0f;
     const int64_t grid = ((int64_t) a.T + p.tb - 1) / p.tb;
     if (grid > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d is too large", what, a.T);
@@ -1206,7 +1300,7 @@ int32_t nxg_qk_norm_rope_rows(const nxg_qk_norm_rope_params * params, const nxg_
 
 int64_t nxg_qk_norm_rope_rows_workspace_bytes(const nxg_qk_norm_rope_params * params) {
     const int32_t rc = check_qk("qk_norm_rope_rows_workspace_bytes", params);
-    return rc ? -rc : (int64_t) NORM_PARTS * 2 * params->head_dim * 4;
+    return rc ? -rc : (int64_t) QK_PARTS * params->head_dim * 4;
 }
 
 int32_t nxg_qk_norm_rope_rows_backward(const nxg_qk_norm_rope_params * params, const nxg_rows * dq_out, const nxg_rows * dk_out,
@@ -1219,7 +1313,7 @@ int32_t nxg_qk_norm_rope_rows_backward(const nxg_qk_norm_rope_params * params, c
     if (!dwq || !aligned(dwq, ws) || (a.n_kv_head && (!dwk || !aligned(dwk, ws)))) {
         return nxg_fail(NXG_EINVAL, "%s: dwq or dwk is null or not aligned to its type", what);
     }
-    if (!workspace || ((uintptr_t) workspace & 15) || workspace_bytes < (int64_t) NORM_PARTS * 2 * a.head_dim * 4) {
+    if (!workspace || ((uintptr_t) workspace & 15) || workspace_bytes < (int64_t) QK_PARTS * a.head_dim * 4) {
         return nxg_fail(NXG_EINVAL, "%s: workspace must be 16-byte aligned memory of %lld bytes", what,
                         (long long) nxg_qk_norm_rope_rows_workspace_bytes(params));
     }
@@ -1237,10 +1331,14 @@ int32_t nxg_qk_norm_rope_rows_backward(const nxg_qk_norm_rope_params * params, c
                     if (o->data == r->data) return nxg_fail(NXG_EINVAL, "%s: an output is another tensor of the call", what);
             }
         }
-        const qk_plan l = plan_qk(a, p);
+        const qk_plan l = plan_qk(a, p, true);
         p.sign = -1.0f;
         p.part = static_cast<float *>(workspace);
-        grid = std::min<int64_t>(NORM_PARTS, ((int64_t) a.T + p.tb - 1) / p.tb);
+        // workgroups shared out by the heads
+        const int64_t groups = ((int64_t) a.T + p.tb - 1) / p.tb;
+        p.n_q = (int32_t) std::min<int64_t>(groups, std::max<int64_t>(1, (int64_t) QK_PARTS * a.n_head / (a.n_head + a.n_kv_head)));
+        if (a.n_kv_head) p.n_q = std::min(p.n_q, QK_PARTS - 1);
+        grid = p.n_q + (a.n_kv_head ? std::min<int64_t>(groups, QK_PARTS - p.n_q) : 0);
         NXG_TRY(nxg_check_device());
         by_qk(a, l, [&](auto e, auto V, auto half, auto P) {
             qk_norm_rope_back_kernel<decltype(e), V(), half(), P()><<<(unsigned) grid, 256, l.lds, s>>>(p);
@@ -1249,14 +1347,12 @@ int32_t nxg_qk_norm_rope_rows_backward(const nxg_qk_norm_rope_params * params, c
     } else {
         NXG_TRY(nxg_check_device());
     }
-    // dw and db of the norm's sums are here dwq and dwk
-    norm_p n = {};
-    n.part = static_cast<float *>(workspace);
-    n.n_part = (int32_t) grid;
-    n.C = a.head_dim;
-    n.dw = dwq;
-    n.db = a.n_kv_head ? dwk : nullptr;
-    by_types(a.type, a.w_type, [&](auto, auto we) { norm_reduce_kernel<decltype(we)><<<(2 * a.head_dim + 15) / 16, 1024, 0, s>>>(n); });
+    p.part = static_cast<float *>(workspace);
+    p.D = a.head_dim;
+    p.dw[0] = dwq;
+    p.dw[1] = dwk;
+    const unsigned blocks = (unsigned) ((a.head_dim + 15) / 16 * (a.n_kv_head ? 2 : 1));
+    by_types(a.type, a.w_type, [&](auto, auto we) { qk_reduce_kernel<decltype(we)><<<blocks, 1024, 0, s>>>(p, (int) grid); });
     return nxg_launch_check(what);
 }
 

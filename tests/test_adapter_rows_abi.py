@@ -43,7 +43,7 @@ def qk(nxg, L, p=None, **kw):
     return L.nxg_qk_norm_rope_rows(ctypes.byref(p or qk_params(nxg)), *(None if at[n] is None else ctypes.byref(at[n]) for n in ("q", "k", "q_out", "k_out")), None)
 
 
-NEED = 512 * 2 * 64 * 4
+NEED = 768 * 64 * 4
 
 
 def qk_back(nxg, L, p=None, dwq=P16, dwk=P16, ws=P16, n=NEED, **kw):
