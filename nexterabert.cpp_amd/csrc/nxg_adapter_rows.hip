@@ -113,10 +113,13 @@ struct adapter_p {
     const int32_t * cu, * ids;
     int32_t T, K, N, r, n, n_seqs;
     float pre, post;               // factors on s and on the second product
+    bool gather;                   // documents of one row that share an adapter go together
 };
 
 struct tile {
     int row, len, id;              // rows row .. row + len - 1 of adapter id
+    int doc;
+    bool whole;                    // the document
 };
 
 // The tile of size rows of a slot. Document d owns the slots from floor(cu[d] / size) + d, at least as many as it has tiles,
@@ -136,6 +139,8 @@ __device__ __forceinline__ tile find_tile(const adapter_p & p, int size, int slo
     tile t;
     t.row = r0 + at * size;
     t.len = at < 0 ? 0 : min(size, r1 - t.row);
+    t.doc = lo;
+    t.whole = t.len == r1 - r0;
     const int id = uni(p.ids[lo]);
     t.id = id >= 0 && id < p.n ? id : -1;
     return t;
@@ -185,6 +190,26 @@ template <class E, int RT> struct ranks {
     }
 };
 
+// Documents of one row that have an adapter in common, 16 at a time: the rows of the tile's document and of those that follow it, into
+// `rows`, and their number; 0 where the document is among those of one before it. By every wave of a workgroup; ends with a barrier.
+__device__ __forceinline__ int gather_rows(const adapter_p & p, const tile & c, int * rows) {
+    const int lane = threadIdx.x & 63;
+    auto alike = [&](int d, int end) { return d < end && p.ids[d] == c.id && offset(p.cu, d + 1, p.T) - offset(p.cu, d, p.T) == 1; };
+    int before = 0, found = 1;
+    for (int d = 0; d < c.doc; d += 64) before += __popcll(__ballot(alike(d + lane, c.doc)));
+    if (before % 16) return 0;
+    if (threadIdx.x == 0) rows[0] = c.row;
+    for (int d = c.doc + 1; d < p.n_seqs && found < 16; d += 64) {
+        const bool mine = alike(d + lane, p.n_seqs);
+        const uint64_t all = __ballot(mine);
+        const int at = found + __popcll(all & ((1ull << lane) - 1));
+        if (mine && at < 16 && threadIdx.x < 64) rows[at] = offset(p.cu, d + lane, p.T);
+        found += __popcll(all);
+    }
+    __syncthreads();
+    return min(found, 16);
+}
+
 // The rows of a document without an adapter: base as it is, s = 0. By a workgroup, V values at a time.
 template <class E, int V>
 __device__ __forceinline__ void copy_rows(const adapter_p & p, const tile & c) {
@@ -224,12 +249,19 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
     constexpr int SUMS = 2 * 16 * LD * 4, LDS = HOW == THROUGH_LDS ? std::max(4 * (X_BYTES + A_BYTES), SUMS) : SUMS;
     typedef typename operand<E>::vec vec;
     __shared__ __align__(16) char lds[LDS];
-    const tile c = find_tile(p, 16, blockIdx.x);
+    __shared__ int gathered[16];
+    tile c = find_tile(p, 16, blockIdx.x);
     if (c.len <= 0) return;
     if (c.id < 0) {
         if (blockIdx.y == 0) copy_rows<E, HOW == BY_VALUE ? 1 : V>(p, c);
         return;
     }
+    const bool many = p.gather && c.whole && c.len == 1;
+    if (many) {
+        c.len = gather_rows(p, c, gathered);
+        if (c.len == 0) return;
+    }
+    auto row_of = [&](int t) { return many ? (int64_t) gathered[t] : c.row + (int64_t) t; };
     const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     char * xs = lds + wave * (X_BYTES + A_BYTES), * as = xs + X_BYTES;     // the wave's own
     const int row8 = lane >> 3, at8 = lane & 7;                            // 8 lanes a row
@@ -249,7 +281,7 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
         const char * x[2];
         int ar[A_LOADS];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) x[i] = p.x + (c.row + (int64_t) min(8 * i + row8, c.len - 1)) * p.x_s;
+        for (int i = 0; i < 2; ++i) x[i] = p.x + row_of(min(8 * i + row8, c.len - 1)) * p.x_s;
 #pragma unroll
         for (int i = 0; i < A_LOADS; ++i) ar[i] = min(A_ROW == 128 ? 8 * i + row8 : 16 * i + (lane >> 2), p.r - 1) * p.K;
         auto load = [&](step & s, int k0) {
@@ -290,7 +322,7 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
             use(s1, k0 + STEP);
         }
     } else {
-        const E * x = reinterpret_cast<const E *>(p.x + (c.row + (int64_t) min(col, c.len - 1)) * p.x_s);
+        const E * x = reinterpret_cast<const E *>(p.x + row_of(min(col, c.len - 1)) * p.x_s);
         for (; k0 < p.K; k0 += STEP) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -322,7 +354,7 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
         const int t = i / RP, r = i % RP;
         const float x = (sums[0][t][r] + sums[1][t][r]) * p.pre;
         sums[0][t][r] = x;
-        if (blockIdx.y == 0 && t < c.len && r < p.r) p.s[(c.row + (int64_t) t) * p.r + r] = x;
+        if (blockIdx.y == 0 && t < c.len && r < p.r) p.s[row_of(t) * p.r + r] = x;
     }
     if (!p.y) return;
     __syncthreads();
@@ -342,6 +374,7 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
         struct block {
             v4i before[2], b[A_LOADS];
         };
+        const int64_t row[2] = {row_of(min(row8, c.len - 1)), row_of(min(8 + row8, c.len - 1))};
         // B's rows of a block lie one after another; in LDS they are 16 bytes apart, where they are whole chunks
         const int row_bytes = p.r * (int) sizeof(W), chunks = 8 * V * row_bytes / 16;
         const bool whole = row_bytes % 16 == 0, aligned = p.r % V == 0;
@@ -359,10 +392,7 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
             for (int i = 0; i < A_LOADS; ++i) k.b[i] = *reinterpret_cast<const v4i *>(from + min(64 * i + lane, last) * 16);
             if (p.base) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const char * row = p.base + (c.row + (int64_t) min(8 * i + row8, c.len - 1)) * p.base_s;
-                    k.before[i] = *reinterpret_cast<const v4i *>(row + min(n0 + at8 * V, p.N - V) * (int) sizeof(E));
-                }
+                for (int i = 0; i < 2; ++i) k.before[i] = *reinterpret_cast<const v4i *>(p.base + row[i] * p.base_s + min(n0 + at8 * V, p.N - V) * (int) sizeof(E));
             }
         };
         auto use = [&](const block & k, int n0) {
@@ -375,13 +405,13 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < M; ++i) {
-                    const char * row = as + b_row(h, i) * stride;
+                    const char * from = as + b_row(h, i) * stride;
                     v4f up = {};
 #pragma unroll
                     for (int q = 0; q < Q; ++q) {
                         vec bf;
-                        if (aligned) bf = taken<E, W>(row + b_rank(q) * (int) sizeof(W), b_rank(q) < p.r);
-                        else bf = fetch<E, false>(reinterpret_cast<const W *>(row), b_rank(q), p.r);
+                        if (aligned) bf = taken<E, W>(from + b_rank(q) * (int) sizeof(W), b_rank(q) < p.r);
+                        else bf = fetch<E, false>(reinterpret_cast<const W *>(from), b_rank(q), p.r);
                         ranks<E, RT>::multiply(up, bf, s[q]);
                     }
                     *reinterpret_cast<v4f *>(xs + col * OUT + (4 * V * h + V * g + 4 * i) * 4) = up;
@@ -395,7 +425,7 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
                 __builtin_memcpy(&before, &k.before[i], 16);
 #pragma unroll
                 for (int e = 0; e < V; ++e) out[e] = (E) __builtin_fmaf(up[e], p.post, p.base ? (float) before[e] : 0.0f);
-                if (t < c.len && n < p.N) *reinterpret_cast<vec *>(p.y + (c.row + (int64_t) t) * p.y_s + (int64_t) n * (int) sizeof(E)) = out;
+                if (t < c.len && n < p.N) *reinterpret_cast<vec *>(p.y + row[i] * p.y_s + (int64_t) n * (int) sizeof(E)) = out;
             }
         };
         block b0, b1;
@@ -409,8 +439,9 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
         }
     } else {
         const bool whole = HOW == WIDE && p.r % V == 0;
-        const E * from = reinterpret_cast<const E *>(p.base + (c.row + (int64_t) col) * p.base_s);
-        E * to = reinterpret_cast<E *>(p.y + (c.row + (int64_t) col) * p.y_s);
+        const int64_t row = row_of(min(col, c.len - 1));
+        const E * from = reinterpret_cast<const E *>(p.base + row * p.base_s);
+        E * to = reinterpret_cast<E *>(p.y + row * p.y_s);
         for (; n0 < p.N; n0 += step) {
             vec before[2], bf[2][M][Q];
 #pragma unroll
@@ -418,9 +449,9 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
                 before[h] = fetch<E, HOW == WIDE>(from, p.base && col < c.len ? n0 + 4 * V * h + V * g : p.N, p.N);
 #pragma unroll
                 for (int i = 0; i < M; ++i) {
-                    const W * row = b + (int64_t) min(n0 + b_row(h, i), p.N - 1) * p.r;
+                    const W * br = b + (int64_t) min(n0 + b_row(h, i), p.N - 1) * p.r;
 #pragma unroll
-                    for (int q = 0; q < Q; ++q) bf[h][i][q] = whole ? fetch<E, true>(row, b_rank(q), p.r) : fetch<E, false>(row, b_rank(q), p.r);
+                    for (int q = 0; q < Q; ++q) bf[h][i][q] = whole ? fetch<E, true>(br, b_rank(q), p.r) : fetch<E, false>(br, b_rank(q), p.r);
                 }
             }
 #pragma unroll
@@ -657,6 +688,7 @@ struct grads_p {
     void * da, * db;
     float scale;
     int32_t w_type, n_out_blocks;
+    bool whole;                    // da and db are 16-byte aligned
 };
 
 __device__ __forceinline__ int scan64(int x) {
@@ -754,6 +786,9 @@ __global__ __launch_bounds__(1024) void adapter_prepare_kernel(grads_p p) {
     __shared__ W lds[MAX_RANK][66];
     const int strips_k = (p.K + 63) / 64, strips = strips_k + (p.N + 63) / 64;
     const int id = (blockIdx.x - 1) / strips, strip = (blockIdx.x - 1) % strips;
+    bool some = false;             // has the adapter rows?
+    for (int d = threadIdx.x; d < p.n_seqs; d += 1024) some |= p.ids[d] == id && offset(p.cu, d + 1, p.T) > offset(p.cu, d, p.T);
+    if (!__syncthreads_or(some)) return;
     const bool down = strip < strips_k;
     const int c0 = (down ? strip : strip - strips_k) * 64, C = down ? p.K : p.N, cols = min(64, C - c0);
     const int64_t first = (int64_t) id * p.r * C;
@@ -774,6 +809,27 @@ __device__ __forceinline__ void put(void * to, int64_t i, float x, int32_t type)
     if (type == NXG_TYPE_F32) static_cast<float *>(to)[i] = x;
     else if (type == NXG_TYPE_F16) static_cast<_Float16 *>(to)[i] = (_Float16) x;
     else static_cast<__bf16 *>(to)[i] = (__bf16) x;
+}
+
+template <int N>
+__device__ __forceinline__ void put(void * to, int64_t i, const float (&x)[N], int32_t type) {
+    typedef float fvec __attribute__((ext_vector_type(4)));
+    typedef _Float16 hvec __attribute__((ext_vector_type(N)));
+    typedef __bf16 bvec __attribute__((ext_vector_type(N)));
+    if (type == NXG_TYPE_F32) {
+#pragma unroll
+        for (int k = 0; k < N; k += 4) *reinterpret_cast<fvec *>(static_cast<float *>(to) + i + k) = fvec{x[k], x[k + 1], x[k + 2], x[k + 3]};
+    } else if (type == NXG_TYPE_F16) {
+        hvec v;
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = (_Float16) x[k];
+        *reinterpret_cast<hvec *>(static_cast<_Float16 *>(to) + i) = v;
+    } else {
+        bvec v;
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = (__bf16) x[k];
+        *reinterpret_cast<bvec *>(static_cast<__bf16 *>(to) + i) = v;
+    }
 }
 
 // The sum over a chunk's rows of u^T z, r x 64 V columns: u = g, z = x (dA), or u = s, z = dy (dB), 32 rows a step. A wave has 16 V columns:
@@ -909,27 +965,40 @@ __global__ __launch_bounds__(256) void adapter_grads_kernel(grads_p p) {
     const float f = down ? 1.0f : p.scale;
     float * part = c.part < 0 ? nullptr : (down ? p.part_a : p.part_b) + (int64_t) c.part * p.r * C;
     const int n = c0 + V * col;
+    if (n >= C) return;
 #pragma unroll
-    for (int j = 0; j < RT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 16 * j + 4 * g + i;
-            if (r >= p.r || n >= C) continue;
-            if (part && WIDE) {
-#pragma unroll
-                for (int v = 0; v < V; v += 4)
-                    *reinterpret_cast<v4f *>(part + (int64_t) r * C + n + v) = v4f{acc[v][j][i], acc[v + 1][j][i], acc[v + 2][j][i], acc[v + 3][j][i]} * f;
-                continue;
-            }
+    for (int j = 0; j < RT; ++j) {
+        const int r0 = 16 * j + 4 * g;
+        if (!part && !down && p.r % 4 == 0 && p.whole) {       // four ranks of a row of db
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                if (n + v >= C) continue;
-                const float x = acc[v][j][i] * f;
-                if (part) part[(int64_t) r * C + n + v] = x;
-                else if (down) put(p.da, ((int64_t) c.id * p.r + r) * C + n + v, x, p.w_type);
-                else put(p.db, ((int64_t) c.id * C + n + v) * p.r + r, x, p.w_type);
+                const float x[4] = {acc[v][j][0] * f, acc[v][j][1] * f, acc[v][j][2] * f, acc[v][j][3] * f};
+                if (r0 < p.r && n + v < C) put<4>(p.db, ((int64_t) c.id * C + n + v) * p.r + r0, x, p.w_type);
+            }
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = r0 + i;
+            if (r >= p.r) continue;
+            float x[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = acc[v][j][i] * f;
+            if (WIDE && part) {
+                put<V>(part, (int64_t) r * C + n, x, NXG_TYPE_F32);
+            } else if (WIDE && down && p.whole) {
+                put<V>(p.da, ((int64_t) c.id * p.r + r) * C + n, x, p.w_type);
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (n + v >= C) continue;
+                    if (part) part[(int64_t) r * C + n + v] = x[v];
+                    else if (down) put(p.da, ((int64_t) c.id * p.r + r) * C + n + v, x[v], p.w_type);
+                    else put(p.db, ((int64_t) c.id * C + n + v) * p.r + r, x[v], p.w_type);
+                }
             }
         }
+    }
 }
 
 // The chunks' sums of the adapters that have several, in order: a value a lane, its four waves every fourth chunk.
@@ -1039,11 +1108,14 @@ int32_t launch_rows(const char * what, adapter_p & p, int32_t type, int32_t w_ty
         else if (p.T / 64 >= (p.r > 64 && !f32 ? 1 : 2) * cus) rows = 64;
     }
     const int64_t slots = p.T / rows + (int64_t) p.n_seqs;
-    if (slots > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d n_seqs=%d is too large", what, p.T, p.n_seqs);
+    if (slots * 8 > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d n_seqs=%d is too large", what, p.T, p.n_seqs);
     const bool direct = !f32 && p.r <= 32 && slots < 4 * cus;
-    // few rows: several workgroups share out the columns, each with the down product of its own
+    // single rows of fewer adapters than rows: those that share one go together
+    p.gather = rows == 16 && p.T <= p.n_seqs && p.n_seqs > p.n;
+    const int64_t tiles = p.gather ? std::min<int64_t>(slots, p.n + p.n_seqs / 16) : slots;
+    // few tiles: several workgroups share out a tile's columns, each with the down product of its own
     int parts = 1;
-    while (p.y && rows == 16 && slots * parts * 2 <= cus && p.N > 32 * V * parts) parts *= 2;
+    while (p.y && rows == 16 && tiles * parts * 2 <= cus && p.N > 32 * V * parts) parts *= 2;
     const dim3 grid((unsigned) slots, (unsigned) parts);
     hipStream_t s = (hipStream_t) stream;
     by_types(type, w_type, [&](auto e, auto we) {
@@ -1212,6 +1284,7 @@ int32_t nxg_adapter_rows_backward(const nxg_adapter_rows_params * params, const 
     p.part_b = reinterpret_cast<float *>(w + l.part_b);
     p.da = da;
     p.db = db;
+    p.whole = (((uintptr_t) da | (uintptr_t) db) & 15) == 0;
     p.scale = a.scale;
     p.w_type = a.w_type;
     const int64_t turned = (int64_t) a.n_adapters * ((a.n_in + 63) / 64 + (a.n_out + 63) / 64);

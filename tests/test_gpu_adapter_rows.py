@@ -282,3 +282,19 @@ def test_refusals_of_the_python_side(nxg, torch, dev):
         nxg.adapter_rows(c.x[:, :32], c.a, c.b, c.cu, c.ids)
     with pytest.raises(ValueError, match="contiguous"):
         nxg.adapter_rows(c.x, c.a.transpose(1, 2), c.b, c.cu, c.ids)
+
+
+@pytest.mark.parametrize("dtype,wtype", TYPES)
+@pytest.mark.parametrize("r,n", [(16, 1), (128, 5)])
+def test_single_rows_that_share_adapters(nxg, torch, dev, dtype, wtype, r, n):
+    """Requests of one row go together by their adapters, beside empty and longer ones: the same bits as one by one."""
+    say(f"adapter_rows {dtype} {wtype} r={r}, requests of one row, {n} adapters")
+    lens = [1] * 70 + [0, 0, 0, 17, 1, 1, 0] + [1] * 200 + [0] * 40
+    ids = [(7 * i + i // 13) % (n + 1) - 1 if i % 5 else 0 for i in range(len(lens))]
+    assert sum(lens) <= len(lens) and len(lens) > n
+    c = Case(torch, dtype, wtype, lens, ids, n, r, 320, 136)
+    y, s = c.check(nxg, torch)[:2]
+    for d in (0, 1, 69, 73, 74, 100, 260):
+        rows = slice(int(c.cu[d]), int(c.cu[d + 1]))
+        one, s_one = nxg.adapter_rows(c.x[rows], c.a, c.b, [0, lens[d]], [ids[d]], c.scale, base=c.base[rows])
+        assert torch.equal(one, y[rows]) and torch.equal(s_one, s[rows]), d
