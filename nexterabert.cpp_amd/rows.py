@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 from typing import Optional
 
 import numpy as np
@@ -36,20 +37,11 @@ class _AttentionParams(ctypes.Structure):
                 ("scale", ctypes.c_float)]
 
 
-class _QkNormRopeParams(ctypes.Structure):
-    """struct nxg_qk_norm_rope_params."""
-    _fields_ = [("type", ctypes.c_int32), ("T", ctypes.c_int32), ("n_head", ctypes.c_int32), ("n_kv_head", ctypes.c_int32),
-                ("head_dim", ctypes.c_int32), ("wq", ctypes.c_void_p), ("wk", ctypes.c_void_p), ("w_type", ctypes.c_int32),
-                ("eps", ctypes.c_float), ("freq", ctypes.c_void_p), ("n_rot", ctypes.c_int32), ("layout", ctypes.c_int32),
-                ("mscale", ctypes.c_float), ("positions", ctypes.c_void_p), ("cu", ctypes.c_void_p), ("n_seqs", ctypes.c_int32)]
-
-
-class _AdapterParams(ctypes.Structure):
-    """struct nxg_adapter_rows_params."""
-    _fields_ = [("type", ctypes.c_int32), ("w_type", ctypes.c_int32), ("T", ctypes.c_int32), ("n_in", ctypes.c_int32),
-                ("n_out", ctypes.c_int32), ("rank", ctypes.c_int32), ("n_adapters", ctypes.c_int32), ("n_seqs", ctypes.c_int32),
-                ("cu", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
-                ("scale", ctypes.c_float)]
+# struct nxg_qk_norm_rope_params: type, T, n_head, n_kv_head, head_dim, wq, wk, w_type, eps, freq, n_rot, layout, mscale, positions,
+# cu, n_seqs; struct nxg_adapter_rows_params: type, w_type, T, n_in, n_out, rank, n_adapters, n_seqs, cu, ids, a, b, scale
+_qk_params = struct.Struct("@5i2PifPiif2Pi0q")
+_adapter_params = struct.Struct("@8i4Pf0q")
+_row = struct.Struct("@P2q")       # struct nxg_rows
 
 
 # The checks below are most of what a call for a few rows costs (10 to 20 us in all), so they look at each
@@ -86,7 +78,7 @@ def _type_of(t, name, allowed=None):
 
 def _device_of(t, name) -> int:
     """The tensor's device, which must be the current one."""
-    dev = t.get_device() if t.is_cuda else -1
+    dev = t.get_device()           # -1: host memory
     if dev < 0 or dev != _raw_device():
         raise ValueError(f"{name} must be a tensor on the current device")
     return dev
@@ -94,7 +86,7 @@ def _device_of(t, name) -> int:
 
 def _head_rows(t, name, dev, dtype, shape=None):
     """A [T][n_head][head_dim] tensor as the words of struct nxg_rows."""
-    if not t.is_cuda or t.get_device() != dev:
+    if t.get_device() != dev:
         raise ValueError(f"{name} must be a tensor on the current device")
     st = t.stride()
     if len(st) != 3 or (st[2] != 1 and t.shape[2] > 1):
@@ -107,16 +99,24 @@ def _head_rows(t, name, dev, dtype, shape=None):
 
 
 def _vector(t, name, n, dev, dtypes):
-    if not t.is_cuda or t.get_device() != dev:
+    if t.get_device() != dev:
         raise ValueError(f"{name} must be a tensor on the current device")
     if t.dtype not in dtypes or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor [{n}] of {' or '.join(map(str, dtypes))}")
     return t.data_ptr()
 
 
+def _float(x, name) -> float:
+    """A number that a 32-bit float can be."""
+    x = float(x)
+    if not -3.4e38 <= x <= 3.4e38:
+        raise ValueError(f"{name} must be a finite number that a 32-bit float holds")
+    return x
+
+
 def _plain_rows(t, name, dev, like=None):
     """A [T][C] tensor with values next to each other: (pointer, row stride)."""
-    if not t.is_cuda or t.get_device() != dev:
+    if t.get_device() != dev:
         raise ValueError(f"{name} must be a tensor on the current device")
     st = t.stride()
     if len(st) != 2 or (st[1] != 1 and t.shape[1] > 1):
@@ -374,42 +374,50 @@ def attention_rows_backward(dout, q, k, v, out, lse, cu_q, cu_k=None, scale: Opt
 # --- norms of queries and keys, and their rotation -----------------------------------------------
 
 def _qk_args(q, k, wq, wk, freq, cu_offsets, positions, eps, layout, mscale):
-    """(params, the words of q and k, cu, device)"""
+    """(params, q's and k's struct nxg_rows, cu, device)"""
     torch = _torch()
-    ty = _type_of(q, "q")
-    dev, dtype = _device_of(q, "q"), q.dtype
-    T, H, D = q.shape if q.dim() == 3 else (0, 0, 0)
-    words = _head_rows(q, "q", dev, dtype)
+    dtype = q.dtype
+    ty, dev = _type_of(q, "q"), _device_of(q, "q")
+    qr = _row.pack(*_head_rows(q, "q", dev, dtype))
+    T, H, D = q.shape
     half = freq.numel()
     if (k is None) != (wk is None):
         raise ValueError("give k and wk together")
-    if k is None:
-        G, kw = 0, None
-    else:
-        G = k.shape[1] if k.dim() == 3 else 0
-        words += _head_rows(k, "k", dev, dtype, torch.Size((T, G, D)))
-        if G == 0:
-            raise ValueError("k has no heads")
-    _sizes(T, H, G, D, half)
-    wt = _type_of(wq, "wq")
-    if wt != TYPE_F32 and wq.dtype != dtype:
-        raise ValueError(f"wq and wk must be float32 or {dtype}")
-    qw = _vector(wq, "wq", D, dev, (wq.dtype,))
+    G, kr = 0, None
     if k is not None:
-        kw = _vector(wk, "wk", D, dev, (wq.dtype,))
+        kr = _row.pack(*_head_rows(k, "k", dev, dtype))
+        Tk, G, Dk = k.shape
+        if Tk != T or Dk != D or G == 0:
+            raise ValueError(f"k must have shape ({T}, n_kv_head, {D})")
+    _sizes(T, H, G, D, half)
+    wdtype = wq.dtype
+    wt = _type_of(wq, "wq")
+    if wt != TYPE_F32 and wdtype != dtype:
+        raise ValueError(f"wq and wk must be float32 or {dtype}")
+    qw = _vector(wq, "wq", D, dev, (wdtype,))
+    kw = 0 if k is None else _vector(wk, "wk", D, dev, (wdtype,))
     fp = _vector(freq, "freq", half, dev, (torch.float64,))
     if layout not in ROPE_LAYOUTS:
         raise ValueError(f"layout must be one of {', '.join(ROPE_LAYOUTS)}")
     if (cu_offsets is None) == (positions is None):
         raise ValueError("give either cu_offsets or positions")
-    cu = None
+    cu, pp, cp, n_seqs = None, 0, 0, 0
     if positions is not None:
-        pp, cp, n_seqs = _vector(positions, "positions", T, dev, (torch.int32,)), None, 0
+        pp = _vector(positions, "positions", T, dev, (torch.int32,))
     else:
         cu = _offsets_arg(cu_offsets, q, dev)
-        pp, cp, n_seqs = None, cu.data_ptr(), cu.numel() - 1
-    p = _QkNormRopeParams(ty, T, H, G, D, qw, kw, wt, float(eps), fp, 2 * half, ROPE_LAYOUTS[layout], float(mscale), pp, cp, n_seqs)
-    return p, words, cu, dev
+        cp, n_seqs = cu.data_ptr(), cu.numel() - 1
+    p = _qk_params.pack(ty, T, H, G, D, qw, kw, wt, _float(eps, "eps"), fp, 2 * half, ROPE_LAYOUTS[layout], _float(mscale, "mscale"),
+                        pp, cp, n_seqs)
+    return p, qr, kr, cu, dev
+
+
+def _rows_out(t, name, dev, like):
+    """(t, its struct nxg_rows): rows of the shape and type of `like`, made where t is None."""
+    if t is None:
+        t = like.new_empty(like.shape)
+        return t, _row.pack(t.data_ptr(), *t.stride()[:2])
+    return t, _row.pack(*_head_rows(t, name, dev, like.dtype, like.shape))
 
 
 def qk_norm_rope_rows(q, k, wq, wk, freq, cu_offsets=None, positions=None, eps: float = 1e-6, layout: str = "half",
@@ -417,21 +425,11 @@ def qk_norm_rope_rows(q, k, wq, wk, freq, cu_offsets=None, positions=None, eps: 
     """The RMS norm of every head of q [T][n_head][head_dim] and k [T][n_kv_head][head_dim] (fp32, fp16 or bf16), times wq or
     wk [head_dim] (of their type or fp32), then rotary positions as rope_rows turns them. k and wk may both be None. Returns
     (q_out, k_out), which may be q and k."""
-    p, words, cu, dev = _qk_args(q, k, wq, wk, freq, cu_offsets, positions, eps, layout, mscale)
-    if q_out is None:
-        q_out = q.new_empty(q.shape)
-    words += _head_rows(q_out, "q_out", dev, q.dtype, q.shape)
-    if k is not None:
-        if k_out is None:
-            k_out = q.new_empty(k.shape)
-        words += _head_rows(k_out, "k_out", dev, q.dtype, k.shape)
-        rows = _words[4](*words)
-        qa, ka, qo, ko = range(ctypes.addressof(rows), ctypes.addressof(rows) + 4 * _ROWS_BYTES, _ROWS_BYTES)
-    else:
-        rows = _words[2](*words)
-        qa, ka, qo, ko = ctypes.addressof(rows), None, ctypes.addressof(rows) + _ROWS_BYTES, None
+    p, qr, kr, cu, dev = _qk_args(q, k, wq, wk, freq, cu_offsets, positions, eps, layout, mscale)
+    q_out, qo = _rows_out(q_out, "q_out", dev, q)
+    k_out, ko = (None, None) if k is None else _rows_out(k_out, "k_out", dev, k)
     _order_on(stream, cu, q_out, k_out)
-    _check(load_library().nxg_qk_norm_rope_rows(ctypes.byref(p), qa, ka, qo, ko, _stream_ptr(stream)), "qk_norm_rope_rows")
+    _check(load_library().nxg_qk_norm_rope_rows(p, qr, kr, qo, ko, _stream_ptr(stream)), "qk_norm_rope_rows")
     return q_out, k_out
 
 
@@ -439,8 +437,8 @@ def qk_norm_rope_rows(q, k, wq, wk, freq, cu_offsets=None, positions=None, eps: 
 def qk_norm_rope_rows_workspace_bytes(head_dim: int) -> int:
     """The workspace qk_norm_rope_rows_backward takes for heads of this size."""
     _sizes(head_dim)
-    p = _QkNormRopeParams(TYPE_F32, 0, 1, 0, head_dim, None, None, TYPE_F32, 0.0, None, 2, 0, 1.0, None, None, 0)
-    n = int(load_library().nxg_qk_norm_rope_rows_workspace_bytes(ctypes.byref(p)))
+    p = _qk_params.pack(TYPE_F32, 0, 1, 0, head_dim, 0, 0, TYPE_F32, 0.0, 0, 2, 0, 1.0, 0, 0, 0)
+    n = int(load_library().nxg_qk_norm_rope_rows_workspace_bytes(p))
     _check(-n if n < 0 else 0, "qk_norm_rope_rows_workspace_bytes")
     return n
 
@@ -451,27 +449,22 @@ def qk_norm_rope_rows_backward(dq_out, dk_out, q, k, wq, wk, freq, cu_offsets=No
     """The gradients of qk_norm_rope_rows: (dq, dk, dwq, dwk), from the gradients of its outputs and its inputs; dwq and dwk of
     wq's type. dq may be dq_out or q, dk dk_out or k. Without k and wk: dk and dwk are None. workspace: None (made for the
     call) or a uint8 device tensor of qk_norm_rope_rows_workspace_bytes(head_dim)."""
-    p, words, cu, dev = _qk_args(q, k, wq, wk, freq, cu_offsets, positions, eps, layout, mscale)
-    dtype, D = q.dtype, q.shape[2]
-    dq = q.new_empty(q.shape) if dq is None else dq
-    words += _head_rows(dq_out, "dq_out", dev, dtype, q.shape) + _head_rows(dq, "dq", dev, dtype, q.shape)
+    p, qr, kr, cu, dev = _qk_args(q, k, wq, wk, freq, cu_offsets, positions, eps, layout, mscale)
+    D = q.shape[2]
+    gq = _row.pack(*_head_rows(dq_out, "dq_out", dev, q.dtype, q.shape))
+    dq, dqr = _rows_out(dq, "dq", dev, q)
     dwq = q.new_empty(D, dtype=wq.dtype) if dwq is None else dwq
-    wqp, wkp = _vector(dwq, "dwq", D, dev, (wq.dtype,)), None
-    if k is not None:
-        dk = q.new_empty(k.shape) if dk is None else dk
-        words += _head_rows(dk_out, "dk_out", dev, dtype, k.shape) + _head_rows(dk, "dk", dev, dtype, k.shape)
+    wqp, wkp, gk, dkr = _vector(dwq, "dwq", D, dev, (wq.dtype,)), None, None, None
+    if k is None:
+        dk = dwk = None
+    else:
+        gk = _row.pack(*_head_rows(dk_out, "dk_out", dev, q.dtype, k.shape))
+        dk, dkr = _rows_out(dk, "dk", dev, k)
         dwk = q.new_empty(D, dtype=wq.dtype) if dwk is None else dwk
         wkp = _vector(dwk, "dwk", D, dev, (wq.dtype,))
-        rows = _words[6](*words)
-        qa, ka, dqo, dqa, dko, dka = range(ctypes.addressof(rows), ctypes.addressof(rows) + 6 * _ROWS_BYTES, _ROWS_BYTES)
-    else:
-        dk = dwk = None
-        rows = _words[4](*words, 0, 0, 0)
-        at = ctypes.addressof(rows)
-        qa, ka, dqo, dqa, dko, dka = at, None, at + _ROWS_BYTES, at + 2 * _ROWS_BYTES, None, None
     ws = _workspace(workspace, qk_norm_rope_rows_workspace_bytes(D), q)
     _order_on(stream, cu, dq, dk, dwq, dwk, ws)
-    _check(load_library().nxg_qk_norm_rope_rows_backward(ctypes.byref(p), dqo, dko, qa, ka, dqa, dka, wqp, wkp, ws.data_ptr(), ws.numel(),
+    _check(load_library().nxg_qk_norm_rope_rows_backward(p, gq, gk, qr, kr, dqr, dkr, wqp, wkp, ws.data_ptr(), ws.numel(),
                                                          _stream_ptr(stream)), "qk_norm_rope_rows_backward")
     return dq, dk, dwq, dwk
 
@@ -494,7 +487,9 @@ def dropout_rows(x, p: float, seed: int, offset: int = 0, step=None, residual=No
     sp = None if step is None else _vector(step, "step", 1, dev, (_torch().int64,))
     if out is None:
         out = x.new_empty((T, C))
-    op, os_ = _plain_rows(out, "out", dev, x)
+        op, os_ = out.data_ptr(), C
+    else:
+        op, os_ = _plain_rows(out, "out", dev, x)
     _order_on(stream, out)
     _check(load_library().nxg_dropout_rows(ty, xp, xs, rp, rs, T, C, float(p), seed, offset, sp, op, os_, _stream_ptr(stream)),
            "dropout_rows")
@@ -506,8 +501,8 @@ def dropout_rows(x, p: float, seed: int, offset: int = 0, step=None, residual=No
 @functools.lru_cache(maxsize=256)
 def _adapter_bytes(dev, ty, wt, T, K, N, r, n, n_seqs):
     """The backward pass's workspace for these sizes on this device."""
-    p = _AdapterParams(ty, wt, T, K, N, r, n, n_seqs, None, None, None, None, 1.0)
-    b = int(load_library().nxg_adapter_rows_backward_workspace_bytes(ctypes.byref(p)))
+    p = _adapter_params.pack(ty, wt, T, K, N, r, n, n_seqs, 0, 0, 0, 0, 1.0)
+    b = int(load_library().nxg_adapter_rows_backward_workspace_bytes(p))
     _check(-b if b < 0 else 0, "adapter_rows_backward")
     return b
 
@@ -526,28 +521,27 @@ def _ids_arg(ids, n_seqs, like, dev):
 
 
 def _adapter_args(x, a, b, cu_offsets, ids, scale):
-    """(params, cu, ids, workspace bytes, device)"""
-    ty = _type_of(x, "x")
-    dev = _device_of(x, "x")
-    wt = _type_of(a, "a")
+    """(params, (type, w_type, T, n_in, n_out, rank, n_adapters, n_seqs), cu, ids, device)"""
+    ty, dev, wt, wdtype = _type_of(x, "x"), _device_of(x, "x"), _type_of(a, "a"), a.dtype
     if wt != ty and ty != TYPE_F32:
         raise ValueError(f"a and b must have type {x.dtype}")
     for t, name in ((a, "a"), (b, "b")):
-        if not t.is_cuda or t.get_device() != dev:
+        if t.get_device() != dev:
             raise ValueError(f"{name} must be a tensor on the current device")
-        if t.dtype != a.dtype or t.dim() != 3 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous tensor of 3 dimensions and type {a.dtype}")
+        if t.dtype != wdtype or t.dim() != 3 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous tensor of 3 dimensions and type {wdtype}")
     n, r, K = a.shape
-    N = b.shape[1]
-    if b.shape[0] != n or b.shape[2] != r or x.dim() != 2 or x.shape[1] != K:
+    nb, N, rb = b.shape
+    if nb != n or rb != r or x.dim() != 2 or x.shape[1] != K:
         raise ValueError("x [T][n_in], a [n_adapters][rank][n_in] and b [n_adapters][n_out][rank] do not fit")
     T = x.shape[0]
     _sizes(T, K, N, r, n)
     cu = _offsets_arg(cu_offsets, x, dev)
     n_seqs = cu.numel() - 1
     ids = _ids_arg(ids, n_seqs, x, dev)
-    p = _AdapterParams(ty, wt, T, K, N, r, n, n_seqs, cu.data_ptr(), ids.data_ptr(), a.data_ptr(), b.data_ptr(), float(scale))
-    return p, cu, ids, dev
+    sizes = ty, wt, T, K, N, r, n, n_seqs
+    p = _adapter_params.pack(*sizes, cu.data_ptr(), ids.data_ptr(), a.data_ptr(), b.data_ptr(), _float(scale, "scale"))
+    return p, sizes, cu, ids, dev
 
 
 def _s_arg(s, T, r, dev):
@@ -569,25 +563,28 @@ def adapter_rows(x, a, b, cu_offsets, ids, scale: float = 1.0, base=None, out=No
     b_i^T, a [n_adapters][rank][n_in] and b [n_adapters][n_out][rank] of x's type (fp32 rows, as the int8 linears leave them: of any
     type). base [T][n_out]: the shared projection's rows, or None. An id that is no adapter leaves base as it is (0 without).
     Returns (out, s), s the fp32 [T][rank] rows x a_i^T, as adapter_rows_backward takes them. out may be base."""
-    p, cu, ids, dev = _adapter_args(x, a, b, cu_offsets, ids, scale)
-    T, N, r = p.T, p.n_out, p.rank
+    p, (_, _, T, _, N, r, _, _), cu, ids, dev = _adapter_args(x, a, b, cu_offsets, ids, scale)
     xp, xs = _plain_rows(x, "x", dev)
     bp, bs = (None, 0) if base is None else _rows_of_width(base, "base", dev, x.dtype, T, N)
     if out is None:
         out = x.new_empty((T, N))
-    op, os_ = _rows_of_width(out, "out", dev, x.dtype, T, N)
+        op, os_ = out.data_ptr(), N
+    else:
+        op, os_ = _rows_of_width(out, "out", dev, x.dtype, T, N)
     if s is None:
         s = x.new_empty((T, r), dtype=_torch().float32)
-    sp = _s_arg(s, T, r, dev)
+        sp = s.data_ptr()
+    else:
+        sp = _s_arg(s, T, r, dev)
     _order_on(stream, cu, ids, out, s)
-    _check(load_library().nxg_adapter_rows(ctypes.byref(p), xp, xs, bp, bs, op, os_, sp, _stream_ptr(stream)), "adapter_rows")
+    _check(load_library().nxg_adapter_rows(p, xp, xs, bp, bs, op, os_, sp, _stream_ptr(stream)), "adapter_rows")
     return out, s
 
 
 def adapter_rows_backward_workspace_bytes(x, a, b, cu_offsets, ids) -> int:
     """The workspace adapter_rows_backward takes for these arguments."""
-    p, _, _, dev = _adapter_args(x, a, b, cu_offsets, ids, 1.0)
-    return _adapter_bytes(dev, p.type, p.w_type, p.T, p.n_in, p.n_out, p.rank, p.n_adapters, p.n_seqs)
+    _, sizes, _, _, dev = _adapter_args(x, a, b, cu_offsets, ids, 1.0)
+    return _adapter_bytes(dev, *sizes)
 
 
 def adapter_rows_backward(dout, x, a, b, s, cu_offsets, ids, scale: float = 1.0, base=None, dx=None, da=None, db=None, workspace=None,
@@ -595,23 +592,23 @@ def adapter_rows_backward(dout, x, a, b, s, cu_offsets, ids, scale: float = 1.0,
     """The gradients of adapter_rows: (dx, da, db), from dout [T][n_out], its inputs and the s that it returned. base [T][n_in]: what
     dx is added to (the shared projection's part), or None; dx may be base. da and db as a and b, zeros for adapters
     that no row has. workspace: None (made for the call) or a uint8 device tensor of adapter_rows_backward_workspace_bytes."""
-    p, cu, ids, dev = _adapter_args(x, a, b, cu_offsets, ids, scale)
-    T, K, N = p.T, p.n_in, p.n_out
+    p, sizes, cu, ids, dev = _adapter_args(x, a, b, cu_offsets, ids, scale)
+    _, _, T, K, N, r, _, _ = sizes
     xp, xs = _plain_rows(x, "x", dev)
     gp, gs = _rows_of_width(dout, "dout", dev, x.dtype, T, N)
-    sp = _s_arg(s, T, p.rank, dev)
+    sp = _s_arg(s, T, r, dev)
     bp, bs = (None, 0) if base is None else _rows_of_width(base, "base", dev, x.dtype, T, K)
     dx = x.new_empty((T, K)) if dx is None else dx
     dp, ds = _rows_of_width(dx, "dx", dev, x.dtype, T, K)
     da = a.new_empty(a.shape) if da is None else da
     db = b.new_empty(b.shape) if db is None else db
     for t, like, name in ((da, a, "da"), (db, b, "db")):
-        if not t.is_cuda or t.get_device() != dev:
+        if t.get_device() != dev:
             raise ValueError(f"{name} must be a tensor on the current device")
         if t.dtype != like.dtype or t.shape != like.shape or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous tensor of type {like.dtype} and shape {tuple(like.shape)}")
-    ws = _workspace(workspace, _adapter_bytes(dev, p.type, p.w_type, T, K, N, p.rank, p.n_adapters, p.n_seqs), x)
+    ws = _workspace(workspace, _adapter_bytes(dev, *sizes), x)
     _order_on(stream, cu, ids, dx, da, db, ws)
-    _check(load_library().nxg_adapter_rows_backward(ctypes.byref(p), gp, gs, xp, xs, sp, bp, bs, dp, ds, da.data_ptr(), db.data_ptr(),
+    _check(load_library().nxg_adapter_rows_backward(p, gp, gs, xp, xs, sp, bp, bs, dp, ds, da.data_ptr(), db.data_ptr(),
                                                     ws.data_ptr(), ws.numel(), _stream_ptr(stream)), "adapter_rows_backward")
     return dx, da, db

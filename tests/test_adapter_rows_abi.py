@@ -10,6 +10,31 @@ import pytest
 P16 = 1 << 20            # an aligned address that no call here dereferences
 
 
+class QkNormRopeParams(ctypes.Structure):
+    """struct nxg_qk_norm_rope_params."""
+    _fields_ = [("type", ctypes.c_int32), ("T", ctypes.c_int32), ("n_head", ctypes.c_int32), ("n_kv_head", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("wq", ctypes.c_void_p), ("wk", ctypes.c_void_p), ("w_type", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("freq", ctypes.c_void_p), ("n_rot", ctypes.c_int32), ("layout", ctypes.c_int32),
+                ("mscale", ctypes.c_float), ("positions", ctypes.c_void_p), ("cu", ctypes.c_void_p), ("n_seqs", ctypes.c_int32)]
+
+
+class AdapterParams(ctypes.Structure):
+    """struct nxg_adapter_rows_params."""
+    _fields_ = [("type", ctypes.c_int32), ("w_type", ctypes.c_int32), ("T", ctypes.c_int32), ("n_in", ctypes.c_int32),
+                ("n_out", ctypes.c_int32), ("rank", ctypes.c_int32), ("n_adapters", ctypes.c_int32), ("n_seqs", ctypes.c_int32),
+                ("cu", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
+                ("scale", ctypes.c_float)]
+
+
+def test_words_of_the_params(nxg):
+    assert nxg.rows._qk_params.size == ctypes.sizeof(QkNormRopeParams)
+    assert nxg.rows._adapter_params.size == ctypes.sizeof(AdapterParams)
+    q = QkNormRopeParams(*range(1, 9), 0.5, *range(10, 13), 0.25, *range(14, 17))
+    assert bytes(q) == nxg.rows._qk_params.pack(*range(1, 9), 0.5, *range(10, 13), 0.25, *range(14, 17))
+    a = AdapterParams(*range(1, 13), 0.5)
+    assert bytes(a) == nxg.rows._adapter_params.pack(*range(1, 13), 0.5)
+
+
 @pytest.fixture()
 def L(nxg):
     return nxg.load_library()
@@ -34,7 +59,7 @@ def qk_params(nxg, **kw):
     d = dict(type=nxg.TYPE_BF16, T=10, n_head=4, n_kv_head=2, head_dim=64, wq=P16, wk=P16, w_type=nxg.TYPE_F32, eps=1e-6, freq=P16, n_rot=64,
              layout=0, mscale=1.0, positions=None, cu=P16, n_seqs=1)
     d.update(kw)
-    return struct(nxg.rows._QkNormRopeParams, **d)
+    return struct(QkNormRopeParams, **d)
 
 
 def qk(nxg, L, p=None, **kw):
@@ -134,7 +159,7 @@ def test_dropout_refused(nxg, L):
 def adapter_params(nxg, **kw):
     d = dict(type=nxg.TYPE_BF16, w_type=nxg.TYPE_BF16, T=10, n_in=64, n_out=128, rank=16, n_adapters=3, n_seqs=2, cu=P16, ids=P16, a=P16, b=2 * P16, scale=1.0)
     d.update(kw)
-    return struct(nxg.rows._AdapterParams, **d)
+    return struct(AdapterParams, **d)
 
 
 def adapter(nxg, L, p=None, x=3 * P16, xs=64, base=4 * P16, bs=128, y=5 * P16, ys=128, s=6 * P16):
