@@ -85,6 +85,11 @@ __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 // A barrier for LDS alone: loads from memory stay under way.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Rows that are read once leave the caches to what is read again (the weights, s and g): with ordinary loads 32,000 rows of 1,024 to
+// 1,024 take 65 us for 46 (bf16) and 114 for 87 (fp32), the gradients over 65,536 rows 70 for 50.
+template <class T>
+__device__ __forceinline__ T once(const void * p) { return __builtin_nontemporal_load(reinterpret_cast<const T *>(p)); }
+
 // x as the sum of two bf16 values: itself rounded, and what is left.
 __device__ __forceinline__ void split(const float (&x)[8], v8b & hi, v8b & lo) {
 #pragma unroll
@@ -286,7 +291,7 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
         for (int i = 0; i < A_LOADS; ++i) ar[i] = min(A_ROW == 128 ? 8 * i + row8 : 16 * i + (lane >> 2), p.r - 1) * p.K;
         auto load = [&](step & s, int k0) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) s.x[i] = *reinterpret_cast<const v4i *>(x[i] + min(k0 + at8 * V, p.K - V) * (int) sizeof(E));
+            for (int i = 0; i < 2; ++i) s.x[i] = once<v4i>(x[i] + min(k0 + at8 * V, p.K - V) * (int) sizeof(E));
 #pragma unroll
             for (int i = 0; i < A_LOADS; ++i) s.a[i] = *reinterpret_cast<const v4i *>(a + ar[i] + min(k0 + (A_ROW == 128 ? at8 : lane & 3) * WV, p.K - WV));
         };
@@ -313,56 +318,66 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
             }
         };
         step s0, s1;
-        if (k0 < p.K) load(s0, k0);
+        load(s0, k0);
         for (; k0 < p.K; k0 += 2 * STEP) {
-            if (k0 + STEP < p.K) load(s1, k0 + STEP);
+            load(s1, k0 + STEP);
             use(s0, k0);
             if (k0 + STEP >= p.K) break;
-            if (k0 + 2 * STEP < p.K) load(s0, k0 + 2 * STEP);
+            load(s0, k0 + 2 * STEP);
             use(s1, k0 + STEP);
         }
     } else {
         const E * x = reinterpret_cast<const E *>(p.x + row_of(min(col, c.len - 1)) * p.x_s);
-        for (; k0 < p.K; k0 += STEP) {
+        constexpr int BATCH = HOW == WIDE ? 8 : 2;         // operands whose loads are under way together
+        for (; k0 < p.K; k0 += BATCH / 2 * STEP) {
+            vec xf[BATCH], af[BATCH][RT];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int k = k0 + (4 * h + g) * V;
-                const vec xf = fetch<E, HOW == WIDE>(x, k, p.K);
+            for (int h = 0; h < BATCH; ++h) {
+                const int k = k0 + h / 2 * STEP + (4 * (h % 2) + g) * V;
+                xf[h] = fetch<E, HOW == WIDE>(x, k, p.K);
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
                     const int r = 16 * j + col;
-                    acc[j] = operand<E>::mul(fetch<E, HOW == WIDE>(a + (int64_t) r * p.K, r < p.r ? k : p.K, p.K), xf, acc[j]);
+                    af[h][j] = fetch<E, HOW == WIDE>(a + (int64_t) r * p.K, r < p.r ? k : p.K, p.K);
                 }
             }
+#pragma unroll
+            for (int h = 0; h < BATCH; ++h)
+#pragma unroll
+                for (int j = 0; j < RT; ++j) acc[j] = operand<E>::mul(af[h][j], xf[h], acc[j]);
         }
     }
-    // the waves' sums: 0 + 2 and 1 + 3, then both
+    // The waves' sums: 0 + 2 and 1 + 3, then both. The first columns' weights and base are under way meanwhile (start).
     typedef float row_sums[16][LD];
     row_sums * sums = reinterpret_cast<row_sums *>(lds);
-    if (HOW == THROUGH_LDS) __syncthreads();
-    for (int turn = 0; turn < 2; ++turn) {
-        if ((wave >> 1) == turn) {
-#pragma unroll
-            for (int j = 0; j < RT; ++j) {
-                v4f * to = reinterpret_cast<v4f *>(&sums[wave & 1][col][16 * j + 4 * g]);
-                *to = turn ? *to + acc[j] : acc[j];
-            }
-        }
-        __syncthreads();
-    }
-    for (int i = threadIdx.x; i < 16 * RP; i += 256) {
-        const int t = i / RP, r = i % RP;
-        const float x = (sums[0][t][r] + sums[1][t][r]) * p.pre;
-        sums[0][t][r] = x;
-        if (blockIdx.y == 0 && t < c.len && r < p.r) p.s[row_of(t) * p.r + r] = x;
-    }
-    if (!p.y) return;
-    __syncthreads();
-
     constexpr int Q = ranks<E, RT>::Q, M = V / 4;          // M results make up a lane's V columns
     typename ranks<E, RT>::vec s[Q][ranks<E, RT>::SV];
-    ranks<E, RT>::operands(s, sums[0][col], g);
-    if (HOW == THROUGH_LDS) __syncthreads();
+    auto join = [&]() {
+        if (HOW == THROUGH_LDS) lds_barrier();
+        for (int turn = 0; turn < 2; ++turn) {
+            if ((wave >> 1) == turn) {
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                    v4f * to = reinterpret_cast<v4f *>(&sums[wave & 1][col][16 * j + 4 * g]);
+                    *to = turn ? *to + acc[j] : acc[j];
+                }
+            }
+            lds_barrier();
+        }
+        for (int i = threadIdx.x; i < 16 * RP; i += 256) {
+            const int t = i / RP, r = i % RP;
+            const float x = (sums[0][t][r] + sums[1][t][r]) * p.pre;
+            sums[0][t][r] = x;
+            if (blockIdx.y == 0 && t < c.len && r < p.r) p.s[row_of(t) * p.r + r] = x;
+        }
+        lds_barrier();
+        ranks<E, RT>::operands(s, sums[0][col], g);
+        if (HOW == THROUGH_LDS) lds_barrier();
+    };
+    if (!p.y) {
+        join();
+        return;
+    }
 
     const W * b = static_cast<const W *>(p.b) + (int64_t) c.id * p.N * p.r;
     // row of B for a lane of result i of columns 4 V h .. of a block; its first rank of operand q
@@ -386,13 +401,14 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
             at[i] = q >= chunks ? -1 : 16 * (whole ? q + q / (row_bytes / 16) : q);
         }
         auto load = [&](block & k, int n0) {
+            n0 = min(n0, (p.N - 1) / (8 * V) * 8 * V);     // behind the last block: that one
             const char * from = reinterpret_cast<const char *>(b + (int64_t) n0 * p.r);
             const int last = min(chunks, (p.N - n0) * row_bytes / 16) - 1;
 #pragma unroll
             for (int i = 0; i < A_LOADS; ++i) k.b[i] = *reinterpret_cast<const v4i *>(from + min(64 * i + lane, last) * 16);
             if (p.base) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) k.before[i] = *reinterpret_cast<const v4i *>(p.base + row[i] * p.base_s + min(n0 + at8 * V, p.N - V) * (int) sizeof(E));
+                for (int i = 0; i < 2; ++i) k.before[i] = once<v4i>(p.base + row[i] * p.base_s + min(n0 + at8 * V, p.N - V) * (int) sizeof(E));
             }
         };
         auto use = [&](const block & k, int n0) {
@@ -425,16 +441,17 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
                 __builtin_memcpy(&before, &k.before[i], 16);
 #pragma unroll
                 for (int e = 0; e < V; ++e) out[e] = (E) __builtin_fmaf(up[e], p.post, p.base ? (float) before[e] : 0.0f);
-                if (t < c.len && n < p.N) *reinterpret_cast<vec *>(p.y + row[i] * p.y_s + (int64_t) n * (int) sizeof(E)) = out;
+                if (t < c.len && n < p.N) __builtin_nontemporal_store(out, reinterpret_cast<vec *>(p.y + row[i] * p.y_s + (int64_t) n * (int) sizeof(E)));
             }
         };
         block b0, b1;
-        if (n0 < p.N) load(b0, n0);
+        load(b0, n0);
+        join();
         for (; n0 < p.N; n0 += 2 * step) {
-            if (n0 + step < p.N) load(b1, n0 + step);
+            load(b1, n0 + step);
             use(b0, n0);
             if (n0 + step >= p.N) break;
-            if (n0 + 2 * step < p.N) load(b0, n0 + 2 * step);
+            load(b0, n0 + 2 * step);
             use(b1, n0 + step);
         }
     } else {
@@ -442,8 +459,8 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
         const int64_t row = row_of(min(col, c.len - 1));
         const E * from = reinterpret_cast<const E *>(p.base + row * p.base_s);
         E * to = reinterpret_cast<E *>(p.y + row * p.y_s);
-        for (; n0 < p.N; n0 += step) {
-            vec before[2], bf[2][M][Q];
+        vec before[2], bf[2][M][Q];
+        auto load = [&]() {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 before[h] = fetch<E, HOW == WIDE>(from, p.base && col < c.len ? n0 + 4 * V * h + V * g : p.N, p.N);
@@ -454,6 +471,11 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(adapter_p p) {
                     for (int q = 0; q < Q; ++q) bf[h][i][q] = whole ? fetch<E, true>(br, b_rank(q), p.r) : fetch<E, false>(br, b_rank(q), p.r);
                 }
             }
+        };
+        if (HOW == WIDE) load();
+        join();
+        for (; n0 < p.N; n0 += step) {
+            if (HOW != WIDE || n0 >= step) load();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int n = n0 + 4 * V * h + V * g;
@@ -521,7 +543,7 @@ __global__ __launch_bounds__(256, 2) void adapter_rows_tall_kernel(adapter_p p) 
         }
         auto load = [&](step & s, int k0) {
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) s.x[i] = *reinterpret_cast<const v4i *>(x[i] + min(k0 + at8 * V, p.K - V) * (int) sizeof(E));
+            for (int i = 0; i < 2 * MT; ++i) s.x[i] = once<v4i>(x[i] + min(k0 + at8 * V, p.K - V) * (int) sizeof(E));
 #pragma unroll
             for (int i = 0; i < A_LOADS; ++i) s.a[i] = *reinterpret_cast<const v4i *>(a + ar[i] + min(k0 + (A_ROW == 128 ? at8 : lane & 3) * WV, p.K - WV));
         };
@@ -605,7 +627,7 @@ __global__ __launch_bounds__(256, 2) void adapter_rows_tall_kernel(adapter_p p) 
 #pragma unroll
             for (int i = 0; i < 2 * MT; ++i) {
                 const char * row = p.base + (c.row + (int64_t) min(t0 + 8 * i + row8, c.len - 1)) * p.base_s;
-                k.before[i] = *reinterpret_cast<const v4i *>(row + min(n0 + at8 * V, p.N - V) * (int) sizeof(E));
+                k.before[i] = once<v4i>(row + min(n0 + at8 * V, p.N - V) * (int) sizeof(E));
             }
         }
     };
@@ -755,8 +777,10 @@ __device__ void plan_rows(const grads_p & p) {
         for (int k = lane; k < o.chunks && o.slot + k < p.n_slots; k += 64) {
             chunk c;
             c.id = id;
-            c.from = o.row + k * p.size;
-            c.count = min(p.size, o.rows - k * p.size);
+            // every chunks-th step of 32 rows: all workgroups go over the rows side by side
+            const int steps = (o.rows + 31) / 32, own = (steps - k + o.chunks - 1) / o.chunks;
+            c.from = o.row + 32 * k;
+            c.count = max(32 * own - (own > 0 && (own - 1) * o.chunks + k == steps - 1 ? 32 * steps - o.rows : 0), 0);
             c.part = o.chunks > 1 ? o.part + k : -1;
             p.slots[o.slot + k] = c;
         }
@@ -840,6 +864,7 @@ constexpr int CHUNK = 2048;        // rows of a chunk, at most
 template <class E, int RT, int V, bool WIDE>
 __global__ __launch_bounds__(256) void adapter_grads_kernel(grads_p p) {
     constexpr bool F32 = std::is_same<E, float>::value, F16 = std::is_same<E, _Float16>::value;
+    constexpr int DEPTH = 2;                                   // steps whose loads are under way (4: 17.9 us for 16.2)
     constexpr int RP = 16 * RT, CW = 64 * V, TP = RP / 8;      // TP: tokens of u of a thread
     constexpr int U_ROW = F32 ? 32 * 4 + 16 : 32 * 2 + 16;     // bytes of a rank's 32 rows (of one part)
     constexpr int PARTS = F32 ? 1 : 2, U_BYTES = RP * U_ROW;
@@ -860,15 +885,16 @@ __global__ __launch_bounds__(256) void adapter_grads_kernel(grads_p p) {
     const int rank = threadIdx.x % RP, tok = threadIdx.x / RP * TP;            // of u
     const float * u = (down ? p.g : p.s) + min(rank, p.r - 1);
 
-    const int doc = p.of[c.id].doc, docs = p.of[c.id].docs;
+    const int doc = p.of[c.id].doc, docs = p.of[c.id].docs, chunks = p.of[c.id].chunks;
     for (int i = threadIdx.x; i < c.count; i += 256) {
+        const int at = c.from + i / 32 * 32 * chunks + i % 32;
         int lo = doc, hi = doc + docs - 1;             // the last document that starts there or before
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (p.pos[mid] <= c.from + i) lo = mid;
+            if (p.pos[mid] <= at) lo = mid;
             else hi = mid - 1;
         }
-        rows[i] = min(max(offset(p.cu, p.order[lo], p.T) + c.from + i - p.pos[lo], 0), p.T - 1);
+        rows[i] = min(max(offset(p.cu, p.order[lo], p.T) + at - p.pos[lo], 0), p.T - 1);
     }
     __syncthreads();
 
@@ -881,23 +907,23 @@ __global__ __launch_bounds__(256) void adapter_grads_kernel(grads_p p) {
         evec z[8];
         float u[TP];
     };
-    const bool mine = c0 < C;
+    // Loads go on without a branch, behind the chunk's end as its last row, and into the registers that a step has just done with: where
+    // the compiler has to move a load's registers, it waits for the load first.
     auto load = [&](step & s, int t0) {
 #pragma unroll
         for (int k = 0; k < TP; ++k) s.u[k] = u[(int64_t) rows[min(t0 + tok + k, c.count - 1)] * p.r];
-        if (!mine) return;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const char * from = z + rows[min(t0 + 8 * g + k, c.count - 1)] * z_s;
             if constexpr (WIDE) {
-                s.z[k] = *reinterpret_cast<const evec *>(from);
+                s.z[k] = once<evec>(from);
             } else {
 #pragma unroll
                 for (int v = 0; v < V; ++v) s.z[k][v] = c0 + V * col + v < C ? reinterpret_cast<const E *>(from)[v] : (E) 0.0f;
             }
         }
     };
-    auto use = [&](step & s, int t0, int buf, int next) {
+    auto use = [&](step & s, int t0, int buf) {
         // rows behind the chunk's end, and ranks behind the last, are zeros, in both operands
         uvec hi;
 #pragma unroll
@@ -909,15 +935,12 @@ __global__ __launch_bounds__(256) void adapter_grads_kernel(grads_p p) {
             for (int k = 0; k < TP; ++k) lo[k] = (U) (s.u[k] - (float) hi[k]);
             *reinterpret_cast<uvec *>(us[buf][1] + rank * U_ROW + tok * (int) sizeof(U)) = lo;
         }
-        evec zv[8];
+        if (t0 + 32 > c.count) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            zv[k] = s.z[k];
-            if (t0 + 32 > c.count && t0 + 8 * g + k >= c.count) zv[k] = evec{};
+            for (int k = 0; k < 8; ++k)
+                if (t0 + 8 * g + k >= c.count) s.z[k] = evec{};
         }
-        if (next < c.count) load(s, next);
         lds_barrier();
-        if (!mine) return;
         if constexpr (F32) {
             v4f uv[RT][2];
 #pragma unroll
@@ -929,7 +952,7 @@ __global__ __launch_bounds__(256) void adapter_grads_kernel(grads_p p) {
 #pragma unroll
                 for (int v = 0; v < V; ++v)
 #pragma unroll
-                    for (int j = 0; j < RT; ++j) acc[v][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(uv[j][k / 4][k % 4], zv[k][v], acc[v][j], 0, 0, 0);
+                    for (int j = 0; j < RT; ++j) acc[v][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(uv[j][k / 4][k % 4], s.z[k][v], acc[v][j], 0, 0, 0);
         } else {
             v8b uh[RT], ul[RT];
 #pragma unroll
@@ -941,7 +964,7 @@ __global__ __launch_bounds__(256) void adapter_grads_kernel(grads_p p) {
             for (int v = 0; v < V; ++v) {
                 typename operand<E>::vec zc;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) zc[k] = zv[k][v];
+                for (int k = 0; k < 8; ++k) zc[k] = s.z[k][v];
                 v8b zh, zl;
                 if constexpr (F16) split(zc, zh, zl);
                 else zh = zc;
@@ -954,14 +977,18 @@ __global__ __launch_bounds__(256) void adapter_grads_kernel(grads_p p) {
             }
         }
     };
-    step s0, s1;
-    if (0 < c.count) load(s0, 0);
-    if (32 < c.count) load(s1, 32);
-    for (int t0 = 0; t0 < c.count; t0 += 64) {
-        use(s0, t0, 0, t0 + 64);
-        if (t0 + 32 < c.count) use(s1, t0 + 32, 1, t0 + 96);
+    if (c.count > 0) {
+        step ahead[DEPTH];
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) load(ahead[i], 32 * i);
+        for (int t0 = 0; t0 < c.count; t0 += 32 * DEPTH) {
+#pragma unroll
+            for (int i = 0; i < DEPTH; ++i) {
+                use(ahead[i], t0 + 32 * i, i % 2);
+                load(ahead[i], t0 + 32 * (i + DEPTH));
+            }
+        }
     }
-    if (!mine) return;
     const float f = down ? 1.0f : p.scale;
     float * part = c.part < 0 ? nullptr : (down ? p.part_a : p.part_b) + (int64_t) c.part * p.r * C;
     const int n = c0 + V * col;
@@ -1097,10 +1124,10 @@ int32_t launch_rows(const char * what, adapter_p & p, int32_t type, int32_t w_ty
     const bool w = wide(p.x, p.x_s) && (!p.base || wide(p.base, p.base_s)) && wide(p.y, p.y ? p.y_s : 0) && p.K % V == 0 && p.N % V == 0 &&
                    p.K * (int64_t) size_of(w_type) % 16 == 0 && p.N * (int64_t) p.r * size_of(w_type) % 16 == 0;
     // Which kernel, and rows of a workgroup: the larger ones read the weights less often, where that leaves work for every CU
-    // (32,768 rows of 1,024 to 1,024: bf16 rank 64 49 us with 64 rows, 70 with 16, rank 32 37 and 40; 16,384 rows of rank 64 43 and
-    // 40, of rank 128 64 and 97; fp32 rank 64 118 and 139, rank 32 110 and 92; 65,536 rows of rank 128 120 with 128 rows, 147
-    // with 64). Straight from memory: one row bf16 rank 16 5.3 us, through LDS 6.2; 8,192 rows 14.0 and 15.3; 16,384 rows 22.5
-    // and 20.6; rank 64 and fp32 are faster through LDS from one row on.
+    // (1,024 to 1,024, caches cold: 32,768 rows of bf16 rank 64 56 us with 64 rows, 82 with 16, of rank 32 45 and 50; 16,384 rows of
+    // rank 64 45 and 44, of rank 128 71 and 106; 8,192 of rank 128 67 and 54; 32,768 of fp32 rank 64 126 and 151; 65,536 of rank 128
+    // 140 with 128 rows, 172 with 64). Straight from memory: one row of bf16 rank 16 6.4 us, through LDS 8.3; 64 requests of one
+    // row 8.7 and 10.0; 2,000 rows 12.5 both; 3,500 rows 13.4 and 12.8, of rank 32 15.2 and 13.6; 8,000 rows 24.6 and 17.8.
     const bool f32 = type == NXG_TYPE_F32;
     int rows = 16;
     if (w && p.r > (f32 ? 32 : 16)) {
@@ -1109,7 +1136,7 @@ int32_t launch_rows(const char * what, adapter_p & p, int32_t type, int32_t w_ty
     }
     const int64_t slots = p.T / rows + (int64_t) p.n_seqs;
     if (slots * 8 > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d n_seqs=%d is too large", what, p.T, p.n_seqs);
-    const bool direct = !f32 && p.r <= 32 && slots < 4 * cus;
+    const bool direct = !f32 && p.r <= 32 && slots < cus / 2;
     // single rows of fewer adapters than rows: those that share one go together
     p.gather = rows == 16 && p.T <= p.n_seqs && p.n_seqs > p.n;
     const int64_t tiles = p.gather ? std::min<int64_t>(slots, p.n + p.n_seqs / 16) : slots;
