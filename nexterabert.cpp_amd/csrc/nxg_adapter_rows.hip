@@ -197,8 +197,8 @@ template <class E, int RT> struct ranks {
 };
 
 // Documents of one row that have an adapter in common, 16 at a time (197 of 64 adapters of rank 128: 54 us, one by one 81): the rows
-// of the tile's document and of those that follow it, into
-// `rows`, and their number; 0 where the document is among those of one before it. By every wave of a workgroup; ends with a barrier.
+// of the tile's document and of those that follow it, into `rows`, and their number; 0 where the document is among those of one
+// before it. By every wave of a workgroup; ends with a barrier.
 __device__ __forceinline__ int gather_rows(const adapter_p & p, const tile & c, int * rows) {
     const int lane = threadIdx.x & 63;
     auto alike = [&](int d, int end) { return d < end && p.ids[d] == c.id && offset(p.cu, d + 1, p.T) - offset(p.cu, d, p.T) == 1; };
