@@ -1351,8 +1351,9 @@ int32_t nxg_adapter_rows_backward(const nxg_adapter_rows_params * params, const 
         NXG_TRY(launch_rows(what, f, a.type, a.w_type, stream));
     }
     if (jobs == 0) return NXG_OK;
+    // V columns at a time, in what is read and in what is written: without rows their number alone decides
     const int V = 16 / es;
-    const bool wd = (!da || !some || (wide(x, p.x_s) && a.n_in % V == 0)) && (!db || !some || (wide(dy, p.dy_s) && a.n_out % V == 0));
+    const bool wd = (!da || (a.n_in % V == 0 && (!some || wide(x, p.x_s)))) && (!db || (a.n_out % V == 0 && (!some || wide(dy, p.dy_s))));
     by_type(a.type, [&](auto e) {
         typedef decltype(e) E;
         by_rank(a.rank, [&](auto rt) {
