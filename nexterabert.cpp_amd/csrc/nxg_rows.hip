@@ -102,8 +102,12 @@ __device__ __forceinline__ void find_turns(float2 * turn, const P & p, int t0, i
         if (p.positions) {
             pos = p.positions[t];
         } else {
-            int d = first;
-            while (d + 1 < p.n_seqs && p.cu[d + 1] <= t) ++d;
+            // steps of 1, 2, 4, .. documents on, then halves: one load where the row is in the first, 2 log2(n) behind n empty ones
+            uint32_t d = first, step = 1;
+            const uint32_t n = p.n_seqs;
+            for (; d + step < n && p.cu[d + step] <= t; step *= 2) d += step;
+            while (step /= 2)
+                if (d + step < n && p.cu[d + step] <= t) d += step;
             pos = t - p.cu[d];
         }
         const double turns = (double) pos * f * 0.15915494309189533577;   // 1 / (2 pi)
