@@ -120,6 +120,7 @@ struct adapter_p {
     int32_t T, K, N, r, n, n_seqs;
     float pre, post;               // factors on s and on the second product
     bool gather;                   // documents of one row that share an adapter go together
+    int32_t window;                // among so many of them
 };
 
 struct tile {
@@ -198,16 +199,17 @@ template <class E, int RT> struct ranks {
 
 // Documents of one row that have an adapter in common, 16 at a time (197 of 64 adapters of rank 128: 54 us, one by one 81): the rows
 // of the tile's document and of those that follow it, into `rows`, and their number; 0 where the document is among those of one
-// before it. By every wave of a workgroup; ends with a barrier.
+// before it. They are looked for in a window of documents, so that what a workgroup looks over does not grow with their number.
+// By every wave of a workgroup; ends with a barrier.
 __device__ __forceinline__ int gather_rows(const adapter_p & p, const tile & c, int * rows) {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, first = c.doc / p.window * p.window, end = min(first + p.window, p.n_seqs);
     auto alike = [&](int d, int end) { return d < end && p.ids[d] == c.id && offset(p.cu, d + 1, p.T) - offset(p.cu, d, p.T) == 1; };
     int before = 0, found = 1;
-    for (int d = 0; d < c.doc; d += 64) before += __popcll(__ballot(alike(d + lane, c.doc)));
+    for (int d = first; d < c.doc; d += 256) before += __syncthreads_count(alike(d + threadIdx.x, c.doc));
     if (before % 16) return 0;
     if (threadIdx.x == 0) rows[0] = c.row;
-    for (int d = c.doc + 1; d < p.n_seqs && found < 16; d += 64) {
-        const bool mine = alike(d + lane, p.n_seqs);
+    for (int d = c.doc + 1; d < end && found < 16; d += 64) {
+        const bool mine = alike(d + lane, end);
         const uint64_t all = __ballot(mine);
         const int at = found + __popcll(all & ((1ull << lane) - 1));
         if (mine && at < 16 && threadIdx.x < 64) rows[at] = offset(p.cu, d + lane, p.T);
@@ -1066,6 +1068,7 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(grads_p p) {
 #define NXG_TRY(call) do { const int32_t rc_ = (call); if (rc_) return rc_; } while (0)
 
 constexpr int64_t MAX_GRID = (1 << 24) - 1;    // workgroups of a launch: less than 2^32 threads
+constexpr int MAX_WINDOW = 4096;               // of documents among which single rows are gathered
 
 int size_of(int32_t type) { return type == NXG_TYPE_F32 ? 4 : type == NXG_TYPE_F16 || type == NXG_TYPE_BF16 ? 2 : 0; }
 
@@ -1143,9 +1146,14 @@ int32_t launch_rows(const char * what, adapter_p & p, int32_t type, int32_t w_ty
     const int64_t slots = p.T / rows + (int64_t) p.n_seqs;
     if (slots * 8 > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d n_seqs=%d is too large", what, p.T, p.n_seqs);
     const bool direct = !f32 && p.r <= 32 && slots < cus / 2;
-    // single rows of fewer adapters than rows: those that share one go together
-    p.gather = rows == 16 && p.T <= p.n_seqs && p.n_seqs > p.n;
-    const int64_t tiles = p.gather ? std::min<int64_t>(slots, p.n + p.n_seqs / 16) : slots;
+    // Single rows, two an adapter on the average: those that share one go together (fp32, ids by chance, together and one by one: 65 rows of
+    // 64 adapters of rank 16 11.0 and 10.3 us, of rank 128 both 35; 1,000 rows of 512 30 and 28, 131 and 161; 4,096 rows of 64 45 and 73,
+    // 167 and 678). The window: so that 16 rows of an adapter are in it, but no larger than keeps its search short (16,384 rows of 512
+    // adapters of rank 16 200, 162 and 200 us with 1,024, 4,096 and 8,192 documents, of rank 128 1,609, 926 and 1,062).
+    p.gather = rows == 16 && p.T <= p.n_seqs && p.n_seqs / 2 >= p.n;
+    p.window = 1024;
+    while (p.window < MAX_WINDOW && p.window < 16 * (int64_t) p.n) p.window *= 2;
+    const int64_t tiles = p.gather ? std::min<int64_t>(slots, (p.n_seqs + p.window - 1) / p.window * (int64_t) p.n + p.n_seqs / 16) : slots;
     // few tiles: several workgroups share out a tile's columns, each with the down product of its own
     int parts = 1;
     while (p.y && rows == 16 && tiles * parts * 2 <= cus && p.N > 32 * V * parts) parts *= 2;

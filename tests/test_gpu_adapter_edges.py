@@ -67,3 +67,47 @@ def check(bufs):
     for buf, t, inside in bufs:
         assert (t == 0).all()
         assert (buf[:inside.start] == 7).all() and (buf[inside.stop:] == 7).all()
+
+
+def single_rows(torch, dtype, n, r, S, extra=()):
+    """Arguments of a call of S documents of one row of n adapters, and of documents of the `extra` lengths behind them."""
+    g = torch.Generator(device="cuda").manual_seed(S)
+    T = S + sum(extra)
+    x, base = (torch.randn(T, c, device="cuda", generator=g).to(getattr(torch, dtype)) for c in (64, 72))
+    a, b = torch.randn(n, r, 64, device="cuda", generator=g).to(x.dtype) / 8, torch.randn(n, 72, r, device="cuda", generator=g).to(x.dtype)
+    ids = torch.randint(-1, n, (S + len(extra),), device="cuda", dtype=torch.int32, generator=g)
+    cu = torch.cumsum(torch.tensor([0] + [1] * S + list(extra), device="cuda"), 0).int()
+    return x, a, b, cu, ids, 1.5, base
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("S,n", [(1023, 5), (1024, 300), (1025, 1), (5000, 300), (9001, 16), (20000, 3000), (40000, 70)])
+def test_single_rows_gathered_or_not(nxg, torch, dev, dtype, S, n):
+    """More rows than one search for an adapter's goes over: the same bits as in a call that takes every row by itself, which a longer
+    document behind them makes of it."""
+    print(f"adapter_rows {dtype} {S} documents of one row, {n} adapters", flush=True)
+    x, a, b, cu, ids, scale, base = single_rows(torch, dtype, n, 16, S, (3,))
+    y, s = nxg.adapter_rows(x[:S], a, b, cu[:S + 1], ids[:S], scale, base=base[:S])
+    want, s_want = nxg.adapter_rows(x, a, b, cu, ids, scale, base=base)
+    assert torch.equal(y, want[:S]) and torch.equal(s, s_want[:S])
+    none = (ids[:S] < 0).nonzero()[:, 0]
+    assert torch.equal(y[none], base[:S][none]) and (s[none] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,r,n", [("float32", 16, 16), ("float32", 8, 64), ("bfloat16", 16, 16)])
+def test_time_of_single_rows(nxg, torch, dev, dtype, r, n):
+    """8 times the rows take about 8 times as long, not 64."""
+    print(f"adapter_rows {dtype} r={r}: 4,096 and 32,768 documents of one row, {n} adapters", flush=True)
+    ms = []
+    for S in (4096, 32768):
+        args = single_rows(torch, dtype, n, r, S)
+        best = float("inf")
+        for _ in range(6):
+            t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            t[0].record()
+            nxg.adapter_rows(*args[:6], base=args[6])
+            t[1].record()
+            torch.cuda.synchronize()
+            best = min(best, t[0].elapsed_time(t[1]))
+        ms.append(best)
+    assert ms[1] < 12 * ms[0], ms
