@@ -1139,8 +1139,12 @@ int32_t launch_rows(const char * what, adapter_p & p, int32_t type, int32_t w_ty
     // row 8.7 and 10.0; 2,000 rows 12.5 both; 3,500 rows 13.4 and 12.8, of rank 32 15.2 and 13.6; 8,000 rows 24.6 and 17.8.
     const bool f32 = type == NXG_TYPE_F32;
     int rows = 16;
-    if (w && p.r > (f32 ? 32 : 16)) {
-        if (p.r > 64 && p.T / 128 >= 2 * cus) rows = 128;
+    // A tile's rows are of one document, so that the documents have to be long enough on the average, too (8 adapters, with 64 rows and
+    // with 16: 65,536 rows of bf16 rank 64 in documents of 48 rows 114 and 200 us, of 32 143 and 164, of 16 226 and 281, of 8 406 and 285,
+    // of 1 2,928 and 583; 32,768 of fp32 rank 128 of 48 rows 279 and 435, of 32 468 and 356, of 1 10,051 and 852).
+    const int mean = p.T / p.n_seqs;
+    if (w && p.r > (f32 ? 32 : 16) && mean >= (f32 ? 48 : 32)) {
+        if (p.r > 64 && p.T / 128 >= 2 * cus && mean >= 128) rows = 128;
         else if (p.T / 64 >= (p.r > 64 && !f32 ? 1 : 2) * cus) rows = 64;
     }
     const int64_t slots = p.T / rows + (int64_t) p.n_seqs;

@@ -69,12 +69,12 @@ def check(bufs):
         assert (buf[:inside.start] == 7).all() and (buf[inside.stop:] == 7).all()
 
 
-def single_rows(torch, dtype, n, r, S, extra=()):
+def single_rows(torch, dtype, n, r, S, extra=(), n_in=256, n_out=264):
     """Arguments of a call of S documents of one row of n adapters, and of documents of the `extra` lengths behind them."""
     g = torch.Generator(device="cuda").manual_seed(S)
     T = S + sum(extra)
-    x, base = (torch.randn(T, c, device="cuda", generator=g).to(getattr(torch, dtype)) for c in (64, 72))
-    a, b = torch.randn(n, r, 64, device="cuda", generator=g).to(x.dtype) / 8, torch.randn(n, 72, r, device="cuda", generator=g).to(x.dtype)
+    x, base = (torch.randn(T, c, device="cuda", generator=g).to(getattr(torch, dtype)) for c in (n_in, n_out))
+    a, b = torch.randn(n, r, n_in, device="cuda", generator=g).to(x.dtype) / 16, torch.randn(n, n_out, r, device="cuda", generator=g).to(x.dtype)
     ids = torch.randint(-1, n, (S + len(extra),), device="cuda", dtype=torch.int32, generator=g)
     cu = torch.cumsum(torch.tensor([0] + [1] * S + list(extra), device="cuda"), 0).int()
     return x, a, b, cu, ids, 1.5, base
@@ -94,6 +94,18 @@ def test_single_rows_gathered_or_not(nxg, torch, dev, dtype, S, n):
     assert torch.equal(y[none], base[:S][none]) and (s[none] == 0).all()
 
 
+def fastest(torch, call):
+    best = float("inf")
+    for _ in range(6):
+        t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        t[0].record()
+        call()
+        t[1].record()
+        torch.cuda.synchronize()
+        best = min(best, t[0].elapsed_time(t[1]))
+    return best
+
+
 @pytest.mark.parametrize("dtype,r,n", [("float32", 16, 16), ("float32", 8, 64), ("bfloat16", 16, 16)])
 def test_time_of_single_rows(nxg, torch, dev, dtype, r, n):
     """8 times the rows take about 8 times as long, not 64."""
@@ -101,13 +113,18 @@ def test_time_of_single_rows(nxg, torch, dev, dtype, r, n):
     ms = []
     for S in (4096, 32768):
         args = single_rows(torch, dtype, n, r, S)
-        best = float("inf")
-        for _ in range(6):
-            t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
-            t[0].record()
-            nxg.adapter_rows(*args[:6], base=args[6])
-            t[1].record()
-            torch.cuda.synchronize()
-            best = min(best, t[0].elapsed_time(t[1]))
-        ms.append(best)
+        ms.append(fastest(torch, lambda: nxg.adapter_rows(*args[:6], base=args[6])))
+    assert ms[1] < 12 * ms[0], ms
+
+
+@pytest.mark.parametrize("dtype,r,T", [("bfloat16", 32, 32768), ("bfloat16", 64, 32768), ("bfloat16", 128, 65536), ("float32", 128, 65536)])
+@pytest.mark.parametrize("length", [1, 6])
+def test_time_of_short_documents(nxg, torch, dev, dtype, r, T, length):
+    """A launch of many rows does not take a tile of 64 or 128 of them for every short document: 8 times the rows, about 8 times as long."""
+    print(f"adapter_rows {dtype} r={r}: {T // 8} and {T} rows, {length} a document", flush=True)
+    ms = []
+    for rows in (T // 8, T):
+        x, a, b, cu, ids, scale, base = single_rows(torch, dtype, 8, r, rows // length * length)
+        cu, ids = cu[::length].contiguous(), ids[:rows // length]
+        ms.append(fastest(torch, lambda: nxg.adapter_rows(x, a, b, cu, ids, scale, base=base)))
     assert ms[1] < 12 * ms[0], ms
