@@ -706,6 +706,7 @@ struct grads_p {
     const void * a, * b;           // [n][r][K], [n][N][r]
     void * at, * bt;               // [n][K][r], [n][r][N]
     int32_t * order, * pos;        // the documents by adapter, and their first rows' places in that order
+    int32_t * counts, runs;        // [runs][n], for the plan: runs of documents, a wave's each
     chunk * slots;
     adapter_rows_of * of;
     const char * x, * dy;
@@ -718,107 +719,181 @@ struct grads_p {
     bool whole;                    // da and db are 16-byte aligned
 };
 
+// The sum of x over a wave's lanes up to this one: within rows of 16, then the last of a row to the next, of two to the others.
 __device__ __forceinline__ int scan64(int x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int k = 1; k < 64; k *= 2) {
-        const int y = __shfl_up(x, k);
-        x += lane >= k ? y : 0;
-    }
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
     return x;
 }
 
-// Who has which rows: by one workgroup, a wave an adapter. Sums are kept at most T, so that offsets that do not rise
-// make no place past the arrays.
-__device__ void plan_rows(const grads_p & p) {
+// The sums of N values over the threads of `waves` waves before this one, and over all of them; a wave's own sum counts as `most` at most.
+template <int N>
+__device__ __forceinline__ void scan_all(int (&x)[N], int (&total)[N], int most, int (*sums)[16], int waves) {
     const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    auto length = [&](int d, int id) {
-        return d < p.n_seqs && p.ids[d] == id ? max(offset(p.cu, d + 1, p.T) - offset(p.cu, d, p.T), 0) : -1;
-    };
-    for (int id = wave; id < p.n; id += 16) {
-        int rows = 0, docs = 0;
-        for (int d0 = 0; d0 < p.n_seqs; d0 += 64) {
-            const int len = length(d0 + lane, id);
-            docs += __popcll(__ballot(len >= 0));
-            rows = min(rows + uni(__shfl(scan64(max(len, 0)), 63)), p.T);
-        }
-        if (lane == 0) {
-            p.of[id].rows = rows;
-            p.of[id].docs = docs;
-        }
+    int upto[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) upto[i] = scan64(x[i]);
+    __syncthreads();
+    if (lane == 63) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) sums[i][wave] = min(upto[i], most);
     }
     __syncthreads();
-    if (wave == 0) {
-        int row = 0, doc = 0, slot = 0, part = 0;
-        for (int i0 = 0; i0 < p.n; i0 += 64) {
-            const int id = i0 + lane;
-            const int rows = id < p.n ? p.of[id].rows : 0, docs = id < p.n ? p.of[id].docs : 0;
-            // 64 times T is below 2^31
-            const int upto = min(row + scan64(rows), p.T), here = min(row + scan64(rows) - rows, p.T);
-            const int chunks = id < p.n ? max((upto - here + p.size - 1) / p.size, 1) : 0, parts = chunks > 1 ? chunks : 0;
-            const int d = doc + scan64(docs), c = slot + scan64(chunks), q = part + scan64(parts);
-            if (id < p.n) {
-                adapter_rows_of o;
-                o.row = here;
-                o.rows = upto - here;
-                o.doc = d - docs;
-                o.docs = docs;
-                o.slot = c - chunks;
-                o.part = q - parts;
-                o.chunks = chunks;
-                o.unused = 0;
-                p.of[id] = o;
-            }
-            row = uni(__shfl(upto, 63));
-            doc = uni(__shfl(d, 63));
-            slot = uni(__shfl(c, 63));
-            part = uni(__shfl(q, 63));
-        }
-        for (int k = slot + lane; k < p.n_slots; k += 64) p.slots[k].id = -1;
-    }
-    __syncthreads();
-    for (int id = wave; id < p.n; id += 16) {
-        const adapter_rows_of o = p.of[id];
-        for (int k = lane; k < o.chunks && o.slot + k < p.n_slots; k += 64) {
-            chunk c;
-            c.id = id;
-            // every chunks-th step of 32 rows: all workgroups go over the rows side by side
-            const int steps = (o.rows + 31) / 32, own = (steps - k + o.chunks - 1) / o.chunks;
-            c.from = o.row + 32 * k;
-            c.count = max(32 * own - (own > 0 && (own - 1) * o.chunks + k == steps - 1 ? 32 * steps - o.rows : 0), 0);
-            c.part = o.chunks > 1 ? o.part + k : -1;
-            p.slots[o.slot + k] = c;
-        }
-        int rows = 0, docs = 0;
-        for (int d0 = 0; d0 < p.n_seqs; d0 += 64) {
-            const int len = length(d0 + lane, id);
-            const uint64_t mine = __ballot(len >= 0);
-            const int upto = scan64(max(len, 0));
-            if (len >= 0) {
-                const int k = o.doc + docs + __popcll(mine & ((1ull << lane) - 1));
-                p.order[k] = d0 + lane;
-                p.pos[k] = o.row + min(rows + upto - len, o.rows);
-            }
-            docs += __popcll(mine);
-            rows = min(rows + uni(__shfl(upto, 63)), p.T);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        x[i] = upto[i] - x[i];
+        total[i] = 0;
+        for (int w = 0; w < waves; ++w) {
+            const int sum = sums[i][w];
+            x[i] += w < wave ? sum : 0;
+            total[i] += sum;
         }
     }
 }
 
+// Who has which rows, by one workgroup: the documents sorted by adapter, an adapter's in their own order, by counting. Every wave counts
+// a run of documents for itself, then, from where its run's first of each adapter goes, places them; so the work goes by the
+// documents and the adapters, and not by their product. Sums are kept at most T, so that offsets that do not rise make no place
+// past the arrays. `room`: of lds, for the counts and then the documents' lengths where they fit.
+__device__ __forceinline__ void plan_rows(const grads_p & p, int * lds, int room, int (*sums)[16]) {
+    const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    // few documents and adapters: one wave, whose barriers wait for no other
+    const int waves = p.n_seqs <= 64 && p.n <= 64 ? 1 : 16, threads = 64 * waves;
+    if (wave >= waves) return;
+    const int64_t n_counts = p.runs * (int64_t) p.n;
+    const bool inside = n_counts + p.n_seqs <= room;
+    int * counts = inside ? lds : p.counts;                // [runs][n]
+    int * lens = inside ? lds + n_counts : p.pos;          // of the documents in their order
+    int * mine = counts + (int64_t) wave * p.n;
+    // the wave's documents, none of them behind the last run
+    const int run = (p.n_seqs + 64 * p.runs - 1) / (64 * p.runs) * 64;
+    const int first = wave < p.runs ? min(wave * run, p.n_seqs) : p.n_seqs, end = wave < p.runs ? min(first + run, p.n_seqs) : p.n_seqs;
+    const int bits = p.n > 1 ? 32 - __clz(p.n - 1) : 0;
+    // a lane's document: its adapter (-1: none), its rows, and the lanes with the same adapter
+    int id, len;
+    uint64_t same;
+    auto take = [&](int d) {
+        id = d < end ? p.ids[d] : -1;
+        len = d < end ? max(offset(p.cu, d + 1, p.T) - offset(p.cu, d, p.T), 0) : 0;
+        if (id < 0 || id >= p.n) id = -1;
+        same = __ballot(id >= 0);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t ones = __ballot(id >> b & 1);
+            same &= id >> b & 1 ? ones : ~ones;
+        }
+    };
+    for (int64_t i = threadIdx.x; i < n_counts; i += threads) counts[i] = 0;
+    __syncthreads();
+    for (int d = first; d < end; d += 64) {
+        take(d + lane);
+        if (id >= 0 && (same & ((1ull << lane) - 1)) == 0) mine[id] += __popcll(same);
+        __threadfence_block();             // the next step's lanes are others
+    }
+    __syncthreads();
+    int docs_all = 0, doc = 0, docs = 0;   // of every adapter, and of a thread's: the first, and their number
+    for (int i0 = 0; i0 < p.n; i0 += threads) {
+        const int i = i0 + threadIdx.x;
+        docs = 0;
+        for (int w = 0; w < p.runs && i < p.n; ++w) docs += counts[(int64_t) w * p.n + i];
+        int before[1] = {docs}, total[1];
+        scan_all(before, total, INT32_MAX, sums, waves);
+        doc = docs_all + before[0];
+        docs_all += total[0];
+        if (i >= p.n) continue;
+        p.of[i].doc = doc;
+        p.of[i].docs = docs;
+        int k = doc;
+        for (int w = 0; w < p.runs; ++w) {
+            int & c = counts[(int64_t) w * p.n + i];
+            const int here = c;
+            c = k;
+            k += here;
+        }
+    }
+    __syncthreads();
+    for (int d = first; d < end; d += 64) {
+        if (run > 64) take(d + lane);      // else they are those of before
+        const int before = __popcll(same & ((1ull << lane) - 1)), k = id >= 0 ? mine[id] : 0;
+        __threadfence_block();
+        if (id >= 0 && before == 0) mine[id] = k + __popcll(same);
+        if (id >= 0) {
+            p.order[k + before] = d + lane;
+            lens[k + before] = len;
+        }
+        __threadfence_block();
+    }
+    __syncthreads();
+    int rows_all = 0;
+    for (int k0 = 0; k0 < docs_all; k0 += threads) {
+        const int k = k0 + threadIdx.x;
+        int before[1] = {k < docs_all ? lens[k] : 0}, total[1];
+        scan_all(before, total, p.T, sums, waves);
+        if (k < docs_all) p.pos[k] = lens[k] = min(rows_all + before[0], p.T);
+        rows_all = min(rows_all + total[0], p.T);
+    }
+    __syncthreads();
+    int slots = 0, parts = 0;
+    for (int i0 = 0; i0 < p.n; i0 += threads) {
+        const int i = i0 + threadIdx.x;
+        adapter_rows_of o = {};
+        if (i < p.n) {
+            o.doc = p.n > threads ? p.of[i].doc : doc;
+            o.docs = p.n > threads ? p.of[i].docs : docs;
+            o.row = o.doc < docs_all ? lens[o.doc] : rows_all;
+            o.rows = (o.doc + o.docs < docs_all ? lens[o.doc + o.docs] : rows_all) - o.row;
+            o.chunks = max((o.rows + p.size - 1) / p.size, 1);
+        }
+        int before[2] = {o.chunks, o.chunks > 1 ? o.chunks : 0}, total[2];
+        scan_all(before, total, INT32_MAX, sums, waves);
+        o.slot = slots + before[0];
+        o.part = parts + before[1];
+        slots += total[0];
+        parts += total[1];
+        if (i < p.n) p.of[i] = o;
+        // Every chunks-th step of 32 rows: all workgroups go over the rows side by side. Adapters of one chunk a lane, others a wave.
+        if (i < p.n && o.chunks == 1 && o.slot < p.n_slots) p.slots[o.slot] = chunk{i, o.row, o.rows, -1};
+        for (uint64_t left = __ballot(o.chunks > 1); left; left &= left - 1) {
+            const int l = __ffsll((unsigned long long) left) - 1;
+            const int chunks = __shfl(o.chunks, l), rows = __shfl(o.rows, l), row = __shfl(o.row, l), slot = __shfl(o.slot, l),
+                      part = __shfl(o.part, l), steps = (rows + 31) / 32;
+            for (int k = lane; k < chunks && slot + k < p.n_slots; k += 64) {
+                const int own = (steps - k + chunks - 1) / chunks;
+                const int count = max(32 * own - (own > 0 && (own - 1) * chunks + k == steps - 1 ? 32 * steps - rows : 0), 0);
+                p.slots[slot + k] = chunk{i - lane + l, row + 32 * k, count, part + k};
+            }
+        }
+    }
+    for (int k = slots + (int) threadIdx.x; k < p.n_slots; k += threads) p.slots[k].id = -1;
+}
+
 // The first workgroup: plan_rows. Each other one: 64 columns of one adapter's down weights, or 64 rows of its up weights, turned round.
-// 4 adapters of rank 16, 32 documents: 4.5 us, the plan's chain of loads.
+// Those go over the documents to see whether their adapter has rows; where documents times adapters are more than FEW_PAIRS they are a
+// launch of their own behind the plan, which says so (gradients of 4,096 documents with 64 adapters of rank 16 117 us in one launch and
+// 128 in two, of 1,000 with 1,000 363 and 334, of 4,096 with 1,000 458 and 392).
+// 4 adapters of rank 16, 32 documents: 4.3 us, the plan's chain of loads.
+constexpr int64_t FEW_PAIRS = 1 << 19;
+enum { PLAN = 1, TURN = 2 };
 template <class W>
-__global__ __launch_bounds__(1024) void adapter_prepare_kernel(grads_p p) {
-    if (blockIdx.x == 0) {
-        plan_rows(p);
+__global__ __launch_bounds__(1024) void adapter_prepare_kernel(grads_p p, int what) {
+    __shared__ __align__(16) W lds[MAX_RANK][66];
+    __shared__ int sums[2][16];
+    if ((what & PLAN) && blockIdx.x == 0) {
+        plan_rows(p, reinterpret_cast<int *>(lds), sizeof(lds) / sizeof(int), sums);
         return;
     }
-    __shared__ W lds[MAX_RANK][66];
-    const int strips_k = (p.K + 63) / 64, strips = strips_k + (p.N + 63) / 64;
-    const int id = (blockIdx.x - 1) / strips, strip = (blockIdx.x - 1) % strips;
-    bool some = false;             // has the adapter rows?
-    for (int d = threadIdx.x; d < p.n_seqs; d += 1024) some |= p.ids[d] == id && offset(p.cu, d + 1, p.T) > offset(p.cu, d, p.T);
-    if (!__syncthreads_or(some)) return;
+    const int strips_k = (p.K + 63) / 64, strips = strips_k + (p.N + 63) / 64, job = blockIdx.x - (what & PLAN ? 1 : 0);
+    const int id = job / strips, strip = job % strips;
+    if (what & PLAN) {
+        bool some = false;         // has the adapter rows?
+        for (int d = threadIdx.x; d < p.n_seqs; d += 1024) some |= p.ids[d] == id && offset(p.cu, d + 1, p.T) > offset(p.cu, d, p.T);
+        if (!__syncthreads_or(some)) return;
+    } else if (p.of[id].rows == 0) {
+        return;
+    }
     const bool down = strip < strips_k;
     const int c0 = (down ? strip : strip - strips_k) * 64, C = down ? p.K : p.N, cols = min(64, C - c0);
     const int64_t first = (int64_t) id * p.r * C;
@@ -1188,7 +1263,8 @@ int32_t launch_rows(const char * what, adapter_p & p, int32_t type, int32_t w_ty
 struct layout {
     int size, cw;                  // rows of a chunk, columns of a slab
     int64_t n_slots, n_parts;
-    int64_t order, pos, slots, of, at, bt, g, part_a, part_b, bytes;
+    int64_t order, pos, counts, slots, of, at, bt, g, part_a, part_b, bytes;
+    int runs;                      // of documents, in the plan
 };
 layout plan_backward(const nxg_adapter_rows_params & p) {
     layout l;
@@ -1209,6 +1285,8 @@ layout plan_backward(const nxg_adapter_rows_params & p) {
     };
     l.order = take(4 * (int64_t) p.n_seqs);
     l.pos = take(4 * (int64_t) p.n_seqs);
+    l.runs = std::min(16, std::max(1, (p.n_seqs + 63) / 64));
+    l.counts = take(4 * (int64_t) l.runs * p.n_adapters);
     l.slots = take((int64_t) sizeof(chunk) * l.n_slots);
     l.of = take((int64_t) sizeof(adapter_rows_of) * p.n_adapters);
     l.at = take((int64_t) p.n_adapters * p.rank * p.n_in * ws);
@@ -1317,6 +1395,8 @@ int32_t nxg_adapter_rows_backward(const nxg_adapter_rows_params * params, const 
     p.bt = w + l.bt;
     p.order = reinterpret_cast<int32_t *>(w + l.order);
     p.pos = reinterpret_cast<int32_t *>(w + l.pos);
+    p.counts = reinterpret_cast<int32_t *>(w + l.counts);
+    p.runs = l.runs;
     p.slots = reinterpret_cast<chunk *>(w + l.slots);
     p.of = reinterpret_cast<adapter_rows_of *>(w + l.of);
     p.x = static_cast<const char *>(x);
@@ -1337,8 +1417,16 @@ int32_t nxg_adapter_rows_backward(const nxg_adapter_rows_params * params, const 
     if (turned >= MAX_GRID || jobs > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d n_adapters=%d is too large", what, a.T, a.n_adapters);
     NXG_TRY(nxg_check_device());
     hipStream_t st = (hipStream_t) stream;
-    by_type(a.w_type, [&](auto we) { adapter_prepare_kernel<decltype(we)><<<(unsigned) (some ? 1 + turned : 1), 1024, 0, st>>>(p); });
-    NXG_TRY(nxg_launch_check(what));
+    auto prepare = [&](int64_t grid, int parts) {
+        by_type(a.w_type, [&](auto we) { adapter_prepare_kernel<decltype(we)><<<(unsigned) grid, 1024, 0, st>>>(p, parts); });
+        return nxg_launch_check(what);
+    };
+    if (some && p.n_seqs * (int64_t) p.n <= FEW_PAIRS) {
+        NXG_TRY(prepare(1 + turned, PLAN | TURN));
+    } else {
+        NXG_TRY(prepare(1, PLAN));
+        if (some) NXG_TRY(prepare(turned, TURN));
+    }
     if (some && (dx || da)) {
         adapter_p f = {};
         f.x = p.dy;

@@ -1,9 +1,13 @@
-"""GPU: adapter_rows and adapter_rows_backward at the edges of their sizes: no rows, gradients inside other tensors."""
+"""GPU: adapter_rows and adapter_rows_backward at the edges of their sizes: no rows, gradients inside other
+tensors, many documents and adapters and the time they take."""
 from __future__ import annotations
 
 import ctypes
+import random
 
 import pytest
+
+from test_gpu_adapter_rows import Case
 
 pytestmark = pytest.mark.gpu
 
@@ -128,3 +132,25 @@ def test_time_of_short_documents(nxg, torch, dev, dtype, r, T, length):
         cu, ids = cu[::length].contiguous(), ids[:rows // length]
         ms.append(fastest(torch, lambda: nxg.adapter_rows(x, a, b, cu, ids, scale, base=base)))
     assert ms[1] < 12 * ms[0], ms
+
+
+@pytest.mark.parametrize("dtype,wtype", [("float32", "bfloat16"), ("bfloat16", "bfloat16")])
+@pytest.mark.parametrize("docs,n", [(64, 3), (65, 1), (1030, 700), (4096, 2), (4097, 40), (1000, 524), (1000, 525), (3, 5000)])
+def test_many_documents(nxg, torch, dev, dtype, wtype, docs, n):
+    """Documents of 0 to 6 rows of many adapters: of one wave and of all, prepared by one launch and by two."""
+    print(f"adapter_rows {dtype} {wtype} {docs} documents of {n} adapters", flush=True)
+    rng = random.Random(docs)
+    lens, ids = [rng.randrange(7) for _ in range(docs)], [rng.randrange(-1, n + 1) if i % 3 else rng.randrange(min(n, 3)) for i in range(docs)]
+    Case(torch, dtype, wtype, lens, ids, n, 8, 40, 24, T=sum(lens) + 5).check(nxg, torch)
+
+
+def test_time_of_many_adapters(nxg, torch, dev):
+    """Gradients of 4,096 documents with 1,000 adapters: what is done goes by the documents and the adapters, not by their product."""
+    print("adapter_rows_backward, 4,096 documents of 4 rows, 10 and 1,000 adapters", flush=True)
+    ms = []
+    for n in (10, 1000):
+        x, a, b, cu, ids, scale, _ = single_rows(torch, "bfloat16", n, 8, 16384, n_in=64, n_out=64)
+        cu, ids = cu[::4].contiguous(), ids[:4096].clamp(min=0)
+        dy, s = torch.ones_like(x), nxg.adapter_rows(x, a, b, cu, ids)[1]
+        ms.append(fastest(torch, lambda: nxg.adapter_rows_backward(dy, x, a, b, s, cu, ids)))
+    assert ms[1] < 4 * ms[0] + 0.1, ms
