@@ -242,7 +242,8 @@ NXG_API int32_t nxg_adapter_rows(const nxg_adapter_rows_params * params, const v
  * The sums are taken in a fixed order: the same call gives the same bits.
  *   dy       device rows of n_out values;  x, s  as the forward call had and left them
  *   base     rows of n_in values (the shared projection's part of dx), or null: 0;  dx  rows, or null; may be base, with its stride
- *   da, db   device, as a and b, or null; zeros for an adapter that no row has
+ *   da, db   device, as a and b, or null; zeros for an adapter that no row has. n_adapters * (n_in / 64 + n_out / 64), each rounded up,
+ *            below 2^22 - 1
  *   workspace  device memory, 16-byte aligned, nxg_adapter_rows_backward_workspace_bytes (on the current device) bytes */
 NXG_API int64_t nxg_adapter_rows_backward_workspace_bytes(const nxg_adapter_rows_params * params);
 NXG_API int32_t nxg_adapter_rows_backward(const nxg_adapter_rows_params * params, const void * dy, int64_t dy_stride, const void * x,

@@ -1414,7 +1414,8 @@ int32_t nxg_adapter_rows_backward(const nxg_adapter_rows_params * params, const 
     p.w_type = a.w_type;
     const int64_t turned = (int64_t) a.n_adapters * ((a.n_in + 63) / 64 + (a.n_out + 63) / 64);
     const int64_t jobs = l.n_slots * (p.slabs_a + p.slabs_b);
-    if (turned >= MAX_GRID || jobs > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d n_adapters=%d is too large", what, a.T, a.n_adapters);
+    // the strips' workgroups have 1,024 threads, four times the others'
+    if (turned >= MAX_GRID / 4 || jobs > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d n_adapters=%d is too large", what, a.T, a.n_adapters);
     NXG_TRY(nxg_check_device());
     hipStream_t st = (hipStream_t) stream;
     auto prepare = [&](int64_t grid, int parts) {

@@ -231,3 +231,10 @@ def test_host_tensors_refused(nxg):
         nxg.adapter_rows(x, torch.zeros(1, 4, 8), torch.zeros(1, 8, 4), [0, 4], [0])
     with pytest.raises(ValueError, match="does not take"):
         nxg.adapter_rows(x.double(), torch.zeros(1, 4, 8), torch.zeros(1, 8, 4), [0, 4], [0])
+
+
+def test_adapter_backward_launches_refused(nxg, L):
+    """More strips of 64 columns than a launch of 1,024 threads each takes: refused, not left to the launch."""
+    for kw in ({"n_adapters": 131072, "rank": 3, "n_in": 1024, "n_out": 1024}, {"n_adapters": 2097152, "rank": 1, "n_in": 64, "n_out": 64}):
+        p = adapter_params(nxg, **kw)
+        refused(nxg, L, adapter_back(nxg, L, p, dys=1024, xs=1024, bs=1024, dxs=1024, n=1 << 50), "too large")
