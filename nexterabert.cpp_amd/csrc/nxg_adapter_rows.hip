@@ -1222,8 +1222,7 @@ int32_t launch_rows(const char * what, adapter_p & p, int32_t type, int32_t w_ty
         if (p.r > 64 && p.T / 128 >= 2 * cus && mean >= 128) rows = 128;
         else if (p.T / 64 >= (p.r > 64 && !f32 ? 1 : 2) * cus) rows = 64;
     }
-    const int64_t slots = p.T / rows + (int64_t) p.n_seqs;
-    if (slots * 8 > MAX_GRID) return nxg_fail(NXG_EINVAL, "%s: T=%d n_seqs=%d is too large", what, p.T, p.n_seqs);
+    const int64_t slots = p.T / rows + (int64_t) p.n_seqs;         // below 2^20 + 2^22
     const bool direct = !f32 && p.r <= 32 && slots < cus / 2;
     // Single rows, two an adapter on the average: those that share one go together (fp32, ids by chance, together and one by one: 65 rows of
     // 64 adapters of rank 16 11.0 and 10.3 us, of rank 128 both 35; 1,000 rows of 512 30 and 28, 131 and 161; 4,096 rows of 64 45 and 73,

@@ -154,3 +154,22 @@ def test_time_of_many_adapters(nxg, torch, dev):
         dy, s = torch.ones_like(x), nxg.adapter_rows(x, a, b, cu, ids)[1]
         ms.append(fastest(torch, lambda: nxg.adapter_rows_backward(dy, x, a, b, s, cu, ids)))
     assert ms[1] < 4 * ms[0] + 0.1, ms
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_millions_of_documents(nxg, torch, dev, dtype):
+    """As many documents as the header allows, nearly all of them empty: the same bits as without the empty ones."""
+    S = (1 << 22) - 1
+    print(f"adapter_rows {dtype} {S} documents", flush=True)
+    x, a, b, _, _, scale, base = single_rows(torch, dtype, 5, 16, 600, n_in=64, n_out=72)
+    at = torch.tensor([0, 3, 1000, 2_000_000, S - 1], device="cuda")             # documents of 120 rows each
+    lens, ids = torch.zeros(S, dtype=torch.int64, device="cuda"), torch.full((S,), 4, dtype=torch.int32, device="cuda")
+    lens[at], ids[at] = 120, torch.tensor([1, 0, -1, 1, 3], dtype=torch.int32, device="cuda")
+    cu = torch.cat([lens.new_zeros(1), torch.cumsum(lens, 0)]).int()
+    few = torch.arange(0, 601, 120, dtype=torch.int32, device="cuda")
+    dy = torch.ones_like(base)
+    for c, i in ((cu, ids), (few, ids[at].contiguous())):
+        y, s = nxg.adapter_rows(x, a, b, c, i, scale, base=base)
+        got = (y, s) + nxg.adapter_rows_backward(dy, x, a, b, s, c, i, scale)
+        want = got if c is cu else want
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
