@@ -508,16 +508,16 @@ def _adapter_bytes(dev, ty, wt, T, K, N, r, n, n_seqs):
 
 
 def _ids_arg(ids, n_seqs, like, dev):
-    """ids (host sequence or device int32 tensor) as a device int32 tensor [n_seqs]."""
+    """ids (host sequence or tensor, or device int32 tensor) as a device int32 tensor [n_seqs]."""
     torch = _torch()
-    if not isinstance(ids, torch.Tensor):
+    if not isinstance(ids, torch.Tensor) or ids.device.type == "cpu":
         host = np.ascontiguousarray(ids)
         if host.ndim == 1 and host.shape[0] == n_seqs and host.dtype.kind in "iu":
             return _uploaded(np.clip(host, -1, _INT32).astype(np.int32), like.device)
     elif ids.is_cuda and ids.get_device() == dev and ids.dtype == torch.int32 and ids.dim() == 1 and ids.shape[0] == n_seqs \
             and ids.is_contiguous():
         return ids
-    raise ValueError(f"ids must be {n_seqs} whole numbers: a host sequence, or a contiguous int32 tensor on the current device")
+    raise ValueError(f"ids must be {n_seqs} whole numbers: a host sequence or tensor, or a contiguous int32 tensor on the current device")
 
 
 def _adapter_args(x, a, b, cu_offsets, ids, scale):

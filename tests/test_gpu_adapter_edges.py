@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes
 import random
 
+import numpy as np
 import pytest
 
 from test_gpu_adapter_rows import Case
@@ -173,3 +174,21 @@ def test_millions_of_documents(nxg, torch, dev, dtype):
         got = (y, s) + nxg.adapter_rows_backward(dy, x, a, b, s, c, i, scale)
         want = got if c is cu else want
         assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+def test_ids_of_the_host(nxg, torch, dev):
+    """Whole numbers of any kind, as cu_offsets takes them: lists, arrays and tensors; past 32 bits they are no adapter."""
+    print("adapter_rows ids of the host", flush=True)
+    x, a, b, _, _, scale, base = single_rows(torch, "bfloat16", 3, 8, 40, n_in=64, n_out=64)
+    cu, ids = [0, 10, 15, 40], [2, 0, 1]
+    want = nxg.adapter_rows(x, a, b, cu, ids, scale, base=base)
+    kinds = [np.array(ids, t) for t in (np.uint8, np.int16, np.uint32, np.int64, np.uint64)]
+    for host in kinds + [torch.tensor(ids, dtype=t) for t in (torch.uint8, torch.int16, torch.int32, torch.int64)] + \
+            [torch.tensor([2, 9, 0, 9, 1, 9])[::2]]:
+        got = nxg.adapter_rows(x, a, b, torch.tensor(cu), host, scale, base=base)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    far = nxg.adapter_rows(x, a, b, cu, np.array([2 ** 32, 2 ** 40 + 1, -2 ** 40]), scale, base=base)
+    assert torch.equal(far[0], base) and (far[1] == 0).all()
+    for bad in (torch.tensor([2.0, 0.0, 1.0]), torch.tensor([[2, 0, 1]]), torch.tensor([2, 0]), [2.0, 0.0, 1.0], torch.tensor(ids, device="cuda")):
+        with pytest.raises(ValueError, match="ids"):
+            nxg.adapter_rows(x, a, b, cu, bad, scale, base=base)
