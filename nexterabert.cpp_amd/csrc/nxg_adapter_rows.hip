@@ -513,7 +513,8 @@ template <class E, class W, int MT, int RT>
 __global__ __launch_bounds__(256, 2) void adapter_rows_tall_kernel(adapter_p p) {
     constexpr int V = operand<E>::V, RP = 16 * RT, LD = RP + 4;
     constexpr int WV = 16 / (int) sizeof(W), A_ROW = 8 * V * (int) sizeof(W);
-    constexpr int A_LOADS = (RP * A_ROW / 1024 + 3) / 4;   // of a wave
+    constexpr int A_LOADS = RP * A_ROW / 4096;             // of a wave
+    static_assert(RP * A_ROW % 4096 == 0, "the four waves' loads are all of a step's weights");
     constexpr int OUT = 8 * V * 4 + 16;
     constexpr int X_BYTES = std::max(std::max(16 * MT * 128, 16 * OUT), 16 * LD * 4), A_BYTES = RP * A_ROW + 8 * V * 16;
     typedef typename operand<E>::vec vec;
@@ -558,7 +559,6 @@ __global__ __launch_bounds__(256, 2) void adapter_rows_tall_kernel(adapter_p p) 
             for (int i = 0; i < 2 * MT; ++i) *reinterpret_cast<v4i *>(xs + (8 * i + row8) * 128 + ((at8 ^ ((4 * i + (lane >> 4)) & 7)) << 4)) = s.x[i];
 #pragma unroll
             for (int i = 0; i < A_LOADS; ++i) {
-                if (rank[i] >= RP) continue;               // a wave without a share (few ranks)
                 if constexpr (A_ROW == 128) *reinterpret_cast<v4i *>(buf + rank[i] * 128 + ((at8 ^ ((rank[i] >> 1) & 7)) << 4)) = s.a[i];
                 else *reinterpret_cast<v4i *>(buf + rank[i] * 64 + (((lane & 3) ^ ((rank[i] >> 2) & 3)) << 4)) = s.a[i];
             }
