@@ -52,3 +52,27 @@ def test_lily_state_many_rows(nxg, torch, dev, docs):
     qa = nxg.lily_state_quantize_rows(a, x, b, torch.randn(2, C, device="cuda", generator=g), cu)
     torch.cuda.synchronize()
     assert qa.T == T
+
+
+@pytest.mark.parametrize("first,docs", [(4000, 100), (4000, 64), (1, 70), (5990, 3)])
+@pytest.mark.parametrize("right", [-1, 0])
+def test_attention_rows_of_documents_behind_other_rows(nxg, torch, dev, first, docs, right):
+    """The documents' rows are those of a call in which the rows in front are a document of their own, forward and back, and the rows
+    in front are left as they were."""
+    print(f"attention_rows, {docs} documents from row {first}, against a document in front", flush=True)
+    T = 6000
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v, dout = (torch.randn(T, n, 64, device="cuda", generator=g).to(torch.bfloat16) for n in (4, 2, 2, 4))
+    cu = torch.tensor(np.linspace(first, T, docs + 1).astype(np.int32), device="cuda")
+    whole = torch.cat([torch.zeros(1, dtype=torch.int32, device="cuda"), cu])
+    want, lse_want = nxg.attention_rows(q, k, v, whole, right=right)
+    grads_want = nxg.attention_rows_backward(dout, q, k, v, want, lse_want, whole, right=right)
+    out, lse = torch.full_like(q, 7.0), torch.full((T, 4), 7.0, device="cuda")
+    nxg.attention_rows(q, k, v, cu, right=right, out=out, lse=lse)
+    grads = [torch.full_like(t, 7.0) for t in (q, k, v)]
+    nxg.attention_rows_backward(dout, q, k, v, want, lse_want, cu, right=right, dq=grads[0], dk=grads[1], dv=grads[2])
+    for name, a, b in zip(("out", "lse", "dq", "dk", "dv"), (out, lse) + tuple(grads), (want, lse_want) + tuple(grads_want)):
+        assert (a[:first] == 7).all(), name
+        # the two launches may share a long sum out differently: fp32 sums of up to 6,000 terms, rounded to bf16 once
+        d = (a[first:].float() - b[first:].float()).abs()
+        assert bool((d <= 2.0 ** -7 * b[first:].float().abs() + 6000 * 2.0 ** -24 * b[first:].float().abs().max()).all()), name
