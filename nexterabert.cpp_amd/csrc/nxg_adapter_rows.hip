@@ -1207,11 +1207,18 @@ int32_t launch_rows(const char * what, adapter_p & p, int32_t type, int32_t w_ty
     const int V = 16 / size_of(type), cus = nxg_device_cus();
     const bool w = wide(p.x, p.x_s) && (!p.base || wide(p.base, p.base_s)) && wide(p.y, p.y ? p.y_s : 0) && p.K % V == 0 && p.N % V == 0 &&
                    p.K * (int64_t) size_of(w_type) % 16 == 0 && p.N * (int64_t) p.r * size_of(w_type) % 16 == 0;
-    // Which kernel, and rows of a workgroup: the larger ones read the weights less often, where that leaves work for every CU
-    // (1,024 to 1,024, caches cold: 32,768 rows of bf16 rank 64 56 us with 64 rows, 82 with 16, of rank 32 45 and 50; 16,384 rows of
-    // rank 64 45 and 44, of rank 128 71 and 106; 8,192 of rank 128 67 and 54; 32,768 of fp32 rank 64 126 and 151; 65,536 of rank 128
-    // 140 with 128 rows, 172 with 64). Straight from memory: one row of bf16 rank 16 6.4 us, through LDS 8.3; 64 requests of one
-    // row 8.7 and 10.0; 2,000 rows 12.5 both; 3,500 rows 13.4 and 12.8, of rank 32 15.2 and 13.6; 8,000 rows 24.6 and 17.8.
+    // Which kernel, and rows of a workgroup: the larger ones read the weights less often, where that leaves work for every CU. 1,024 to
+    // 1,024, caches cold, one document and 32, with 64 rows and with 16 (320, 2,304 and 4,096 columns give the same answers):
+    //   bf16 rank 32   24,000 rows 38, 39 and 39, 42 us   32,768 42, 49 and 51, 52   65,536 73, 85 and 98, 98
+    //   bf16 rank 64   16,000 43, 47 and 38, 40           32,768 53, 63 and 77, 78   65,536 86, 88 and 152, 159
+    //   bf16 rank 128  8,192 62, 62 and 51, 72            16,000 64, 74 and 97, 99   32,768 80, 126 and 191, 193
+    //   fp32 rank 64   24,000 110, 111 and 99, 101        32,768 116, 150 and 132, 134   40,000 152, 152 and 162, 164
+    //   fp32 rank 128  24,000 192, 193 and 236, 240       32,768 197, 275 and 314, 319   65,536 381, 387 and 614, 628
+    // With 128 rows and with 64, bf16 rank 128: 65,536 rows 122, 189 and 149, 149; 100,000 219, 221 and 251, 253. fp32 has none of them: 65,536
+    // rows 356, 525 and 381, 387; 80,000 545, 623 and 449, 450; 130,000 683, 684 and 700, 700. The steps are those of 512 workgroups at a time.
+    // Straight from memory: one row of bf16 rank 16 6.4 us, through LDS 8.3; 64 requests of one row 8.7 and 10.0; 2,000 rows 12.5 both;
+    // 3,500 rows 13.4 and 12.8, of rank 32 15.2 and 13.6; 8,000 rows 24.6 and 17.8. fp32 rows go through LDS always: one row of rank 16 6.4 us,
+    // straight 7.1; 64 requests 7.9 and 9.4; 500 rows 7.2 and 9.4; 1,900 rows 12.7 and 15.1, of rank 32 14.3 and 19.3.
     const bool f32 = type == NXG_TYPE_F32;
     int rows = 16;
     // A tile's rows are of one document, so that the documents have to be long enough on the average, too (8 adapters, with 64 rows and
@@ -1219,7 +1226,7 @@ int32_t launch_rows(const char * what, adapter_p & p, int32_t type, int32_t w_ty
     // of 1 2,928 and 583; 32,768 of fp32 rank 128 of 48 rows 279 and 435, of 32 468 and 356, of 1 10,051 and 852).
     const int mean = p.T / p.n_seqs;
     if (w && p.r > (f32 ? 32 : 16) && mean >= (f32 ? 48 : 32)) {
-        if (p.r > 64 && p.T / 128 >= 2 * cus && mean >= 128) rows = 128;
+        if (p.r > 64 && !f32 && p.T / 128 >= 2 * cus && mean >= 128) rows = 128;
         else if (p.T / 64 >= (p.r > 64 && !f32 ? 1 : 2) * cus) rows = 64;
     }
     const int64_t slots = p.T / rows + (int64_t) p.n_seqs;         // below 2^20 + 2^22
@@ -1246,7 +1253,7 @@ int32_t launch_rows(const char * what, adapter_p & p, int32_t type, int32_t w_ty
             if constexpr (!F32 && rt() <= 2) {
                 if (direct) return adapter_rows_kernel<E, W, rt(), WIDE><<<grid, 256, 0, s>>>(p);
             }
-            if constexpr (rt() == 8) {
+            if constexpr (!F32 && rt() == 8) {
                 if (rows == 128) return adapter_rows_tall_kernel<E, W, 2, rt()><<<grid, 256, 0, s>>>(p);
             }
             if constexpr (rt() > (F32 ? 2 : 1)) {
