@@ -7,9 +7,10 @@
  *   nxg_rope_rows        rotary positions                     (beside nxg_qk_prep)
  *   nxg_layer_norm_rows  layer norm, forward and backward     (beside nxg_layer_norm)
  *   nxg_attention_rows   attention, forward and backward      (beside nxg_attention)
- *   nxg_qk_norm_rope_rows  norms of queries and keys for each head, then their rotation, forward and backward (beside nxg_qk_prep)
+ *   nxg_qk_norm_rope_rows  RMS norms of queries and keys for each head, then their rotation, forward and backward: of layers that have
+ *                          them (the encoder's own heads have nxg_qk_prep's tanh there, which has no gradient here)
  *   nxg_dropout_rows     dropout whose mask is drawn again where it is needed
- *   nxg_adapter_rows     low-rank adapters of many requests, forward and backward (beside nxg_linear_i8)
+ *   nxg_adapter_rows     low-rank adapters of many requests, forward and backward (beside nxg_linear_i8, which has no gradient)
  *
  * They have no counterpart in the reference (NexteraBERT.cpp), which only infers. Conventions
  * are nxg_linear.h's: device pointers on the current device, `stream` a hipStream_t, NXG_OK or an
@@ -19,7 +20,8 @@
  * another array of its call, except where it may be that array itself.
  *
  * Types are nxg_type's numbers: NXG_TYPE_F32, NXG_TYPE_F16, NXG_TYPE_BF16. Sums, statistics and
- * products are fp32 or wider whatever the rows' type; a result is rounded to it once.
+ * products are fp32 or wider whatever the rows' type, but where a function says what it carries in
+ * fewer bits; a result is rounded to its type once.
  *
  * Rows of several heads are given as a pointer and two strides in values (not bytes): value
  * (t, h, d) is at data + t * token_stride + h * head_stride + d. So the heads may lie inside a fused
@@ -27,8 +29,8 @@
  *
  * Packed documents: cu is device int32, n_seqs + 1 offsets, from 0 and not decreasing (an empty
  * document is allowed). Rows that no document covers have no part in a result of
- * nxg_attention_rows and its gradient, and are not written. Other offsets give unspecified rows but
- * no access out of bounds.
+ * nxg_attention_rows, nxg_adapter_rows and their gradients, and are not written. Other offsets give
+ * unspecified rows but no access out of bounds.
  */
 #ifndef NXG_ROWS_H
 #define NXG_ROWS_H
@@ -215,7 +217,8 @@ NXG_API int32_t nxg_dropout_rows(int32_t type, const void * x, int64_t x_stride,
  * Low-rank adapters
  * ------------------------------------------------------------------------- */
 
-/* Document d has adapter i = ids[d], or none (an id that is not in 0 .. n_adapters - 1). */
+/* Document d has adapter i = ids[d], or none (an id that is not in 0 .. n_adapters - 1). All adapters have one rank and one
+ * scale: a smaller rank is filled up with zeros in a and b, another scale multiplied into b (db is then that product's gradient). */
 typedef struct nxg_adapter_rows_params {
     int32_t type;              /* of the rows */
     int32_t w_type;            /* of a and b: `type`; F32 rows take F32, F16 or BF16 */
@@ -230,8 +233,11 @@ typedef struct nxg_adapter_rows_params {
     float   scale;             /* of every adapter's share, finite */
 } nxg_adapter_rows_params;
 
-/* s = x a_i^T,  y = base + scale * s b_i^T  per row of a document; rows of a document without an adapter get base, and 0 as s. A row
- * of x or base that holds an infinity or a NaN may give NaN where it would give an infinity; it has no part in other rows.
+/* s = x a_i^T,  y = base + scale * s b_i^T  per row of a document; rows of a document without an adapter get base, and 0 as s.
+ * s is fp32. Beside F16 and BF16 rows it enters the product with b as the sum of two bf16 values, off by at most 2^-16 of it, and F16
+ * weights as such a sum too, without the product of both second parts (2^-16 of a term more); beside F32 rows every product is
+ * fp32. A row of x or base that holds an infinity or a NaN, or whose s does, may give NaN where it would give an infinity; it has no
+ * part in other rows.
  *   x      device rows of n_in values, base, y  of n_out (their strides in values); base may be null: 0. y may be base, with its stride
  *   s      device float [T][rank]: what nxg_adapter_rows_backward takes */
 NXG_API int32_t nxg_adapter_rows(const nxg_adapter_rows_params * params, const void * x, int64_t x_stride, const void * base,
@@ -239,7 +245,9 @@ NXG_API int32_t nxg_adapter_rows(const nxg_adapter_rows_params * params, const v
 
 /* The gradients, with g = scale * dy b_i:
  *   dx = base + g a_i,  da_i = sum of g^T x,  db_i = scale * sum of dy^T s  over the rows of the documents with adapter i
- * The sums are taken in a fixed order: the same call gives the same bits.
+ * The sums are taken in a fixed order: the same call gives the same bits. g and s are carried as s in the forward call. A row of dy or x
+ * that holds an infinity or a NaN, or whose g or s does, may give NaN for infinities in its row of dx and anywhere in da_i and db_i of
+ * its adapter; it has no part in other rows' dx and other adapters' gradients.
  *   dy       device rows of n_out values;  x, s  as the forward call had and left them
  *   base     rows of n_in values (the shared projection's part of dx), or null: 0;  dx  rows, or null; may be base, with its stride
  *   da, db   device, as a and b, or null; zeros for an adapter that no row has. n_adapters * (n_in / 64 + n_out / 64), each rounded up,

@@ -4,7 +4,8 @@ attention in fp32 too).
 
 Rows of several heads are tensors [T][n_head][head_dim] with any strides whose last is 1 (a slice of a
 fused projection, or head-major storage as a transposed view). Documents are given by cu_offsets, a host
-sequence or a device int32 tensor, with empty documents allowed. Every function takes the streams and
+sequence or a device int32 tensor, with empty documents allowed. Rows of no document are not written by attention_rows, adapter_rows
+and their gradients: an output that the call makes holds anything there. Every function takes the streams and
 raises the errors that the package's other functions do, and keeps nothing between calls.
 """
 from __future__ import annotations
@@ -423,7 +424,8 @@ def _rows_out(t, name, dev, like):
 def qk_norm_rope_rows(q, k, wq, wk, freq, cu_offsets=None, positions=None, eps: float = 1e-6, layout: str = "half",
                       mscale: float = 1.0, q_out=None, k_out=None, stream=None):
     """The RMS norm of every head of q [T][n_head][head_dim] and k [T][n_kv_head][head_dim] (fp32, fp16 or bf16), times wq or
-    wk [head_dim] (of their type or fp32), then rotary positions as rope_rows turns them. k and wk may both be None. Returns
+    wk [head_dim] (of their type or fp32), then rotary positions as rope_rows turns them: for layers whose heads have RMS norms
+    (the encoder's own have qkv_prep's tanh there). k and wk may both be None. Returns
     (q_out, k_out), which may be q and k."""
     p, qr, kr, cu, dev = _qk_args(q, k, wq, wk, freq, cu_offsets, positions, eps, layout, mscale)
     q_out, qo = _rows_out(q_out, "q_out", dev, q)
@@ -562,7 +564,8 @@ def adapter_rows(x, a, b, cu_offsets, ids, scale: float = 1.0, base=None, out=No
     """Low-rank adapters of many requests: document d's rows of x [T][n_in] through adapter i = ids[d], base + scale * (x a_i^T)
     b_i^T, a [n_adapters][rank][n_in] and b [n_adapters][n_out][rank] of x's type (fp32 rows, as the int8 linears leave them: of any
     type). base [T][n_out]: the shared projection's rows, or None. An id that is no adapter leaves base as it is (0 without).
-    Returns (out, s), s the fp32 [T][rank] rows x a_i^T, as adapter_rows_backward takes them. out may be base."""
+    Returns (out, s), s the fp32 [T][rank] rows x a_i^T, as adapter_rows_backward takes them. out may be base. Rows of no document
+    are left as they were (uninitialised where the call makes out or s). ids: a host sequence or tensor, or device int32."""
     p, (_, _, T, _, N, r, _, _), cu, ids, dev = _adapter_args(x, a, b, cu_offsets, ids, scale)
     xp, xs = _plain_rows(x, "x", dev)
     bp, bs = (None, 0) if base is None else _rows_of_width(base, "base", dev, x.dtype, T, N)
@@ -591,7 +594,8 @@ def adapter_rows_backward(dout, x, a, b, s, cu_offsets, ids, scale: float = 1.0,
                           stream=None):
     """The gradients of adapter_rows: (dx, da, db), from dout [T][n_out], its inputs and the s that it returned. base [T][n_in]: what
     dx is added to (the shared projection's part), or None; dx may be base. da and db as a and b, zeros for adapters
-    that no row has. workspace: None (made for the call) or a uint8 device tensor of adapter_rows_backward_workspace_bytes."""
+    that no row has. Rows of no document are left as they were in dx. workspace: None (made for the call) or a uint8 device tensor of
+    adapter_rows_backward_workspace_bytes."""
     p, sizes, cu, ids, dev = _adapter_args(x, a, b, cu_offsets, ids, scale)
     _, _, T, K, N, r, _, _ = sizes
     xp, xs = _plain_rows(x, "x", dev)
