@@ -512,7 +512,7 @@ def _adapter_bytes(dev, ty, wt, T, K, N, r, n, n_seqs):
 def _ids_arg(ids, n_seqs, like, dev):
     """ids (host sequence or tensor, or device int32 tensor) as a device int32 tensor [n_seqs]."""
     torch = _torch()
-    if not isinstance(ids, torch.Tensor) or ids.device.type == "cpu":
+    if not isinstance(ids, torch.Tensor) or (ids.device.type == "cpu" and not ids.is_floating_point()):
         host = np.ascontiguousarray(ids)
         if host.ndim == 1 and host.shape[0] == n_seqs and host.dtype.kind in "iu":
             return _uploaded(np.clip(host, -1, _INT32).astype(np.int32), like.device)

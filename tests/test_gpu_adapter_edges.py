@@ -189,6 +189,35 @@ def test_ids_of_the_host(nxg, torch, dev):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     far = nxg.adapter_rows(x, a, b, cu, np.array([2 ** 32, 2 ** 40 + 1, -2 ** 40]), scale, base=base)
     assert torch.equal(far[0], base) and (far[1] == 0).all()
-    for bad in (torch.tensor([2.0, 0.0, 1.0]), torch.tensor([[2, 0, 1]]), torch.tensor([2, 0]), [2.0, 0.0, 1.0], torch.tensor(ids, device="cuda")):
+    for bad in (torch.tensor([2.0, 0.0, 1.0]), torch.tensor(ids, dtype=torch.bfloat16), torch.tensor([True, False, True]), torch.tensor([[2, 0, 1]]), torch.tensor([2, 0]), [2.0, 0.0, 1.0], torch.tensor(ids, device="cuda")):
         with pytest.raises(ValueError, match="ids"):
             nxg.adapter_rows(x, a, b, cu, bad, scale, base=base)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("docs,n,rows", [(3000, 200, 1), (3000, 200, 3), (40, 5, 30)])
+def test_replays_with_other_documents_and_adapters(nxg, torch, dev, dtype, docs, n, rows):
+    """A captured call of many documents, replayed after its offsets and ids have changed, on another stream than it was made for:
+    the bits of the same call made then."""
+    print(f"adapter_rows {dtype} {docs} documents of {n} adapters, captured", flush=True)
+    x, a, b, _, ids, scale, base = single_rows(torch, dtype, n, 8, docs * rows, n_in=64, n_out=72)
+    cu = (torch.arange(docs + 1, device="cuda") * rows).int()
+    ids, dy = ids[:docs].contiguous(), torch.ones_like(base)
+
+    def both():
+        y, s = nxg.adapter_rows(x, a, b, cu, ids, scale, base=base)
+        return (y, s) + nxg.adapter_rows_backward(dy, x, a, b, s, cu, ids, scale)
+    both()
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        got = both()
+    for turn in range(4):
+        ids.copy_(torch.roll(ids, 1 + 7 * turn))
+        if turn % 2:
+            cu[docs // 3:docs // 2] = int(cu[docs // 3])             # empty ones, and a longer one behind them
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(u, v) for u, v in zip(got, both())), turn
